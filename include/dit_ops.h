@@ -1,0 +1,137 @@
+/*
+ * dit_ops.h — C ABI of the operators around a projection in 8-bit floating
+ * point on MI355X (gfx950): rows and weights in e4m3 with a power-of-two scale
+ * for each block of 128, their product, and rotary positions on what comes out.
+ * No counterpart in the reference, whose projections are fp16 / bf16
+ * (dit_vk.cpp:321-322) and whose rotation is part of its attention
+ * (dit_vk.cpp:62-71).
+ *
+ *   q, s   = quant(rows)                 once per activation
+ *   w, sw  = quant(weight, 128 x 128)    once per weight
+ *   qkv    = product(q, s, w, sw)
+ *   rope(q and k columns of qkv, positions)
+ *
+ * Conventions as awa_capi.h: device pointers, stream-ordered and asynchronous,
+ * 0 / AWA_EARG / AWA_EHIP, messages through awa_last_error of the context.
+ * These calls allocate nothing and use no scratch of the context, so they may
+ * be captured into graphs, and calls on different streams may overlap.
+ */
+#ifndef SEEDVR2_DIT_OPS_H
+#define SEEDVR2_DIT_OPS_H
+
+#include <stdint.h>
+
+#include "awa_capi.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Sizes that the calls below accept: rows (or tokens), and columns. */
+enum { DIT_OPS_ROWS_MAX = 1 << 24, DIT_OPS_COLS_MAX = 1 << 20 };
+
+/* ---- e4m3 rows --------------------------------------------------------------
+ *
+ * A matrix [rows][cols] in 8 bits is
+ *   q      e4m3 (OCP: finite to 448, no infinity) [rows][kp], kp = cols rounded
+ *          up to a multiple of 128, columns past cols zero; 16-byte aligned
+ *   scale  uint32 words [groups][ld], groups = ceil(cols / 512): word [g][r]
+ *          holds the scales of blocks 4 g .. 4 g + 3 (128 columns each) of row r
+ *          (of rows 128 r .. 128 r + 127 in the form for weights), the first in
+ *          the low byte; a scale byte b stands for 2^(b - 127) (E8M0), bytes of
+ *          blocks past the last one are 0; ld words from group to group.
+ * The value of an element is q 2^(b - 127).  Rows can be cut anywhere: rows from
+ * r0 on are q + r0 kp and scale + r0 (r0 / 128 for weights, r0 a multiple of
+ * 128), with the same ld.
+ *
+ * Scales are powers of two because the matrix instructions of CDNA4 apply such
+ * scales by themselves.  e4m3 is a floating-point format: a scale between two
+ * powers of two would move a block's range, not the values' relative precision.
+ */
+enum { DIT_FP8_BLOCK = 128 };
+
+/* Quantises d_x [M][K] of type dtype (AWA_F32 or AWA_BF16), rows ldx elements
+ * apart.  block_rows 1: a scale for each 128 columns of a row (activations);
+ * block_rows 128: for each 128 x 128 block (weights).  A block's scale is the
+ * smallest 2^e with every finite magnitude at most 448 2^e, e >= -127; values
+ * are rounded to the nearest (ties to even).  Infinities and NaNs become NaN and
+ * take no part in the scale.  M may be 0.  d_x needs its elements' alignment only.
+ * Rejected (AWA_EARG): M or K out of range, ldx < K (for M > 1), ld_scale less
+ * than the rows (row blocks), d_q not 16-byte or d_scale not 4-byte aligned,
+ * outputs that lie over d_x. */
+int dit_quant_fp8(awa_ctx* ctx, int dtype, const void* d_x, int64_t ldx, int M, int K, int block_rows,
+                  uint8_t* d_q, uint32_t* d_scale, int64_t ld_scale, awa_stream_t stream);
+
+/* C[m][n] = sum over k of A[m][k] W[n][k], plus bias[n] (fp32, may be NULL): A is
+ * [M][K] in e4m3 rows with a scale per row and block, W [N][K] with a scale per
+ * 128 x 128 block (both as dit_quant_fp8 writes them; K is their padded width, a
+ * multiple of 128).  fp32 accumulation; C of type dtype_c (AWA_F32 or AWA_BF16),
+ * rows ldc elements apart, rounded once.  M (also 0) and N are any size.
+ * The result of a row does not depend on the other rows of A, but on their number
+ * in the order of its sums.
+ * Rejected (AWA_EARG): sizes out of range, K not a multiple of 128, ldc < N (for
+ * M > 1), ld_as < M, ld_ws < ceil(N / 128), a misaligned pointer (A and W 16
+ * bytes, scales and bias 4, C its elements), C over an input. */
+int dit_gemm_fp8(awa_ctx* ctx, const uint8_t* d_a, const uint32_t* d_as, int64_t ld_as, const uint8_t* d_w,
+                 const uint32_t* d_ws, int64_t ld_ws, const float* d_bias, int dtype_c, void* d_c,
+                 int64_t ldc, int M, int N, int K, awa_stream_t stream);
+
+/* ---- rotary positions -------------------------------------------------------
+ *
+ * Channel pair i of a head turns by the angle pos[axis of i] freq[i]:
+ *   (a, b) -> scale (a cos - b sin, a sin + b cos)
+ * with (a, b) channels (2 i, 2 i + 1) (DIT_ROPE_INTERLEAVED) or (i, pairs + i)
+ * (DIT_ROPE_HALF); channels from 2 pairs on pass through unchanged.
+ */
+enum { DIT_ROPE_INTERLEAVED = 0, DIT_ROPE_HALF = 1 };
+enum { DIT_ROPE_MAX_PAIRS = 128, DIT_ROPE_MAX_AXES = 4 };
+
+typedef struct {
+    int layout;                        /* DIT_ROPE_INTERLEAVED or DIT_ROPE_HALF               */
+    int axes;                          /* positions per token, 1 .. DIT_ROPE_MAX_AXES         */
+    int pairs[DIT_ROPE_MAX_AXES];      /* pairs that turn with each axis, axis after axis     */
+    int inverse;                       /* 1: the angles negated (the adjoint: gradients)      */
+    double scale;                      /* factor of cos and sin (1, or a long context's)      */
+    double freq[DIT_ROPE_MAX_PAIRS];   /* radians per position, pair after pair               */
+} dit_rope_plan;
+
+/* One tensor of the call: heads x head_d channels per token.  Strides count
+ * elements; a head's channels are contiguous. */
+typedef struct {
+    const void* x;
+    void* out;                         /* x itself (same strides) or memory apart from it     */
+    int heads;
+    int64_t x_token, x_head;
+    int64_t out_token, out_head;
+} dit_rope_rows;
+
+/* Rotates one or two tensors (queries and keys) of n_tokens tokens, type dtype
+ * (AWA_F32 or AWA_BF16), at positions d_pos int32 [n_tokens][axes] (any int32).
+ * The plan is copied before the call returns.  Angles are reduced to a turn in
+ * fp64, so far positions keep their precision; products are fp32, rounded once.
+ * n_tokens may be 0.  Rejected (AWA_EARG): head_d over 256 or under twice the
+ * pairs, frequencies or a scale that are not finite, negative strides, outputs
+ * whose elements could coincide, with each other's or with an input's, other than
+ * out = x with the same strides (views of one buffer are accepted where equal
+ * token or head strides keep them apart: q, k and v parts of a row). */
+int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int n_tokens, int head_d,
+             const dit_rope_plan* plan, const int32_t* d_pos, awa_stream_t stream);
+
+/* Frequencies of n pairs for base b (host only): f_i = b^(-i / n), and for a
+ * context stretched by `factor` (at least 1):
+ *   DIT_ROPE_PLAIN   f_i
+ *   DIT_ROPE_LINEAR  f_i / factor                    (positions interpolated)
+ *   DIT_ROPE_BASE    with base b factor^(n / (n - 1)) (the slowest pair is
+ *                    stretched by factor, the fastest not; n > 1)
+ *   DIT_ROPE_BANDS   r = trained f_i / (2 pi) turns over the trained length,
+ *                    t = (r - low) / (high - low) clamped to 0 .. 1,
+ *                    f_i (t + (1 - t) / factor)      (low < high)
+ * trained, low and high are read by DIT_ROPE_BANDS only.  0, or AWA_EARG. */
+enum { DIT_ROPE_PLAIN = 0, DIT_ROPE_LINEAR = 1, DIT_ROPE_BASE = 2, DIT_ROPE_BANDS = 3 };
+int dit_rope_freqs(int kind, int n, double base, double factor, double trained, double low, double high,
+                   double* h_freq);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

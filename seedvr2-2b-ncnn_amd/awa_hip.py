@@ -52,6 +52,23 @@ class DitTimeWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("w_in", "b_in", "w_hid", "b_hid", "w_out", "b_out")]
 
 
+ROPE_MAX_PAIRS, ROPE_MAX_AXES = 128, 4
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "bands": 3}
+
+
+class RopePlan(C.Structure):
+    """dit_rope_plan of include/dit_ops.h."""
+    _fields_ = [("layout", C.c_int), ("axes", C.c_int), ("pairs", C.c_int * ROPE_MAX_AXES), ("inverse", C.c_int),
+                ("scale", C.c_double), ("freq", C.c_double * ROPE_MAX_PAIRS)]
+
+
+class RopeRows(C.Structure):
+    """dit_rope_rows of include/dit_ops.h."""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int)] + [
+        (n, C.c_int64) for n in ("x_token", "x_head", "out_token", "out_head")]
+
+
 class GeomInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in
                 ("t", "h", "w", "nwin", "sumf", "Lv", "txt_len", "max_S", "n_tiles", "n_items")]
@@ -148,6 +165,11 @@ def lib():
         L.dit_reserve.argtypes = [vp, vp, C.c_int]
         L.awa_time_phases.argtypes = [vp, vp, C.c_int, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp,
                                       C.c_float, vp, vp, C.c_int, C.POINTER(C.c_double), vp]
+        L.dit_quant_fp8.argtypes = [vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int64, vp]
+        L.dit_gemm_fp8.argtypes = [vp, vp, vp, C.c_int64, vp, vp, C.c_int64, vp, C.c_int, vp, C.c_int64, C.c_int,
+                                   C.c_int, C.c_int, vp]
+        L.dit_rope.argtypes = [vp, C.c_int, C.POINTER(RopeRows), C.c_int, C.c_int, C.c_int, C.POINTER(RopePlan), vp, vp]
+        L.dit_rope_freqs.argtypes = [C.c_int, C.c_int] + 5 * [C.c_double] + [vp]
         _lib = L
     return _lib
 
@@ -245,6 +267,35 @@ def plan_windows(t, h, w, num_windows, shifted):
     out = np.zeros((max(n, 1), 6), np.int32)
     lib().awa_plan_windows(t, h, w, _ptr(nw), int(bool(shifted)), _ptr(out), n)
     return out[:n]
+
+
+def rope_freqs(n, base=10000.0, kind="plain", factor=1.0, trained=0.0, low=1.0, high=32.0):
+    """dit_rope_freqs: the radians per position of n channel pairs (float64 [n]), for a
+    context stretched by `factor` over a trained length where kind is not "plain"."""
+    out = np.empty(max(int(n), 1), np.float64)
+    rc = lib().dit_rope_freqs(ROPE_KINDS[kind], int(n), float(base), float(factor), float(trained), float(low),
+                              float(high), out.ctypes.data)
+    if rc != AWA_OK:
+        raise AwaError(rc, "dit_rope_freqs rejected the arguments")
+    return out
+
+
+_FP8 = {"e": "float8_e8m0fnu", "q": "float8_e4m3fn", "a": "float8_e4m3fn", "w": "float8_e4m3fn"}
+
+
+def _bytes_of(t, shape, name):
+    """Whether t is a contiguous tensor of this shape of scales (names that end so) or e4m3 values, or of their bytes."""
+    return tuple(t.shape) == shape and t.is_contiguous() and str(t.dtype)[6:] in (_FP8[name[-1]], "uint8")
+
+
+def fp8_values(q, scale, cols=None):
+    """The fp32 values of an 8-bit matrix as quant_fp8 returns it (either form), cut to `cols` columns."""
+    import torch
+    rows, kp = q.shape
+    s = scale.view(torch.uint8).transpose(0, 1).flatten(1)[:, :kp // 128].int() - 127
+    s = s if s.shape[0] == rows else s.repeat_interleave(128, 0)[:rows]
+    v = torch.ldexp(q.view(torch.float8_e4m3fn).float().unflatten(1, (-1, 128)), s[:, :, None]).flatten(1)
+    return v if cols is None else v[:, :cols]
 
 
 def _stream_ptr(stream=None):
@@ -446,6 +497,130 @@ class Context:
                                       C.c_void_p(emb.data_ptr()), _stream_ptr(stream))
         self.check(rc, "dit_time_embedding")
         return emb
+
+    # ---- operators around a projection in 8 bits (include/dit_ops.h)
+    def _on(self, what, *tensors):
+        """Every tensor lives on the context's device."""
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != self.device):
+                raise ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
+
+    def _stream(self, stream, *made):
+        """The stream of a call: the given one, else the current one of the context's device.  Tensors that
+        the call made on the current stream are marked as used on another."""
+        import torch
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        for t in made:
+            t.record_stream(stream)
+        return stream.cuda_stream
+
+    @staticmethod
+    def _dtype(what, dtype):
+        import torch
+        if dtype == torch.bfloat16:
+            return AWA_BF16
+        if dtype == torch.float32:
+            return AWA_F32
+        raise TypeError(f"{what}: unsupported dtype {dtype}")
+
+    def quant_fp8(self, x, blocks=False, q=None, scale=None, stream=None):
+        """dit_quant_fp8: x [rows, cols] bf16 or fp32 (columns contiguous) to (q, scale): q float8_e4m3fn
+        [rows, cols padded to 128], scale float8_e8m0fnu [groups of four column blocks, rows, 4] (blocks=True:
+        a scale per 128 x 128 values, [groups, ceil(rows / 128), 4])."""
+        import torch
+        dtype = self._dtype("quant_fp8", x.dtype)
+        if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+            raise ValueError("quant_fp8: x must be [rows, cols] with contiguous columns")
+        rows, cols = x.shape
+        qs, ss = (rows, (cols + 127) // 128 * 128), ((cols + 511) // 512, (rows + 127) // 128 if blocks else rows, 4)
+        made = []
+        if q is None:
+            q = torch.empty(qs, dtype=torch.float8_e4m3fn, device=x.device)
+            made.append(q)
+        if scale is None:
+            scale = torch.empty(ss, dtype=torch.float8_e8m0fnu, device=x.device)
+            made.append(scale)
+        self._on("quant_fp8", x, q, scale)
+        for t, shape, name in ((q, qs, "q"), (scale, ss, "scale")):
+            if not _bytes_of(t, shape, name):
+                raise ValueError(f"quant_fp8: {name} must be a contiguous {_FP8[name[-1]]} tensor {list(shape)}")
+        if rows:
+            self.check(lib().dit_quant_fp8(self.ptr, dtype, x.data_ptr(), x.stride(0), rows, cols, 128 if blocks else 1,
+                                           q.data_ptr(), scale.data_ptr(), ss[1], self._stream(stream, *made)),
+                       "dit_quant_fp8")
+        return q, scale
+
+    def gemm_fp8(self, a, a_scale, w, w_scale, bias=None, out=None, dtype=None, stream=None):
+        """dit_gemm_fp8: [M, N] = A W^T (+ bias fp32 [N]) of matrices as quant_fp8 returns them, A by rows and W
+        with blocks=True; `dtype` bf16 (default) or fp32, or that of `out` (rows may be strided)."""
+        import torch
+        M, K = a.shape
+        N = w.shape[0]
+        if out is None:
+            out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=a.device)
+            made = (out,)
+        else:
+            made = ()
+            if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (dtype or out.dtype) != out.dtype:
+                raise ValueError(f"gemm_fp8: out must be [{M}, {N}] of dtype {dtype} with contiguous columns")
+        self._on("gemm_fp8", a, a_scale, w, w_scale, bias, out)
+        groups = (K + 511) // 512
+        for t, shape, name in ((a, (M, K), "a"), (w, (N, K), "w"), (a_scale, (groups, M, 4), "a_scale"),
+                               (w_scale, (groups, (N + 127) // 128, 4), "w_scale")):
+            if not _bytes_of(t, shape, name):
+                raise ValueError(f"gemm_fp8: {name} must be a contiguous {_FP8[name[-1]]} tensor {list(shape)}")
+        if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+            raise ValueError(f"gemm_fp8: bias must be a contiguous fp32 tensor [{N}]")
+        ct = self._dtype("gemm_fp8", out.dtype)
+        if M:
+            self.check(lib().dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), M, w.data_ptr(),
+                                          w_scale.data_ptr(), w_scale.shape[1], bias.data_ptr() if bias is not None else None,
+                                          ct, out.data_ptr(), out.stride(0), M, N, K, self._stream(stream, *made)),
+                       "dit_gemm_fp8")
+        return out
+
+    def rope(self, x, positions, freqs, pairs=None, layout="interleaved", scale=1.0, inverse=False, out=None,
+             stream=None):
+        """dit_rope: x [tokens, heads, head_d] (or a pair of such tensors, queries and keys; channels contiguous)
+        rotated at positions int32 [tokens] or [tokens, axes].  freqs: radians per position of each pair
+        (rope_freqs, float64), axis after axis; pairs: how many belong to each axis.  inverse=True is the adjoint,
+        which takes gradients of the output to those of the input.  out: x itself for a rotation in place."""
+        import torch
+        xs = list(x) if isinstance(x, (tuple, list)) else [x]
+        outs = [None] * len(xs) if out is None else list(out) if isinstance(out, (tuple, list)) else [out]
+        if len(xs) not in (1, 2) or len(outs) != len(xs):
+            raise ValueError("rope: one or two tensors, and as many outputs")
+        f = np.ascontiguousarray(freqs, np.float64)
+        axes = positions.shape[1] if positions.dim() == 2 else 1
+        pairs = (f.size,) if pairs is None else tuple(pairs)
+        tokens, _, head_d = xs[0].shape
+        if (positions.dtype != torch.int32 or not positions.is_contiguous() or positions.dim() > 2 or
+                positions.shape[0] != tokens):
+            raise ValueError(f"rope: positions must be contiguous int32 [{tokens}] or [{tokens}, axes]")
+        if len(pairs) != axes or axes > ROPE_MAX_AXES or sum(pairs) != f.size or f.size > ROPE_MAX_PAIRS:
+            raise ValueError(f"rope: pairs {pairs} must name each axis of the positions and sum to the {f.size} freqs")
+        dtype = self._dtype("rope", xs[0].dtype)
+        plan = RopePlan(ROPE_LAYOUTS[layout], axes, pairs, int(bool(inverse)), scale)
+        C.memmove(C.addressof(plan) + RopePlan.freq.offset, f.ctypes.data, 8 * f.size)
+        rows, made = (RopeRows * len(xs))(), []
+        for i, t in enumerate(xs):
+            if t.dim() != 3 or t.dtype != xs[0].dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
+                    head_d > 1 and t.stride(2) != 1):
+                raise ValueError("rope: tensors must be [tokens, heads, head_d] of one dtype with contiguous channels")
+            o = outs[i]
+            if o is None:
+                o = outs[i] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                made.append(o)
+            elif o.shape != t.shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):
+                raise ValueError("rope: out must have x's shape and dtype and contiguous channels")
+            self._on("rope", t, o)
+            rows[i] = RopeRows(t.data_ptr(), o.data_ptr(), t.shape[1], t.stride(0), t.stride(1), o.stride(0),
+                               o.stride(1))
+        self._on("rope", positions)
+        self.check(lib().dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, C.byref(plan), positions.data_ptr(),
+                                  self._stream(stream, *made)), "dit_rope")
+        return tuple(outs) if isinstance(x, (tuple, list)) else outs[0]
 
     def reserve(self, geom, dtype="bf16"):
         """awa_reserve: size the op's scratch for geom in this storage dtype."""

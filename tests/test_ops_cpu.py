@@ -1,0 +1,74 @@
+"""dit_ops.h on the CPU: the refusals of its entry points (tests/cpp/test_ops_args.cpp, which compiles
+csrc/dit_ops.cpp with stubs for the launches and never reads the addresses it passes), the frequencies
+against their formulas, and the shapes that the binding refuses."""
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PKG = os.path.join(ROOT, "seedvr2-2b-ncnn_amd")
+HIPCC = "/opt/rocm/bin/hipcc"
+
+
+def test_refusals(tmp_path):
+    if not os.path.exists(HIPCC):
+        pytest.skip("hipcc not present")
+    exe = str(tmp_path / "test_ops_args")
+    # the shared header holds device helpers, so hipcc compiles the driver (host code only)
+    cmd = [HIPCC, "--offload-arch=gfx950", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(PKG, "csrc"), os.path.join(ROOT, "tests", "cpp", "test_ops_args.cpp"),
+           os.path.join(PKG, "csrc", "dit_ops.cpp"), "-o", exe]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+    assert int(r.stdout.split("checks=")[1].split()[0]) > 100
+
+
+@pytest.mark.parametrize("n,base,factor", [(1, 10000.0, 1.0), (21, 10000.0, 4.0), (64, 500000.0, 32.0), (128, 2.0, 1.5)])
+def test_freqs(awa, n, base, factor):
+    i = np.arange(n)
+    f = base ** (-i / n)
+    close = dict(rtol=1e-14)  # a few roundings of 2^-53 in pow and the products
+    np.testing.assert_allclose(awa.rope_freqs(n, base), f, **close)
+    np.testing.assert_allclose(awa.rope_freqs(n, base, "linear", factor), f / factor, **close)
+    if n > 1:
+        g = awa.rope_freqs(n, base, "base", factor)
+        assert g[0] == 1.0
+        assert math.isclose(g[-1], f[-1] / factor, rel_tol=1e-13)
+    trained, lo, hi = 4096.0, 1.0, 32.0
+    g = awa.rope_freqs(n, base, "bands", factor, trained, lo, hi)
+    turns = trained * f / (2 * np.pi)
+    np.testing.assert_allclose(g[turns >= hi], f[turns >= hi], **close)
+    np.testing.assert_allclose(g[turns <= lo], f[turns <= lo] / factor, **close)
+    t = np.clip((turns - lo) / (hi - lo), 0, 1)
+    np.testing.assert_allclose(g, f * (t + (1 - t) / factor), **close)
+    assert (np.diff(g) < 0).all()
+
+
+def test_freqs_refused(awa):
+    for args in ((0,), (129,), (8, -1.0), (8, 1e4, "linear", 0.5), (8, 1e4, "bands", 2.0, 0.0)):
+        with pytest.raises(awa.AwaError):
+            awa.rope_freqs(*args)
+
+
+def test_binding_refuses_host_tensors(awa):
+    """Refused before any device call (a context object without a device)."""
+    import torch
+    ctx = awa.Context.__new__(awa.Context)
+    ctx.ptr, ctx.device = None, 0
+    x = torch.zeros((3, 256))
+    q, s = torch.zeros((3, 256), dtype=torch.uint8), torch.zeros((1, 3, 4), dtype=torch.uint8)
+    w, ws = torch.zeros((5, 256), dtype=torch.uint8), torch.zeros((1, 1, 4), dtype=torch.uint8)
+    pos = torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: ctx.quant_fp8(x), lambda: ctx.gemm_fp8(q, s, w, ws), lambda: ctx.rope(x[:, None], pos, [1.0]),
+                 lambda: ctx.quant_fp8(x.T), lambda: ctx.rope(x[:, None], pos.long(), [1.0]),
+                 lambda: ctx.rope(x[:, None], pos, [1.0], pairs=(1, 0))):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ctx.quant_fp8(x.half()), lambda: ctx.rope(x[:, None].half(), pos, [1.0])):
+        with pytest.raises(TypeError):
+            call()

@@ -1,0 +1,428 @@
+"""GPU tests of the operators of dit_ops.h against plain forms in 64 bits.
+
+Quantising is exact arithmetic up to one rounding that both sides make alike: bytes are compared for
+equality.  The product's inputs are its 8-bit values, so its reference has no rounding; an fp32 sum of
+products p_i is off by at most half a step (2^-24) of a partial sum per addition.  A partial sum is at most
+S = sum |p_i|; a block of 128 is four bf16 instructions, and the parts of a split K are added at the end (at
+most 16): bar (4 K / 128 + 16) 2^-24 S, and half a step of C's type.  Rotation: a sine or cosine is off by at most 2^-22
+(rounding the reduced angle, its product with pi / 2, the polynomial, the factor: under 2^-24 each) and by the
+angle's own 2^-51 of itself in fp64; products and sum are fp32: bar (|a| + |b|) scale (2^-21 + |angle| 2^-51)
+and half a step of the type.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = "bfloat16", "float32"
+
+
+def dt(name):
+    import torch
+    return getattr(torch, name)
+
+
+def half_step(dtype):
+    import torch
+    return torch.finfo(dtype).eps / 2
+
+
+def within(out, ref, bar):
+    """out within bar of ref everywhere; NaN where ref is, and only there."""
+    import torch
+    out = out.double()
+    assert torch.equal(out.isnan(), ref.isnan())
+    d = torch.nan_to_num((out - ref).abs() - bar, nan=-1.0)
+    assert float(d.max() if d.numel() else -1) <= 0, f"over the bar by {float(d.max())}"
+
+
+# ------------------------------------------------------------------ quantising
+
+def plain_quant(x, per):
+    """(e4m3 values as fp64, scale exponents [row blocks][blocks]) of the definition, for finite and other values."""
+    import torch
+    rows, cols = x.shape
+    kp, rp = -(-cols // 128) * 128, -(-max(rows, 1) // per) * per
+    v = torch.zeros((rp, kp), dtype=torch.float64, device=x.device)
+    v[:rows, :cols] = x.double()
+    fin = torch.where(v.isfinite(), v.abs(), 0.0).reshape(rp // per, per, kp // 128, 128).amax((1, 3))
+    e = torch.ceil(torch.log2(fin / 448.0)).clamp(min=-127.0)
+    y = v / torch.exp2(e).repeat_interleave(per, 0).repeat_interleave(128, 1)
+    step = torch.exp2(torch.floor(torch.log2(y.abs())).clamp(min=-6.0) - 3)
+    q = torch.where(y.isfinite(), torch.round(y / step) * step, math.nan)
+    q = torch.where(y == 0, 0.0, q)
+    return q[:rows], e.int()
+
+
+def check_quant(q, scale, x, per):
+    import torch
+    ref, e = plain_quant(x, per)
+    assert q.shape == ref.shape
+    got = q.view(torch.float8_e4m3fn).double()
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got.nan_to_num(nan=0.0), ref.nan_to_num(nan=0.0))
+    b = scale.view(torch.uint8).transpose(0, 1).flatten(1).int()
+    want = torch.zeros_like(b)
+    want[:, :e.shape[1]] = e + 127
+    assert torch.equal(b, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols,ld", [(1, 1, 1), (1, 128, 128), (3, 129, 129), (5, 511, 517), (4, 512, 520),
+                                          (33, 513, 513), (58, 2560, 2560), (300, 130, 131), (2000, 2693, 2701),
+                                          (1700, 2560, 7680)])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_quant(ctx, dtype, rows, cols, ld, blocks):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    x = torch.randn((rows, ld), generator=g, device="cuda")
+    x = (x * torch.exp2(torch.randint(-20, 20, (rows, 1), generator=g, device="cuda").float())).to(dt(dtype))
+    x = x[:, ld - cols:]  # begins at any element
+    q, s = ctx.quant_fp8(x, blocks=blocks)
+    check_quant(q, s, x, 128 if blocks else 1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_quant_special_values(ctx, dtype, blocks):
+    """Zeros, values of 448 2^e and just over, ties, the ends of the type's range, subnormals, infinities, NaN."""
+    import torch
+    t = dt(dtype)
+    x = torch.zeros((256, 640), dtype=t, device="cuda")
+    x[1, :128] = torch.linspace(-448, 448, 128)
+    x[2, :128] = torch.linspace(-449, 449, 128)
+    x[2, 5] = 452.0  # over 448 in either type
+    x[3, :128] = (torch.arange(128) + 0.5) * 2.0 ** -9  # ties of e4m3's subnormals and small values
+    x[3, 0] = 448.0
+    x[4, :128] = torch.finfo(t).max
+    x[5, :128] = torch.finfo(t).tiny
+    x[6, :128] = torch.finfo(t).smallest_normal * 2.0 ** -7  # subnormal
+    x[6, 1] = 0.0
+    x[7, :256] = 1.0
+    x[7, 3], x[7, 130] = math.inf, -math.inf
+    x[8, 128:256] = 3.0
+    x[8, 131] = math.nan
+    x[9, :128] = math.nan
+    x[10, :128] = math.inf
+    x[130:, 512:] = 2.0 ** -100
+    x[200, 513] = -(2.0 ** -90)
+    q, s = ctx.quant_fp8(x, blocks=blocks)
+    check_quant(q, s, x, 128 if blocks else 1)
+
+
+def test_quant_leaves_what_is_not_its_own(ctx, awa):
+    """Rows and words past the last one, at a wider scale stride."""
+    import torch
+    x = torch.randn((5, 700), device="cuda")
+    q = torch.full((7, 768), 99, dtype=torch.uint8, device="cuda")
+    s = torch.full((3, 9), 77, dtype=torch.int32, device="cuda")
+    ctx.check(awa.lib().dit_quant_fp8(ctx.ptr, awa.AWA_F32, x.data_ptr(), 700, 5, 700, 1, q.data_ptr(), s.data_ptr(), 9,
+                                      torch.cuda.current_stream().cuda_stream), "dit_quant_fp8")
+    check_quant(q[:5], s[:2, :5].contiguous().view(torch.uint8).reshape(2, 5, 4), x, 1)
+    assert bool((q[5:] == 99).all()) and bool((s[2] == 77).all()) and bool((s[:, 5:] == 77).all())
+    assert ctx.quant_fp8(x[:0])[0].shape == (0, 768)
+
+
+# ------------------------------------------------------------------ the product
+
+def fp8_matrix(awa, ctx, rows, k, blocks, g, spread=0):
+    """Rows quantised by the plain form above: (q, scale, values in fp64)."""
+    import torch
+    x = torch.randn((rows, k), generator=g, device="cuda")
+    if spread:
+        x = x * torch.exp2(torch.randint(-spread, spread, (rows, k // 128), generator=g, device="cuda")
+                           .float()).repeat_interleave(128, 1)
+    per = 128 if blocks else 1
+    ref, e = plain_quant(x, per)
+    b = torch.zeros((e.shape[0], -(-k // 512) * 4), dtype=torch.uint8, device="cuda")
+    b[:, :e.shape[1]] = (e + 127).to(torch.uint8)
+    s = b.reshape(e.shape[0], -1, 4).transpose(0, 1).contiguous().view(torch.float8_e8m0fnu)
+    v = ref * torch.exp2(e.double()).repeat_interleave(per, 0)[:rows].repeat_interleave(128, 1)
+    return ref.float().to(torch.float8_e4m3fn), s, v
+
+
+def gemm_bar(va, vw, ref, dtype, k):
+    return (4 * k / 128 + 16) * 2.0 ** -24 * (va.abs() @ vw.abs().T) + half_step(dtype) * ref.abs()
+
+
+SIZES = [(1, 1, 128), (1, 7680, 2560), (2, 130, 640), (15, 257, 384), (16, 16, 512), (17, 2560, 1664), (31, 100, 128),
+         (33, 129, 512), (58, 7680, 2560), (64, 256, 6912), (65, 384, 1024), (127, 511, 256), (129, 1000, 640),
+         (257, 513, 896), (300, 2560, 512), (679, 2560, 6912), (1000, 1536, 2560), (1237, 1999, 2816),
+         (2100, 5120, 384), (4440, 2560, 256)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gemm(awa, ctx, m, n, k, dtype):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    a, sa, va = fp8_matrix(awa, ctx, m, k, False, g, spread=6)
+    w, sw, vw = fp8_matrix(awa, ctx, n, k, True, g, spread=3)
+    bias = torch.randn(n, generator=g, device="cuda") * 100
+    ref = va @ vw.T
+    # rows inside a wider buffer whose other values stay: an odd stride when n is odd
+    buf = torch.full((m + 2, n + (n & 1) * 2 + 8), 7.0, dtype=dt(dtype), device="cuda")
+    out = buf[1:-1, :n]
+    ctx.gemm_fp8(a, sa, w, sw, out=out)
+    bar = gemm_bar(va, vw, ref, dt(dtype), k)
+    within(out, ref, bar)
+    assert bool((buf[0] == 7).all()) and bool((buf[-1] == 7).all()) and bool((buf[:, n:] == 7).all())
+    again = ctx.gemm_fp8(a, sa, w, sw, dtype=dt(dtype))
+    assert torch.equal(again, out)  # the same sums, whatever the output's strides
+    ref = ref + bias.double()
+    within(ctx.gemm_fp8(a, sa, w, sw, bias=bias, dtype=dt(dtype)), ref,
+           bar + (2.0 ** -24 + half_step(dt(dtype))) * (ref.abs() + bias.abs()))
+
+
+def test_gemm_misaligned_output(awa, ctx):
+    """An output that begins at an odd element: no 16-byte stores."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a, sa, va = fp8_matrix(awa, ctx, 300, 512, False, g)
+    w, sw, vw = fp8_matrix(awa, ctx, 520, 512, True, g)
+    for t in (BF16, F32):
+        buf = torch.full((300 * 520 + 2,), 7.0, dtype=dt(t), device="cuda")
+        out = buf[1:-1].view(300, 520)
+        ctx.gemm_fp8(a, sa, w, sw, out=out)
+        ref = va @ vw.T
+        within(out, ref, gemm_bar(va, vw, ref, dt(t), 512))
+        assert float(buf[0]) == 7 and float(buf[-1]) == 7
+
+
+@pytest.mark.parametrize("m", [3, 40, 200, 700])
+def test_gemm_rows_apart(awa, ctx, m):
+    """A row with NaN, a row of zeros and one with scales at the ends of their range stay their own."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m)
+    a, sa, va = fp8_matrix(awa, ctx, m, 1024, False, g)
+    w, sw, vw = fp8_matrix(awa, ctx, 300, 1024, True, g)
+    a[0, 700] = math.nan
+    a[1] = 0
+    va[0], va[1] = math.nan, 0
+    sa.view(torch.uint8)[:, 1] = 0
+    sa.view(torch.uint8)[1, 2] = 0  # blocks 4 .. 7 of row 2: 2^-127, nothing beside the others
+    va[2, 512:] = a[2, 512:].double() * 2.0 ** -127
+    ref = va @ vw.T
+    out = ctx.gemm_fp8(a, sa, w, sw, dtype=torch.float32)
+    within(out, ref, gemm_bar(va.nan_to_num(nan=0.0), vw, ref.nan_to_num(nan=0.0), torch.float32, 1024))
+    assert bool((out[1] == 0).all()) and bool(out[0].isnan().all())
+
+
+def test_gemm_slices(awa, ctx):
+    """Rows cut from a larger quantised matrix (the scale stride of the whole), through the C entry."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+    a, sa, va = fp8_matrix(awa, ctx, 100, 640, False, g)
+    w, sw, vw = fp8_matrix(awa, ctx, 600, 640, True, g)
+    out = torch.empty((31, 300), device="cuda")
+    ctx.check(awa.lib().dit_gemm_fp8(ctx.ptr, a[13:].data_ptr(), sa.data_ptr() + 13 * 4, 100, w[256:].data_ptr(),
+                                     sw.data_ptr() + 2 * 4, 5, None, awa.AWA_F32, out.data_ptr(), 300, 31, 300, 640,
+                                     torch.cuda.current_stream().cuda_stream), "dit_gemm_fp8")
+    ref = va[13:44] @ vw[256:556].T
+    within(out, ref, gemm_bar(va[13:44], vw[256:556], ref, torch.float32, 640))
+    assert ctx.gemm_fp8(a[:0], sa[:, :0].contiguous(), w, sw).shape == (0, 600)
+
+
+# ------------------------------------------------------------------ rotary positions
+
+def plain_rope(x, pos, freqs, pairs, layout, scale, inverse):
+    """(the rotation in fp64, its bar without the type's half step)."""
+    import torch
+    y, bar = x.double().clone(), torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    p = sum(pairs)
+    axis = torch.tensor([i for i, n in enumerate(pairs) for _ in range(n)], dtype=torch.long, device=x.device)
+    f = torch.as_tensor(np.asarray(freqs), device=x.device)
+    ang = pos.reshape(pos.shape[0], -1)[:, axis].double() * f
+    c, s = scale * ang.cos()[:, None], scale * ang.sin()[:, None] * (-1 if inverse else 1)
+    i = torch.arange(p, device=x.device)
+    first, second = (i, i + p) if layout == "half" else (2 * i, 2 * i + 1)
+    a, b = x[..., first].double(), x[..., second].double()
+    y[..., first], y[..., second] = a * c - b * s, a * s + b * c
+    e = (a.abs() + b.abs()) * abs(scale) * (2.0 ** -21 + ang.abs()[:, None] * 2.0 ** -51)
+    bar[..., first], bar[..., second] = e, e
+    return y, bar
+
+
+ROPES = [  # tokens, heads, head_d, pairs per axis, layout, extra elements between tokens
+    (1, 40, 128, (21, 21, 21), "interleaved", 0), (1, 1, 2, (1,), "half", 0), (7, 3, 64, (32,), "half", 0),
+    (300, 40, 128, (21, 21, 21), "interleaved", 2560), (65, 5, 96, (32,), "half", 3), (65, 5, 96, (32,), "interleaved", 3),
+    (129, 1, 256, (64, 64), "half", 256), (33, 2, 77, (11, 7), "half", 0), (33, 2, 77, (11, 7), "interleaved", 0),
+    (50, 9, 80, (40,), "interleaved", 16), (50, 9, 80, (20,), "half", 16), (11, 4, 128, (16, 0, 8, 24), "half", 8),
+    (3000, 2, 64, (16,), "interleaved", 0), (5, 70, 8, (4,), "half", 0), (9, 2, 32, (0,), "half", 0),
+]
+
+
+@pytest.mark.parametrize("tokens,heads,head_d,pairs,layout,extra", ROPES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rope(awa, ctx, tokens, heads, head_d, pairs, layout, extra, dtype):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(tokens * heads + head_d)
+    buf = torch.randn((tokens, heads * head_d + extra), generator=g, device="cuda").to(dt(dtype))
+    x = buf[:, :heads * head_d].unflatten(1, (heads, head_d))
+    pos = torch.randint(-100, 5000, (tokens, len(pairs)), generator=g, device="cuda", dtype=torch.int32)
+    freqs = np.concatenate([awa.rope_freqs(n) for n in pairs if n] or [np.zeros(0)])
+    args = dict(pairs=pairs, layout=layout)
+    for scale, inverse in ((1.0, False), (1.25, True)):
+        ref, bar = plain_rope(x, pos, freqs, pairs, layout, scale, inverse)
+        out = ctx.rope(x, pos, freqs, scale=scale, inverse=inverse, **args)
+        within(out, ref, bar + half_step(dt(dtype)) * ref.abs())
+        turned = torch.zeros(head_d, dtype=torch.bool)
+        turned[:2 * sum(pairs)] = True
+        assert torch.equal(out[..., ~turned], x[..., ~turned])
+    # in place, inside the buffer, whose other values stay
+    rest = buf[:, heads * head_d:].clone()
+    out = ctx.rope(x, pos, freqs, **args)
+    assert ctx.rope(x, pos, freqs, out=x, **args) is x
+    assert torch.equal(x, out) and torch.equal(buf[:, heads * head_d:], rest)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_far_positions(awa, ctx, layout):
+    import torch
+    pos = torch.tensor([0, 1, 2 ** 20 + 1, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31, -12345679], dtype=torch.int32, device="cuda")
+    freqs = awa.rope_freqs(32, kind="bands", factor=8.0, trained=4096.0)
+    x = torch.randn((7, 3, 64), device="cuda")
+    ref, bar = plain_rope(x, pos, freqs, (32,), layout, 1.0, False)
+    within(ctx.rope(x, pos, freqs, layout=layout), ref, bar + 2.0 ** -24 * ref.abs())
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_quarter_turns(awa, ctx, layout):
+    """Angles at and around the borders of the reduction: multiples of a sixteenth turn."""
+    import torch
+    pos = torch.arange(-40, 41, dtype=torch.int32, device="cuda")
+    freqs = np.array([2 * np.pi / 16, 2 * np.pi / 16 * (1 + 2.0 ** -40), 0.0, 2 * np.pi])
+    x = torch.randn((81, 2, 8), device="cuda")
+    ref, bar = plain_rope(x, pos, freqs, (4,), layout, 1.0, False)
+    within(ctx.rope(x, pos, freqs, layout=layout), ref, bar + 2.0 ** -24 * ref.abs())
+
+
+def test_rope_not_finite_stays_in_its_pair(awa, ctx):
+    import torch
+    for t in (BF16, F32):
+        for layout, other in (("interleaved", 5), ("half", 36)):
+            x = torch.randn((2, 1, 72), device="cuda").to(dt(t))
+            x[0, 0, 4], x[1, 0, 70] = math.nan, math.inf
+            out = ctx.rope(x, torch.tensor([3, 4], dtype=torch.int32, device="cuda"), awa.rope_freqs(32), layout=layout)
+            bad = ~out.isfinite().cpu()
+            want = torch.zeros((2, 72), dtype=torch.bool)
+            want[0, 4] = want[0, other] = want[1, 70] = True
+            assert torch.equal(bad[:, 0], want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rope_queries_and_keys(awa, ctx, dtype):
+    """Both tensors of a call, in place inside qkv rows: the same bits as one by one; v stays."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tok, hq, hk, d = 37, 12, 3, 64
+    buf = torch.randn((tok, (hq + 2 * hk) * d), generator=g, device="cuda").to(dt(dtype))
+    was = buf.clone()
+    q, k = buf[:, :hq * d].unflatten(1, (hq, d)), buf[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d))
+    pos = torch.arange(tok, dtype=torch.int32, device="cuda")
+    f = awa.rope_freqs(32)
+    wq, wk = ctx.rope(q, pos, f, layout="half"), ctx.rope(k, pos, f, layout="half")
+    oq, ok = ctx.rope((q, k), pos, f, layout="half")
+    assert torch.equal(oq, wq) and torch.equal(ok, wk)
+    ctx.rope((q, k), pos, f, layout="half", out=(q, k))
+    assert torch.equal(q, wq) and torch.equal(k, wk) and torch.equal(buf[:, (hq + hk) * d:], was[:, (hq + hk) * d:])
+    # heads outside tokens, into such memory
+    out = torch.empty((hq, tok, d), dtype=dt(dtype), device="cuda").transpose(0, 1)
+    ctx.rope(was[:, :hq * d].unflatten(1, (hq, d)), pos, f, layout="half", out=out)
+    assert torch.equal(out, wq)
+    with pytest.raises(awa.AwaError):
+        ctx.rope((q, q), pos, f, layout="half", out=(q, q))
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_gradient(awa, ctx, layout):
+    """inverse=True takes gradients back: <g, R x> = <R' g, x>, against differences of the forward pass too."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((6, 2, 20), generator=gen, device="cuda")
+    g = torch.randn((6, 2, 20), generator=gen, device="cuda")
+    pos = torch.arange(6, dtype=torch.int32, device="cuda") * 7
+    f = awa.rope_freqs(8)
+    args = dict(layout=layout, scale=1.3)
+    grad = ctx.rope(g, pos, f, inverse=True, **args)
+    ref, bar = plain_rope(g, pos, f, (8,), layout, 1.3, True)
+    within(grad, ref, bar + 2.0 ** -24 * ref.abs())
+    # the map is linear, so a difference of any step is the derivative: each of the two passes is off by its
+    # bar of at most 4 (|a| + |b| with |x| < 4 and scale 1.3, times 2^-21 and a half step), over 2 h = 2
+    for i in (0, 3, 9, 17):
+        e = torch.zeros_like(x)
+        e[..., i] = 1.0
+        up, down = ctx.rope(x + e, pos, f, **args).double(), ctx.rope(x - e, pos, f, **args).double()
+        d = ((up - down) / 2 * g.double()).sum(-1)
+        assert float((d - grad[..., i].double()).abs().max()) <= 20 * 4 * 13 * 2.0 ** -21
+
+
+# ------------------------------------------------------------------ together
+
+def layer(ctx, x, w, bias, pos, freqs, stream=None):
+    """Rows in 8 bits, the qkv projection, queries and keys rotated in place."""
+    q, s = ctx.quant_fp8(x, stream=stream)
+    qkv = ctx.gemm_fp8(q, s, *w, bias=bias, stream=stream)
+    h = qkv[:, :2 * 512].unflatten(1, (8, 128))
+    ctx.rope(h, pos, freqs, pairs=(21, 21, 21), out=h, stream=stream)
+    return qkv
+
+
+def layer_inputs(awa, ctx, m, seed):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((m, 700), generator=g, device="cuda").bfloat16()
+    wt = torch.randn((3 * 512, 700), generator=g, device="cuda") * 0.02
+    bias = torch.randn(3 * 512, generator=g, device="cuda")
+    pos = torch.randint(0, 99, (m, 3), generator=g, device="cuda", dtype=torch.int32)
+    return x, wt, bias, pos, np.tile(awa.rope_freqs(21), 3)
+
+
+@pytest.mark.parametrize("m", [1, 58, 700])
+def test_projection_and_rotation(awa, ctx, m):
+    import torch
+    x, wt, bias, pos, freqs = layer_inputs(awa, ctx, m, m)
+    w = ctx.quant_fp8(wt, blocks=True)
+    out = layer(ctx, x, w, bias, pos, freqs)
+    va, vw = [q * torch.exp2(e.double()).repeat_interleave(per, 0)[:q.shape[0]].repeat_interleave(128, 1)
+              for per, (q, e) in ((1, plain_quant(x, 1)), (128, plain_quant(wt, 128)))]
+    assert torch.equal(awa.fp8_values(*ctx.quant_fp8(x), cols=700).double(), va[:, :700])
+    assert torch.equal(awa.fp8_values(*w, cols=700).double(), vw[:, :700])
+    c = va @ vw.T + bias.double()
+    ce = gemm_bar(va, vw, c, torch.bfloat16, 768) + (2.0 ** -24 + 2.0 ** -8) * (c.abs() + bias.abs())
+    within(out[:, 1024:], c[:, 1024:], ce[:, 1024:])
+    y, bar = plain_rope(c[:, :1024].unflatten(1, (8, 128)), pos, freqs, (21, 21, 21), "interleaved", 1.0, False)
+    # a rotated channel is off by both channels' errors before it
+    e = ce[:, :1024].unflatten(1, (8, 64, 2)).sum(-1, keepdim=True).expand(-1, -1, -1, 2).flatten(2)
+    within(out[:, :1024].unflatten(1, (8, 128)), y, bar + e * 1.01 + 2.0 ** -8 * (y.abs() + e))
+
+
+def test_captured_and_replayed(awa, ctx):
+    """The run as a graph, replayed over changed inputs with eager work between; another context and stream at once."""
+    import torch
+    x, wt, bias, pos, freqs = layer_inputs(awa, ctx, 130, 9)
+    w = ctx.quant_fp8(wt, blocks=True)
+    want = layer(ctx, x, w, bias, pos, freqs).clone()
+    torch.cuda.synchronize()
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        out = layer(ctx, x, w, bias, pos, freqs)
+    x0 = x.clone()
+    for k in range(4):
+        x.copy_(x0.roll(k, 0) * (k + 1))
+        eager = layer(ctx, x, w, bias, pos, freqs)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+    x.copy_(x0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    other, side = awa.Context(0), [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [layer(c, x, w, bias, pos, freqs, stream=s) for _ in range(3) for c, s in ((ctx, side[0]), (other, side[1]))]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    other.close()
