@@ -4,7 +4,11 @@ Quantising is exact arithmetic up to one rounding that both sides make alike: by
 equality.  The product's inputs are its 8-bit values, so its reference has no rounding; an fp32 sum of
 products p_i is off by at most half a step (2^-24) of a partial sum per addition.  A partial sum is at most
 S = sum |p_i|; a block of 128 is four bf16 instructions, and the parts of a split K are added at the end (at
-most 16): bar (4 K / 128 + 16) 2^-24 S, and half a step of C's type.  Rotation: a sine or cosine is off by at most 2^-22
+most 16): bar (4 K / 128 + 16) 2^-24 S, and half a step of C's type.  For bf16 C the 8-bit instructions may sum:
+they align the products of eight consecutive columns to the exponent e of the largest of them and drop what lies
+below 2^(e - 13) (2^3 stays beside a product of 2^16, 2^2 does not), so each of the seven others loses less than
+2^-13 of the largest, which is at most the product of the two rows' largest magnitudes in those columns: 7 2^-13
+sum over the groups of those products in addition.  Rotation: a sine or cosine is off by at most 2^-22
 (rounding the reduced angle, its product with pi / 2, the polynomial, the factor: under 2^-24 each) and by the
 angle's own 2^-51 of itself in fp64; products and sum are fp32: bar (|a| + |b|) scale (2^-21 + |angle| 2^-51)
 and half a step of the type.
@@ -145,7 +149,11 @@ def fp8_matrix(awa, ctx, rows, k, blocks, g, spread=0):
 
 
 def gemm_bar(va, vw, ref, dtype, k):
-    return (4 * k / 128 + 16) * 2.0 ** -24 * (va.abs() @ vw.abs().T) + half_step(dtype) * ref.abs()
+    import torch
+    e = (4 * k / 128 + 16) * 2.0 ** -24 * (va.abs() @ vw.abs().T)
+    if dtype == torch.bfloat16:
+        e = e + 7 * 2.0 ** -13 * (va.abs().unflatten(1, (-1, 8)).amax(2) @ vw.abs().unflatten(1, (-1, 8)).amax(2).T)
+    return e + half_step(dtype) * (ref.abs() + e)
 
 
 SIZES = [(1, 1, 128), (1, 7680, 2560), (2, 130, 640), (15, 257, 384), (16, 16, 512), (17, 2560, 1664), (31, 100, 128),
