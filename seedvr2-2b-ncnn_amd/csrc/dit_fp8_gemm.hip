@@ -131,13 +131,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 // chunk ^ ((row >> 1) & 7), and each half block (64 columns, one instruction per
 // accumulator) runs with the next half's fragment reads and, in the half that
 // refills the freed stage, the DMA pieces between its instructions.  A row's scale
-// word travels with its stage (256 bytes per 64 rows beside 8 KiB of them); W's is
-// the same for a whole wave and comes by scalar loads.
+// word travels with its stage, and W's, which are the same for a whole wave.
 //
 // EXACT (fp32 C): the fragments are widened to bf16 with their scales and take four
 // 32x32x16 bf16 instructions in place of one 8-bit one.
 constexpr int ROW = 128;  // bytes of a block's row
-__device__ inline int swz(int row, int chunk) { return row * ROW + ((chunk ^ ((row >> 1) & 7)) << 4); }
 
 // A buffer resource with wave-uniform fields (as in dit_gemm.hip): loads past
 // `bytes` read zeros and stores past it are dropped.
@@ -153,76 +151,81 @@ template <int N>
 __device__ inline void wait_vmem_lds() {
     asm volatile("s_waitcnt vmcnt(%c0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
-// A word that no kernel writes while this one runs, at a wave-uniform address.
-__device__ inline uint32_t uniform_word(const uint32_t* p) {
-    return *(const __attribute__((address_space(4))) uint32_t*)reinterpret_cast<uint64_t>(p);
-}
 
 // Lane (c = lane % 32, g = lane / 32) of accumulator (i, j): row 32 j + c, features
-// 32 i + 8 t + 4 g + e in register 4 t + e.  Through LDS, so that global memory sees
-// whole rows: chunk k of staged row r at k ^ (r's low bits).
-template <bool F32, int NI, int MJ>
-__device__ inline void epilogue(const Fp8Gemm& p, f32x16 (&acc)[NI][MJ], int n_base, int m_base, int lane, uint8_t* stg) {
-    constexpr int SZ = F32 ? 4 : 2, NC = 2 * NI * SZ, RPI = 64 / NC;  // 16-byte chunks per row, rows per read
-    constexpr int EPC = 16 / SZ;                                     // elements per chunk
-    auto swc = [](int r, int k) __attribute__((always_inline)) {
-        return k ^ (NC >= 16 ? r & (NC - 1) : NC == 8 ? (r >> 1) & 7 : (r >> 2) & 3);
+// 32 i + 8 t + 4 g + e in register 4 t + e.  Pieces of 32 rows go through the wave's
+// 4 KiB of LDS so that global memory sees 128 bytes of a row at once (chunk k of
+// staged row r at k ^ (r's low bits)).
+constexpr int STG = 4096;
+template <bool F32, bool BIAS, int NI, int MJ>
+__device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], int n_base, int m_base, int lane, uint8_t* stg) {
+    constexpr int SZ = F32 ? 4 : 2, EPC = 16 / SZ;   // elements per 16-byte chunk
+    constexpr int FW = F32 || NI == 1 ? 1 : 2;       // accumulators side by side in a piece
+    constexpr int NC = 2 * FW * SZ, RPI = 64 / NC;   // chunks per staged row, rows per read
+    constexpr int STEPS = 32 / RPI;
+    auto at = [&](int r, int k) __attribute__((always_inline)) {
+        return stg + r * (16 * NC) + ((k ^ (NC == 8 ? (r >> 1) & 7 : (r >> 2) & 3)) << 4);
     };
     const int c = lane & 31, g = lane >> 5;
-    const __amdgpu_buffer_rsrc_t bres = uniform_rsrc(p.bias, p.bias ? p.N * 4 : 0);
-#pragma unroll
-    for (int i = 0; i < NI; i++)
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(bres, 4u * (n_base + 32 * i + 8 * t + 4 * g), 0, 0);
-#pragma unroll
-            for (int j = 0; j < MJ; j++) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[i][j][4 * t + e] + __uint_as_float(b[e]);
-                const int r = 32 * j + c;
-                if constexpr (F32) {
-                    *reinterpret_cast<float4*>(stg + r * (16 * NC) + (swc(r, 8 * i + 2 * t + g) << 4)) =
-                        make_float4(v[0], v[1], v[2], v[3]);
-                } else {
-                    *reinterpret_cast<uint2*>(stg + r * (16 * NC) + (swc(r, 4 * i + t) << 4) + 8 * g) =
-                        make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
-                }
-            }
-        }
-    const int k = lane % NC, r0 = lane / NC, n = n_base + k * EPC;
+    const int k = lane % NC, r0 = lane / NC;
+    const bool vec = p.c_vec && p.N % EPC == 0;
+    // a resource that ends at row M
     const int rows = min(max(p.M - m_base, 0), 32 * MJ);
+    const uint32_t row_bytes = (uint32_t)p.ldc * SZ;
     uint8_t* crow = reinterpret_cast<uint8_t*>(p.C) + (int64_t)m_base * p.ldc * SZ;
-    constexpr int STEPS = 32 * MJ / RPI, AT = STEPS < 8 ? STEPS : 8;  // rows per lane, rows in flight
-    if (p.c_vec && p.N % EPC == 0) {
-        // a resource that ends at row M, and an offset past it for chunks past N
-        const __amdgpu_buffer_rsrc_t cres = uniform_rsrc(crow, (uint32_t)rows * (uint32_t)p.ldc * SZ);
-        const uint32_t step = (uint32_t)(RPI * p.ldc * SZ);
-        const uint32_t ofs0 = n < p.N ? (uint32_t)((r0 * p.ldc + n) * SZ) : 0x80000000u;
+    const __amdgpu_buffer_rsrc_t cres = uniform_rsrc(crow, (uint32_t)rows * row_bytes);
 #pragma unroll
-        for (int s = 0; s < STEPS; s += AT) {
-            u32x4 v[AT];
+    for (int i0 = 0; i0 < NI; i0 += FW) {
+        f32x4 b[FW][4];
+        if constexpr (BIAS) {
+            const __amdgpu_buffer_rsrc_t bres = uniform_rsrc(p.bias, p.N * 4);
 #pragma unroll
-            for (int u = 0; u < AT; u++) {
-                const int r = RPI * (s + u) + r0;
-                v[u] = *reinterpret_cast<const u32x4*>(stg + r * (16 * NC) + (swc(r, k) << 4));
-            }
+            for (int f = 0; f < FW; f++)
 #pragma unroll
-            for (int u = 0; u < AT; u++) __builtin_amdgcn_raw_buffer_store_b128(v[u], cres, ofs0 + (s + u) * step, 0, 0);
+                for (int t = 0; t < 4; t++)
+                    b[f][t] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                            bres, 4u * (n_base + 32 * (i0 + f) + 8 * t + 4 * g), 0, 0));
         }
-    } else {
-        typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
-        for (int s = 0; s < STEPS; s++) {
-            const int r = RPI * s + r0;
-            if (r >= rows || n >= p.N) continue;
-            const uint8_t* at = stg + r * (16 * NC) + (swc(r, k) << 4);
-            uint8_t* to = crow + (r * p.ldc + n) * SZ;
-            if (n + EPC <= p.N) {
-                *reinterpret_cast<u32x4_u*>(to) = *reinterpret_cast<const u32x4*>(at);
+        const int n = n_base + 32 * i0 + k * EPC;
+        // an offset past the resource for chunks past N
+        const uint32_t ofs0 = n < p.N ? r0 * row_bytes + n * SZ : 0x80000000u;
+#pragma unroll
+        for (int j = 0; j < MJ; j++) {
+#pragma unroll
+            for (int f = 0; f < FW; f++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const f32x16& x = acc[i0 + f][j];
+                    f32x4 v = {x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                    if constexpr (BIAS) v += b[f][t];
+                    if constexpr (F32) {
+                        *reinterpret_cast<f32x4*>(at(c, 2 * t + g)) = v;
+                    } else {
+                        *reinterpret_cast<uint2*>(at(c, 4 * f + t) + 8 * g) =
+                            make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
+                    }
+                }
+            if (vec) {
+                u32x4 v[STEPS];
+#pragma unroll
+                for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+#pragma unroll
+                for (int u = 0; u < STEPS; u++)
+                    __builtin_amdgcn_raw_buffer_store_b128(v[u], cres, ofs0 + (32 * j + RPI * u) * row_bytes, 0, 0);
             } else {
-                for (int e = 0; e < p.N - n; e++) {
-                    if constexpr (F32) reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(at)[e];
-                    else reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(at)[e];
+                // rows at any alignment: whole chunks as they are, the last one of a row in elements
+                typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll 1
+                for (int r = r0; r < min(rows - 32 * j, 32); r += RPI) {
+                    uint8_t* to = crow + ((32 * j + r) * p.ldc + n) * SZ;
+                    const uint8_t* from = at(r, k);
+                    if (n + EPC <= p.N) {
+                        *reinterpret_cast<u32x4_u*>(to) = *reinterpret_cast<const u32x4*>(from);
+                    } else {
+#pragma unroll 1
+                        for (int e = 0; e < (p.N - n) * (SZ / 2); e++)
+                            reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+                    }
                 }
             }
         }
@@ -232,30 +235,37 @@ __device__ inline void epilogue(const Fp8Gemm& p, f32x16 (&acc)[NI][MJ], int n_b
 template <bool EXACT, int NI, int MJ, int NS>
 __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     constexpr int BN = 64 * NI, BM = 64 * MJ;
-    constexpr int SCALES = (BN + BM) * ROW, STAGE = SCALES + BM * 4;
-    constexpr int STG = 32 * MJ * 32 * NI * (EXACT ? 4 : 2);  // the epilogue's staging area, per wave
-    constexpr int LDS = NS * STAGE > 4 * STG ? NS * STAGE : 4 * STG;
-    __shared__ __align__(16) uint8_t lds[LDS];
+    constexpr int SCALES = (BN + BM) * ROW, STAGE = SCALES + 2048;  // words of A's rows, then W's
+    // two-stage forms walk several tiles: the next tile's first stages land during this
+    // one's epilogue, which therefore has LDS of its own
+    constexpr bool WALK = NS == 2;
+    __shared__ __align__(16) uint8_t lds[NS * STAGE + (WALK ? 4 * STG : 0)];
     const int total = p.n_tiles * p.m_tiles;
-    const int lid = xcd_remap(total);
-    if (lid >= total) return;
-    // four m-tiles per group, n advancing across the group
-    constexpr int GM = 4;
-    const int group = lid / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
-    const int in_group = lid % (GM * p.n_tiles);
-    const int m0 = (first_m + in_group % gm) * BM, n0 = in_group / gm * BN;
+    // tiles lid, lid + stride, .. of the XCD's contiguous range up to `end`
+    const int per = (total + 7) >> 3, stride = gridDim.x >> 3;
+    const int end = min(((int)blockIdx.x & 7) * per + per, total);
+    int tile = ((int)blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (tile >= end) return;
+    auto place = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
+        // four m-tiles per group, n advancing across the group
+        constexpr int GM = 4;
+        const int group = t / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
+        const int in_group = t - group * (GM * p.n_tiles);
+        m0 = (first_m + in_group % gm) * BM;
+        n0 = in_group / gm * BN;
+    };
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int wn = wave >> 1, wm = wave & 1;
     const int c = lane & 31, g = lane >> 5;
+    const int nk = p.K >> 7;
+    int nk_wrap = nk;
+    asm("" : "+s"(nk_wrap));  // so that no last stage is peeled off the loop for its one comparison
 
     // DMA: one instruction of a wave fills 8 rows; lane l lands in row l / 8, chunk
     // l % 8, so it fetches the chunk that the swizzle maps there.  Rows past N or M
     // lie past their resource and read zeros.
     const int lrow = lane >> 3;
-    const int wrows = min(BN, p.N - n0), arows = min(BM, p.M - m0);
-    const __amdgpu_buffer_rsrc_t wres = uniform_rsrc(p.W + (int64_t)n0 * p.K, (uint32_t)wrows * p.K);
-    const __amdgpu_buffer_rsrc_t ares = uniform_rsrc(p.A + (int64_t)m0 * p.K, (uint32_t)arows * p.K);
     int woff[2 * NI], aoff[2 * MJ];
 #pragma unroll
     for (int i = 0; i < 2 * NI; i++) {
@@ -268,63 +278,83 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         aoff[i] = row * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
     }
     constexpr int NP = 2 * NI + 2 * MJ + 1;  // DMA instructions of a wave per stage
-    const int srow = (wave % MJ) * 64;       // the wave's 64 scale words (waves past MJ repeat the first ones')
-    auto load_piece = [&](int kt, int slot, int x) __attribute__((always_inline)) {
+    // the last of them: waves 0 and 2 A's words, 1 and 3 W's (alike, so that every wave waits for one count)
+    const bool w_words = wave & 1;
+    const int64_t words_ld = w_words ? p.ld_ws : p.ld_as;
+    // the stage fetched next: block f_kt of tile f_tile; past the last tile empty
+    // resources, whose loads write zeros without memory traffic
+    int f_tile = tile, f_kt = 0;
+    __amdgpu_buffer_rsrc_t wres, ares;
+    const uint32_t* words;
+    uint32_t words_bytes;
+    auto fetch_from = [&](int t) __attribute__((always_inline)) {
+        int m0 = 0, n0 = 0, wrows = 0, arows = 0;
+        if (t < end) {
+            place(t, m0, n0);
+            wrows = min(BN, p.N - n0);
+            arows = min(BM, p.M - m0);
+        }
+        wres = uniform_rsrc(p.W + (int64_t)n0 * p.K, (uint32_t)wrows * p.K);
+        ares = uniform_rsrc(p.A + (int64_t)m0 * p.K, (uint32_t)arows * p.K);
+        words = w_words ? p.ws + (n0 >> 7) : p.as + m0;
+        words_bytes = 4u * (w_words ? (wrows + 127) >> 7 : arows);
+    };
+    auto fetch_next = [&]() __attribute__((always_inline)) {
+        if (++f_kt == nk) {
+            f_kt = 0;
+            f_tile += stride;
+            fetch_from(WALK ? f_tile : end);
+        }
+    };
+    auto load_piece = [&](int slot, int x) __attribute__((always_inline)) {
         uint8_t* st = lds + slot * STAGE;
         if (x == NP - 1) {
-            const uint32_t* words = p.as + (int64_t)(kt >> 2) * p.ld_as + m0;
-            const __amdgpu_buffer_rsrc_t sres = uniform_rsrc(words, (uint32_t)arows * 4);
-            uint8_t* dst = st + SCALES + srow * 4;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 4, (srow + lane) * 4, 0, 0, 0);
+            const __amdgpu_buffer_rsrc_t sres = uniform_rsrc(words + (int64_t)(f_kt >> 2) * words_ld, words_bytes);
+            uint8_t* dst = st + SCALES + 1024 * w_words;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 16, 16 * lane, 0, 0, 0);
             return;
         }
         const bool is_a = x >= 2 * NI;
         const int i = is_a ? x - 2 * NI : x;
         uint8_t* dst = st + (is_a ? BN * ROW + (wave * 2 * MJ + i) * 1024 : (wave * 2 * NI + i) * 1024);
         const int ofs = is_a ? aoff[i < 2 * MJ ? i : 0] : woff[i];
-        if (is_a) __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lptr_t)dst, 16, ofs, kt * ROW, 0, 0);
-        else __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (lptr_t)dst, 16, ofs, kt * ROW, 0, 0);
+        if (is_a) __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
     };
 
     f32x16 acc[NI][MJ];
-    const int nk = p.K >> 7, last = nk - 1;
-    int wrow[NI], arow[MJ];
-#pragma unroll
-    for (int i = 0; i < NI; i++) wrow[i] = wn * 32 * NI + 32 * i + c;
-#pragma unroll
-    for (int j = 0; j < MJ; j++) arow[j] = wm * 32 * MJ + 32 * j + c;
+    // fragment rows: blocks of 32 rows are 4 KiB apart and have the same swizzle
+    const int wrow = (wn * 32 * NI + c) * ROW, arow = BN * ROW + (wm * 32 * MJ + c) * ROW, sx = (c >> 1) & 7;
     i32x8 wf[2][NI], af[2][MJ];
     int sw, sa[MJ], sw_next = 0, sa_next[MJ];
-    const int nb = min(n0 + wn * 32 * NI, p.N - 1) >> 7;
     // piece x of the fragments of half s of a stage (into buffer buf): two chunks of a row each
     auto read_piece = [&](int slot, int s, int buf, int x) __attribute__((always_inline)) {
-        const uint8_t* ws = lds + slot * STAGE;
-        const uint8_t* as = ws + BN * ROW;
-        const int f = x >> 1, h = x & 1, ch = 4 * s + 2 * g + h;
-        const i32x4 v = *reinterpret_cast<const i32x4*>(f < NI ? ws + swz(wrow[f < NI ? f : 0], ch)
-                                                              : as + swz(arow[f < NI ? 0 : f - NI], ch));
+        const int f = x >> 1, h = x & 1, at = ((4 * s + 2 * g + h) ^ sx) << 4;
+        const uint8_t* from = lds + slot * STAGE + at + (f < NI ? wrow + 32 * ROW * f : arow + 32 * ROW * (f - NI));
+        const i32x4 v = *reinterpret_cast<const i32x4*>(from);
         i32x8& d = f < NI ? wf[buf][f < NI ? f : 0] : af[buf][f < NI ? 0 : f - NI];
 #pragma unroll
         for (int e = 0; e < 4; e++) d[4 * h + e] = v[e];
     };
     constexpr int NR = 2 * (NI + MJ);
-    auto read_scales = [&](int kt, int slot) __attribute__((always_inline)) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(lds + slot * STAGE + SCALES);
+    auto read_scales = [&](int slot) __attribute__((always_inline)) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(lds + slot * STAGE + SCALES);
 #pragma unroll
-        for (int j = 0; j < MJ; j++) sa_next[j] = (int)words[arow[j]];
-        sw_next = (int)uniform_word(p.ws + (int64_t)(kt >> 2) * p.ld_ws + nb);
+        for (int j = 0; j < MJ; j++) sa_next[j] = (int)w[wm * 32 * MJ + 32 * j + c];
+        sw_next = (int)w[256 + ((wn * 32 * NI) >> 7)];
     };
     auto take_scales = [&](int kt) __attribute__((always_inline)) {  // byte kt % 4 of the words
         const int sh = 8 * (kt & 3);
-        sw = sw_next >> sh;
+        sw = __builtin_amdgcn_readfirstlane(sw_next) >> sh;
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa[j] = sa_next[j] >> sh;
     };
     // One half block on fragment buffer `buf`; between its instructions the reads of
     // the next half (slot rslot, half rs, into buffer buf ^ 1) and, when `dma`, the DMA
-    // pieces of stage dma_kt, all in the first half of them.
-    auto half = [&](int buf, int rslot, int rs, bool do_read, bool dma, int dma_kt, int dma_slot, bool zc)
-        __attribute__((always_inline)) {
+    // pieces of the next stage into slot dma_slot, spread evenly: an instruction of 64
+    // cycles hides one read and one piece, not two (5498 x 13824 x 2560 188 us with them
+    // in the first eight of sixteen, 175 so).
+    auto half = [&](int buf, int rslot, int rs, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
         bf16x8 wb[EXACT ? NI : 1][4], ab[EXACT ? MJ : 1][4];
         if constexpr (EXACT) {
             const float fw = scale_of(sw & 0xff);
@@ -339,7 +369,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
                 for (int e = 0; e < 4; e++) ab[j][e] = widen(af[buf][j][2 * e], af[buf][j][2 * e + 1], fa);
             }
         }
-        constexpr int T = NI * MJ, RS = (2 * NR + T - 1) / T, DS = (2 * NP + T - 1) / T;
+        constexpr int T = NI * MJ;
 #pragma unroll
         for (int x = 0; x < T; x++) {
             const int i = x / MJ, j = x % MJ;
@@ -357,59 +387,70 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < RS; e++)
-                if (do_read && x * RS + e < NR) read_piece(rslot, rs, buf ^ 1, x * RS + e);
+            for (int e = 0; e < NR; e++)
+                if (e * T / NR == x) read_piece(rslot, rs, buf ^ 1, e);
 #pragma unroll
-            for (int e = 0; e < DS; e++)
-                if (dma && x * DS + e < NP) load_piece(dma_kt, dma_slot, x * DS + e);
+            for (int e = 0; e < NP; e++)
+                if (dma && e * T / NP == x) load_piece(dma_slot, e);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    // While stage kt is computed from slot kt % NS, stages kt + 1 .. kt + NS - 1 land
-    // in the others.  Half 0 of stage kt reads half 1's fragments from the same slot;
-    // then every wave waits for its own DMA of stage kt + 1 and for its LDS reads, and
-    // the barrier makes stage kt + 1 visible and slot kt % NS free: half 1 reads stage
-    // kt + 1's first fragments and refills slot kt % NS with stage kt + NS (past the
-    // last stage it repeats the last one, so that the count waited for stays fixed).
+    // A stream of stages, tile after tile: while one is computed from slot `slot`, the
+    // NS - 1 after it land in the others.  Half 0 reads half 1's fragments from the same
+    // slot; then every wave waits for its own DMA of the next stage and for its LDS
+    // reads, and the barrier makes that stage visible and this slot free: half 1 reads
+    // the next stage's first fragments and refills this slot with the stage NS on.
+    int slot = 0;
+    auto next = [](int t) __attribute__((always_inline)) { return t + 1 == NS ? 0 : t + 1; };
+    auto stage = [&](int kt, bool zc) __attribute__((always_inline)) {
+        half(0, slot, 1, false, 0, zc);
+        wait_vmem_lds<(NS - 2) * NP>();
+        __builtin_amdgcn_s_barrier();
+        read_scales(next(slot));
+        half(1, next(slot), 0, true, slot, false);
+        // the sums stay here: the compiler would move the instructions that no one reads
+        // yet past the branch below, behind all the loads between them
 #pragma unroll
-    for (int i = 0; i < NS; i++)
+        for (int x = 0; x < NI * MJ; x++) asm volatile("" : "+a"(acc[x / MJ][x % MJ]));
+        fetch_next();
+        take_scales(kt + 1 == nk_wrap ? 0 : kt + 1);
+        slot = next(slot);
+    };
+    fetch_from(tile);
 #pragma unroll
-        for (int x = 0; x < NP; x++) load_piece(min(i, last), i, x);
+    for (int i = 0; i < NS; i++) {
+#pragma unroll
+        for (int x = 0; x < NP; x++) load_piece(i, x);
+        fetch_next();
+    }
     wait_vmem_lds<(NS - 1) * NP>();
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int x = 0; x < NR; x++) read_piece(0, 0, 0, x);
-    read_scales(0, 0);
+    read_scales(0);
     take_scales(0);
-    int slot = 0;
-    auto next = [](int t) __attribute__((always_inline)) { return t + 1 == NS ? 0 : t + 1; };
-    if (last == 0) {
-        half(0, 0, 1, true, false, 0, 0, true);
-        half(1, 0, 0, false, false, 0, 0, false);
-    } else {
-        half(0, 0, 1, true, false, 0, 0, true);
-        wait_vmem_lds<(NS - 2) * NP>();
-        __builtin_amdgcn_s_barrier();
-        read_scales(1, 1);
-        half(1, 1, 0, true, true, min(NS, last), 0, false);
-        take_scales(1);
-        slot = 1;
-        for (int kt = 1; kt < last; kt++) {
-            half(0, slot, 1, true, false, 0, 0, false);
-            wait_vmem_lds<(NS - 2) * NP>();
+    while (true) {
+        stage(0, true);
+        for (int kt = 1; kt < nk; kt++) stage(kt, false);
+        int m0, n0;
+        place(tile, m0, n0);
+        if constexpr (!WALK) {  // the slots are free once every DMA (of nothing, by now) and read is done
+            wait_vmem_lds<0>();
             __builtin_amdgcn_s_barrier();
-            read_scales(kt + 1, next(slot));
-            half(1, next(slot), 0, true, true, min(kt + NS, last), slot, false);
-            take_scales(kt + 1);
-            slot = next(slot);
         }
-        half(0, slot, 1, true, false, 0, 0, false);
-        half(1, slot, 0, false, false, 0, 0, false);
+        uint8_t* stg = lds + (WALK ? NS * STAGE : 0) + wave * STG;
+        // the lane anew, so that the epilogue's addresses are formed here: hoisted, they
+        // would cost the stages registers
+        int l = 0;
+        asm volatile("" : "+v"(l));
+        l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, l));
+        if (p.bias) epilogue<EXACT, true, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
+        else epilogue<EXACT, false, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
+        tile += stride;
+        if (!WALK || tile >= end) break;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last refills, which nobody reads
-    __syncthreads();  // every wave is done with the operands: LDS becomes the staging area
-    epilogue<EXACT, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, lane, lds + wave * STG);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives its LDS
 }
 
 struct Tile {
@@ -454,7 +495,9 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
         if (tile_cost(p, *x, cus) < tile_cost(p, *t, cus)) t = x;
     p.n_tiles = (p.N + 64 * t->ni - 1) / (64 * t->ni);
     p.m_tiles = (p.M + 64 * t->mj - 1) / (64 * t->mj);
-    const dim3 grid(xcd_grid((long)p.n_tiles * p.m_tiles)), block(256);
+    // two-stage forms: a workgroup per CU walks its tiles
+    const long tiles = (long)p.n_tiles * p.m_tiles;
+    const dim3 grid(xcd_grid(t->ns == 2 && tiles > cus ? cus : tiles)), block(256);
 #define TILE(E, NI, MJ, NS)                                                     \
     if (p.c_f32 == E && t->ni == NI && t->mj == MJ) {                           \
         hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS>), grid, block, 0, s, p); \
