@@ -235,7 +235,12 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
 template <bool EXACT, int NI, int MJ, int NS>
 __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     constexpr int BN = 64 * NI, BM = 64 * MJ;
-    constexpr int SCALES = (BN + BM) * ROW, STAGE = SCALES + 2048;  // words of A's rows, then W's
+    constexpr int SCALES = (BN + BM) * ROW;
+    // a stage's scale words: A's rows', then W's.  Each wave has one instruction for them (so
+    // that all wait for one count): 256 rows take one of 16 bytes a lane (waves 0 and 2, W's
+    // 1 and 3), fewer one of 4 (a wave for each 64 rows, W's the others).
+    constexpr int WORD_B = MJ == 4 ? 16 : 4, W_WORDS = MJ == 4 ? 256 : 64 * MJ;
+    constexpr int STAGE = SCALES + 4 * W_WORDS + 64 * WORD_B;
     // two-stage forms walk several tiles: the next tile's first stages land during this
     // one's epilogue, which therefore has LDS of its own
     constexpr bool WALK = NS == 2;
@@ -278,8 +283,8 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         aoff[i] = row * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
     }
     constexpr int NP = 2 * NI + 2 * MJ + 1;  // DMA instructions of a wave per stage
-    // the last of them: waves 0 and 2 A's words, 1 and 3 W's (alike, so that every wave waits for one count)
-    const bool w_words = wave & 1;
+    const bool w_words = MJ == 4 ? wave & 1 : wave >= MJ;
+    const int words0 = MJ == 4 || w_words ? 0 : 64 * wave;  // the first of the wave's words
     const int64_t words_ld = w_words ? p.ld_ws : p.ld_as;
     // the stage fetched next: block f_kt of tile f_tile; past the last tile empty
     // resources, whose loads write zeros without memory traffic
@@ -310,8 +315,9 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         uint8_t* st = lds + slot * STAGE;
         if (x == NP - 1) {
             const __amdgpu_buffer_rsrc_t sres = uniform_rsrc(words + (int64_t)(f_kt >> 2) * words_ld, words_bytes);
-            uint8_t* dst = st + SCALES + 1024 * w_words;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 16, 16 * lane, 0, 0, 0);
+            uint8_t* dst = st + SCALES + 4 * (w_words ? W_WORDS : words0);
+            if constexpr (WORD_B == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 16, 16 * lane, 0, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 4, 4 * (words0 + lane), 0, 0, 0);
             return;
         }
         const bool is_a = x >= 2 * NI;
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(lds + slot * STAGE + SCALES);
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa_next[j] = (int)w[wm * 32 * MJ + 32 * j + c];
-        sw_next = (int)w[256 + ((wn * 32 * NI) >> 7)];
+        sw_next = (int)w[W_WORDS + ((wn * 32 * NI) >> 7)];
     };
     auto take_scales = [&](int kt) __attribute__((always_inline)) {  // byte kt % 4 of the words
         const int sh = 8 * (kt & 3);
@@ -349,12 +355,12 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa[j] = sa_next[j] >> sh;
     };
-    // One half block on fragment buffer `buf`; between its instructions the reads of
-    // the next half (slot rslot, half rs, into buffer buf ^ 1) and, when `dma`, the DMA
+    // One half block on fragment buffer `buf`; between its instructions, when `read`, the
+    // reads of the next half (slot rslot, half rs, into buffer buf ^ 1) and, when `dma`, the DMA
     // pieces of the next stage into slot dma_slot, spread evenly: an instruction of 64
     // cycles hides one read and one piece, not two (5498 x 13824 x 2560 188 us with them
     // in the first eight of sixteen, 175 so).
-    auto half = [&](int buf, int rslot, int rs, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
+    auto half = [&](int buf, int rslot, int rs, bool read, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
         bf16x8 wb[EXACT ? NI : 1][4], ab[EXACT ? MJ : 1][4];
         if constexpr (EXACT) {
             const float fw = scale_of(sw & 0xff);
@@ -388,7 +394,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < NR; e++)
-                if (e * T / NR == x) read_piece(rslot, rs, buf ^ 1, e);
+                if (read && e * T / NR == x) read_piece(rslot, rs, buf ^ 1, e);
 #pragma unroll
             for (int e = 0; e < NP; e++)
                 if (dma && e * T / NP == x) load_piece(dma_slot, e);
@@ -404,11 +410,11 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     int slot = 0;
     auto next = [](int t) __attribute__((always_inline)) { return t + 1 == NS ? 0 : t + 1; };
     auto stage = [&](int kt, bool zc) __attribute__((always_inline)) {
-        half(0, slot, 1, false, 0, zc);
+        half(0, slot, 1, true, false, 0, zc);
         wait_vmem_lds<(NS - 2) * NP>();
         __builtin_amdgcn_s_barrier();
         read_scales(next(slot));
-        half(1, next(slot), 0, true, slot, false);
+        half(1, next(slot), 0, true, true, slot, false);
         // the sums stay here: the compiler would move the instructions that no one reads
         // yet past the branch below, behind all the loads between them
 #pragma unroll
@@ -431,9 +437,21 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     read_scales(0);
     take_scales(0);
     while (true) {
-        stage(0, true);
-        for (int kt = 1; kt < nk; kt++) stage(kt, false);
         int m0, n0;
+        if constexpr (WALK) {
+            stage(0, true);
+            for (int kt = 1; kt < nk; kt++) stage(kt, false);
+        } else {
+            // no stage follows the last one, which only reads its own second half
+            if (nk > 1) {
+                stage(0, true);
+                for (int kt = 1; kt + 1 < nk; kt++) stage(kt, false);
+                half(0, slot, 1, true, false, 0, false);
+            } else {
+                half(0, slot, 1, true, false, 0, true);
+            }
+            half(1, slot, 0, false, false, 0, false);
+        }
         place(tile, m0, n0);
         if constexpr (!WALK) {  // the slots are free once every DMA (of nothing, by now) and read is done
             wait_vmem_lds<0>();
