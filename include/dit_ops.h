@@ -109,7 +109,7 @@ typedef struct {
  * (AWA_F32 or AWA_BF16), at positions d_pos int32 [n_tokens][axes] (any int32).
  * The plan is copied before the call returns.  Angles are reduced to a turn in
  * fp64, so far positions keep their precision; products are fp32, rounded once.
- * n_tokens may be 0.  Rejected (AWA_EARG): head_d over 256 or under twice the
+ * n_tokens may be 0.  Rejected (AWA_EARG): over 32767 heads, head_d over 256 or under twice the
  * pairs, frequencies or a scale that are not finite, negative strides, outputs
  * whose elements could coincide, with each other's or with an input's, other than
  * out = x with the same strides (views of one buffer are accepted where equal

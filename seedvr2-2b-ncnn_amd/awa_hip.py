@@ -21,6 +21,9 @@ AWA_F32, AWA_BF16 = 0, 1
 HEADS, HEAD_D, DIM, QKV, ROPE_ROT = 20, 128, 2560, 7680, 126
 
 _lib = None
+# set by lib(), which imports torch: the module, the 8-bit types that the operators take (values or scales
+# first, then plain bytes) and the storage types by torch's
+_torch, _e4m3, _e8m0, _storage = None, (), (), {}
 
 
 class AwaError(RuntimeError):
@@ -69,6 +72,9 @@ class RopeRows(C.Structure):
         (n, C.c_int64) for n in ("x_token", "x_head", "out_token", "out_head")]
 
 
+_RopeRows2 = RopeRows * 2
+
+
 class GeomInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in
                 ("t", "h", "w", "nwin", "sumf", "Lv", "txt_len", "max_S", "n_tiles", "n_items")]
@@ -81,7 +87,7 @@ def build():
 
 
 def lib():
-    global _lib
+    global _lib, _torch, _e4m3, _e8m0, _storage
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise ImportError(f"{LIB_PATH} is missing: build it (make -C {HERE}) before use")
@@ -89,7 +95,7 @@ def lib():
         # (libamdhip64.so.7).  Load it first so the library binds to that one
         # runtime instead of starting a second one from /opt/rocm in the same
         # process: torch's tensors and streams then belong to our runtime too.
-        import torch  # noqa: F401
+        import torch
         L = C.CDLL(LIB_PATH)
         vp, i32p, f32p = C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_float)
         L.awa_create.argtypes = [C.POINTER(vp), C.c_int]
@@ -170,8 +176,17 @@ def lib():
                                    C.c_int, C.c_int, vp]
         L.dit_rope.argtypes = [vp, C.c_int, C.POINTER(RopeRows), C.c_int, C.c_int, C.c_int, C.POINTER(RopePlan), vp, vp]
         L.dit_rope_freqs.argtypes = [C.c_int, C.c_int] + 5 * [C.c_double] + [vp]
+        _torch, _storage = torch, {torch.float32: AWA_F32, torch.bfloat16: AWA_BF16}
+        _e4m3, _e8m0 = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
         _lib = L
     return _lib
+
+
+def _dtype_of(what, t):
+    d = _storage.get(t.dtype)
+    if d is None:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype}")
+    return d
 
 
 def _host_array(ptr, n, dtype):
@@ -278,14 +293,6 @@ def rope_freqs(n, base=10000.0, kind="plain", factor=1.0, trained=0.0, low=1.0, 
     if rc != AWA_OK:
         raise AwaError(rc, "dit_rope_freqs rejected the arguments")
     return out
-
-
-_FP8 = {"e": "float8_e8m0fnu", "q": "float8_e4m3fn", "a": "float8_e4m3fn", "w": "float8_e4m3fn"}
-
-
-def _bytes_of(t, shape, name):
-    """Whether t is a contiguous tensor of this shape of scales (names that end so) or e4m3 values, or of their bytes."""
-    return tuple(t.shape) == shape and t.is_contiguous() and str(t.dtype)[6:] in (_FP8[name[-1]], "uint8")
 
 
 def fp8_values(q, scale, cols=None):
@@ -499,85 +506,89 @@ class Context:
         return emb
 
     # ---- operators around a projection in 8 bits (include/dit_ops.h)
-    def _on(self, what, *tensors):
-        """Every tensor lives on the context's device."""
-        for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != self.device):
-                raise ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
-
     def _stream(self, stream, *made):
         """The stream of a call: the given one, else the current one of the context's device.  Tensors that
         the call made on the current stream are marked as used on another."""
-        import torch
         if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return _torch._C._cuda_getCurrentRawStream(self.device)
         for t in made:
             t.record_stream(stream)
         return stream.cuda_stream
 
-    @staticmethod
-    def _dtype(what, dtype):
-        import torch
-        if dtype == torch.bfloat16:
-            return AWA_BF16
-        if dtype == torch.float32:
-            return AWA_F32
-        raise TypeError(f"{what}: unsupported dtype {dtype}")
+    def _elsewhere(self, what, t):
+        return ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
+
+    def _bytes_of(self, what, t, name, kind, *shape):
+        """t is a contiguous tensor of this shape of the given 8-bit type (or of plain bytes) on the context's device."""
+        if t.dtype not in kind or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous {str(kind[0])[6:]} tensor {list(shape)}, got "
+                             f"{str(t.dtype)[6:]} {list(t.shape)} with strides {t.stride()}")
+        if t.get_device() != self.device:
+            raise self._elsewhere(what, t)
 
     def quant_fp8(self, x, blocks=False, q=None, scale=None, stream=None):
         """dit_quant_fp8: x [rows, cols] bf16 or fp32 (columns contiguous) to (q, scale): q float8_e4m3fn
         [rows, cols padded to 128], scale float8_e8m0fnu [groups of four column blocks, rows, 4] (blocks=True:
         a scale per 128 x 128 values, [groups, ceil(rows / 128), 4])."""
-        import torch
-        dtype = self._dtype("quant_fp8", x.dtype)
-        if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+        lib_ = lib()
+        dtype = _dtype_of("quant_fp8", x)
+        rows, cols = x.shape if x.dim() == 2 else (0, 0)
+        if cols < 1 or (cols > 1 and x.stride(1) != 1):
             raise ValueError("quant_fp8: x must be [rows, cols] with contiguous columns")
-        rows, cols = x.shape
-        qs, ss = (rows, (cols + 127) // 128 * 128), ((cols + 511) // 512, (rows + 127) // 128 if blocks else rows, 4)
-        made = []
+        if x.get_device() != self.device:
+            raise self._elsewhere("quant_fp8", x)
+        kp, groups, srows = (cols + 127) // 128 * 128, (cols + 511) // 512, (rows + 127) // 128 if blocks else rows
+        made = ()
         if q is None:
-            q = torch.empty(qs, dtype=torch.float8_e4m3fn, device=x.device)
-            made.append(q)
+            q = x.new_empty((rows, kp), dtype=_e4m3[0])
+            made = (q,)
+        else:
+            self._bytes_of("quant_fp8", q, "q", _e4m3, rows, kp)
         if scale is None:
-            scale = torch.empty(ss, dtype=torch.float8_e8m0fnu, device=x.device)
-            made.append(scale)
-        self._on("quant_fp8", x, q, scale)
-        for t, shape, name in ((q, qs, "q"), (scale, ss, "scale")):
-            if not _bytes_of(t, shape, name):
-                raise ValueError(f"quant_fp8: {name} must be a contiguous {_FP8[name[-1]]} tensor {list(shape)}")
+            scale = x.new_empty((groups, srows, 4), dtype=_e8m0[0])
+            made += (scale,)
+        else:
+            self._bytes_of("quant_fp8", scale, "scale", _e8m0, groups, srows, 4)
         if rows:
-            self.check(lib().dit_quant_fp8(self.ptr, dtype, x.data_ptr(), x.stride(0), rows, cols, 128 if blocks else 1,
-                                           q.data_ptr(), scale.data_ptr(), ss[1], self._stream(stream, *made)),
-                       "dit_quant_fp8")
+            rc = lib_.dit_quant_fp8(self.ptr, dtype, x.data_ptr(), x.stride(0), rows, cols, 128 if blocks else 1,
+                                    q.data_ptr(), scale.data_ptr(), srows, self._stream(stream, *made))
+            if rc:
+                self.check(rc, "dit_quant_fp8")
         return q, scale
 
     def gemm_fp8(self, a, a_scale, w, w_scale, bias=None, out=None, dtype=None, stream=None):
         """dit_gemm_fp8: [M, N] = A W^T (+ bias fp32 [N]) of matrices as quant_fp8 returns them, A by rows and W
         with blocks=True; `dtype` bf16 (default) or fp32, or that of `out` (rows may be strided)."""
-        import torch
+        lib_ = lib()
+        if a.dim() != 2 or w.dim() != 2:
+            raise ValueError("gemm_fp8: a [M, K] and w [N, K]")
         M, K = a.shape
         N = w.shape[0]
+        groups, nb = (K + 511) // 512, (N + 127) // 128
+        self._bytes_of("gemm_fp8", a, "a", _e4m3, M, K)
+        self._bytes_of("gemm_fp8", w, "w", _e4m3, N, K)
+        self._bytes_of("gemm_fp8", a_scale, "a_scale", _e8m0, groups, M, 4)
+        self._bytes_of("gemm_fp8", w_scale, "w_scale", _e8m0, groups, nb, 4)
+        made = ()
         if out is None:
-            out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=a.device)
+            out = a.new_empty((M, N), dtype=dtype or _torch.bfloat16)
             made = (out,)
-        else:
-            made = ()
-            if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (dtype or out.dtype) != out.dtype:
-                raise ValueError(f"gemm_fp8: out must be [{M}, {N}] of dtype {dtype} with contiguous columns")
-        self._on("gemm_fp8", a, a_scale, w, w_scale, bias, out)
-        groups = (K + 511) // 512
-        for t, shape, name in ((a, (M, K), "a"), (w, (N, K), "w"), (a_scale, (groups, M, 4), "a_scale"),
-                               (w_scale, (groups, (N + 127) // 128, 4), "w_scale")):
-            if not _bytes_of(t, shape, name):
-                raise ValueError(f"gemm_fp8: {name} must be a contiguous {_FP8[name[-1]]} tensor {list(shape)}")
-        if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
-            raise ValueError(f"gemm_fp8: bias must be a contiguous fp32 tensor [{N}]")
-        ct = self._dtype("gemm_fp8", out.dtype)
+        elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (dtype or out.dtype) != out.dtype:
+            raise ValueError(f"gemm_fp8: out must be [{M}, {N}] of dtype {dtype} with contiguous columns")
+        elif out.get_device() != self.device:
+            raise self._elsewhere("gemm_fp8", out)
+        ct = _dtype_of("gemm_fp8", out)
+        if bias is not None:
+            if bias.dtype != _torch.float32 or bias.shape != (N,) or not bias.is_contiguous():
+                raise ValueError(f"gemm_fp8: bias must be a contiguous fp32 tensor [{N}]")
+            if bias.get_device() != self.device:
+                raise self._elsewhere("gemm_fp8", bias)
         if M:
-            self.check(lib().dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), M, w.data_ptr(),
-                                          w_scale.data_ptr(), w_scale.shape[1], bias.data_ptr() if bias is not None else None,
-                                          ct, out.data_ptr(), out.stride(0), M, N, K, self._stream(stream, *made)),
-                       "dit_gemm_fp8")
+            rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), M, w.data_ptr(), w_scale.data_ptr(), nb,
+                                   bias.data_ptr() if bias is not None else None, ct, out.data_ptr(), out.stride(0), M, N,
+                                   K, self._stream(stream, *made))
+            if rc:
+                self.check(rc, "dit_gemm_fp8")
         return out
 
     def rope(self, x, positions, freqs, pairs=None, layout="interleaved", scale=1.0, inverse=False, out=None,
@@ -586,41 +597,53 @@ class Context:
         rotated at positions int32 [tokens] or [tokens, axes].  freqs: radians per position of each pair
         (rope_freqs, float64), axis after axis; pairs: how many belong to each axis.  inverse=True is the adjoint,
         which takes gradients of the output to those of the input.  out: x itself for a rotation in place."""
-        import torch
-        xs = list(x) if isinstance(x, (tuple, list)) else [x]
-        outs = [None] * len(xs) if out is None else list(out) if isinstance(out, (tuple, list)) else [out]
-        if len(xs) not in (1, 2) or len(outs) != len(xs):
+        lib_ = lib()
+        many = isinstance(x, (tuple, list))
+        xs = x if many else (x,)
+        outs = (None,) * len(xs) if out is None else out if isinstance(out, (tuple, list)) else (out,)
+        if not 1 <= len(xs) <= 2 or len(outs) != len(xs):
             raise ValueError("rope: one or two tensors, and as many outputs")
+        first = xs[0]
+        dtype = _dtype_of("rope", first)
+        if first.dim() != 3:
+            raise ValueError("rope: tensors must be [tokens, heads, head_d]")
+        tokens, _, head_d = first.shape
         f = np.ascontiguousarray(freqs, np.float64)
         axes = positions.shape[1] if positions.dim() == 2 else 1
         pairs = (f.size,) if pairs is None else tuple(pairs)
-        tokens, _, head_d = xs[0].shape
-        if (positions.dtype != torch.int32 or not positions.is_contiguous() or positions.dim() > 2 or
-                positions.shape[0] != tokens):
+        if (positions.dtype != _torch.int32 or positions.dim() > 2 or positions.shape[0] != tokens or
+                not positions.is_contiguous()):
             raise ValueError(f"rope: positions must be contiguous int32 [{tokens}] or [{tokens}, axes]")
         if len(pairs) != axes or axes > ROPE_MAX_AXES or sum(pairs) != f.size or f.size > ROPE_MAX_PAIRS:
             raise ValueError(f"rope: pairs {pairs} must name each axis of the positions and sum to the {f.size} freqs")
-        dtype = self._dtype("rope", xs[0].dtype)
-        plan = RopePlan(ROPE_LAYOUTS[layout], axes, pairs, int(bool(inverse)), scale)
-        C.memmove(C.addressof(plan) + RopePlan.freq.offset, f.ctypes.data, 8 * f.size)
-        rows, made = (RopeRows * len(xs))(), []
+        if layout not in ROPE_LAYOUTS:
+            raise ValueError(f"rope: layout must be one of {list(ROPE_LAYOUTS)}")
+        if positions.get_device() != self.device:
+            raise self._elsewhere("rope", positions)
+        plan = RopePlan(ROPE_LAYOUTS[layout], axes, pairs, 1 if inverse else 0, scale)
+        C.memmove(C.byref(plan, RopePlan.freq.offset), f.ctypes.data, 8 * f.size)
+        rows, made, res = _RopeRows2(), (), []
         for i, t in enumerate(xs):
-            if t.dim() != 3 or t.dtype != xs[0].dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
-                    head_d > 1 and t.stride(2) != 1):
+            ts = t.stride()
+            if t.dim() != 3 or t.dtype != first.dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
+                    head_d > 1 and ts[2] != 1):
                 raise ValueError("rope: tensors must be [tokens, heads, head_d] of one dtype with contiguous channels")
             o = outs[i]
             if o is None:
-                o = outs[i] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                made.append(o)
+                o = t.new_empty(t.shape)
+                made += (o,)
             elif o.shape != t.shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):
                 raise ValueError("rope: out must have x's shape and dtype and contiguous channels")
-            self._on("rope", t, o)
-            rows[i] = RopeRows(t.data_ptr(), o.data_ptr(), t.shape[1], t.stride(0), t.stride(1), o.stride(0),
-                               o.stride(1))
-        self._on("rope", positions)
-        self.check(lib().dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, C.byref(plan), positions.data_ptr(),
-                                  self._stream(stream, *made)), "dit_rope")
-        return tuple(outs) if isinstance(x, (tuple, list)) else outs[0]
+            if t.get_device() != self.device or o.get_device() != self.device:
+                raise self._elsewhere("rope", t)
+            res.append(o)
+            os_ = o.stride()
+            rows[i] = (t.data_ptr(), o.data_ptr(), t.shape[1], ts[0], ts[1], os_[0], os_[1])
+        rc = lib_.dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, plan, positions.data_ptr(),
+                           self._stream(stream, *made))
+        if rc:
+            self.check(rc, "dit_rope")
+        return tuple(res) if many else res[0]
 
     def reserve(self, geom, dtype="bf16"):
         """awa_reserve: size the op's scratch for geom in this storage dtype."""

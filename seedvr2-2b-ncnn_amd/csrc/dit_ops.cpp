@@ -192,11 +192,10 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
     const size_t size = elem(dtype);
     // strides far enough below 2^63 for the checks' own arithmetic
     constexpr int64_t STRIDE_MAX = (int64_t)1 << 36;
-    a.vec = 1;
     for (int t = 0; t < n_rows; t++) {
         const dit_rope_rows& r = rows[t];
-        if (r.heads < 0 || r.heads > 65536) {
-            set_err(ctx, "dit_rope: heads=%d of tensor %d (0 .. 65536)", r.heads, t);
+        if (r.heads < 0 || r.heads > 32767) {
+            set_err(ctx, "dit_rope: heads=%d of tensor %d (0 .. 32767)", r.heads, t);
             return AWA_EARG;
         }
         if (r.heads == 0 || n_tokens == 0) continue;
@@ -220,9 +219,6 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
             return AWA_EARG;
         }
         if (!same) in_place = false;
-        for (int64_t st : {vx[t].token, vx[t].head, vo[t].token, vo[t].head})
-            if (st % 16) a.vec = 0;
-        if (!aligned(r.x, 16) || !aligned(r.out, 16)) a.vec = 0;
     }
     if (n_rows == 2 && rows[0].heads && rows[1].heads && n_tokens &&
         (!apart(vo[0], vo[1]) || !apart(vo[0], vx[1]) || !apart(vx[0], vo[1]))) {

@@ -43,7 +43,6 @@ struct RopeArgs {
     int pairs;               // rotated pairs, all axes
     int axes, axis_end[DIT_ROPE_MAX_AXES];  // pairs up to each axis's end
     int copy;                // channels past the pairs go from x to out (not in place)
-    int vec;                 // 16-byte pieces everywhere
     int rot_units, units;    // pieces of a head that turn, and all; filled by launch_rope
     int heads_per_block;
     const int32_t* pos;
