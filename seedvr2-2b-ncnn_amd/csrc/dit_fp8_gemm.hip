@@ -41,56 +41,51 @@ __device__ inline bf16x8 widen(int lo, int hi, float scale) {
 
 // ---- few rows ---------------------------------------------------------------
 //
-// 16 features x 16 MJ rows per workgroup, the blocks of K in turn over its waves,
+// Up to 16 rows: 16 NI features per workgroup, the blocks of K in turn over its waves,
 // whose sums meet in LDS (in the waves' order).  Bound by W, which is read once,
-// straight into registers; nothing is shared that LDS could hold for others.
-template <int MJ, int WAVES>
+// straight into registers; A comes from the L2 again for every workgroup.
+template <int NI, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
-    __shared__ f32x4 part[WAVES][MJ][64];
+    __shared__ f32x4 part[WAVES][NI][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int n0 = (blockIdx.x % p.n_tiles) * 16, m0 = (blockIdx.x / p.n_tiles) * (16 * MJ);
+    const int n0 = blockIdx.x * (16 * NI);
     // rows past the end repeat the last
-    const uint8_t* wp = p.W + (int64_t)min(n0 + r, p.N - 1) * p.K + 16 * q;
-    const uint8_t* wsp = reinterpret_cast<const uint8_t*>(p.ws + (n0 >> 7));
-    const uint8_t* ap[MJ];
-    const uint8_t* asp[MJ];
+    const int row = min(r, p.M - 1);
+    const uint8_t* ap = p.A + (int64_t)row * p.K + 16 * q;
+    const uint8_t* asp = reinterpret_cast<const uint8_t*>(p.as + row);
+    const uint8_t* wp[NI];
 #pragma unroll
-    for (int j = 0; j < MJ; j++) {
-        const int row = min(m0 + 16 * j + r, p.M - 1);
-        ap[j] = p.A + (int64_t)row * p.K + 16 * q;
-        asp[j] = reinterpret_cast<const uint8_t*>(p.as + row);
-    }
+    for (int i = 0; i < NI; i++) wp[i] = p.W + (int64_t)min(n0 + 16 * i + r, p.N - 1) * p.K + 16 * q;
+    const uint8_t* wsp = reinterpret_cast<const uint8_t*>(p.ws + (n0 >> 7));
     const int nk = p.K >> 7;
     struct Block {
-        i32x4 w[2], a[MJ][2];
-        int sw, sa[MJ];
+        i32x4 a[2], w[NI][2];
+        int sw, sa;
     };
     auto load = [&](Block& b, int kb) __attribute__((always_inline)) {
         const int64_t g = kb >> 2;
 #pragma unroll
-        for (int h = 0; h < 2; h++) b.w[h] = *reinterpret_cast<const i32x4*>(wp + kb * 128 + 64 * h);
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) b.w[i][h] = *reinterpret_cast<const i32x4*>(wp[i] + kb * 128 + 64 * h);
+#pragma unroll
+        for (int h = 0; h < 2; h++) b.a[h] = *reinterpret_cast<const i32x4*>(ap + kb * 128 + 64 * h);
         b.sw = wsp[4 * g * p.ld_ws + (kb & 3)];
-#pragma unroll
-        for (int j = 0; j < MJ; j++) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) b.a[j][h] = *reinterpret_cast<const i32x4*>(ap[j] + kb * 128 + 64 * h);
-            b.sa[j] = asp[j][4 * g * p.ld_as + (kb & 3)];
-        }
+        b.sa = asp[4 * g * p.ld_as + (kb & 3)];
     };
-    f32x4 acc[MJ];
+    f32x4 acc[NI];
 #pragma unroll
-    for (int j = 0; j < MJ; j++) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NI; i++) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     auto sum = [&](const Block& b) __attribute__((always_inline)) {
-        const float sw = scale_of(b.sw);
+        const float sw = scale_of(b.sw), sa = scale_of(b.sa);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const bf16x8 w0 = widen(b.w[h][0], b.w[h][1], sw), w1 = widen(b.w[h][2], b.w[h][3], sw);
+            const bf16x8 a0 = widen(b.a[h][0], b.a[h][1], sa), a1 = widen(b.a[h][2], b.a[h][3], sa);
 #pragma unroll
-            for (int j = 0; j < MJ; j++) {
-                const float sa = scale_of(b.sa[j]);
-                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, widen(b.a[j][h][0], b.a[j][h][1], sa), acc[j], 0, 0, 0);
-                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, widen(b.a[j][h][2], b.a[j][h][3], sa), acc[j], 0, 0, 0);
+            for (int i = 0; i < NI; i++) {
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(b.w[i][h][0], b.w[i][h][1], sw), a0, acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(b.w[i][h][2], b.w[i][h][3], sw), a1, acc[i], 0, 0, 0);
             }
         }
     };
@@ -104,23 +99,22 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
         if (kb + WAVES < nk) sum(b1);
     }
 #pragma unroll
-    for (int j = 0; j < MJ; j++) part[wave][j][lane] = acc[j];
+    for (int i = 0; i < NI; i++) part[wave][i][lane] = acc[i];
     __syncthreads();
-    // wave j finishes row block j
-    for (int j = wave; j < MJ; j += WAVES) {
-        f32x4 c = part[0][j][lane];
+    // wave i finishes feature block i
+    if (wave >= NI) return;
+    f32x4 c = part[0][wave][lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) c += part[w][j][lane];
-        const int m = m0 + 16 * j + r, n = n0 + 4 * q;
-        if (m >= p.M) continue;
+    for (int w = 1; w < WAVES; w++) c += part[w][wave][lane];
+    const int n = n0 + 16 * wave + 4 * q;
+    if (r >= p.M) return;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (n + i < p.N) {
-                const float v = c[i] + (p.bias ? p.bias[n + i] : 0.f);
-                if (p.c_f32) reinterpret_cast<float*>(p.C)[m * p.ldc + n + i] = v;
-                else reinterpret_cast<uint16_t*>(p.C)[m * p.ldc + n + i] = (uint16_t)bf16x2_rne(v, v);
-            }
-    }
+    for (int i = 0; i < 4; i++)
+        if (n + i < p.N) {
+            const float v = c[i] + (p.bias ? p.bias[n + i] : 0.f);
+            if (p.c_f32) reinterpret_cast<float*>(p.C)[r * p.ldc + n + i] = v;
+            else reinterpret_cast<uint16_t*>(p.C)[r * p.ldc + n + i] = (uint16_t)bf16x2_rne(v, v);
+        }
 }
 
 // ---- tiles ------------------------------------------------------------------
@@ -232,8 +226,10 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
     }
 }
 
-template <bool EXACT, int NI, int MJ, int NS>
-__global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
+// KG: groups of four waves that take the blocks of K in turn, each with stages of its own,
+// for products of few tiles; their sums meet in LDS at the end, in the groups' order.
+template <bool EXACT, int NI, int MJ, int NS, int KG>
+__global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     constexpr int BN = 64 * NI, BM = 64 * MJ;
     constexpr int SCALES = (BN + BM) * ROW;
     // a stage's scale words: A's rows', then W's.  Each wave has one instruction for them (so
@@ -243,8 +239,9 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     constexpr int STAGE = SCALES + 4 * W_WORDS + 64 * WORD_B;
     // two-stage forms walk several tiles: the next tile's first stages land during this
     // one's epilogue, which therefore has LDS of its own
-    constexpr bool WALK = NS == 2;
-    __shared__ __align__(16) uint8_t lds[NS * STAGE + (WALK ? 4 * STG : 0)];
+    constexpr bool WALK = NS == 2 && KG == 1;
+    __shared__ __align__(16) uint8_t lds[KG * NS * STAGE + (WALK ? 4 * STG : 0)];
+    static_assert(sizeof(lds) <= 160 * 1024 && 4 * STG + (KG - 1) * NI * MJ * 16384 <= (int)sizeof(lds), "LDS");
     const int total = p.n_tiles * p.m_tiles;
     // tiles lid, lid + stride, .. of the XCD's contiguous range up to `end`
     const int per = (total + 7) >> 3, stride = gridDim.x >> 3;
@@ -260,12 +257,14 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         n0 = in_group / gm * BN;
     };
 
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int kg = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
     const int wn = wave >> 1, wm = wave & 1;
     const int c = lane & 31, g = lane >> 5;
-    const int nk = p.K >> 7;
-    int nk_wrap = nk;
-    asm("" : "+s"(nk_wrap));  // so that no last stage is peeled off the loop for its one comparison
+    const int nk = p.K >> 7, ns = (nk + KG - 1) / KG;  // blocks, and stages of every group
+    int ns_wrap = ns;
+    asm("" : "+s"(ns_wrap));  // so that no last stage is peeled off the loop for its one comparison
+    uint8_t* const ring = lds + kg * (NS * STAGE);
 
     // DMA: one instruction of a wave fills 8 rows; lane l lands in row l / 8, chunk
     // l % 8, so it fetches the chunk that the swizzle maps there.  Rows past N or M
@@ -286,9 +285,9 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     const bool w_words = MJ == 4 ? wave & 1 : wave >= MJ;
     const int words0 = MJ == 4 || w_words ? 0 : 64 * wave;  // the first of the wave's words
     const int64_t words_ld = w_words ? p.ld_ws : p.ld_as;
-    // the stage fetched next: block f_kt of tile f_tile; past the last tile empty
+    // the stage fetched next: block f_kt of tile f_tile; past the last block (tile) empty
     // resources, whose loads write zeros without memory traffic
-    int f_tile = tile, f_kt = 0;
+    int f_tile = tile, f_kt = kg;
     __amdgpu_buffer_rsrc_t wres, ares;
     const uint32_t* words;
     uint32_t words_bytes;
@@ -305,14 +304,15 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         words_bytes = 4u * (w_words ? (wrows + 127) >> 7 : arows);
     };
     auto fetch_next = [&]() __attribute__((always_inline)) {
-        if (++f_kt == nk) {
+        f_kt += KG;
+        if (f_kt >= nk) {
             f_kt = 0;
-            f_tile += stride;
-            fetch_from(WALK ? f_tile : end);
+            f_tile = WALK ? f_tile + stride : end;
+            fetch_from(f_tile);
         }
     };
     auto load_piece = [&](int slot, int x) __attribute__((always_inline)) {
-        uint8_t* st = lds + slot * STAGE;
+        uint8_t* st = ring + slot * STAGE;
         if (x == NP - 1) {
             const __amdgpu_buffer_rsrc_t sres = uniform_rsrc(words + (int64_t)(f_kt >> 2) * words_ld, words_bytes);
             uint8_t* dst = st + SCALES + 4 * (w_words ? W_WORDS : words0);
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     // piece x of the fragments of half s of a stage (into buffer buf): two chunks of a row each
     auto read_piece = [&](int slot, int s, int buf, int x) __attribute__((always_inline)) {
         const int f = x >> 1, h = x & 1, at = ((4 * s + 2 * g + h) ^ sx) << 4;
-        const uint8_t* from = lds + slot * STAGE + at + (f < NI ? wrow + 32 * ROW * f : arow + 32 * ROW * (f - NI));
+        const uint8_t* from = ring + slot * STAGE + at + (f < NI ? wrow + 32 * ROW * f : arow + 32 * ROW * (f - NI));
         const i32x4 v = *reinterpret_cast<const i32x4*>(from);
         i32x8& d = f < NI ? wf[buf][f < NI ? f : 0] : af[buf][f < NI ? 0 : f - NI];
 #pragma unroll
@@ -344,13 +344,13 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     };
     constexpr int NR = 2 * (NI + MJ);
     auto read_scales = [&](int slot) __attribute__((always_inline)) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(lds + slot * STAGE + SCALES);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(ring + slot * STAGE + SCALES);
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa_next[j] = (int)w[wm * 32 * MJ + 32 * j + c];
         sw_next = (int)w[W_WORDS + ((wn * 32 * NI) >> 7)];
     };
-    auto take_scales = [&](int kt) __attribute__((always_inline)) {  // byte kt % 4 of the words
-        const int sh = 8 * (kt & 3);
+    auto take_scales = [&](int st) __attribute__((always_inline)) {  // the group's stage st: byte kt % 4 of the words
+        const int sh = 8 * ((st * KG + kg) & 3);
         sw = __builtin_amdgcn_readfirstlane(sw_next) >> sh;
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa[j] = sa_next[j] >> sh;
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     // the next stage's first fragments and refills this slot with the stage NS on.
     int slot = 0;
     auto next = [](int t) __attribute__((always_inline)) { return t + 1 == NS ? 0 : t + 1; };
-    auto stage = [&](int kt, bool zc) __attribute__((always_inline)) {
+    auto stage = [&](int st, bool zc) __attribute__((always_inline)) {
         half(0, slot, 1, true, false, 0, zc);
         wait_vmem_lds<(NS - 2) * NP>();
         __builtin_amdgcn_s_barrier();
@@ -420,10 +420,10 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
 #pragma unroll
         for (int x = 0; x < NI * MJ; x++) asm volatile("" : "+a"(acc[x / MJ][x % MJ]));
         fetch_next();
-        take_scales(kt + 1 == nk_wrap ? 0 : kt + 1);
+        take_scales(st + 1 == ns_wrap ? 0 : st + 1);
         slot = next(slot);
     };
-    fetch_from(tile);
+    fetch_from(kg < nk ? tile : end);
 #pragma unroll
     for (int i = 0; i < NS; i++) {
 #pragma unroll
@@ -440,12 +440,12 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         int m0, n0;
         if constexpr (WALK) {
             stage(0, true);
-            for (int kt = 1; kt < nk; kt++) stage(kt, false);
+            for (int st = 1; st < ns; st++) stage(st, false);
         } else {
             // no stage follows the last one, which only reads its own second half
-            if (nk > 1) {
+            if (ns > 1) {
                 stage(0, true);
-                for (int kt = 1; kt + 1 < nk; kt++) stage(kt, false);
+                for (int st = 1; st + 1 < ns; st++) stage(st, false);
                 half(0, slot, 1, true, false, 0, false);
             } else {
                 half(0, slot, 1, true, false, 0, true);
@@ -456,6 +456,34 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         if constexpr (!WALK) {  // the slots are free once every DMA (of nothing, by now) and read is done
             wait_vmem_lds<0>();
             __builtin_amdgcn_s_barrier();
+        }
+        if constexpr (KG > 1) {
+            // the other groups' sums to group 0, past its staging area
+            f32x4* sums = reinterpret_cast<f32x4*>(lds + 4 * STG) + (tid & 255);
+            auto at = [&](int from, int x, int q) __attribute__((always_inline)) {
+                return sums + 256 * ((from * NI * MJ + x) * 4 + q);
+            };
+            if (kg) {
+#pragma unroll
+                for (int x = 0; x < NI * MJ; x++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f32x16& v = acc[x / MJ][x % MJ];
+                        *at(kg - 1, x, q) = (f32x4){v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                    }
+            }
+            __syncthreads();
+            if (kg) return;
+#pragma unroll
+            for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+                for (int x = 0; x < NI * MJ; x++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f32x4 v = *at(o, x, q);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[x / MJ][x % MJ][4 * q + e] += v[e];
+                    }
         }
         uint8_t* stg = lds + (WALK ? NS * STAGE : 0) + wave * STG;
         // the lane anew, so that the epilogue's addresses are formed here: hoisted, they
@@ -471,42 +499,46 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives its LDS
 }
 
+// The tile forms.  The large ones have the fewest operand bytes per product, the small
+// ones the most workgroups, and those with groups of waves over K the most of a
+// workgroup's blocks in flight.
 struct Tile {
-    int ni, mj, ns;
-    float step, ends;  // measured, us: a block of K with every CU busy, and a tile's ends
+    int ni, mj, ns, kg;
+    // measured, us: a block of K with one tile at work and with every CU busy, and a tile's ends
+    float alone, full, ends;
 };
-constexpr Tile FAST[] = {{4, 4, 2, 1.0f, 6.f}, {4, 3, 2, 0.8f, 6.f}, {4, 2, 3, 0.55f, 5.f}, {2, 3, 3, 0.45f, 5.f},
-                         {2, 2, 4, 0.32f, 4.f}, {2, 1, 4, 0.22f, 4.f}, {1, 1, 4, 0.15f, 3.f}};
-constexpr Tile FULL[] = {{4, 2, 3, 1.0f, 6.f}, {2, 2, 4, 0.5f, 5.f}, {2, 1, 4, 0.3f, 4.f}, {1, 1, 4, 0.2f, 3.f}};
+constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.34f, 6.0f}, {4, 3, 2, 1, 0.88f, 0.97f, 5.0f}, {2, 3, 3, 1, 0.55f, 0.62f, 4.3f},
+                         {2, 2, 4, 1, 0.43f, 0.47f, 4.1f}, {2, 1, 3, 2, 0.25f, 0.31f, 4.3f}, {1, 1, 4, 2, 0.18f, 0.25f, 3.9f},
+                         {1, 1, 2, 4, 0.15f, 0.22f, 4.2f}};
+constexpr Tile FULL[] = {{4, 2, 3, 1, 1.46f, 1.63f, 5.0f}, {2, 2, 2, 2, 0.65f, 0.75f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.46f, 5.5f},
+                         {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
 
-long tiles_of(const Fp8Gemm& p, const Tile& t) {
-    return ((long)p.N + 64 * t.ni - 1) / (64 * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
-}
-// rounds of one tile per CU, the last at 0.7 of a full round plus 0.3 of its share (as for the bf16 GEMM)
+// Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
+// round plus 0.3 of its share (as for the bf16 GEMM).  Of the forms above and five others
+// that were timed on 24 products of 58 to 5498 rows it takes the fastest or one within 5 %.
 float tile_cost(const Fp8Gemm& p, const Tile& t, int cus) {
-    const float r = (float)tiles_of(p, t) / cus;
+    const long tiles = ((long)p.N + 64 * t.ni - 1) / (64 * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
+    const float r = (float)tiles / cus, share = r < 1.f ? r : 1.f;
     const float rounds = r <= 1.f ? 1.f : 0.7f * (float)(long)(r + 0.9999f) + 0.3f * r;
-    return rounds * (t.step * (float)(p.K / 128) + t.ends);
+    return rounds * ((t.alone + (t.full - t.alone) * share) * (float)(p.K / 128) + t.ends);
 }
 
-template <int MJ>
-void few_launch(Fp8Gemm& p, hipStream_t s) {
-    constexpr int WAVES = 8;
-    p.n_tiles = (p.N + 15) / 16;
-    p.m_tiles = (p.M + 16 * MJ - 1) / (16 * MJ);
-    hipLaunchKernelGGL((gemm_fp8_few_kernel<MJ, WAVES>), dim3(p.n_tiles * p.m_tiles), dim3(64 * WAVES), 0, s, p);
+template <int NI, int WAVES>
+void few_launch(const Fp8Gemm& p, hipStream_t s) {
+    hipLaunchKernelGGL((gemm_fp8_few_kernel<NI, WAVES>), dim3((p.N + 16 * NI - 1) / (16 * NI)), dim3(64 * WAVES), 0, s, p);
 }
 
 }  // namespace
 
 hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
-    if (p.M <= 64) {
-        if (p.M <= 16) few_launch<1>(p, s);
-        else if (p.M <= 32) few_launch<2>(p, s);
-        else few_launch<4>(p, s);
+    const int cus = device_cus();
+    if (p.M <= 16) {
+        // 32 features a workgroup where they leave one for every other CU (1 row, K = 2560: 5120
+        // features 7.7 us against 8.3, 2560 features 5.1 against 3.9)
+        if ((p.N + 31) / 32 >= cus / 2) few_launch<2, 4>(p, s);
+        else few_launch<1, 8>(p, s);
         return hipGetLastError();
     }
-    const int cus = device_cus();
     const Tile* t = p.c_f32 ? FULL : FAST;
     const Tile* end = p.c_f32 ? FULL + sizeof(FULL) / sizeof(Tile) : FAST + sizeof(FAST) / sizeof(Tile);
     for (const Tile* x = t + 1; x < end; x++)
@@ -515,23 +547,23 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     p.m_tiles = (p.M + 64 * t->mj - 1) / (64 * t->mj);
     // two-stage forms: a workgroup per CU walks its tiles
     const long tiles = (long)p.n_tiles * p.m_tiles;
-    const dim3 grid(xcd_grid(t->ns == 2 && tiles > cus ? cus : tiles)), block(256);
-#define TILE(E, NI, MJ, NS)                                                     \
-    if (p.c_f32 == E && t->ni == NI && t->mj == MJ) {                           \
-        hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS>), grid, block, 0, s, p); \
-        return hipGetLastError();                                               \
+    const dim3 grid(xcd_grid(t->ns == 2 && t->kg == 1 && tiles > cus ? cus : tiles)), block(256 * t->kg);
+#define TILE(E, NI, MJ, NS, KG)                                                         \
+    if (p.c_f32 == E && t->ni == NI && t->mj == MJ && t->kg == KG) {                   \
+        hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS, KG>), grid, block, 0, s, p); \
+        return hipGetLastError();                                                       \
     }
-    TILE(0, 4, 4, 2)
-    TILE(0, 4, 3, 2)
-    TILE(0, 4, 2, 3)
-    TILE(0, 2, 3, 3)
-    TILE(0, 2, 2, 4)
-    TILE(0, 2, 1, 4)
-    TILE(0, 1, 1, 4)
-    TILE(1, 4, 2, 3)
-    TILE(1, 2, 2, 4)
-    TILE(1, 2, 1, 4)
-    TILE(1, 1, 1, 4)
+    TILE(0, 4, 4, 2, 1)
+    TILE(0, 4, 3, 2, 1)
+    TILE(0, 2, 3, 3, 1)
+    TILE(0, 2, 2, 4, 1)
+    TILE(0, 2, 1, 3, 2)
+    TILE(0, 1, 1, 4, 2)
+    TILE(0, 1, 1, 2, 4)
+    TILE(1, 4, 2, 3, 1)
+    TILE(1, 2, 2, 2, 2)
+    TILE(1, 2, 1, 3, 2)
+    TILE(1, 1, 1, 2, 4)
 #undef TILE
     return hipErrorInvalidValue;
 }

@@ -159,7 +159,8 @@ def gemm_bar(va, vw, ref, dtype, k):
 SIZES = [(1, 1, 128), (1, 7680, 2560), (2, 130, 640), (15, 257, 384), (16, 16, 512), (17, 2560, 1664), (31, 100, 128),
          (33, 129, 512), (58, 7680, 2560), (64, 256, 6912), (65, 384, 1024), (127, 511, 256), (129, 1000, 640),
          (257, 513, 896), (300, 2560, 512), (679, 2560, 6912), (1000, 1536, 2560), (1237, 1999, 2816),
-         (2100, 5120, 384), (4440, 2560, 256)]
+         (2100, 5120, 384), (4440, 2560, 256), (671, 7601, 640), (700, 3000, 256), (2500, 7681, 256), (6000, 4104, 384),
+         (1300, 20001, 128)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -366,6 +367,31 @@ def test_rope_gradient(awa, ctx, layout):
         up, down = ctx.rope(x + e, pos, f, **args).double(), ctx.rope(x - e, pos, f, **args).double()
         d = ((up - down) / 2 * g.double()).sum(-1)
         assert float((d - grad[..., i].double()).abs().max()) <= 20 * 4 * 13 * 2.0 ** -21
+
+
+# ------------------------------------------------------------------ far apart
+
+def test_offsets_past_32_bits(awa, ctx):
+    """Rows of a buffer of 9 GB (elements past 2^32, bytes past 2^33)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(6)
+    buf = torch.empty(4400 * 2 ** 20, dtype=torch.bfloat16, device="cuda")
+    rows = buf.view(4400, 2 ** 20)
+    x = torch.randn((4400, 200), generator=g, device="cuda").bfloat16()
+    rows[:, 1000:1200] = x
+    q, s = ctx.quant_fp8(rows[:, 1000:1200])
+    wq, ws = ctx.quant_fp8(x)
+    assert torch.equal(q.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(s.view(torch.uint8), ws.view(torch.uint8))
+    w = ctx.quant_fp8(torch.randn((300, 200), generator=g, device="cuda"), blocks=True)
+    want = ctx.gemm_fp8(q, s, *w)
+    assert torch.equal(ctx.gemm_fp8(q, s, *w, out=rows[:, 5:305]), want) and torch.equal(rows[:, 1000:1200], x)
+    h = rows[:, 2000:2192].unflatten(1, (3, 64))
+    h.copy_(want[:, :192].unflatten(1, (3, 64)))
+    pos = torch.arange(4400, dtype=torch.int32, device="cuda")
+    for layout in ("half", "interleaved"):
+        ref = ctx.rope(h.contiguous(), pos, awa.rope_freqs(32), layout=layout)
+        ctx.rope(h, pos, awa.rope_freqs(32), layout=layout, out=h)
+        assert torch.equal(h, ref)
 
 
 # ------------------------------------------------------------------ together
