@@ -84,7 +84,7 @@ int dit_gemm_fp8(awa_ctx* ctx, const uint8_t* d_a, const uint32_t* d_as, int64_t
  * (DIT_ROPE_HALF); channels from 2 pairs on pass through unchanged.
  */
 enum { DIT_ROPE_INTERLEAVED = 0, DIT_ROPE_HALF = 1 };
-enum { DIT_ROPE_MAX_PAIRS = 128, DIT_ROPE_MAX_AXES = 4 };
+enum { DIT_ROPE_MAX_PAIRS = 128, DIT_ROPE_MAX_AXES = 4, DIT_ROPE_MAX_FREQ = 65536 };
 
 typedef struct {
     int layout;                        /* DIT_ROPE_INTERLEAVED or DIT_ROPE_HALF               */
@@ -92,7 +92,8 @@ typedef struct {
     int pairs[DIT_ROPE_MAX_AXES];      /* pairs that turn with each axis, axis after axis     */
     int inverse;                       /* 1: the angles negated (the adjoint: gradients)      */
     double scale;                      /* factor of cos and sin (1, or a long context's)      */
-    double freq[DIT_ROPE_MAX_PAIRS];   /* radians per position, pair after pair               */
+    double freq[DIT_ROPE_MAX_PAIRS];   /* radians per position, pair after pair; each within
+                                          DIT_ROPE_MAX_FREQ either way                        */
 } dit_rope_plan;
 
 /* One tensor of the call: heads x head_d channels per token.  Strides count
@@ -110,7 +111,7 @@ typedef struct {
  * The plan is copied before the call returns.  Angles are reduced to a turn in
  * fp64, so far positions keep their precision; products are fp32, rounded once.
  * n_tokens may be 0.  Rejected (AWA_EARG): over 32767 heads, head_d over 256 or under twice the
- * pairs, frequencies or a scale that are not finite, negative strides, outputs
+ * pairs, frequencies out of range, a scale that is not finite, negative strides, outputs
  * whose elements could coincide, with each other's or with an input's, other than
  * out = x with the same strides (views of one buffer are accepted where equal
  * token or head strides keep them apart: q, k and v parts of a row). */

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -60,19 +61,10 @@ ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "bands": 3}
 
 
-class RopePlan(C.Structure):
-    """dit_rope_plan of include/dit_ops.h."""
-    _fields_ = [("layout", C.c_int), ("axes", C.c_int), ("pairs", C.c_int * ROPE_MAX_AXES), ("inverse", C.c_int),
-                ("scale", C.c_double), ("freq", C.c_double * ROPE_MAX_PAIRS)]
-
-
-class RopeRows(C.Structure):
-    """dit_rope_rows of include/dit_ops.h."""
-    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int)] + [
-        (n, C.c_int64) for n in ("x_token", "x_head", "out_token", "out_head")]
-
-
-_RopeRows2 = RopeRows * 2
+# dit_rope_plan of include/dit_ops.h up to its frequencies, and dit_rope_rows
+_PLAN = struct.Struct("@7i4xd")
+_NO_PAIRS, _NO_FREQS = (0,) * ROPE_MAX_AXES, bytes(8 * ROPE_MAX_PAIRS)
+_ROWS = struct.Struct("@PPi4x4q")
 
 
 class GeomInfo(C.Structure):
@@ -174,7 +166,7 @@ def lib():
         L.dit_quant_fp8.argtypes = [vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int64, vp]
         L.dit_gemm_fp8.argtypes = [vp, vp, vp, C.c_int64, vp, vp, C.c_int64, vp, C.c_int, vp, C.c_int64, C.c_int,
                                    C.c_int, C.c_int, vp]
-        L.dit_rope.argtypes = [vp, C.c_int, C.POINTER(RopeRows), C.c_int, C.c_int, C.c_int, C.POINTER(RopePlan), vp, vp]
+        L.dit_rope.argtypes = [vp, C.c_int, C.c_char_p, C.c_int, C.c_int, C.c_int, C.c_char_p, vp, vp]
         L.dit_rope_freqs.argtypes = [C.c_int, C.c_int] + 5 * [C.c_double] + [vp]
         _torch, _storage = torch, {torch.float32: AWA_F32, torch.bfloat16: AWA_BF16}
         _e4m3, _e8m0 = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
@@ -620,9 +612,9 @@ class Context:
             raise ValueError(f"rope: layout must be one of {list(ROPE_LAYOUTS)}")
         if positions.get_device() != self.device:
             raise self._elsewhere("rope", positions)
-        plan = RopePlan(ROPE_LAYOUTS[layout], axes, pairs, 1 if inverse else 0, scale)
-        C.memmove(C.byref(plan, RopePlan.freq.offset), f.ctypes.data, 8 * f.size)
-        rows, made, res = _RopeRows2(), (), []
+        plan = b"".join((_PLAN.pack(ROPE_LAYOUTS[layout], axes, *pairs, *_NO_PAIRS[axes:], 1 if inverse else 0, scale),
+                         f.tobytes(), _NO_FREQS[8 * f.size:]))
+        rows, made, res = b"", (), []
         for i, t in enumerate(xs):
             ts = t.stride()
             if t.dim() != 3 or t.dtype != first.dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
@@ -638,7 +630,7 @@ class Context:
                 raise self._elsewhere("rope", t)
             res.append(o)
             os_ = o.stride()
-            rows[i] = (t.data_ptr(), o.data_ptr(), t.shape[1], ts[0], ts[1], os_[0], os_[1])
+            rows += _ROWS.pack(t.data_ptr(), o.data_ptr(), t.shape[1], ts[0], ts[1], os_[0], os_[1])
         rc = lib_.dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, plan, positions.data_ptr(),
                            self._stream(stream, *made))
         if rc:

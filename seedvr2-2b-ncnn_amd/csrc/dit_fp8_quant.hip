@@ -13,6 +13,7 @@ namespace awa {
 
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // rows are only known to be aligned to their elements
 typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -94,11 +95,13 @@ __device__ inline void store(const u32x4 (&r)[Piece<T>::N], float inv, uint8_t* 
         int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
         w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], p, true);
     }
+    // past the caches: 5498 x 6912 bf16 24 -> 20 us (the product reads it from memory
+    // either way where it is large)
     if constexpr (Piece<T>::N == 1) {
-        *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+        __builtin_nontemporal_store((u32x2){w[0], w[1]}, reinterpret_cast<u32x2*>(q));
     } else {
-        *reinterpret_cast<uint32_t*>(q) = w[0];
-        *reinterpret_cast<uint32_t*>(q + 64) = w[1];
+        __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t*>(q));
+        __builtin_nontemporal_store(w[1], reinterpret_cast<uint32_t*>(q + 64));
     }
 }
 // column of the lane's piece k inside its block
@@ -115,41 +118,45 @@ __device__ inline void load_block(u32x4 (&r)[Piece<T>::N], const T* row, int col
     }
 }
 
-// A wave takes R rows of one group (512 columns, a scale word a row); the four
-// waves of a workgroup take neighbouring rows, whose words are neighbours too.
+// A wave takes R rows of one group (512 columns, a scale word a row), the four waves of
+// a workgroup neighbouring rows, whose words are neighbours too, and workgroups one
+// after another the groups of the same rows.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = lane & 15, g = blockIdx.y;
-    const int col0 = g * 512 + (lane >> 4) * 128;
-    const int row0 = (blockIdx.x * 4 + wave) * R;
-    if (row0 >= a.M) return;
-    const bool in = col0 < a.kp;  // the last group may have fewer blocks
-    u32x4 r[R][Piece<T>::N];
+    const int c = lane & 15, groups = (a.K + 511) >> 9;
+    const int64_t pieces = ((int64_t)a.M + 4 * R - 1) / (4 * R) * groups;
+    for (int64_t at = blockIdx.x; at < pieces; at += gridDim.x) {
+        const int g = (int)(at % groups), row0 = ((int)(at / groups) * 4 + wave) * R;
+        const int col0 = g * 512 + (lane >> 4) * 128;
+        const bool in = col0 < a.kp;  // the last group may have fewer blocks
+        u32x4 r[R][Piece<T>::N];
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const T* row = reinterpret_cast<const T*>(a.x) + (int64_t)min(row0 + i, a.M - 1) * a.ldx;
-        load_block<T>(r[i], row, col0, in ? a.K : 0, c);
+        for (int i = 0; i < R; i++) {
+            const T* row = reinterpret_cast<const T*>(a.x) + (int64_t)min(row0 + i, a.M - 1) * a.ldx;
+            load_block<T>(r[i], row, col0, in ? a.K : 0, c);
+        }
+        uint32_t word = 0;  // lane i: the word of row row0 + i
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int byte = scale_byte(max16(top_of<T>(r[i])));
+            uint32_t w = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b++) w |= (uint32_t)__builtin_amdgcn_readlane(byte, 16 * b) << (8 * b);
+            if (lane == i) word = w;
+            if (in && row0 + i < a.M)
+                store<T>(r[i], inverse_scale(byte), a.q + (int64_t)(row0 + i) * a.kp + col0 + piece_col<T>(c, 0));
+        }
+        if (lane < R && row0 + lane < a.M) a.scale[g * a.ld_scale + row0 + lane] = word;
     }
-    uint32_t word = 0;  // lane i: the word of row row0 + i
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int byte = scale_byte(max16(top_of<T>(r[i])));
-        uint32_t w = 0;
-#pragma unroll
-        for (int b = 0; b < 4; b++) w |= (uint32_t)__builtin_amdgcn_readlane(byte, 16 * b) << (8 * b);
-        if (lane == i) word = w;
-        if (in && row0 + i < a.M)
-            store<T>(r[i], inverse_scale(byte), a.q + (int64_t)(row0 + i) * a.kp + col0 + piece_col<T>(c, 0));
-    }
-    if (lane < R && row0 + lane < a.M) a.scale[g * a.ld_scale + row0 + lane] = word;
 }
 
 // A workgroup takes a block of 128 x 128: 16 rows a pass, all of it in registers.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_blocks_kernel(QuantArgs a) {
     __shared__ uint32_t tops[4];
-    const int kb = blockIdx.y, nb = blockIdx.x, tid = threadIdx.x;
+    const int kbs = (a.K + 511) / 512 * 4;
+    const int kb = blockIdx.x % kbs, nb = blockIdx.x / kbs, tid = threadIdx.x;
     uint8_t* byte_at = reinterpret_cast<uint8_t*>(a.scale + (kb >> 2) * a.ld_scale + nb) + (kb & 3);
     if (kb * 128 >= a.kp) {  // a byte of the last word without a block
         if (tid == 0) *byte_at = 0;
@@ -181,26 +188,30 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(QuantArgs a) {
     }
 }
 
-template <typename T>
+template <typename T, int R>
 void rows_launch(const QuantArgs& a, hipStream_t s) {
-    const unsigned groups = (a.K + 511) / 512;
-    if ((long)a.M * groups >= 8192) {
-        hipLaunchKernelGGL((quant_rows_kernel<T, 8>), dim3((a.M + 31) / 32, groups), dim3(256), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((quant_rows_kernel<T, 1>), dim3((a.M + 3) / 4, groups), dim3(256), 0, s, a);
-    }
+    const int64_t pieces = ((int64_t)a.M + 4 * R - 1) / (4 * R) * ((a.K + 511) / 512);
+    const unsigned blocks = (unsigned)(pieces < (1 << 22) ? pieces : 1 << 22);
+    hipLaunchKernelGGL((quant_rows_kernel<T, R>), dim3(blocks), dim3(256), 0, s, a);
+}
+// two rows a wave once that leaves 8 workgroups per CU (27258 x 2560 bf16 36.5 us; one row
+// 38.0, four 37.6)
+template <typename T>
+void rows(const QuantArgs& a, hipStream_t s) {
+    if ((int64_t)a.M * ((a.K + 511) / 512) >= 16384) rows_launch<T, 2>(a, s);
+    else rows_launch<T, 1>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_quant_rows(int dtype, const QuantArgs& a, hipStream_t s) {
-    if (dtype == AWA_F32) rows_launch<float>(a, s);
-    else rows_launch<uint16_t>(a, s);
+    if (dtype == AWA_F32) rows<float>(a, s);
+    else rows<uint16_t>(a, s);
     return hipGetLastError();
 }
 
 hipError_t launch_quant_blocks(int dtype, const QuantArgs& a, hipStream_t s) {
-    const dim3 grid((a.M + 127) / 128, (a.K + 511) / 512 * 4);
+    const dim3 grid((unsigned)((a.M + 127) / 128 * ((a.K + 511) / 512 * 4)));
     if (dtype == AWA_F32) hipLaunchKernelGGL((quant_blocks_kernel<float>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((quant_blocks_kernel<uint16_t>), grid, dim3(256), 0, s, a);
     return hipGetLastError();

@@ -175,11 +175,12 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
         a.axis_end[i] = a.pairs;
     }
     for (int i = 0; i < a.pairs; i++) {
-        if (!std::isfinite(plan->freq[i])) {
-            set_err(ctx, "dit_rope: frequency %d is not finite", i);
+        if (!(std::fabs(plan->freq[i]) <= DIT_ROPE_MAX_FREQ)) {
+            set_err(ctx, "dit_rope: frequency %d is %g (a finite number of at most %d either way)", i, plan->freq[i],
+                    DIT_ROPE_MAX_FREQ);
             return AWA_EARG;
         }
-        a.turns[i] = plan->freq[i] / (2.0 * M_PI);
+        a.quarters[i] = plan->freq[i] / (0.5 * M_PI);
     }
     a.axes = plan->axes;
     a.cos_scale = (float)plan->scale;
@@ -227,14 +228,13 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
     }
     for (int t = 0; t < n_rows; t++) {
         if (rows[t].heads == 0) continue;
-        const int i = a.heads0 ? 1 : 0;
+        const int i = a.heads[0] ? 1 : 0;
         a.x[i] = rows[t].x; a.out[i] = rows[t].out;
         a.x_token[i] = rows[t].x_token; a.x_head[i] = rows[t].x_head;
         a.out_token[i] = rows[t].out_token; a.out_head[i] = rows[t].out_head;
-        if (i == 0) a.heads0 = rows[t].heads;
-        a.heads += rows[t].heads;
+        a.heads[i] = rows[t].heads;
     }
-    if (n_tokens == 0 || a.heads == 0) return AWA_OK;
+    if (n_tokens == 0 || a.heads[0] == 0) return AWA_OK;
     a.copy = !in_place;
     DeviceGuard dg(ctx->device);
     HIPCK(ctx, launch_rope(dtype, plan->layout, a, reinterpret_cast<hipStream_t>(stream)));

@@ -38,16 +38,16 @@ struct RopeArgs {
     const void* x[2];
     void* out[2];
     int64_t x_token[2], x_head[2], out_token[2], out_head[2];
-    int heads0, heads;       // of the first tensor, of both
+    int heads[2];
     int tokens, head_d;
     int pairs;               // rotated pairs, all axes
     int axes, axis_end[DIT_ROPE_MAX_AXES];  // pairs up to each axis's end
     int copy;                // channels past the pairs go from x to out (not in place)
     int rot_units, units;    // pieces of a head that turn, and all; filled by launch_rope
-    int heads_per_block;
+    int lanes[2];            // threads per token and piece, each with every lanes-th head; likewise
     const int32_t* pos;
     float cos_scale, sin_scale;
-    double turns[DIT_ROPE_MAX_PAIRS];  // turns per position
+    double quarters[DIT_ROPE_MAX_PAIRS];  // quarter turns per position
 };
 hipError_t launch_rope(int dtype, int layout, RopeArgs& a, hipStream_t s);
 

@@ -133,7 +133,7 @@ int main() {
     check("rope no tokens", rope({q}, 0), ok, 0);
     check("rope no heads", rope({rows(X, X, 0, 0, 0, 0, 0)}), ok, 0);
     check("rope no heads of the first", (rope({rows(nullptr, nullptr, 0, 0, 0, 0, 0), k})), ok);
-    if (last_rope.heads != 4 || last_rope.heads0 != 4 || last_rope.x[0] != k.x) { failures++; printf("FAILED second alone\n"); }
+    if (last_rope.heads[0] != 4 || last_rope.heads[1] != 0 || last_rope.x[0] != k.x) { failures++; printf("FAILED second alone\n"); }
     check("rope heads outside tokens", rope({rows(X, X, 4, 64, 640, 64, 640)}), ok);
     check("rope per head q|k|v", rope({rows(X, X, 4, 768, 192, 768, 192), rows(X + 256, X + 256, 4, 768, 192, 768, 192)}), ok);
     check("rope into other columns", rope({rows(X, X + 2048, 4, 768, 64, 768, 64)}), ok);
@@ -177,6 +177,7 @@ int main() {
     with("rope pairs over the head", [](dit_rope_plan& p) { p.pairs[1] = 17; });
     with("rope pairs overflow", [](dit_rope_plan& p) { p.pairs[1] = std::numeric_limits<int>::max(); });
     with("rope infinite frequency", [](dit_rope_plan& p) { p.freq[23] = INFINITY; });
+    with("rope large frequency", [](dit_rope_plan& p) { p.freq[1] = -65537.0; });
     with("rope NaN frequency", [](dit_rope_plan& p) { p.freq[0] = NAN; });
     with("rope infinite scale", [](dit_rope_plan& p) { p.scale = 1e300; });
 

@@ -303,7 +303,7 @@ def test_rope_quarter_turns(awa, ctx, layout):
     """Angles at and around the borders of the reduction: multiples of a sixteenth turn."""
     import torch
     pos = torch.arange(-40, 41, dtype=torch.int32, device="cuda")
-    freqs = np.array([2 * np.pi / 16, 2 * np.pi / 16 * (1 + 2.0 ** -40), 0.0, 2 * np.pi])
+    freqs = np.array([2 * np.pi / 16, -2 * np.pi / 16 * (1 + 2.0 ** -40), 0.0, 2 * np.pi])
     x = torch.randn((81, 2, 8), device="cuda")
     ref, bar = plain_rope(x, pos, freqs, (4,), layout, 1.0, False)
     within(ctx.rope(x, pos, freqs, layout=layout), ref, bar + 2.0 ** -24 * ref.abs())
