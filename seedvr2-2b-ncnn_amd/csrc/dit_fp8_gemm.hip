@@ -186,10 +186,11 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
 #pragma unroll
         for (int j = 0; j < MJ; j++) {
 #pragma unroll
-            for (int f = 0; f < FW; f++)
+            for (int f = 0; f < FW; f++) {
+                f32x16 x = acc[i0 + f][j];
+                asm volatile("" : "+a"(x));  // read here, not all of them ahead of the branches
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const f32x16& x = acc[i0 + f][j];
                     f32x4 v = {x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
                     if constexpr (BIAS) v += b[f][t];
                     if constexpr (F32) {
@@ -199,6 +200,7 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
                             make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
                     }
                 }
+            }
             if (vec) {
                 u32x4 v[STEPS];
 #pragma unroll
@@ -331,7 +333,9 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     f32x16 acc[NI][MJ];
     // fragment rows: blocks of 32 rows are 4 KiB apart and have the same swizzle
     const int wrow = (wn * 32 * NI + c) * ROW, arow = BN * ROW + (wm * 32 * MJ + c) * ROW, sx = (c >> 1) & 7;
-    i32x8 wf[2][NI], af[2][MJ];
+    // EXACT widens a fragment before the next half's is read into its registers
+    constexpr int BUFS = EXACT ? 1 : 2;
+    i32x8 wf[BUFS][NI], af[BUFS][MJ];
     int sw, sa[MJ], sw_next = 0, sa_next[MJ];
     // piece x of the fragments of half s of a stage (into buffer buf): two chunks of a row each
     auto read_piece = [&](int slot, int s, int buf, int x) __attribute__((always_inline)) {
@@ -355,25 +359,29 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
 #pragma unroll
         for (int j = 0; j < MJ; j++) sa[j] = sa_next[j] >> sh;
     };
-    // One half block on fragment buffer `buf`; between its instructions, when `read`, the
-    // reads of the next half (slot rslot, half rs, into buffer buf ^ 1) and, when `dma`, the DMA
+    // One half block (of: 0 or 1 of its stage); between its instructions, when `read`, the
+    // reads of the next half (slot rslot, half rs) and, when `dma`, the DMA
     // pieces of the next stage into slot dma_slot, spread evenly: an instruction of 64
     // cycles hides one read and one piece, not two (5498 x 13824 x 2560 188 us with them
     // in the first eight of sixteen, 175 so).
-    auto half = [&](int buf, int rslot, int rs, bool read, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
-        bf16x8 wb[EXACT ? NI : 1][4], ab[EXACT ? MJ : 1][4];
+    auto half = [&](int of, int rslot, int rs, bool read, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
+        const int buf = of % BUFS, rbuf = (of + 1) % BUFS;
+        // EXACT: fragments widen while the instructions before their first use run (all of
+        // them ahead of the half: 5498 x 13824 x 2560 375 us, so 358)
+        bf16x8 wb[2][4], ab[MJ][4];
+        auto widen_w = [&](int i) __attribute__((always_inline)) {
+            const float f = scale_of(sw & 0xff);
+#pragma unroll
+            for (int e = 0; e < 4; e++) wb[i & 1][e] = widen(wf[buf][i][2 * e], wf[buf][i][2 * e + 1], f);
+        };
+        auto widen_a = [&](int j) __attribute__((always_inline)) {
+            const float f = scale_of(sa[j] & 0xff);
+#pragma unroll
+            for (int e = 0; e < 4; e++) ab[j][e] = widen(af[buf][j][2 * e], af[buf][j][2 * e + 1], f);
+        };
         if constexpr (EXACT) {
-            const float fw = scale_of(sw & 0xff);
-#pragma unroll
-            for (int i = 0; i < NI; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) wb[i][e] = widen(wf[buf][i][2 * e], wf[buf][i][2 * e + 1], fw);
-#pragma unroll
-            for (int j = 0; j < MJ; j++) {
-                const float fa = scale_of(sa[j] & 0xff);
-#pragma unroll
-                for (int e = 0; e < 4; e++) ab[j][e] = widen(af[buf][j][2 * e], af[buf][j][2 * e + 1], fa);
-            }
+            widen_w(0);
+            widen_a(0);
         }
         constexpr int T = NI * MJ;
 #pragma unroll
@@ -383,18 +391,23 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
 #pragma unroll
             for (int e = 0; e < 16; e++) z[e] = 0.f;
             if constexpr (EXACT) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i][0], ab[j][0], zc ? z : acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i & 1][0], ab[j][0], zc ? z : acc[i][j], 0, 0, 0);
 #pragma unroll
                 for (int e = 1; e < 4; e++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i][e], ab[j][e], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[i & 1][e], ab[j][e], acc[i][j], 0, 0, 0);
+                if (i == 0 && j + 1 < MJ) widen_a(j + 1);
+                if (j + 1 == MJ && i + 1 < NI) widen_w(i + 1);
             } else {
                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[buf][i], af[buf][j], zc ? z : acc[i][j], 0, 0, 0,
                                                                            sw, 0, sa[j]);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < NR; e++)
-                if (read && e * T / NR == x) read_piece(rslot, rs, buf ^ 1, e);
+            for (int e = 0; e < NR; e++) {
+                // EXACT: W's first fragment, A's, W's others, as they fall free
+                const int k = e >> 1, f = !EXACT ? k : k == 0 ? 0 : k <= MJ ? NI + k - 1 : k - MJ;
+                if (read && e * T / NR == x) read_piece(rslot, rs, rbuf, 2 * f + (e & 1));
+            }
 #pragma unroll
             for (int e = 0; e < NP; e++)
                 if (dma && e * T / NP == x) load_piece(dma_slot, e);
@@ -510,8 +523,8 @@ struct Tile {
 constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.34f, 6.0f}, {4, 3, 2, 1, 0.88f, 0.97f, 5.0f}, {2, 3, 3, 1, 0.55f, 0.62f, 4.3f},
                          {2, 2, 4, 1, 0.43f, 0.47f, 4.1f}, {2, 1, 3, 2, 0.25f, 0.31f, 4.3f}, {1, 1, 4, 2, 0.18f, 0.25f, 3.9f},
                          {1, 1, 2, 4, 0.15f, 0.22f, 4.2f}};
-constexpr Tile FULL[] = {{4, 2, 3, 1, 1.46f, 1.63f, 5.0f}, {2, 2, 2, 2, 0.65f, 0.75f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.46f, 5.5f},
-                         {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
+constexpr Tile FULL[] = {{4, 4, 2, 1, 2.16f, 2.65f, 9.0f}, {4, 3, 2, 1, 1.69f, 1.92f, 6.5f}, {4, 2, 2, 1, 1.26f, 1.47f, 6.0f},
+                         {2, 2, 2, 2, 0.62f, 0.76f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
 
 // Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
 // round plus 0.3 of its share (as for the bf16 GEMM).  Of the forms above and five others
@@ -560,7 +573,9 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     TILE(0, 2, 1, 3, 2)
     TILE(0, 1, 1, 4, 2)
     TILE(0, 1, 1, 2, 4)
-    TILE(1, 4, 2, 3, 1)
+    TILE(1, 4, 4, 2, 1)
+    TILE(1, 4, 3, 2, 1)
+    TILE(1, 4, 2, 2, 1)
     TILE(1, 2, 2, 2, 2)
     TILE(1, 2, 1, 3, 2)
     TILE(1, 1, 1, 2, 4)

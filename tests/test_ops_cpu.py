@@ -72,3 +72,10 @@ def test_binding_refuses_host_tensors(awa):
     for call in (lambda: ctx.quant_fp8(x.half()), lambda: ctx.rope(x[:, None].half(), pos, [1.0])):
         with pytest.raises(TypeError):
             call()
+
+
+def test_product_reads_sums_after_their_wait_states(tmp_path):
+    """The static check of the other matrix kernels over the 8-bit product's: its sums pass through empty asm
+    statements, which the compiler does not wait before."""
+    import test_sdpa_asm
+    test_sdpa_asm.test_other_mfma_kernels_wait_states(tmp_path, "dit_fp8_gemm")
