@@ -518,6 +518,20 @@ class Context:
         if t.get_device() != self.device:
             raise self._elsewhere(what, t)
 
+    def _scale_ld(self, what, t, name, groups, rows):
+        """Words from group to group of a scale tensor [groups, rows, 4], cut from a wider one or not."""
+        if t.dtype not in _e8m0 or t.shape != (groups, rows, 4):
+            raise ValueError(f"{what}: {name} must be a {str(_e8m0[0])[6:]} tensor [{groups}, {rows}, 4], got "
+                             f"{str(t.dtype)[6:]} {list(t.shape)}")
+        if t.get_device() != self.device:
+            raise self._elsewhere(what, t)
+        if t.is_contiguous():
+            return rows
+        g, r, b = t.stride()
+        if b != 1 or (rows > 1 and r != 4) or g % 4 or g < 4 * rows:
+            raise ValueError(f"{what}: {name} must be whole words of contiguous rows, got strides {t.stride()}")
+        return g // 4
+
     def quant_fp8(self, x, blocks=False, q=None, scale=None, stream=None):
         """dit_quant_fp8: x [rows, cols] bf16 or fp32 (columns contiguous) to (q, scale): q float8_e4m3fn
         [rows, cols padded to 128], scale float8_e8m0fnu [groups of four column blocks, rows, 4] (blocks=True:
@@ -550,17 +564,21 @@ class Context:
 
     def gemm_fp8(self, a, a_scale, w, w_scale, bias=None, out=None, dtype=None, stream=None):
         """dit_gemm_fp8: [M, N] = A W^T (+ bias fp32 [N]) of matrices as quant_fp8 returns them, A by rows and W
-        with blocks=True; `dtype` bf16 (default) or fp32, or that of `out` (rows may be strided)."""
+        with blocks=True, or of rows cut from them (a[i:j], a_scale[:, i:j]); `dtype` bf16 (default) or fp32, or that
+        of `out` (rows may be strided)."""
         lib_ = lib()
         if a.dim() != 2 or w.dim() != 2:
             raise ValueError("gemm_fp8: a [M, K] and w [N, K]")
         M, K = a.shape
         N = w.shape[0]
         groups, nb = (K + 511) // 512, (N + 127) // 128
-        self._bytes_of("gemm_fp8", a, "a", _e4m3, M, K)
-        self._bytes_of("gemm_fp8", w, "w", _e4m3, N, K)
-        self._bytes_of("gemm_fp8", a_scale, "a_scale", _e8m0, groups, M, 4)
-        self._bytes_of("gemm_fp8", w_scale, "w_scale", _e8m0, groups, nb, 4)
+        dev = self.device
+        if not (a.dtype in _e4m3 and w.dtype in _e4m3 and w.shape[1] == K and a.is_contiguous() and w.is_contiguous() and
+                a.get_device() == dev and w.get_device() == dev):
+            self._bytes_of("gemm_fp8", a, "a", _e4m3, M, K)
+            self._bytes_of("gemm_fp8", w, "w", _e4m3, N, K)
+        ld_as = self._scale_ld("gemm_fp8", a_scale, "a_scale", groups, M)
+        ld_ws = self._scale_ld("gemm_fp8", w_scale, "w_scale", groups, nb)
         made = ()
         if out is None:
             out = a.new_empty((M, N), dtype=dtype or _torch.bfloat16)
@@ -576,7 +594,7 @@ class Context:
             if bias.get_device() != self.device:
                 raise self._elsewhere("gemm_fp8", bias)
         if M:
-            rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), M, w.data_ptr(), w_scale.data_ptr(), nb,
+            rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), ld_as, w.data_ptr(), w_scale.data_ptr(), ld_ws,
                                    bias.data_ptr() if bias is not None else None, ct, out.data_ptr(), out.stride(0), M, N,
                                    K, self._stream(stream, *made))
             if rc:

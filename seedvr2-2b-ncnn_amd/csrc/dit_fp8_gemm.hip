@@ -201,26 +201,28 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
                     }
                 }
             }
-            if (vec) {
-                u32x4 v[STEPS];
+            u32x4 v[STEPS];
 #pragma unroll
-                for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+            for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+            if (vec) {
 #pragma unroll
                 for (int u = 0; u < STEPS; u++)
                     __builtin_amdgcn_raw_buffer_store_b128(v[u], cres, ofs0 + (32 * j + RPI * u) * row_bytes, 0, 0);
             } else {
                 // rows at any alignment: whole chunks as they are, the last one of a row in elements
                 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+                uint8_t* to = crow + ((32 * j + r0) * p.ldc + n) * SZ;
+                const bool whole = n + EPC <= p.N;
+#pragma unroll
+                for (int u = 0; u < STEPS; u++, to += RPI * p.ldc * SZ)
+                    if (whole && 32 * j + RPI * u + r0 < rows) *reinterpret_cast<u32x4_u*>(to) = v[u];
+                if (!whole && n < p.N) {
 #pragma unroll 1
-                for (int r = r0; r < min(rows - 32 * j, 32); r += RPI) {
-                    uint8_t* to = crow + ((32 * j + r) * p.ldc + n) * SZ;
-                    const uint8_t* from = at(r, k);
-                    if (n + EPC <= p.N) {
-                        *reinterpret_cast<u32x4_u*>(to) = *reinterpret_cast<const u32x4*>(from);
-                    } else {
+                    for (int r = r0; r < min(rows - 32 * j, 32); r += RPI) {
+                        to = crow + ((32 * j + r) * p.ldc + n) * SZ;
 #pragma unroll 1
                         for (int e = 0; e < (p.N - n) * (SZ / 2); e++)
-                            reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+                            reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(at(r, k))[e];
                     }
                 }
             }
@@ -360,11 +362,11 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         for (int j = 0; j < MJ; j++) sa[j] = sa_next[j] >> sh;
     };
     // One half block (of: 0 or 1 of its stage); between its instructions, when `read`, the
-    // reads of the next half (slot rslot, half rs) and, when `dma`, the DMA
-    // pieces of the next stage into slot dma_slot, spread evenly: an instruction of 64
-    // cycles hides one read and one piece, not two (5498 x 13824 x 2560 188 us with them
-    // in the first eight of sixteen, 175 so).
-    auto half = [&](int of, int rslot, int rs, bool read, bool dma, int dma_slot, bool zc) __attribute__((always_inline)) {
+    // reads of the next half (slot rslot, half rs) and pieces d0 .. d1 - 1 of the next
+    // stage's DMA into slot dma_slot, spread evenly: an instruction of 64 cycles hides one
+    // read and one piece, not two (5498 x 13824 x 2560 188 us with them in the first eight
+    // of sixteen, 175 so).
+    auto half = [&](int of, int rslot, int rs, bool read, int d0, int d1, int dma_slot, bool zc) __attribute__((always_inline)) {
         const int buf = of % BUFS, rbuf = (of + 1) % BUFS;
         // EXACT: fragments widen while the instructions before their first use run (all of
         // them ahead of the half: 5498 x 13824 x 2560 375 us, so 358)
@@ -409,8 +411,8 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
                 if (read && e * T / NR == x) read_piece(rslot, rs, rbuf, 2 * f + (e & 1));
             }
 #pragma unroll
-            for (int e = 0; e < NP; e++)
-                if (dma && e * T / NP == x) load_piece(dma_slot, e);
+            for (int e = d0; e < d1; e++)
+                if ((e - d0) * T / (d1 - d0) == x) load_piece(dma_slot, e);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -422,17 +424,29 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     // the next stage's first fragments and refills this slot with the stage NS on.
     int slot = 0;
     auto next = [](int t) __attribute__((always_inline)) { return t + 1 == NS ? 0 : t + 1; };
-    auto stage = [&](int st, bool zc) __attribute__((always_inline)) {
-        half(0, slot, 1, true, false, 0, zc);
+    // With three stages or more the refill goes on through half 0 of the next stage (`more`:
+    // there is one to go on with), an even stream in place of a burst that the pieces of four
+    // waves queue up in (679 x 2560 x 6912 in 128 x 128 tiles 27.1 -> 23.5 us).
+    constexpr int NP1 = NS > 2 ? NP / 2 : NP;
+    // The sums stay where they are formed: the compiler would move the instructions whose
+    // results no one reads yet past the branch of fetch_next, behind all the loads between.
+    auto pin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < NI * MJ; x++) asm volatile("" : "+a"(acc[x / MJ][x % MJ]));
+    };
+    auto stage = [&](int st, bool zc, bool more) __attribute__((always_inline)) {
+        const int before = slot == 0 ? NS - 1 : slot - 1;
+        half(0, slot, 1, true, more ? NP1 : NP, NP, before, zc);
+        if (more && NP1 < NP) {
+            pin();
+            fetch_next();
+        }
         wait_vmem_lds<(NS - 2) * NP>();
         __builtin_amdgcn_s_barrier();
         read_scales(next(slot));
-        half(1, next(slot), 0, true, true, slot, false);
-        // the sums stay here: the compiler would move the instructions that no one reads
-        // yet past the branch below, behind all the loads between them
-#pragma unroll
-        for (int x = 0; x < NI * MJ; x++) asm volatile("" : "+a"(acc[x / MJ][x % MJ]));
-        fetch_next();
+        half(1, next(slot), 0, true, 0, NP1, slot, false);
+        pin();
+        if (NP1 == NP) fetch_next();
         take_scales(st + 1 == ns_wrap ? 0 : st + 1);
         slot = next(slot);
     };
@@ -452,18 +466,18 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     while (true) {
         int m0, n0;
         if constexpr (WALK) {
-            stage(0, true);
-            for (int st = 1; st < ns; st++) stage(st, false);
+            stage(0, true, false);
+            for (int st = 1; st < ns; st++) stage(st, false, false);
         } else {
             // no stage follows the last one, which only reads its own second half
             if (ns > 1) {
-                stage(0, true);
-                for (int st = 1; st + 1 < ns; st++) stage(st, false);
-                half(0, slot, 1, true, false, 0, false);
+                stage(0, true, false);
+                for (int st = 1; st + 1 < ns; st++) stage(st, false, NS > 2);
+                half(0, slot, 1, true, NP, NP, 0, false);
             } else {
-                half(0, slot, 1, true, false, 0, true);
+                half(0, slot, 1, true, NP, NP, 0, true);
             }
-            half(1, slot, 0, false, false, 0, false);
+            half(1, slot, 0, false, NP, NP, 0, false);
         }
         place(tile, m0, n0);
         if constexpr (!WALK) {  // the slots are free once every DMA (of nothing, by now) and read is done
@@ -520,9 +534,8 @@ struct Tile {
     // measured, us: a block of K with one tile at work and with every CU busy, and a tile's ends
     float alone, full, ends;
 };
-constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.34f, 6.0f}, {4, 3, 2, 1, 0.88f, 0.97f, 5.0f}, {2, 3, 3, 1, 0.55f, 0.62f, 4.3f},
-                         {2, 2, 4, 1, 0.43f, 0.47f, 4.1f}, {2, 1, 3, 2, 0.25f, 0.31f, 4.3f}, {1, 1, 4, 2, 0.18f, 0.25f, 3.9f},
-                         {1, 1, 2, 4, 0.15f, 0.22f, 4.2f}};
+constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.34f, 6.0f}, {4, 3, 2, 1, 0.88f, 0.97f, 5.0f}, {2, 3, 3, 1, 0.42f, 0.66f, 4.3f},
+                         {2, 2, 4, 1, 0.30f, 0.42f, 4.2f}, {2, 1, 3, 2, 0.19f, 0.29f, 4.0f}, {1, 1, 4, 2, 0.13f, 0.20f, 3.9f}};
 constexpr Tile FULL[] = {{4, 4, 2, 1, 2.16f, 2.65f, 9.0f}, {4, 3, 2, 1, 1.69f, 1.92f, 6.5f}, {4, 2, 2, 1, 1.26f, 1.47f, 6.0f},
                          {2, 2, 2, 2, 0.62f, 0.76f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
 
@@ -572,7 +585,6 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     TILE(0, 2, 2, 4, 1)
     TILE(0, 2, 1, 3, 2)
     TILE(0, 1, 1, 4, 2)
-    TILE(0, 1, 1, 2, 4)
     TILE(1, 4, 4, 2, 1)
     TILE(1, 4, 3, 2, 1)
     TILE(1, 4, 2, 2, 1)

@@ -22,6 +22,8 @@ size_t elem(int dtype) { return dtype == AWA_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == AWA_F32 || dtype == AWA_BF16; }
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 int64_t groups_of(int k) { return ((int64_t)k + 511) / 512; }
+// strides far enough below 2^63 for the checks' own arithmetic
+constexpr int64_t STRIDE_MAX = (int64_t)1 << 36;
 // bytes from the first to past the last element of rows ld elements apart
 size_t span(int64_t rows, int64_t ld, int64_t cols, size_t size) {
     return rows > 0 ? (size_t)((rows - 1) * ld + cols) * size : 0;
@@ -82,8 +84,8 @@ int dit_quant_fp8(awa_ctx* ctx, int dtype, const void* d_x, int64_t ldx, int M, 
         return AWA_EARG;
     }
     const int64_t srows = block_rows == 1 ? M : (M + DIT_FP8_BLOCK - 1) / DIT_FP8_BLOCK;
-    if ((M > 1 && ldx < K) || ld_scale < srows) {
-        set_err(ctx, "dit_quant_fp8: ldx=%lld (at least K=%d), ld_scale=%lld (at least %lld)", (long long)ldx, K,
+    if ((M > 1 && (ldx < K || ldx > STRIDE_MAX)) || ld_scale < srows || ld_scale > STRIDE_MAX) {
+        set_err(ctx, "dit_quant_fp8: ldx=%lld (at least K=%d), ld_scale=%lld (at least %lld; both at most 2^36)", (long long)ldx, K,
                 (long long)ld_scale, (long long)srows);
         return AWA_EARG;
     }
@@ -120,8 +122,9 @@ int dit_gemm_fp8(awa_ctx* ctx, const uint8_t* d_a, const uint32_t* d_as, int64_t
         return AWA_EARG;
     }
     const int64_t nb = (N + DIT_FP8_BLOCK - 1) / DIT_FP8_BLOCK;
-    if ((M > 1 && ldc < N) || ldc > DIT_OPS_COLS_MAX || ld_as < M || ld_ws < nb) {
-        set_err(ctx, "dit_gemm_fp8: ldc=%lld (%d .. %d), ld_as=%lld (at least %d), ld_ws=%lld (at least %lld)",
+    if ((M > 1 && (ldc < N || ldc > DIT_OPS_COLS_MAX)) || ld_as < M || ld_as > STRIDE_MAX || ld_ws < nb ||
+        ld_ws > STRIDE_MAX) {
+        set_err(ctx, "dit_gemm_fp8: ldc=%lld (%d .. %d), ld_as=%lld (at least %d), ld_ws=%lld (at least %lld; both at most 2^36)",
                 (long long)ldc, N, DIT_OPS_COLS_MAX, (long long)ld_as, M, (long long)ld_ws, (long long)nb);
         return AWA_EARG;
     }
@@ -191,8 +194,6 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
     View vx[2], vo[2];
     bool in_place = true;
     const size_t size = elem(dtype);
-    // strides far enough below 2^63 for the checks' own arithmetic
-    constexpr int64_t STRIDE_MAX = (int64_t)1 << 36;
     for (int t = 0; t < n_rows; t++) {
         const dit_rope_rows& r = rows[t];
         if (r.heads < 0 || r.heads > 32767) {

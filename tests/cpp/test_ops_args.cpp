@@ -68,6 +68,8 @@ int main() {
     check("quant too many columns", quant(AWA_BF16, X, 1 << 21, 7, DIT_OPS_COLS_MAX + 1, 1, Q, S, 7), bad);
     check("quant block_rows", quant(AWA_BF16, X, 200, 7, 200, 64, Q, S, 7), bad);
     check("quant ldx", quant(AWA_BF16, X, 199, 7, 200, 1, Q, S, 7), bad);
+    check("quant huge ldx", quant(AWA_BF16, X, (int64_t)1 << 60, 7, 200, 1, Q, S, 7), bad);
+    check("quant huge ld_scale", quant(AWA_BF16, X, 200, 7, 2000, 1, Q, S, (int64_t)1 << 61), bad);
     check("quant ld_scale", quant(AWA_BF16, X, 200, 7, 200, 1, Q, S, 6), bad);
     check("quant ld_scale blocks", quant(AWA_BF16, X, 200, 129, 200, 128, Q, S, 1), bad);
     check("quant q alignment", quant(AWA_BF16, X, 200, 7, 200, 1, Q + 8, S, 7), bad);
@@ -100,6 +102,8 @@ int main() {
     check("gemm K large", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, DIT_OPS_COLS_MAX + 128), bad);
     check("gemm ldc", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16, C, 199, 5, 200, 256), bad);
     check("gemm ldc large", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16, C, DIT_OPS_COLS_MAX + 1, 5, 200, 256), bad);
+    check("gemm huge ld_as", gemm(Q, S, (int64_t)1 << 61, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 1024), bad);
+    check("gemm huge ld_ws", gemm(Q, S, 5, W, SW, (int64_t)1 << 61, nullptr, AWA_BF16, C, 200, 5, 200, 1024), bad);
     check("gemm ld_as", gemm(Q, S, 4, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);
     check("gemm ld_ws", gemm(Q, S, 5, W, SW, 1, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);
     check("gemm a alignment", gemm(Q + 8, S, 5, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);

@@ -232,7 +232,12 @@ def test_gemm_slices(awa, ctx):
                                      torch.cuda.current_stream().cuda_stream), "dit_gemm_fp8")
     ref = va[13:44] @ vw[256:556].T
     within(out, ref, gemm_bar(va[13:44], vw[256:556], ref, torch.float32, 640))
-    assert ctx.gemm_fp8(a[:0], sa[:, :0].contiguous(), w, sw).shape == (0, 600)
+    assert torch.equal(ctx.gemm_fp8(a[13:44], sa[:, 13:44], w[256:556], sw[:, 2:], dtype=torch.float32), out)
+    one = ctx.gemm_fp8(a[20:21], sa[:, 20:21], w[256:300], sw[:, 2:3])
+    within(one, ref[7:8, :44], gemm_bar(va[20:21], vw[256:300], ref[7:8, :44], torch.bfloat16, 640))
+    assert ctx.gemm_fp8(a[:0], sa[:, :0], w, sw).shape == (0, 600)
+    with pytest.raises(ValueError):
+        ctx.gemm_fp8(a[::2], sa[:, ::2], w, sw)
 
 
 # ------------------------------------------------------------------ rotary positions
