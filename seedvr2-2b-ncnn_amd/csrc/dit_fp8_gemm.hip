@@ -526,6 +526,278 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives its LDS
 }
 
+// The same for accumulators of 16 x 16: lane (c = lane % 16, q = lane / 16) of (i, j) holds row
+// 16 j + c (of the other 64 rows, where kind is 1), features 16 i + 4 q + e.
+template <bool BIAS>
+__device__ inline void wide_epilogue(const Fp8Gemm& p, const f32x4 (&acc)[8][8], int n_base, int m_base, int kind, int lane,
+                                     uint8_t* stg) {
+    constexpr int SZ = 2, EPC = 8, RPI = 8, STEPS = 4;
+    auto at = [&](int r, int k) __attribute__((always_inline)) { return stg + r * 128 + ((k ^ ((r >> 1) & 7)) << 4); };
+    const int c = lane & 15, q = lane >> 4, k = lane & 7, r0 = lane >> 3;
+    const bool vec = p.c_vec && p.N % EPC == 0;
+    const int rows = min(max(p.M - m_base, 0), 128);
+    const uint32_t row_bytes = (uint32_t)p.ldc * SZ;
+    uint8_t* crow = reinterpret_cast<uint8_t*>(p.C) + (int64_t)m_base * p.ldc * SZ;
+    const __amdgpu_buffer_rsrc_t cres = uniform_rsrc(crow, (uint32_t)rows * row_bytes);
+#pragma unroll
+    for (int i0 = 0; i0 < 8; i0 += 4) {
+        f32x4 b[4];
+        if constexpr (BIAS) {
+            const __amdgpu_buffer_rsrc_t bres = uniform_rsrc(p.bias, p.N * 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bres, 4u * (n_base + 16 * (i0 + i) + 4 * q), 0, 0));
+        }
+        const int n = n_base + 16 * i0 + k * EPC;
+        const uint32_t ofs0 = n < p.N ? r0 * row_bytes + n * SZ : 0x80000000u;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int rj = 32 * (j ^ 2 * kind);
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    f32x4 v = acc[i0 + i][2 * j + jj];
+                    asm volatile("" : "+a"(v));
+                    if constexpr (BIAS) v += b[i];
+                    *reinterpret_cast<uint2*>(at(16 * jj + c, 2 * i + (q >> 1)) + 8 * (q & 1)) =
+                        make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
+                }
+            if (vec) {
+                u32x4 v[STEPS];
+#pragma unroll
+                for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+#pragma unroll
+                for (int u = 0; u < STEPS; u++)
+                    __builtin_amdgcn_raw_buffer_store_b128(v[u], cres, ofs0 + (rj + RPI * u) * row_bytes, 0, 0);
+            } else {
+                typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll 1
+                for (int r = r0; r < min(rows - rj, 32); r += RPI) {
+                    uint8_t* to = crow + ((rj + r) * p.ldc + n) * SZ;
+                    const uint8_t* from = at(r, k);
+                    if (n + EPC <= p.N) {
+                        *reinterpret_cast<u32x4_u*>(to) = *reinterpret_cast<const u32x4*>(from);
+                    } else {
+#pragma unroll 1
+                        for (int e = 0; e < p.N - n; e++) reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---- the largest tiles --------------------------------------------------------
+//
+// 256 x 256 for bf16 C, a wave 128 x 128 in accumulators of 16 x 16 (one
+// v_mfma_scale_f32_16x16x128_f8f6f4 a block of K), which draw a little less power than
+// those of 32 x 32.  A stage is four quarters of its 64 instructions: with W's blocks in
+// two halves w0, w1 and A's in f (first) and s,
+//   w0 f   reads s            of this stage      DMA of w0, f of the stage after next
+//   w0 s   reads w1           of this stage
+//   w1 s   reads w0           of the next stage  DMA of s, w1 of the stage after next
+//   w1 f   reads the next f   of the next stage
+// Each fragment is read into registers whose last use is over (the next stage's f is
+// this one's s: they change places from stage to stage), and each half of a slot is
+// refilled as soon as every wave has read it: two barriers a stage, fragment reads and
+// DMA even over all of it, and a whole stage for a refill to land, with two stages of
+// LDS (5498 x 13824 x 2560 165.5 -> 161 us, 8192^3 379 -> 358 us).
+__global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
+    constexpr int BN = 256, BM = 256;
+    constexpr int SCALES = (BN + BM) * ROW, W_WORDS = 256, STAGE = SCALES + 2048;  // words of A's rows, then W's
+    __shared__ __align__(16) uint8_t lds[2 * STAGE + 4 * STG];
+    const int total = p.n_tiles * p.m_tiles;
+    // tiles lid, lid + stride, .. of the XCD's contiguous range up to `end`
+    const int per = (total + 7) >> 3, stride = gridDim.x >> 3;
+    const int end = min(((int)blockIdx.x & 7) * per + per, total);
+    int tile = ((int)blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (tile >= end) return;
+    auto place = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
+        constexpr int GM = 4;
+        const int group = t / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
+        const int in_group = t - group * (GM * p.n_tiles);
+        m0 = (first_m + in_group % gm) * BM;
+        n0 = in_group / gm * BN;
+    };
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave >> 1, wm = wave & 1;
+    const int nk = p.K >> 7;
+    int nk_wrap = nk;
+    asm("" : "+s"(nk_wrap));
+
+    // DMA as in the other tiles.  A half of an operand is rows 0 .. 63 and 128 .. 191 of the
+    // tile, or 64 more: a wave's four pieces of a half are 32 neighbouring rows.
+    const int row0 = (wave >> 1) * 128 + (wave & 1) * 32, lrow = lane >> 3;
+    int off[2], k16;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int row = row0 + 8 * i + lrow;
+        off[i] = row * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+    const bool w_words = wave & 1;  // waves 0 and 2 fetch A's words, 1 and 3 W's
+    const int64_t words_ld = w_words ? p.ld_ws : p.ld_as;
+    int f_tile = tile, f_kt = 0;
+    __amdgpu_buffer_rsrc_t wres, ares;
+    const uint32_t* words;
+    uint32_t words_bytes;
+    auto fetch_from = [&](int t) __attribute__((always_inline)) {
+        int m0 = 0, n0 = 0, wrows = 0, arows = 0;
+        if (t < end) {
+            place(t, m0, n0);
+            wrows = min(BN, p.N - n0);
+            arows = min(BM, p.M - m0);
+        }
+        wres = uniform_rsrc(p.W + (int64_t)n0 * p.K, (uint32_t)wrows * p.K);
+        ares = uniform_rsrc(p.A + (int64_t)m0 * p.K, (uint32_t)arows * p.K);
+        words = w_words ? p.ws + (n0 >> 7) : p.as + m0;
+        words_bytes = 4u * (w_words ? (wrows + 127) >> 7 : arows);
+    };
+    auto fetch_next = [&]() __attribute__((always_inline)) {
+        if (++f_kt == nk) {
+            f_kt = 0;
+            f_tile += stride;
+            fetch_from(f_tile);
+        }
+    };
+    // A tile's first stage begins with A's rows of half `kind`: it goes on from the tile before.
+    int kind = 0;
+    // piece x (of four) of a half of W or A (A's half of this kind), or (x = 4) the words
+    auto load_piece = [&](int slot, bool is_a, int half, int x) __attribute__((always_inline)) {
+        uint8_t* st = lds + slot * STAGE;
+        if (x == 4) {
+            const __amdgpu_buffer_rsrc_t sres = uniform_rsrc(words + (int64_t)(f_kt >> 2) * words_ld, words_bytes);
+            uint8_t* dst = st + SCALES + 4 * (w_words ? W_WORDS : 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (lptr_t)dst, 16, 16 * lane, 0, 0, 0);
+            return;
+        }
+        const int h = is_a ? half ^ kind : half;
+        uint8_t* dst = st + ((is_a ? BN : 0) + row0 + 64 * h + 8 * x) * ROW;
+        const int ofs = off[x & 1] + (4 * h + (x >> 1)) * k16;
+        if (is_a) __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
+    };
+    constexpr int G1 = 9, G2 = 8;  // DMA instructions with the first two quarters and the others
+
+    f32x4 acc[8][8];
+    const int c = lane & 15, q = lane >> 4;
+    // fragment rows: blocks of 16 rows are 2 KiB apart and have the same swizzle
+    const int wrow = (wn * 128 + c) * ROW, arow = BN * ROW + (wm * 128 + c) * ROW, sx = (c >> 1) & 7;
+    const int at0 = ((2 * q) ^ sx) << 4, at1 = ((2 * q + 1) ^ sx) << 4, arow_words = 4 * (wm * 128 + c);
+    i32x8 wf[8], af[8];
+    int sw, sa[8], sw_next = 0, sa_next[8];
+    // piece x (of eight) of the four fragments of a half
+    auto read_piece = [&](int slot, bool is_a, int half, int x) __attribute__((always_inline)) {
+        const int f = 4 * half + (x >> 1), h = x & 1;
+        const uint8_t* from = lds + slot * STAGE + (is_a ? 64 * ROW * (half ^ kind) : 64 * ROW * half);
+        const i32x4 v = *reinterpret_cast<const i32x4*>(from + (h ? at1 : at0) + (is_a ? arow : wrow) + 16 * ROW * (x >> 1));
+        i32x8& d = is_a ? af[f] : wf[f];
+#pragma unroll
+        for (int e = 0; e < 4; e++) d[4 * h + e] = v[e];
+    };
+    auto read_scales = [&](int slot, int kind) __attribute__((always_inline)) {
+        const uint8_t* w = lds + slot * STAGE + SCALES;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            sa_next[j] = *reinterpret_cast<const int*>(w + arow_words + 256 * ((j >> 2) ^ kind) + 64 * (j & 3));
+        sw_next = *reinterpret_cast<const int*>(w + 4 * (W_WORDS + wn));
+    };
+    auto take_scales = [&](int kt) __attribute__((always_inline)) {  // byte kt % 4 of the words
+        const int sh = 8 * (kt & 3);
+        sw = __builtin_amdgcn_readfirstlane(sw_next) >> sh;
+#pragma unroll
+        for (int j = 0; j < 8; j++) sa[j] = sa_next[j] >> sh;
+    };
+    // W's half wi with A's half aj; a read of (rslot, W or A, half rh) after every other
+    // instruction, and after the odd ones, evenly, the DMA of up to two operands' halves
+    auto quarter = [&](int wi, int aj, int rslot, bool rd_a, int rh, int slot, bool dma_a, int dh, int nd, bool zc)
+        __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+            const int i = 4 * wi + (x >> 2), j = 4 * aj + (x & 3);
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[i], af[j], zc ? z : acc[i][j], 0, 0, 0, sw, 0, sa[j]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!(x & 1)) read_piece(rslot, rd_a, rh, x >> 1);
+#pragma unroll
+            for (int e = 0; e < nd; e++)
+                if (e * 16 / nd + 1 == x) load_piece(slot, dma_a, dh, e);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int slot = 0;
+    auto stage = [&](int kt, bool odd, bool zc) __attribute__((always_inline)) {
+        const int f = odd ? 1 : 0, s = 1 - f;
+        k16 = 16 * p.K;
+        asm volatile("" : "+s"(k16));  // the pieces' offsets are formed at the pieces: hoisted, they would take 16 registers
+        // Every wave's DMA of this stage's s and w1 has landed, and its w0, f and words are read.
+        wait_vmem_lds<G1 + G2>();
+        __builtin_amdgcn_s_barrier();
+        quarter(0, f, slot, true, s, slot, false, 0, 5, zc);
+        quarter(0, s, slot, false, 1, slot, true, f, 4, zc);
+        // The next stage's w0, f and words have landed, and this one's s and w1 are read.
+        wait_vmem_lds<G1 + G2>();
+        __builtin_amdgcn_s_barrier();
+        read_scales(slot ^ 1, kt + 1 == nk_wrap ? kind ^ (nk_wrap & 1) : kind);
+        quarter(1, s, slot ^ 1, false, 0, slot, true, s, 4, zc);
+        quarter(1, f, slot ^ 1, true, s, slot, false, 1, 4, zc);
+        // (the sums stay where they are formed, as in the other tiles)
+#pragma unroll
+        for (int x = 0; x < 64; x++) asm volatile("" : "+a"(acc[x >> 3][x & 7]));
+        fetch_next();
+        take_scales(kt + 1 == nk_wrap ? 0 : kt + 1);
+        slot ^= 1;
+    };
+    fetch_from(tile);
+    k16 = 16 * p.K;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#pragma unroll
+        for (int x = 0; x < 5; x++) load_piece(i, false, 0, x);
+#pragma unroll
+        for (int x = 0; x < 4; x++) load_piece(i, true, i, x);  // the first half of A of its kind of stage
+#pragma unroll
+        for (int x = 0; x < 4; x++) load_piece(i, true, 1 - i, x);
+#pragma unroll
+        for (int x = 0; x < 4; x++) load_piece(i, false, 1, x);
+        fetch_next();
+    }
+    wait_vmem_lds<G2 + G1 + G2>();
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int x = 0; x < 8; x++) read_piece(0, false, 0, x);
+#pragma unroll
+    for (int x = 0; x < 8; x++) read_piece(0, true, 0, x);
+    read_scales(0, 0);
+    take_scales(0);
+    while (true) {
+        stage(0, false, true);
+        int kt = 1;
+        for (; kt + 1 < nk; kt += 2) {
+            stage(kt, true, false);
+            stage(kt + 1, false, false);
+        }
+        if (kt < nk) {
+            stage(kt, true, false);
+        } else {  // the next tile's first fragments of A are in s's registers
+#pragma unroll
+            for (int i = 0; i < 4; i++) af[i] = af[4 + i];
+        }
+        int m0, n0;
+        place(tile, m0, n0);
+        int l = 0;  // the lane anew: see the other tiles
+        asm volatile("" : "+v"(l));
+        l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, l));
+        uint8_t* stg = lds + 2 * STAGE + wave * STG;
+        if (p.bias) wide_epilogue<true>(p, acc, n0 + wn * 128, m0 + wm * 128, kind, l, stg);
+        else wide_epilogue<false>(p, acc, n0 + wn * 128, m0 + wm * 128, kind, l, stg);
+        kind ^= nk & 1;
+        tile += stride;
+        if (tile >= end) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives its LDS
+}
+
 // The tile forms.  The large ones have the fewest operand bytes per product, the small
 // ones the most workgroups, and those with groups of waves over K the most of a
 // workgroup's blocks in flight.
@@ -579,7 +851,10 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
         hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS, KG>), grid, block, 0, s, p); \
         return hipGetLastError();                                                       \
     }
-    TILE(0, 4, 4, 2, 1)
+    if (!p.c_f32 && t->ni == 4 && t->mj == 4) {
+        hipLaunchKernelGGL(gemm_fp8_wide_kernel, grid, block, 0, s, p);
+        return hipGetLastError();
+    }
     TILE(0, 4, 3, 2, 1)
     TILE(0, 2, 3, 3, 1)
     TILE(0, 2, 2, 4, 1)
