@@ -563,24 +563,27 @@ __device__ inline void wide_epilogue(const Fp8Gemm& p, const f32x4 (&acc)[8][8],
                     *reinterpret_cast<uint2*>(at(16 * jj + c, 2 * i + (q >> 1)) + 8 * (q & 1)) =
                         make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
                 }
-            if (vec) {
-                u32x4 v[STEPS];
+            u32x4 v[STEPS];
 #pragma unroll
-                for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+            for (int u = 0; u < STEPS; u++) v[u] = *reinterpret_cast<const u32x4*>(at(RPI * u + r0, k));
+            if (vec) {
 #pragma unroll
                 for (int u = 0; u < STEPS; u++)
                     __builtin_amdgcn_raw_buffer_store_b128(v[u], cres, ofs0 + (rj + RPI * u) * row_bytes, 0, 0);
             } else {
                 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+                uint8_t* to = crow + ((rj + r0) * p.ldc + n) * SZ;
+                const bool whole = n + EPC <= p.N;
+#pragma unroll
+                for (int u = 0; u < STEPS; u++, to += RPI * p.ldc * SZ)
+                    if (whole && rj + RPI * u + r0 < rows) *reinterpret_cast<u32x4_u*>(to) = v[u];
+                if (!whole && n < p.N) {
 #pragma unroll 1
-                for (int r = r0; r < min(rows - rj, 32); r += RPI) {
-                    uint8_t* to = crow + ((rj + r) * p.ldc + n) * SZ;
-                    const uint8_t* from = at(r, k);
-                    if (n + EPC <= p.N) {
-                        *reinterpret_cast<u32x4_u*>(to) = *reinterpret_cast<const u32x4*>(from);
-                    } else {
+                    for (int r = r0; r < min(rows - rj, 32); r += RPI) {
+                        to = crow + ((rj + r) * p.ldc + n) * SZ;
 #pragma unroll 1
-                        for (int e = 0; e < p.N - n; e++) reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+                        for (int x = 0; x < p.N - n; x++)
+                            reinterpret_cast<uint16_t*>(to)[x] = reinterpret_cast<const uint16_t*>(at(r, k))[x];
                     }
                 }
             }
@@ -806,14 +809,15 @@ struct Tile {
     // measured, us: a block of K with one tile at work and with every CU busy, and a tile's ends
     float alone, full, ends;
 };
-constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.34f, 6.0f}, {4, 3, 2, 1, 0.88f, 0.97f, 5.0f}, {2, 3, 3, 1, 0.42f, 0.66f, 4.3f},
+constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.30f, 6.0f}, {4, 3, 2, 1, 0.95f, 0.97f, 5.5f}, {2, 3, 3, 1, 0.42f, 0.66f, 4.3f},
                          {2, 2, 4, 1, 0.30f, 0.42f, 4.2f}, {2, 1, 3, 2, 0.19f, 0.29f, 4.0f}, {1, 1, 4, 2, 0.13f, 0.20f, 3.9f}};
 constexpr Tile FULL[] = {{4, 4, 2, 1, 2.16f, 2.65f, 9.0f}, {4, 3, 2, 1, 1.69f, 1.92f, 6.5f}, {4, 2, 2, 1, 1.26f, 1.47f, 6.0f},
                          {2, 2, 2, 2, 0.62f, 0.76f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
 
 // Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
-// round plus 0.3 of its share (as for the bf16 GEMM).  Of the forms above and five others
-// that were timed on 24 products of 58 to 5498 rows it takes the fastest or one within 5 %.
+// round plus 0.3 of its share (as for the bf16 GEMM).  All six forms were timed on 26 products
+// with bf16 C and 14 with fp32 C of 58 to 5498 rows: it takes the fastest of each, or in one
+// case a form 3 % behind it (5498 x 7680 x 2560, fp32 C: 182 us, 177).
 float tile_cost(const Fp8Gemm& p, const Tile& t, int cus) {
     const long tiles = ((long)p.N + 64 * t.ni - 1) / (64 * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
     const float r = (float)tiles / cus, share = r < 1.f ? r : 1.f;
