@@ -684,9 +684,10 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
 
     f32x4 acc[8][8];
     const int c = lane & 15, q = lane >> 4;
-    // fragment rows: blocks of 16 rows are 2 KiB apart and have the same swizzle
+    // Fragment rows: blocks of 16 rows are 2 KiB apart and have the same swizzle.  A lane takes
+    // chunks q and q + 4, which keeps the lanes of one LDS pass on different banks.
     const int wrow = (wn * 128 + c) * ROW, arow = BN * ROW + (wm * 128 + c) * ROW, sx = (c >> 1) & 7;
-    const int at0 = ((2 * q) ^ sx) << 4, at1 = ((2 * q + 1) ^ sx) << 4, arow_words = 4 * (wm * 128 + c);
+    const int at0 = (q ^ sx) << 4, at1 = ((q + 4) ^ sx) << 4, arow_words = 4 * (wm * 128 + c);
     i32x8 wf[8], af[8];
     int sw, sa[8], sw_next = 0, sa_next[8];
     // piece x (of eight) of the four fragments of a half
