@@ -43,7 +43,10 @@ __device__ inline bf16x8 widen(int lo, int hi, float scale) {
 //
 // Up to 16 rows: 16 NI features per workgroup, the blocks of K in turn over its waves,
 // whose sums meet in LDS (in the waves' order).  Bound by W, which is read once,
-// straight into registers; A comes from the L2 again for every workgroup.
+// straight into registers; A comes from the L2 again for every workgroup.  One row of
+// 7680 x 2560 takes 5.4 us (19.7 MB of W: 3.6 TB/s), of 2560 x 6912 6.5, 16 rows of 7680 x
+// 2560 6.3 (of which a launch and the fill of the chip are 2 to 3).  Widened to bf16: an
+// 8-bit instruction would save nothing where W's bytes bound.
 template <int NI, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
     __shared__ f32x4 part[WAVES][NI][64];
@@ -129,6 +132,13 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 //
 // EXACT (fp32 C): the fragments are widened to bf16 with their scales and take four
 // 32x32x16 bf16 instructions in place of one 8-bit one.
+//
+// Bound by what a tile's operands take from the L2 where the tiles are small, and by the
+// chip's power where they are large (a loop of 8-bit instructions alone reaches 4.0 to 4.1
+// PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 7.0 us, 679 x 2560 x 6912 19.7 (1.22
+// PFLOP/s), 1237 x 1999 x 2816 15.3, 1400 x 13824 x 2560 50 to 53 (1.9).  fp32 C: 679 x
+// 2560 x 6912 32 to 34 us (0.72), 5498 x 13824 x 2560 322 (1.21), 8192^3 752 (1.46; the
+// library's bf16 product 1.31).
 constexpr int ROW = 128;  // bytes of a block's row
 
 // A buffer resource with wave-uniform fields (as in dit_gemm.hip): loads past
@@ -605,7 +615,10 @@ __device__ inline void wide_epilogue(const Fp8Gemm& p, const f32x4 (&acc)[8][8],
 // this one's s: they change places from stage to stage), and each half of a slot is
 // refilled as soon as every wave has read it: two barriers a stage, fragment reads and
 // DMA even over all of it, and a whole stage for a refill to land, with two stages of
-// LDS (5498 x 13824 x 2560 165.5 -> 161 us, 8192^3 379 -> 358 us).
+// LDS.  5498 x 13824 x 2560 takes 160 us (2.43 PFLOP/s; tiles as above 165), 8192^3 354 to
+// 366 (3.0 to 3.1; 374), the matrix cores busy for 60 % of the cycles.  Bound by power: the
+// first stages of a tile without a wait for the stores of the tile before, and LDS reads
+// without bank conflicts, changed neither.
 __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
     constexpr int BN = 256, BM = 256;
     constexpr int SCALES = (BN + BM) * ROW, W_WORDS = 256, STAGE = SCALES + 2048;  // words of A's rows, then W's

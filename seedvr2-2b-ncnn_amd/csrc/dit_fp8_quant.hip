@@ -6,7 +6,10 @@
 // product x 2^-e is exact (or below e4m3's range), so the one rounding is the
 // conversion's, to nearest even.
 //
-// HBM-bound: each value is read once (2 or 4 bytes) and a byte written.
+// HBM-bound: each value is read once (2 or 4 bytes) and a byte written.  Rows of 27258 x
+// 2560 bf16 take 36.9 us (5.7 TB/s), 5498 x 6912 fp32 34.0 (5.6), weights of 13824 x 2560
+// bf16 17.6 (6.0) and 2560 x 6912 fp32 14.9 (5.9), where device copies of 50 to 100 MiB
+// reach 4.8 to 5.1 TB/s; rows of 58 x 2560 2.3 us, of 679 x 2560 2.9.
 #include "dit_ops_internal.hpp"
 
 namespace awa {
