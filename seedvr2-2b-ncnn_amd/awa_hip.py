@@ -498,14 +498,25 @@ class Context:
         return emb
 
     # ---- operators around a projection in 8 bits (include/dit_ops.h)
-    def _stream(self, stream, *made):
-        """The stream of a call: the given one, else the current one of the context's device.  Tensors that
-        the call made on the current stream are marked as used on another."""
+    def _stream(self, stream):
+        """The stream of a call: the given one, else the current one of the context's device."""
         if stream is None:
             return _torch._C._cuda_getCurrentRawStream(self.device)
-        for t in made:
-            t.record_stream(stream)
+        if stream.device_index != self.device:
+            raise ValueError(f"stream must be of device {self.device}, got {stream.device}")
         return stream.cuda_stream
+
+    def _empty(self, like, shape, dtype, stream):
+        """A result, from the memory of the stream that writes it.  Where that is not the current stream, which
+        will read it, it is marked as used there too."""
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype)
+        self._stream(stream)
+        current = _torch.cuda.current_stream(self.device)
+        with _torch.cuda.stream(stream):
+            t = like.new_empty(shape, dtype=dtype)
+        t.record_stream(current)
+        return t
 
     def _elsewhere(self, what, t):
         return ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
@@ -544,20 +555,17 @@ class Context:
         if x.get_device() != self.device:
             raise self._elsewhere("quant_fp8", x)
         kp, groups, srows = (cols + 127) // 128 * 128, (cols + 511) // 512, (rows + 127) // 128 if blocks else rows
-        made = ()
         if q is None:
-            q = x.new_empty((rows, kp), dtype=_e4m3[0])
-            made = (q,)
+            q = self._empty(x, (rows, kp), _e4m3[0], stream)
         else:
             self._bytes_of("quant_fp8", q, "q", _e4m3, rows, kp)
         if scale is None:
-            scale = x.new_empty((groups, srows, 4), dtype=_e8m0[0])
-            made += (scale,)
+            scale = self._empty(x, (groups, srows, 4), _e8m0[0], stream)
         else:
             self._bytes_of("quant_fp8", scale, "scale", _e8m0, groups, srows, 4)
         if rows:
             rc = lib_.dit_quant_fp8(self.ptr, dtype, x.data_ptr(), x.stride(0), rows, cols, 128 if blocks else 1,
-                                    q.data_ptr(), scale.data_ptr(), srows, self._stream(stream, *made))
+                                    q.data_ptr(), scale.data_ptr(), srows, self._stream(stream))
             if rc:
                 self.check(rc, "dit_quant_fp8")
         return q, scale
@@ -579,10 +587,8 @@ class Context:
             self._bytes_of("gemm_fp8", w, "w", _e4m3, N, K)
         ld_as = self._scale_ld("gemm_fp8", a_scale, "a_scale", groups, M)
         ld_ws = self._scale_ld("gemm_fp8", w_scale, "w_scale", groups, nb)
-        made = ()
         if out is None:
-            out = a.new_empty((M, N), dtype=dtype or _torch.bfloat16)
-            made = (out,)
+            out = self._empty(a, (M, N), dtype or _torch.bfloat16, stream)
         elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (dtype or out.dtype) != out.dtype:
             raise ValueError(f"gemm_fp8: out must be [{M}, {N}] of dtype {dtype} with contiguous columns")
         elif out.get_device() != self.device:
@@ -596,7 +602,7 @@ class Context:
         if M:
             rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), ld_as, w.data_ptr(), w_scale.data_ptr(), ld_ws,
                                    bias.data_ptr() if bias is not None else None, ct, out.data_ptr(), out.stride(0), M, N,
-                                   K, self._stream(stream, *made))
+                                   K, self._stream(stream))
             if rc:
                 self.check(rc, "dit_gemm_fp8")
         return out
@@ -632,7 +638,7 @@ class Context:
             raise self._elsewhere("rope", positions)
         plan = b"".join((_PLAN.pack(ROPE_LAYOUTS[layout], axes, *pairs, *_NO_PAIRS[axes:], 1 if inverse else 0, scale),
                          f.tobytes(), _NO_FREQS[8 * f.size:]))
-        rows, made, res = b"", (), []
+        rows, res = b"", []
         for i, t in enumerate(xs):
             ts = t.stride()
             if t.dim() != 3 or t.dtype != first.dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
@@ -640,8 +646,7 @@ class Context:
                 raise ValueError("rope: tensors must be [tokens, heads, head_d] of one dtype with contiguous channels")
             o = outs[i]
             if o is None:
-                o = t.new_empty(t.shape)
-                made += (o,)
+                o = self._empty(t, t.shape, t.dtype, stream)
             elif o.shape != t.shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):
                 raise ValueError("rope: out must have x's shape and dtype and contiguous channels")
             if t.get_device() != self.device or o.get_device() != self.device:
@@ -650,7 +655,7 @@ class Context:
             os_ = o.stride()
             rows += _ROWS.pack(t.data_ptr(), o.data_ptr(), t.shape[1], ts[0], ts[1], os_[0], os_[1])
         rc = lib_.dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, plan, positions.data_ptr(),
-                           self._stream(stream, *made))
+                           self._stream(stream))
         if rc:
             self.check(rc, "dit_rope")
         return tuple(res) if many else res[0]

@@ -465,3 +465,26 @@ def test_captured_and_replayed(awa, ctx):
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
     other.close()
+
+
+def test_results_of_another_stream(awa, ctx):
+    """A result is not put where the current stream's earlier work, still running, has yet to write."""
+    import torch
+    x, wt, bias, pos, freqs = layer_inputs(awa, ctx, 700, 3)
+    w = ctx.quant_fp8(wt, blocks=True)
+    q, s = ctx.quant_fp8(x)
+    want = ctx.gemm_fp8(q, s, *w)
+    turned = ctx.rope(want.unflatten(1, (12, 128)), pos, freqs, pairs=(21, 21, 21))
+    side, big = torch.cuda.Stream(), torch.ones(1 << 28, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(8):  # 8 passes over 1 GiB: over a millisecond
+        big.mul_(1.0)
+    late = [torch.empty_like(t) for t in (q, s, want, turned) for _ in range(4)]
+    for t in late:
+        t.view(torch.uint8).fill_(85)
+    del late, t  # given back before the fills have run
+    got = [*ctx.quant_fp8(x, stream=side), ctx.gemm_fp8(q, s, *w, stream=side),
+           ctx.rope(want.unflatten(1, (12, 128)), pos, freqs, pairs=(21, 21, 21), stream=side)]
+    torch.cuda.synchronize()
+    for g, r in zip(got, (q, s, want, turned)):
+        assert torch.equal(g.view(torch.uint8), r.view(torch.uint8))
