@@ -149,6 +149,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
                 for (int j = 0; j < V; j++) {
                     const float m = Chan<T>::get(f[r].v[2 * j]), n = Chan<T>::get(f[r].v[2 * j + 1]);
                     Chan<T>::put(p.v + 2 * j, m * c[j] - n * s[j], m * s[j] + n * c[j]);
+                    if (V > 1 && u * V + j >= a.pairs) {  // channels that only pass, as they are (also infinities)
+                        p.v[2 * j] = f[r].v[2 * j];
+                        p.v[2 * j + 1] = f[r].v[2 * j + 1];
+                    }
                 }
                 p.store(o);
             }

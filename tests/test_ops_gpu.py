@@ -327,6 +327,23 @@ def test_rope_not_finite_stays_in_its_pair(awa, ctx):
             assert torch.equal(bad[:, 0], want)
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rope_passes_every_bit(awa, ctx, layout, dtype):
+    """Channels past the pairs, some inside the last piece of the pairs: infinities, NaN with their bits, -0."""
+    import torch
+    ints = torch.int16 if dtype == BF16 else torch.int32
+    for head_d, pairs in ((128, 63), (128, 61), (64, 1), (24, 9), (10, 3)):
+        x = torch.randn((5, 3, head_d), device="cuda").to(dt(dtype))
+        tail = x[..., 2 * pairs:]
+        tail.copy_(torch.tensor([math.inf, 1.0, -0.0, math.nan, -1.0, -math.inf, 0.0, -2.0] * 32,
+                                device="cuda")[torch.randint(0, 256, tail.shape, device="cuda")].to(dt(dtype)))
+        x.view(ints)[0, 0, 2 * pairs] |= 3  # a NaN of some bits, or a number
+        out = ctx.rope(x, torch.arange(5, dtype=torch.int32, device="cuda"), awa.rope_freqs(pairs), layout=layout)
+        assert torch.equal(out.view(ints)[..., 2 * pairs:], x.view(ints)[..., 2 * pairs:])
+        assert out[..., :2 * pairs].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rope_queries_and_keys(awa, ctx, dtype):
     """Both tensors of a call, in place inside qkv rows: the same bits as one by one; v stays."""
@@ -397,6 +414,28 @@ def test_offsets_past_32_bits(awa, ctx):
         ref = ctx.rope(h.contiguous(), pos, awa.rope_freqs(32), layout=layout)
         ctx.rope(h, pos, awa.rope_freqs(32), layout=layout, out=h)
         assert torch.equal(h, ref)
+
+
+def test_most_rows(awa, ctx):
+    """2^24 rows: more pieces than one grid of the quantiser holds, and nearly 2^32 threads of the rotation."""
+    import torch
+    n = 1 << 24
+    x = torch.empty((n, 1025), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, n // 64):  # a part's rows are its first ones, times a power of two of its own
+        x[i:i + n // 64].copy_((torch.arange(1025, device="cuda") % 251 - 99).bfloat16() * 2.0 ** (i // (n // 64) - 32))
+    q, s = ctx.quant_fp8(x)
+    for i in range(0, n, n // 64):
+        wq, ws = ctx.quant_fp8(x[i:i + 1])
+        assert bool((q[i:i + n // 64].view(torch.int32) == wq.view(torch.int32)).all())
+        assert bool((s[:, i:i + n // 64].view(torch.uint8) == ws.view(torch.uint8)).all())
+    del x, q, s
+    h = torch.ones((n, 1, 256), dtype=torch.bfloat16, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    out = ctx.rope(h, pos, np.array([0.001]), layout="half")
+    for i in (0, 12345, n // 2 - 3, n - 10):
+        some = ctx.rope(h[i:i + 10].clone(), pos[i:i + 10], np.array([0.001]), layout="half")
+        assert torch.equal(out[i:i + 10], some)
+    assert bool((out[..., 2:] == 1).all()) and bool((out[..., 0].float() ** 2 + out[..., 1].float() ** 2 - 2).abs().max() < 0.05)
 
 
 # ------------------------------------------------------------------ together
