@@ -161,9 +161,11 @@ SIZES = [(1, 1, 128), (1, 7680, 2560), (2, 130, 640), (15, 257, 384), (16, 16, 5
          (257, 513, 896), (300, 2560, 512), (679, 2560, 6912), (1000, 1536, 2560), (1237, 1999, 2816),
          (2100, 5120, 384), (4440, 2560, 256), (671, 7601, 640), (700, 3000, 256), (2500, 7681, 256), (6000, 4104, 384),
          (1300, 20001, 128)]
+# 256 x 256 tiles, more of them than CUs, of even and odd numbers of blocks over several scale words
+LARGE = [(6000, 4104, 256), (4300, 6600, 512), (5890, 4601, 1152), (6100, 4101, 1792), (4000, 4001, 1280)]
 
 
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + LARGE)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_gemm(awa, ctx, m, n, k, dtype):
     import torch
@@ -218,6 +220,28 @@ def test_gemm_rows_apart(awa, ctx, m):
     out = ctx.gemm_fp8(a, sa, w, sw, dtype=torch.float32)
     within(out, ref, gemm_bar(va.nan_to_num(nan=0.0), vw, ref.nan_to_num(nan=0.0), torch.float32, 1024))
     assert bool((out[1] == 0).all()) and bool(out[0].isnan().all())
+
+
+@pytest.mark.parametrize("m,n", [(20, 300), (200, 1000), (700, 2560), (700, 7601), (2500, 7681), (6000, 4104)])
+@pytest.mark.parametrize("k", [768, 896])
+def test_gemm_rows_apart_in_8_bits(awa, ctx, m, n, k):
+    """The same for bf16 C of more rows, in every form of tile, and at each row's place of a tile."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    a, sa, va = fp8_matrix(awa, ctx, m, k, False, g)
+    w, sw, vw = fp8_matrix(awa, ctx, n, k, True, g)
+    nans, zeros, lows = (slice(i, None, 37) for i in (0, 1, 2))
+    a[nans, 300] = math.nan
+    a[zeros] = 0
+    va[nans], va[zeros] = 0, 0
+    sa.view(torch.uint8)[:, zeros] = 0
+    sa.view(torch.uint8)[1, lows] = 0  # blocks from the fifth on: 2^-127
+    va[lows, 512:] = a[lows, 512:].double() * 2.0 ** -127
+    ref = va @ vw.T
+    out = ctx.gemm_fp8(a, sa, w, sw)
+    assert bool(out[nans].isnan().all()) and bool((out[zeros] == 0).all())
+    out[nans] = 0
+    within(out, ref, gemm_bar(va, vw, ref, torch.bfloat16, k))
 
 
 def test_gemm_slices(awa, ctx):
