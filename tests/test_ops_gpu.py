@@ -244,6 +244,26 @@ def test_gemm_rows_apart_in_8_bits(awa, ctx, m, n, k):
     within(out, ref, gemm_bar(va, vw, ref, torch.bfloat16, k))
 
 
+@pytest.mark.parametrize("m", [4, 40, 700])
+def test_gemm_ends_of_the_range(awa, ctx, m):
+    """Rows that quantise to 2^128: infinite where products enter whole, values like others in 8 bits."""
+    import torch
+    x = torch.zeros((m, 128), device="cuda")
+    x[:, 0] = 3.4e38
+    x[1, 0] = -247.0 * 2.0 ** 120  # to 240 2^120
+    x[2, 0] = 2.0 ** -120
+    wt = torch.zeros((300, 128), device="cuda")
+    wt[:, 0] = 2.0 ** -10
+    a, w = ctx.quant_fp8(x), ctx.quant_fp8(wt, blocks=True)
+    for t in (F32, BF16):
+        out = ctx.gemm_fp8(*a, *w, dtype=dt(t)).double()
+        whole = t == F32 or m <= 16
+        assert bool((out[0] == (math.inf if whole else 2.0 ** 118)).all())
+        assert bool((out[1] == -240.0 * 2.0 ** 110).all())
+        assert bool((out[2] == 2.0 ** -130).all()) or bool((out[2] == 0).all())
+        assert bool((out[3:] == out[0]).all())
+
+
 def test_gemm_slices(awa, ctx):
     """Rows cut from a larger quantised matrix (the scale stride of the whole), through the C entry."""
     import torch
