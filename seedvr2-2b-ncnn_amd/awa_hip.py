@@ -312,6 +312,7 @@ class Context:
         if rc != AWA_OK:
             raise AwaError(rc, f"awa_create(device={device}) failed")
         self.device = int(device)
+        self._on = _torch.device("cuda", self.device)
 
     def error(self):
         return lib().awa_last_error(self.ptr).decode()
@@ -506,15 +507,15 @@ class Context:
             raise ValueError(f"stream must be of device {self.device}, got {stream.device}")
         return stream.cuda_stream
 
-    def _empty(self, like, shape, dtype, stream):
+    def _empty(self, dtype, stream, *shape):
         """A result, from the memory of the stream that writes it.  Where that is not the current stream, which
         will read it, it is marked as used there too."""
         if stream is None:
-            return like.new_empty(shape, dtype=dtype)
+            return _torch.empty(*shape, dtype=dtype, device=self._on)
         self._stream(stream)
         current = _torch.cuda.current_stream(self.device)
         with _torch.cuda.stream(stream):
-            t = like.new_empty(shape, dtype=dtype)
+            t = _torch.empty(*shape, dtype=dtype, device=self._on)
         t.record_stream(current)
         return t
 
@@ -549,22 +550,23 @@ class Context:
         a scale per 128 x 128 values, [groups, ceil(rows / 128), 4])."""
         lib_ = lib()
         dtype = _dtype_of("quant_fp8", x)
-        rows, cols = x.shape if x.dim() == 2 else (0, 0)
-        if cols < 1 or (cols > 1 and x.stride(1) != 1):
+        shape, st = x.shape, x.stride()
+        rows, cols = shape if len(shape) == 2 else (0, 0)
+        if cols < 1 or (cols > 1 and st[1] != 1):
             raise ValueError("quant_fp8: x must be [rows, cols] with contiguous columns")
         if x.get_device() != self.device:
             raise self._elsewhere("quant_fp8", x)
         kp, groups, srows = (cols + 127) // 128 * 128, (cols + 511) // 512, (rows + 127) // 128 if blocks else rows
         if q is None:
-            q = self._empty(x, (rows, kp), _e4m3[0], stream)
+            q = self._empty(_e4m3[0], stream, rows, kp)
         else:
             self._bytes_of("quant_fp8", q, "q", _e4m3, rows, kp)
         if scale is None:
-            scale = self._empty(x, (groups, srows, 4), _e8m0[0], stream)
+            scale = self._empty(_e8m0[0], stream, groups, srows, 4)
         else:
             self._bytes_of("quant_fp8", scale, "scale", _e8m0, groups, srows, 4)
         if rows:
-            rc = lib_.dit_quant_fp8(self.ptr, dtype, x.data_ptr(), x.stride(0), rows, cols, 128 if blocks else 1,
+            rc = lib_.dit_quant_fp8(self.ptr, dtype, x.data_ptr(), st[0], rows, cols, 128 if blocks else 1,
                                     q.data_ptr(), scale.data_ptr(), srows, self._stream(stream))
             if rc:
                 self.check(rc, "dit_quant_fp8")
@@ -575,20 +577,21 @@ class Context:
         with blocks=True, or of rows cut from them (a[i:j], a_scale[:, i:j]); `dtype` bf16 (default) or fp32, or that
         of `out` (rows may be strided)."""
         lib_ = lib()
-        if a.dim() != 2 or w.dim() != 2:
+        shape, wshape = a.shape, w.shape
+        if len(shape) != 2 or len(wshape) != 2:
             raise ValueError("gemm_fp8: a [M, K] and w [N, K]")
-        M, K = a.shape
-        N = w.shape[0]
+        M, K = shape
+        N = wshape[0]
         groups, nb = (K + 511) // 512, (N + 127) // 128
         dev = self.device
-        if not (a.dtype in _e4m3 and w.dtype in _e4m3 and w.shape[1] == K and a.is_contiguous() and w.is_contiguous() and
+        if not (a.dtype in _e4m3 and w.dtype in _e4m3 and wshape[1] == K and a.is_contiguous() and w.is_contiguous() and
                 a.get_device() == dev and w.get_device() == dev):
             self._bytes_of("gemm_fp8", a, "a", _e4m3, M, K)
             self._bytes_of("gemm_fp8", w, "w", _e4m3, N, K)
         ld_as = self._scale_ld("gemm_fp8", a_scale, "a_scale", groups, M)
         ld_ws = self._scale_ld("gemm_fp8", w_scale, "w_scale", groups, nb)
         if out is None:
-            out = self._empty(a, (M, N), dtype or _torch.bfloat16, stream)
+            out = self._empty(dtype or _torch.bfloat16, stream, M, N)
         elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (dtype or out.dtype) != out.dtype:
             raise ValueError(f"gemm_fp8: out must be [{M}, {N}] of dtype {dtype} with contiguous columns")
         elif out.get_device() != self.device:
@@ -621,39 +624,39 @@ class Context:
             raise ValueError("rope: one or two tensors, and as many outputs")
         first = xs[0]
         dtype = _dtype_of("rope", first)
-        if first.dim() != 3:
+        shape = first.shape
+        if len(shape) != 3:
             raise ValueError("rope: tensors must be [tokens, heads, head_d]")
-        tokens, _, head_d = first.shape
+        tokens, _, head_d = shape
         f = np.ascontiguousarray(freqs, np.float64)
-        axes = positions.shape[1] if positions.dim() == 2 else 1
-        pairs = (f.size,) if pairs is None else tuple(pairs)
-        if (positions.dtype != _torch.int32 or positions.dim() > 2 or positions.shape[0] != tokens or
-                not positions.is_contiguous()):
+        n, at = f.size, positions.shape
+        axes = at[1] if len(at) == 2 else 1
+        pairs = (n,) if pairs is None else tuple(pairs)
+        if positions.dtype != _torch.int32 or not 1 <= len(at) <= 2 or at[0] != tokens or not positions.is_contiguous():
             raise ValueError(f"rope: positions must be contiguous int32 [{tokens}] or [{tokens}, axes]")
-        if len(pairs) != axes or axes > ROPE_MAX_AXES or sum(pairs) != f.size or f.size > ROPE_MAX_PAIRS:
-            raise ValueError(f"rope: pairs {pairs} must name each axis of the positions and sum to the {f.size} freqs")
+        if len(pairs) != axes or axes > ROPE_MAX_AXES or sum(pairs) != n or n > ROPE_MAX_PAIRS:
+            raise ValueError(f"rope: pairs {pairs} must name each axis of the positions and sum to the {n} freqs")
         if layout not in ROPE_LAYOUTS:
             raise ValueError(f"rope: layout must be one of {list(ROPE_LAYOUTS)}")
         if positions.get_device() != self.device:
             raise self._elsewhere("rope", positions)
         plan = b"".join((_PLAN.pack(ROPE_LAYOUTS[layout], axes, *pairs, *_NO_PAIRS[axes:], 1 if inverse else 0, scale),
-                         f.tobytes(), _NO_FREQS[8 * f.size:]))
+                         f.tobytes(), _NO_FREQS[8 * n:]))
         rows, res = b"", []
-        for i, t in enumerate(xs):
-            ts = t.stride()
-            if t.dim() != 3 or t.dtype != first.dtype or t.shape[0] != tokens or t.shape[2] != head_d or (
+        for t, o in zip(xs, outs):
+            shape, ts = t.shape, t.stride()
+            if len(shape) != 3 or t.dtype != first.dtype or shape[0] != tokens or shape[2] != head_d or (
                     head_d > 1 and ts[2] != 1):
                 raise ValueError("rope: tensors must be [tokens, heads, head_d] of one dtype with contiguous channels")
-            o = outs[i]
             if o is None:
-                o = self._empty(t, t.shape, t.dtype, stream)
-            elif o.shape != t.shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):
+                o = self._empty(t.dtype, stream, *shape)
+            elif o.shape != shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):
                 raise ValueError("rope: out must have x's shape and dtype and contiguous channels")
             if t.get_device() != self.device or o.get_device() != self.device:
                 raise self._elsewhere("rope", t)
             res.append(o)
             os_ = o.stride()
-            rows += _ROWS.pack(t.data_ptr(), o.data_ptr(), t.shape[1], ts[0], ts[1], os_[0], os_[1])
+            rows += _ROWS.pack(t.data_ptr(), o.data_ptr(), shape[1], ts[0], ts[1], os_[0], os_[1])
         rc = lib_.dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, plan, positions.data_ptr(),
                            self._stream(stream))
         if rc:
