@@ -227,12 +227,15 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
                 for (int u = 0; u < STEPS; u++, to += RPI * p.ldc * SZ)
                     if (whole && 32 * j + RPI * u + r0 < rows) *reinterpret_cast<u32x4_u*>(to) = v[u];
                 if (!whole && n < p.N) {
+                    to = crow + ((32 * j + r0) * p.ldc + n) * SZ;
 #pragma unroll 1
-                    for (int r = r0; r < min(rows - 32 * j, 32); r += RPI) {
-                        to = crow + ((32 * j + r) * p.ldc + n) * SZ;
-#pragma unroll 1
-                        for (int e = 0; e < (p.N - n) * (SZ / 2); e++)
-                            reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(at(r, k))[e];
+                    for (int e = 0; e < (p.N - n) * (SZ / 2); e++) {
+                        uint16_t h[STEPS];
+#pragma unroll
+                        for (int u = 0; u < STEPS; u++) h[u] = reinterpret_cast<const uint16_t*>(at(RPI * u + r0, k))[e];
+#pragma unroll
+                        for (int u = 0; u < STEPS; u++)
+                            if (32 * j + RPI * u + r0 < rows) reinterpret_cast<uint16_t*>(to + RPI * u * p.ldc * SZ)[e] = h[u];
                     }
                 }
             }
@@ -588,12 +591,15 @@ __device__ inline void wide_epilogue(const Fp8Gemm& p, const f32x4 (&acc)[8][8],
                 for (int u = 0; u < STEPS; u++, to += RPI * p.ldc * SZ)
                     if (whole && rj + RPI * u + r0 < rows) *reinterpret_cast<u32x4_u*>(to) = v[u];
                 if (!whole && n < p.N) {
+                    to = crow + ((rj + r0) * p.ldc + n) * SZ;
 #pragma unroll 1
-                    for (int r = r0; r < min(rows - rj, 32); r += RPI) {
-                        to = crow + ((rj + r) * p.ldc + n) * SZ;
-#pragma unroll 1
-                        for (int x = 0; x < p.N - n; x++)
-                            reinterpret_cast<uint16_t*>(to)[x] = reinterpret_cast<const uint16_t*>(at(r, k))[x];
+                    for (int e = 0; e < p.N - n; e++) {
+                        uint16_t h[STEPS];
+#pragma unroll
+                        for (int u = 0; u < STEPS; u++) h[u] = reinterpret_cast<const uint16_t*>(at(RPI * u + r0, k))[e];
+#pragma unroll
+                        for (int u = 0; u < STEPS; u++)
+                            if (rj + RPI * u + r0 < rows) reinterpret_cast<uint16_t*>(to + RPI * u * p.ldc * SZ)[e] = h[u];
                     }
                 }
             }
