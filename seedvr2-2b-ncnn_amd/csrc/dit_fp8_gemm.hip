@@ -835,8 +835,8 @@ constexpr Tile FULL[] = {{4, 4, 2, 1, 2.16f, 2.65f, 9.0f}, {4, 3, 2, 1, 1.69f, 1
                          {2, 2, 2, 2, 0.62f, 0.76f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
 
 // Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
-// round plus 0.3 of its share (as for the bf16 GEMM).  All six forms were timed on 26 products
-// with bf16 C and 14 with fp32 C of 58 to 5498 rows: it takes the fastest of each, or in one
+// round plus 0.3 of its share (as for the bf16 GEMM).  All six forms were timed on 33 products
+// with bf16 C and 21 with fp32 C of 58 to 5498 rows: it takes the fastest of each, or in one
 // case a form 3 % behind it (5498 x 7680 x 2560, fp32 C: 182 us, 177).
 float tile_cost(const Fp8Gemm& p, const Tile& t, int cus) {
     const long tiles = ((long)p.N + 64 * t.ni - 1) / (64 * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
