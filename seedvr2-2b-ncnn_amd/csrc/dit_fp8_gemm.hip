@@ -122,8 +122,8 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 
 // ---- tiles ------------------------------------------------------------------
 //
-// Workgroup tile 64 NI (n) x 64 MJ (m), a block of K per stage, four wave64 in a
-// 2 x 2 grid, NI x MJ accumulators of 32 x 32 per wave.  As in the bf16 GEMM the
+// Workgroup tile 32 NW NI (n) x 64 MJ (m), a block of K per stage, wave64 in a
+// NW x 2 grid, NI x MJ accumulators of 32 x 32 per wave.  As in the bf16 GEMM the
 // operands' 128-byte rows reach LDS by direct DMA into NS stages, 16-byte chunks at
 // chunk ^ ((row >> 1) & 7), and each half block (64 columns, one instruction per
 // accumulator) runs with the next half's fragment reads and, in the half that
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 //
 // Bound by what a tile's operands take from the L2 where the tiles are small, and by the
 // chip's power where they are large (a loop of 8-bit instructions alone reaches 4.0 to 4.1
-// PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 7.0 us, 679 x 2560 x 6912 19.7 (1.22
+// PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 6.1 us, 679 x 2560 x 6912 19.7 (1.22
 // PFLOP/s), 1237 x 1999 x 2816 15.3, 1400 x 13824 x 2560 50 to 53 (1.9).  fp32 C: 679 x
 // 2560 x 6912 32 to 34 us (0.72), 5498 x 13824 x 2560 322 (1.21), 8192^3 752 (1.46; the
 // library's bf16 product 1.31).
@@ -243,22 +243,25 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
     }
 }
 
-// KG: groups of four waves that take the blocks of K in turn, each with stages of its own,
-// for products of few tiles; their sums meet in LDS at the end, in the groups' order.
-template <bool EXACT, int NI, int MJ, int NS, int KG>
-__global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
-    constexpr int BN = 64 * NI, BM = 64 * MJ;
+// A group of 2 NW waves (NW over n, two over m) makes the tile; KG of them take the blocks of
+// K in turn, each with stages of its own, for products of few tiles; their sums meet in LDS at
+// the end, in the groups' order.
+template <bool EXACT, int NI, int MJ, int NS, int KG, int NW>
+__global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
+    constexpr int BN = 32 * NW * NI, BM = 64 * MJ;
+    constexpr int GW = 2 * NW, GT = 64 * GW;  // waves and threads of a group
+    constexpr int PA = 4 * MJ / NW;           // a wave's DMA instructions for A (2 NI for W)
     constexpr int SCALES = (BN + BM) * ROW;
     // a stage's scale words: A's rows', then W's.  Each wave has one instruction for them (so
     // that all wait for one count): 256 rows take one of 16 bytes a lane (waves 0 and 2, W's
-    // 1 and 3), fewer one of 4 (a wave for each 64 rows, W's the others).
+    // 1 and 3), fewer one of 4 (a wave for each 64 rows, W's the others).  NW = 1: MJ = 1.
     constexpr int WORD_B = MJ == 4 ? 16 : 4, W_WORDS = MJ == 4 ? 256 : 64 * MJ;
     constexpr int STAGE = SCALES + 4 * W_WORDS + 64 * WORD_B;
     // two-stage forms walk several tiles: the next tile's first stages land during this
     // one's epilogue, which therefore has LDS of its own
     constexpr bool WALK = NS == 2 && KG == 1;
     __shared__ __align__(16) uint8_t lds[KG * NS * STAGE + (WALK ? 4 * STG : 0)];
-    static_assert(sizeof(lds) <= 160 * 1024 && 4 * STG + (KG - 1) * NI * MJ * 16384 <= (int)sizeof(lds), "LDS");
+    static_assert(sizeof(lds) <= 160 * 1024 && 4 * STG + (KG - 1) * NI * MJ * GT * 64 <= (int)sizeof(lds), "LDS");
     const int total = p.n_tiles * p.m_tiles;
     // tiles lid, lid + stride, .. of the XCD's contiguous range up to `end`
     const int per = (total + 7) >> 3, stride = gridDim.x >> 3;
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     };
 
     const int tid = threadIdx.x, lane = tid & 63;
-    const int kg = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
+    const int kg = __builtin_amdgcn_readfirstlane(tid / GT), wave = __builtin_amdgcn_readfirstlane((tid >> 6) % GW);
     const int wn = wave >> 1, wm = wave & 1;
     const int c = lane & 31, g = lane >> 5;
     const int nk = p.K >> 7, ns = (nk + KG - 1) / KG;  // blocks, and stages of every group
@@ -287,18 +290,18 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     // l % 8, so it fetches the chunk that the swizzle maps there.  Rows past N or M
     // lie past their resource and read zeros.
     const int lrow = lane >> 3;
-    int woff[2 * NI], aoff[2 * MJ];
+    int woff[2 * NI], aoff[PA];
 #pragma unroll
     for (int i = 0; i < 2 * NI; i++) {
         const int row = (wave * 2 * NI + i) * 8 + lrow;
         woff[i] = row * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * MJ; i++) {
-        const int row = (wave * 2 * MJ + i) * 8 + lrow;
+    for (int i = 0; i < PA; i++) {
+        const int row = (wave * PA + i) * 8 + lrow;
         aoff[i] = row * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
     }
-    constexpr int NP = 2 * NI + 2 * MJ + 1;  // DMA instructions of a wave per stage
+    constexpr int NP = 2 * NI + PA + 1;  // DMA instructions of a wave per stage
     const bool w_words = MJ == 4 ? wave & 1 : wave >= MJ;
     const int words0 = MJ == 4 || w_words ? 0 : 64 * wave;  // the first of the wave's words
     const int64_t words_ld = w_words ? p.ld_ws : p.ld_as;
@@ -339,8 +342,8 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         }
         const bool is_a = x >= 2 * NI;
         const int i = is_a ? x - 2 * NI : x;
-        uint8_t* dst = st + (is_a ? BN * ROW + (wave * 2 * MJ + i) * 1024 : (wave * 2 * NI + i) * 1024);
-        const int ofs = is_a ? aoff[i < 2 * MJ ? i : 0] : woff[i];
+        uint8_t* dst = st + (is_a ? BN * ROW + (wave * PA + i) * 1024 : (wave * 2 * NI + i) * 1024);
+        const int ofs = is_a ? aoff[i < PA ? i : 0] : woff[i];
         if (is_a) __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
         else __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (lptr_t)dst, 16, ofs, f_kt * ROW, 0, 0);
     };
@@ -499,9 +502,9 @@ __global__ __launch_bounds__(256 * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         }
         if constexpr (KG > 1) {
             // the other groups' sums to group 0, past its staging area
-            f32x4* sums = reinterpret_cast<f32x4*>(lds + 4 * STG) + (tid & 255);
+            f32x4* sums = reinterpret_cast<f32x4*>(lds + 4 * STG) + tid % GT;
             auto at = [&](int from, int x, int q) __attribute__((always_inline)) {
-                return sums + 256 * ((from * NI * MJ + x) * 4 + q);
+                return sums + GT * ((from * NI * MJ + x) * 4 + q);
             };
             if (kg) {
 #pragma unroll
@@ -823,23 +826,29 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
 
 // The tile forms.  The large ones have the fewest operand bytes per product, the small
 // ones the most workgroups, and those with groups of waves over K the most of a
-// workgroup's blocks in flight.
+// workgroup's blocks in flight: what bounds few tiles is how many bytes are on their way
+// (58 x 2560 x 6912 in 64 x 64 tiles, 40 workgroups, 11.7 us; in 32 x 64, 80 of them, 9.4;
+// fp32 C 17.3 and 11.6).
 struct Tile {
-    int ni, mj, ns, kg;
+    int ni, mj, ns, kg, nw;
     // measured, us: a block of K with one tile at work and with every CU busy, and a tile's ends
     float alone, full, ends;
 };
-constexpr Tile FAST[] = {{4, 4, 2, 1, 1.05f, 1.30f, 6.0f}, {4, 3, 2, 1, 0.95f, 0.97f, 5.5f}, {2, 3, 3, 1, 0.42f, 0.66f, 4.3f},
-                         {2, 2, 4, 1, 0.30f, 0.42f, 4.2f}, {2, 1, 3, 2, 0.19f, 0.29f, 4.0f}, {1, 1, 4, 2, 0.13f, 0.20f, 3.9f}};
-constexpr Tile FULL[] = {{4, 4, 2, 1, 2.16f, 2.65f, 9.0f}, {4, 3, 2, 1, 1.69f, 1.92f, 6.5f}, {4, 2, 2, 1, 1.26f, 1.47f, 6.0f},
-                         {2, 2, 2, 2, 0.62f, 0.76f, 6.3f}, {2, 1, 3, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 0.23f, 0.30f, 5.0f}};
+constexpr Tile FAST[] = {{4, 4, 2, 1, 2, 1.05f, 1.30f, 6.0f}, {4, 3, 2, 1, 2, 0.95f, 0.97f, 5.5f},
+                         {2, 3, 3, 1, 2, 0.42f, 0.66f, 4.3f}, {2, 2, 4, 1, 2, 0.30f, 0.42f, 4.2f},
+                         {2, 1, 3, 2, 2, 0.19f, 0.29f, 4.0f}, {1, 1, 4, 2, 2, 0.13f, 0.20f, 3.9f},
+                         {1, 1, 3, 4, 1, 0.105f, 0.125f, 3.7f}};
+constexpr Tile FULL[] = {{4, 4, 2, 1, 2, 2.16f, 2.50f, 9.0f}, {4, 3, 2, 1, 2, 1.69f, 1.92f, 6.5f},
+                         {4, 2, 2, 1, 2, 1.26f, 1.47f, 6.0f}, {2, 2, 2, 2, 2, 0.62f, 0.76f, 6.3f},
+                         {2, 1, 3, 2, 2, 0.39f, 0.48f, 5.7f}, {1, 1, 2, 4, 2, 0.23f, 0.30f, 5.0f},
+                         {1, 1, 3, 4, 1, 0.13f, 0.165f, 4.3f}};
 
 // Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
-// round plus 0.3 of its share (as for the bf16 GEMM).  All six forms were timed on 33 products
-// with bf16 C and 21 with fp32 C of 58 to 5498 rows: it takes the fastest of each, or in one
-// case a form 3 % behind it (5498 x 7680 x 2560, fp32 C: 182 us, 177).
+// round plus 0.3 of its share (as for the bf16 GEMM).  All seven forms were timed on 36 products
+// of 17 to 5498 rows with either C: it takes the fastest of each but one, there a form 5 %
+// behind it (58 x 7680 x 512, bf16 C: 4.5 us, 4.3).
 float tile_cost(const Fp8Gemm& p, const Tile& t, int cus) {
-    const long tiles = ((long)p.N + 64 * t.ni - 1) / (64 * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
+    const long tiles = ((long)p.N + 32 * t.nw * t.ni - 1) / (32 * t.nw * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
     const float r = (float)tiles / cus, share = r < 1.f ? r : 1.f;
     const float rounds = r <= 1.f ? 1.f : 0.7f * (float)(long)(r + 0.9999f) + 0.3f * r;
     return rounds * ((t.alone + (t.full - t.alone) * share) * (float)(p.K / 128) + t.ends);
@@ -865,31 +874,33 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     const Tile* end = p.c_f32 ? FULL + sizeof(FULL) / sizeof(Tile) : FAST + sizeof(FAST) / sizeof(Tile);
     for (const Tile* x = t + 1; x < end; x++)
         if (tile_cost(p, *x, cus) < tile_cost(p, *t, cus)) t = x;
-    p.n_tiles = (p.N + 64 * t->ni - 1) / (64 * t->ni);
+    p.n_tiles = (p.N + 32 * t->nw * t->ni - 1) / (32 * t->nw * t->ni);
     p.m_tiles = (p.M + 64 * t->mj - 1) / (64 * t->mj);
     // two-stage forms: a workgroup per CU walks its tiles
     const long tiles = (long)p.n_tiles * p.m_tiles;
-    const dim3 grid(xcd_grid(t->ns == 2 && t->kg == 1 && tiles > cus ? cus : tiles)), block(256 * t->kg);
-#define TILE(E, NI, MJ, NS, KG)                                                         \
-    if (p.c_f32 == E && t->ni == NI && t->mj == MJ && t->kg == KG) {                   \
-        hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS, KG>), grid, block, 0, s, p); \
+    const dim3 grid(xcd_grid(t->ns == 2 && t->kg == 1 && tiles > cus ? cus : tiles)), block(128 * t->nw * t->kg);
+#define TILE(E, NI, MJ, NS, KG, NW)                                                        \
+    if (p.c_f32 == E && t->ni == NI && t->mj == MJ && t->ns == NS && t->kg == KG && t->nw == NW) { \
+        hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS, KG, NW>), grid, block, 0, s, p); \
         return hipGetLastError();                                                       \
     }
     if (!p.c_f32 && t->ni == 4 && t->mj == 4) {
         hipLaunchKernelGGL(gemm_fp8_wide_kernel, grid, block, 0, s, p);
         return hipGetLastError();
     }
-    TILE(0, 4, 3, 2, 1)
-    TILE(0, 2, 3, 3, 1)
-    TILE(0, 2, 2, 4, 1)
-    TILE(0, 2, 1, 3, 2)
-    TILE(0, 1, 1, 4, 2)
-    TILE(1, 4, 4, 2, 1)
-    TILE(1, 4, 3, 2, 1)
-    TILE(1, 4, 2, 2, 1)
-    TILE(1, 2, 2, 2, 2)
-    TILE(1, 2, 1, 3, 2)
-    TILE(1, 1, 1, 2, 4)
+    TILE(0, 4, 3, 2, 1, 2)
+    TILE(0, 2, 3, 3, 1, 2)
+    TILE(0, 2, 2, 4, 1, 2)
+    TILE(0, 2, 1, 3, 2, 2)
+    TILE(0, 1, 1, 4, 2, 2)
+    TILE(1, 4, 4, 2, 1, 2)
+    TILE(1, 4, 3, 2, 1, 2)
+    TILE(1, 4, 2, 2, 1, 2)
+    TILE(1, 2, 2, 2, 2, 2)
+    TILE(1, 2, 1, 3, 2, 2)
+    TILE(1, 1, 1, 2, 4, 2)
+    TILE(0, 1, 1, 3, 4, 1)
+    TILE(1, 1, 1, 3, 4, 1)
 #undef TILE
     return hipErrorInvalidValue;
 }
