@@ -44,9 +44,9 @@ __device__ inline bf16x8 widen(int lo, int hi, float scale) {
 // Up to 16 rows: 16 NI features per workgroup, the blocks of K in turn over its waves,
 // whose sums meet in LDS (in the waves' order).  Bound by W, which is read once,
 // straight into registers; A comes from the L2 again for every workgroup.  One row of
-// 7680 x 2560 takes 5.4 us (19.7 MB of W: 3.6 TB/s), of 2560 x 6912 6.5, 16 rows of 7680 x
-// 2560 6.3 (of which a launch and the fill of the chip are 2 to 3).  Widened to bf16: an
-// 8-bit instruction would save nothing where W's bytes bound.
+// 7680 x 2560 takes 5.4 us (19.7 MB of W: 3.6 TB/s), of 2560 x 6912 6.4, of 4096 x 11008 10.0
+// (4.5 TB/s), 16 rows of 7680 x 2560 6.1, of which a launch and the fill of the chip are 2 to
+// 3.  Widened to bf16: an 8-bit instruction would save nothing where W's bytes bound.
 template <int NI, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
     __shared__ f32x4 part[WAVES][NI][64];
@@ -864,10 +864,13 @@ void few_launch(const Fp8Gemm& p, hipStream_t s) {
 hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     const int cus = device_cus();
     if (p.M <= 16) {
-        // 32 features a workgroup where they leave one for every other CU (1 row, K = 2560: 5120
-        // features 7.7 us against 8.3, 2560 features 5.1 against 3.9)
-        if ((p.N + 31) / 32 >= cus / 2) few_launch<2, 4>(p, s);
-        else few_launch<1, 8>(p, s);
+        // 16 features a workgroup where its CU then has at most 3/4 of the features that 32 would
+        // give the busiest one (1 row: 4096 x 11008 10.0 us against 14.4, 12288 x 5120 12.4 against
+        // 13.8), else 32, which fetch A half as often (8000 x 5120 9.2 us either way, 16 rows 10.3
+        // against 12.6)
+        const int one = ((p.N + 15) / 16 + cus - 1) / cus, two = 2 * (((p.N + 31) / 32 + cus - 1) / cus);
+        if (4 * one <= 3 * two) few_launch<1, 8>(p, s);
+        else few_launch<2, 4>(p, s);
         return hipGetLastError();
     }
     const Tile* t = p.c_f32 ? FULL : FAST;
