@@ -864,13 +864,15 @@ void few_launch(const Fp8Gemm& p, hipStream_t s) {
 hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     const int cus = device_cus();
     if (p.M <= 16) {
-        // 16 features a workgroup where its CU then has at most 3/4 of the features that 32 would
-        // give the busiest one (1 row: 4096 x 11008 10.0 us against 14.4, 12288 x 5120 12.4 against
-        // 13.8), else 32, which fetch A half as often (8000 x 5120 9.2 us either way, 16 rows 10.3
-        // against 12.6)
-        const int one = ((p.N + 15) / 16 + cus - 1) / cus, two = 2 * (((p.N + 31) / 32 + cus - 1) / cus);
-        if (4 * one <= 3 * two) few_launch<1, 8>(p, s);
-        else few_launch<2, 4>(p, s);
+        // 16, 32 or 64 features a workgroup, by what the busiest CU fetches: its features, and for
+        // each of its workgroups A, as much as 4 + 3/4 M features (1 row: 4096 x 11008 10.0 us with
+        // 16, 14.4 with 32; 8000 x 5120 9.2 with 32 and 16; 24000 x 2560 12.5, 11.8 and 13.9; 16
+        // rows of 13824 x 2560 12.4, 10.2 and 9.3)
+        auto fetched = [&](int ni) { return ((p.N + 16 * ni - 1) / (16 * ni) + cus - 1) / cus * (64 * ni + 16 + 3 * p.M); };
+        const int f1 = fetched(1), f2 = fetched(2), f4 = fetched(4);
+        if (f4 < f1 && f4 < f2) few_launch<4, 4>(p, s);
+        else if (f2 < f1) few_launch<2, 4>(p, s);
+        else few_launch<1, 8>(p, s);
         return hipGetLastError();
     }
     const Tile* t = p.c_f32 ? FULL : FAST;

@@ -165,9 +165,11 @@ SIZES = [(1, 1, 128), (1, 7680, 2560), (2, 130, 640), (15, 257, 384), (16, 16, 5
 LARGE = [(6000, 4104, 256), (4300, 6600, 512), (5890, 4601, 1152), (6100, 4101, 1792), (4000, 4001, 1280)]
 # 64 x 64 tiles in groups of waves: more than a workgroup of 32 x 64 per CU
 WIDE = [(58, 15360, 640), (120, 9001, 896), (40, 16001, 128), (250, 2600, 1152)]
+# up to 16 rows: the widest share of features a workgroup, whole and cut
+FEW = [(16, 13824, 640), (9, 13801, 384), (1, 16000, 1152), (5, 4099, 1408)]
 
 
-@pytest.mark.parametrize("m,n,k", SIZES + LARGE + WIDE)
+@pytest.mark.parametrize("m,n,k", SIZES + LARGE + WIDE + FEW)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_gemm(awa, ctx, m, n, k, dtype):
     import torch
