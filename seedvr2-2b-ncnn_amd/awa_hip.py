@@ -56,6 +56,8 @@ class DitTimeWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("w_in", "b_in", "w_hid", "b_hid", "w_out", "b_out")]
 
 
+# the sizes that include/dit_ops.h accepts; checked here, since ctypes cuts what passes 32 bits
+OPS_ROWS_MAX, OPS_COLS_MAX, ROPE_MAX_HEADS = 1 << 24, 1 << 20, 32767
 ROPE_MAX_PAIRS, ROPE_MAX_AXES = 128, 4
 ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "bands": 3}
@@ -519,6 +521,10 @@ class Context:
         t.record_stream(current)
         return t
 
+    def _sizes(self, what, rows, *cols):
+        if rows > OPS_ROWS_MAX or max(cols, default=0) > OPS_COLS_MAX:
+            raise ValueError(f"{what}: at most {OPS_ROWS_MAX} rows and {OPS_COLS_MAX} columns, got {[rows, *cols]}")
+
     def _elsewhere(self, what, t):
         return ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
 
@@ -554,6 +560,7 @@ class Context:
         rows, cols = shape if len(shape) == 2 else (0, 0)
         if cols < 1 or (cols > 1 and st[1] != 1):
             raise ValueError("quant_fp8: x must be [rows, cols] with contiguous columns")
+        self._sizes("quant_fp8", rows, cols)
         if x.get_device() != self.device:
             raise self._elsewhere("quant_fp8", x)
         kp, groups, srows = (cols + 127) // 128 * 128, (cols + 511) // 512, (rows + 127) // 128 if blocks else rows
@@ -582,6 +589,7 @@ class Context:
             raise ValueError("gemm_fp8: a [M, K] and w [N, K]")
         M, K = shape
         N = wshape[0]
+        self._sizes("gemm_fp8", M, N, K)
         groups, nb = (K + 511) // 512, (N + 127) // 128
         dev = self.device
         if not (a.dtype in _e4m3 and w.dtype in _e4m3 and wshape[1] == K and a.is_contiguous() and w.is_contiguous() and
@@ -628,6 +636,7 @@ class Context:
         if len(shape) != 3:
             raise ValueError("rope: tensors must be [tokens, heads, head_d]")
         tokens, _, head_d = shape
+        self._sizes("rope", tokens)
         f = np.ascontiguousarray(freqs, np.float64)
         n, at = f.size, positions.shape
         axes = at[1] if len(at) == 2 else 1
@@ -648,6 +657,8 @@ class Context:
             if len(shape) != 3 or t.dtype != first.dtype or shape[0] != tokens or shape[2] != head_d or (
                     head_d > 1 and ts[2] != 1):
                 raise ValueError("rope: tensors must be [tokens, heads, head_d] of one dtype with contiguous channels")
+            if shape[1] > ROPE_MAX_HEADS:
+                raise ValueError(f"rope: at most {ROPE_MAX_HEADS} heads, got {shape[1]}")
             if o is None:
                 o = self._empty(t.dtype, stream, *shape)
             elif o.shape != shape or o.dtype != t.dtype or (head_d > 1 and o.stride(2) != 1):

@@ -74,6 +74,50 @@ def test_binding_refuses_host_tensors(awa):
             call()
 
 
+def meta_context(awa, monkeypatch):
+    """(a context for tensors without memory, the calls that reach the library), whose entry points only count."""
+    import torch
+
+    class Entries:
+        def __getattr__(self, name):
+            return lambda *args: calls.append((name, args)) or 0
+
+    ctx, calls = awa.Context.__new__(awa.Context), []
+    ctx.ptr, ctx.device, ctx._on = None, -1, torch.device("meta")
+    monkeypatch.setattr(awa, "lib", Entries)
+    monkeypatch.setattr(awa.Context, "_stream", lambda self, stream: 0)
+    return ctx, calls
+
+
+def test_binding_refuses_sizes_past_32_bits(awa, monkeypatch):
+    """Sizes whose low 32 bits the entry points would take: the rest was neither computed nor refused."""
+    import torch
+    ctx, calls = meta_context(awa, monkeypatch)
+    e4m3, e8m0, far = torch.float8_e4m3fn, torch.float8_e8m0fnu, 2 ** 32
+
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    def matrix(rows, cols, blocks):
+        return (empty(rows, cols, dtype=e4m3),
+                empty((cols + 511) // 512, (rows + 127) // 128 if blocks else rows, 4, dtype=e8m0))
+
+    ctx.quant_fp8(empty(5, 128))
+    ctx.gemm_fp8(*matrix(5, 128, False), *matrix(7, 128, True))
+    ctx.rope(empty(5, 1, 2), empty(5, dtype=torch.int32), [1.0])
+    assert [name for name, _ in calls] == ["dit_quant_fp8", "dit_gemm_fp8", "dit_rope"]
+    for call in (lambda: ctx.quant_fp8(empty(far + 5, 128)), lambda: ctx.quant_fp8(empty(5, far + 128)),
+                 lambda: ctx.quant_fp8(empty(2 ** 24 + 1, 128)), lambda: ctx.quant_fp8(empty(5, 2 ** 20 + 1), blocks=True),
+                 lambda: ctx.gemm_fp8(*matrix(far + 5, 128, False), *matrix(7, 128, True)),
+                 lambda: ctx.gemm_fp8(*matrix(5, 128, False), *matrix(far + 7, 128, True)),
+                 lambda: ctx.gemm_fp8(*matrix(5, far + 128, False), *matrix(7, far + 128, True)),
+                 lambda: ctx.rope(empty(far + 5, 1, 2), empty(far + 5, dtype=torch.int32), [1.0]),
+                 lambda: ctx.rope(empty(5, far + 1, 2), empty(5, dtype=torch.int32), [1.0])):
+        with pytest.raises(ValueError, match="at most"):
+            call()
+    assert len(calls) == 3
+
+
 def test_product_reads_sums_after_their_wait_states(tmp_path):
     """The static check of the other matrix kernels over the 8-bit product's: its sums pass through empty asm
     statements, which the compiler does not wait before."""
