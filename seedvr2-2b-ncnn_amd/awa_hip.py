@@ -501,6 +501,9 @@ class Context:
         return emb
 
     # ---- operators around a projection in 8 bits (include/dit_ops.h)
+    # stream= (default: the current stream of the context's device) orders nothing: the caller lets that stream wait
+    # for what made a call's tensors, and waits for it before reading results or changing inputs.  Tensors may be
+    # dropped as soon as a call returns: their memory is marked as used on its stream.
     def _stream(self, stream):
         """The stream of a call: the given one, else the current one of the context's device."""
         if stream is None:
@@ -520,6 +523,12 @@ class Context:
             t = _torch.empty(*shape, dtype=dtype, device=self._on)
         t.record_stream(current)
         return t
+
+    def _used(self, stream, *tensors):
+        """Keeps the memory of a call's tensors from other use until the given stream has passed the call."""
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
 
     def _sizes(self, what, rows, *cols):
         if rows > OPS_ROWS_MAX or max(cols, default=0) > OPS_COLS_MAX:
@@ -573,6 +582,8 @@ class Context:
         else:
             self._bytes_of("quant_fp8", scale, "scale", _e8m0, groups, srows, 4)
         if rows:
+            if stream is not None:
+                self._used(stream, x, q, scale)
             rc = lib_.dit_quant_fp8(self.ptr, dtype, x.data_ptr(), st[0], rows, cols, 128 if blocks else 1,
                                     q.data_ptr(), scale.data_ptr(), srows, self._stream(stream))
             if rc:
@@ -611,6 +622,8 @@ class Context:
             if bias.get_device() != self.device:
                 raise self._elsewhere("gemm_fp8", bias)
         if M:
+            if stream is not None:
+                self._used(stream, a, a_scale, w, w_scale, bias, out)
             rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), ld_as, w.data_ptr(), w_scale.data_ptr(), ld_ws,
                                    bias.data_ptr() if bias is not None else None, ct, out.data_ptr(), out.stride(0), M, N,
                                    K, self._stream(stream))
@@ -668,6 +681,8 @@ class Context:
             res.append(o)
             os_ = o.stride()
             rows += _ROWS.pack(t.data_ptr(), o.data_ptr(), shape[1], ts[0], ts[1], os_[0], os_[1])
+        if stream is not None:
+            self._used(stream, positions, *xs, *res)
         rc = lib_.dit_rope(self.ptr, dtype, rows, len(xs), tokens, head_d, plan, positions.data_ptr(),
                            self._stream(stream))
         if rc:

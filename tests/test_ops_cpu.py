@@ -118,6 +118,37 @@ def test_binding_refuses_sizes_past_32_bits(awa, monkeypatch):
     assert len(calls) == 3
 
 
+def test_tensors_of_another_stream_are_marked(awa, monkeypatch):
+    """Each tensor of a call on a given stream is marked as used there, so that its memory outlives the call."""
+    import torch
+    ctx, calls = meta_context(awa, monkeypatch)
+    monkeypatch.setattr(awa.Context, "_empty", lambda self, dtype, stream, *shape: torch.empty(shape, dtype=dtype, device="meta"))
+    marked, stream = [], object()
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: marked.append((t, s)))
+
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    def check(*tensors):
+        assert all(s is stream for _, s in marked)
+        assert {id(t) for t in tensors} <= {id(t) for t, _ in marked}
+        marked.clear()
+
+    x, wt, bias = empty(5, 128), empty(130, 128), empty(130, dtype=torch.float32)
+    a, w = ctx.quant_fp8(x), ctx.quant_fp8(wt, blocks=True)
+    assert not marked
+    check(x, *ctx.quant_fp8(x, stream=stream))
+    ctx.quant_fp8(x, q=a[0], scale=a[1], stream=stream)
+    check(x, *a)
+    check(*a, *w, bias, ctx.gemm_fp8(*a, *w, bias=bias, stream=stream))
+    out = empty(5, 130)
+    ctx.gemm_fp8(*a, *w, out=out, stream=stream)
+    check(*a, *w, out)
+    q, k, pos = empty(5, 3, 64), empty(5, 1, 64), empty(5, dtype=torch.int32)
+    check(q, k, pos, *ctx.rope((q, k), pos, [1.0] * 32, stream=stream))
+    assert len(calls) == 7
+
+
 def test_product_reads_sums_after_their_wait_states(tmp_path):
     """The static check of the other matrix kernels over the 8-bit product's: its sums pass through empty asm
     statements, which the compiler does not wait before."""

@@ -575,3 +575,31 @@ def test_results_of_another_stream(awa, ctx):
     torch.cuda.synchronize()
     for g, r in zip(got, (q, s, want, turned)):
         assert torch.equal(g.view(torch.uint8), r.view(torch.uint8))
+
+
+def test_inputs_dropped_before_another_stream_has_read_them(awa, ctx):
+    """Inputs given up as the call returns are not overwritten while its stream, still busy, has yet to read them."""
+    import torch
+    x, wt, bias, pos, freqs = layer_inputs(awa, ctx, 700, 3)
+    w = ctx.quant_fp8(wt, blocks=True)
+    q, s = ctx.quant_fp8(x)
+    qkv = ctx.gemm_fp8(q, s, *w, bias=bias)
+    heads, args = qkv.unflatten(1, (12, 128)), dict(pairs=(21, 21, 21))
+    want = [q, s, qkv, ctx.rope(heads, pos, freqs, **args)]
+    side, big = torch.cuda.Stream(), torch.ones(1 << 28, device="cuda")
+    temps = [t.clone() for t in (x, q, s, *w, bias, heads, pos)]
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):  # 8 passes over 1 GiB: over a millisecond
+            big.mul_(1.0)
+    got = [*ctx.quant_fp8(temps[0], stream=side), ctx.gemm_fp8(*temps[1:5], bias=temps[5], stream=side),
+           ctx.rope(temps[6], temps[7], freqs, stream=side, **args)]
+    shapes = [(t.shape, t.dtype) for t in temps]
+    del temps
+    late = [torch.empty(*shape, dtype=dtype, device="cuda") for shape, dtype in shapes for _ in range(2)]
+    for t in late:
+        t.view(torch.uint8).fill_(85)
+    torch.cuda.synchronize()
+    for g, r in zip(got, want):
+        assert torch.equal(g.view(torch.uint8), r.view(torch.uint8))
