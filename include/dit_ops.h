@@ -74,9 +74,15 @@ int dit_quant_fp8(awa_ctx* ctx, int dtype, const void* d_x, int64_t ldx, int M, 
  * round to 2^128 (of fp32 magnitudes from 248 2^120 on) as infinite.  For bf16 C
  * of more rows the 8-bit matrix instructions sum: they align the products of
  * eight consecutive columns to the largest of them and drop what lies 13 bits
- * below its leading one, about 1.5e-5 of a sum and a hundredth of bf16's step.
+ * below its leading one.  Each of the seven others loses less than 2^-13 of the
+ * largest (nothing where its exponent is up to 6 lower): less than 7 2^-13 of the
+ * sum of the groups' largest magnitudes for any data.  Measured at K = 2560 and
+ * 6912 before C's rounding: 1.5e-5 of the sums (both as root mean squares) for
+ * normal data, 9e-5 where one column in eight is 256 or 2048 times the others, a
+ * 260th and a 43rd of bf16's step.  A sum that cancels keeps its error whole.
  * The result of a row does not depend on the other rows of A, but on their number
- * in the order of its sums; the same call gives the same bits.
+ * in the order of its sums (and, past 16 with bf16 C, in what enters them); the same
+ * call gives the same bits.
  * Rejected (AWA_EARG): sizes out of range, K not a multiple of 128, ldc < N (for
  * M > 1), ld_as < M, ld_ws < ceil(N / 128), a misaligned pointer (A and W 16
  * bytes, scales and bias 4, C its elements), C over an input. */

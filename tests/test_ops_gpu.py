@@ -192,6 +192,38 @@ def test_gemm(awa, ctx, m, n, k, dtype):
            bar + (2.0 ** -24 + half_step(dt(dtype))) * (ref.abs() + bias.abs()))
 
 
+@pytest.mark.parametrize("m", [17, 32, 300, 1500, 6000])
+@pytest.mark.parametrize("times", [1, 16, 256, 2048])
+@pytest.mark.parametrize("k", [640, 2560])
+def test_gemm_loses_no_more_than_stated(awa, ctx, m, times, k):
+    """What the 8-bit sums of bf16 C drop, before C's rounding: rows alike and a bias of minus the exact result (in
+    fp32, the difference kept) leave the error itself.  A product loses less than s = 2^(e - 13), e the exponent of its
+    group's largest, and nothing if it is a multiple of s.  Bars: for each result the sum of s over the products that
+    are none (and what an fp32 sum may lose, as in gemm_bar); over all of them, since the losses have their products'
+    signs, which are independent here, the root of the mean sum of s^2 (and K / 8 + 1 random additions of half a step
+    of sums no larger than the last, in the root mean square)."""
+    import torch
+    n = 2048
+    g = torch.Generator(device="cuda").manual_seed(m + k + times)
+    x = torch.randn((1, k), generator=g, device="cuda")
+    x[:, ::8] *= times
+    a, w = ctx.quant_fp8(x), ctx.quant_fp8(torch.randn((n, k), generator=g, device="cuda") * 0.02, blocks=True)
+    va, vw = awa.fp8_values(*a).double(), awa.fp8_values(*w).double()
+    p = (va * vw).abs().unflatten(1, (-1, 8))
+    exact = (va * vw).sum(1)
+    bias = -exact.float()
+    out = ctx.gemm_fp8(a[0].view(torch.uint8).expand(m, -1).contiguous(), a[1].view(torch.uint8).expand(-1, m, -1).contiguous(),
+                       *w, bias=bias)
+    assert bool((out == out[0]).all())
+    e = out[0].double() - (exact + bias.double())
+    s = torch.exp2(torch.floor(torch.log2(p.amax(2, keepdim=True))) - 13)
+    s = torch.where(torch.remainder(p, s) != 0, s, 0.0)
+    most = s.sum((1, 2)) + (4 * k / 128 + 16) * 2.0 ** -24 * p.sum((1, 2)) + 2.0 ** -24 * exact.abs()
+    within(e, torch.zeros_like(e), most * (1 + 2.0 ** -8))
+    rms = math.sqrt(float((s ** 2).sum((1, 2)).mean())) + math.sqrt(k / 8 + 1) * 2.0 ** -24 * math.sqrt(float((exact ** 2).mean()))
+    assert math.sqrt(float((e ** 2).mean())) <= rms * (1 + 2.0 ** -8)
+
+
 def test_gemm_misaligned_output(awa, ctx):
     """An output that begins at an odd element: no 16-byte stores."""
     import torch
