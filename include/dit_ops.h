@@ -64,6 +64,8 @@ enum { DIT_FP8_BLOCK = 128 };
 int dit_quant_fp8(awa_ctx* ctx, int dtype, const void* d_x, int64_t ldx, int M, int K, int block_rows,
                   uint8_t* d_q, uint32_t* d_scale, int64_t ld_scale, awa_stream_t stream);
 
+enum { DIT_FP8_WHOLE = 256 };
+
 /* C[m][n] = sum over k of A[m][k] W[n][k], plus bias[n] (fp32, may be NULL): A is
  * [M][K] in e4m3 rows with a scale per row and block, W [N][K] with a scale per
  * 128 x 128 block (both as dit_quant_fp8 writes them; K is their padded width, a
@@ -80,6 +82,8 @@ int dit_quant_fp8(awa_ctx* ctx, int dtype, const void* d_x, int64_t ldx, int M, 
  * 6912 before C's rounding: 1.5e-5 of the sums (both as root mean squares) for
  * normal data, 9e-5 where one column in eight is 256 or 2048 times the others, a
  * 260th and a 43rd of bf16's step.  A sum that cancels keeps its error whole.
+ * dtype_c AWA_BF16 | DIT_FP8_WHOLE lets products enter whole for any number of rows,
+ * at the time of fp32 C: the bits are those of the fp32 C, rounded.
  * The result of a row does not depend on the other rows of A, but on their number
  * in the order of its sums (and, past 16 with bf16 C, in what enters them); the same
  * call gives the same bits.

@@ -19,6 +19,7 @@ HEADER_DIR = os.path.join(os.path.dirname(HERE), "include")
 
 AWA_OK, AWA_EARG, AWA_EHIP = 0, -1, -2
 AWA_F32, AWA_BF16 = 0, 1
+DIT_FP8_WHOLE = 256
 HEADS, HEAD_D, DIM, QKV, ROPE_ROT = 20, 128, 2560, 7680, 126
 
 _lib = None
@@ -590,10 +591,11 @@ class Context:
                 self.check(rc, "dit_quant_fp8")
         return q, scale
 
-    def gemm_fp8(self, a, a_scale, w, w_scale, bias=None, out=None, dtype=None, stream=None):
+    def gemm_fp8(self, a, a_scale, w, w_scale, bias=None, out=None, dtype=None, stream=None, whole=False):
         """dit_gemm_fp8: [M, N] = A W^T (+ bias fp32 [N]) of matrices as quant_fp8 returns them, A by rows and W
         with blocks=True, or of rows cut from them (a[i:j], a_scale[:, i:j]); `dtype` bf16 (default) or fp32, or that
-        of `out` (rows may be strided)."""
+        of `out` (rows may be strided).  whole=True (DIT_FP8_WHOLE): for bf16 too, sums as exact as those of fp32
+        results, in their time."""
         lib_ = lib()
         shape, wshape = a.shape, w.shape
         if len(shape) != 2 or len(wshape) != 2:
@@ -625,8 +627,8 @@ class Context:
             if stream is not None:
                 self._used(stream, a, a_scale, w, w_scale, bias, out)
             rc = lib_.dit_gemm_fp8(self.ptr, a.data_ptr(), a_scale.data_ptr(), ld_as, w.data_ptr(), w_scale.data_ptr(), ld_ws,
-                                   bias.data_ptr() if bias is not None else None, ct, out.data_ptr(), out.stride(0), M, N,
-                                   K, self._stream(stream))
+                                   bias.data_ptr() if bias is not None else None, ct | DIT_FP8_WHOLE if whole else ct,
+                                   out.data_ptr(), out.stride(0), M, N, K, self._stream(stream))
             if rc:
                 self.check(rc, "dit_gemm_fp8")
         return out

@@ -135,15 +135,17 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 // refills the freed stage, the DMA pieces between its instructions.  A row's scale
 // word travels with its stage, and W's, which are the same for a whole wave.
 //
-// EXACT (fp32 C): the fragments are widened to bf16 with their scales and take four
-// 32x32x16 bf16 instructions in place of one 8-bit one.
+// EXACT (fp32 C, and bf16 C where the caller asks for whole products): the fragments are
+// widened to bf16 with their scales and take four 32x32x16 bf16 instructions in place of
+// one 8-bit one.
 //
 // Bound by what a tile's operands take from the L2 where the tiles are small, and by the
 // chip's power where they are large (a loop of 8-bit instructions alone reaches 4.0 to 4.1
 // PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 6.1 us, 679 x 2560 x 6912 19.7 (1.22
 // PFLOP/s), 1237 x 1999 x 2816 15.3, 1400 x 13824 x 2560 50 to 53 (1.9).  fp32 C: 679 x
 // 2560 x 6912 32 to 34 us (0.72), 5498 x 13824 x 2560 322 (1.21), 8192^3 752 (1.46; the
-// library's bf16 product 1.31).
+// library's bf16 product 1.31).  bf16 C of whole products: 58 x 7680 x 2560 7.6 us, 1237 x
+// 1999 x 2816 24.1, 679 x 2560 x 6912 32.5, 5498 x 13824 x 2560 305.
 constexpr int ROW = 128;  // bytes of a block's row
 
 // A buffer resource with wave-uniform fields (as in dit_gemm.hip): loads past
@@ -251,7 +253,7 @@ __device__ inline void epilogue(const Fp8Gemm& p, const f32x16 (&acc)[NI][MJ], i
 // A group of 2 NW waves (NW over n, two over m) makes the tile; KG of them take the blocks of
 // K in turn, each with stages of its own, for products of few tiles; their sums meet in LDS at
 // the end, in the groups' order.
-template <bool EXACT, int NI, int MJ, int NS, int KG, int NW>
+template <bool EXACT, bool F32, int NI, int MJ, int NS, int KG, int NW>
 __global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     constexpr int BN = 32 * NW * NI, BM = 64 * MJ;
     constexpr int GW = 2 * NW, GT = 64 * GW;  // waves and threads of a group
@@ -539,8 +541,8 @@ __global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
         int l = 0;
         asm volatile("" : "+v"(l));
         l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, l));
-        if (p.bias) epilogue<EXACT, true, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
-        else epilogue<EXACT, false, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
+        if (p.bias) epilogue<F32, true, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
+        else epilogue<F32, false, NI, MJ>(p, acc, n0 + wn * 32 * NI, m0 + wm * 32 * MJ, l, stg);
         tile += stride;
         if (!WALK || tile >= end) break;
     }
@@ -880,8 +882,9 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
         else few_launch<1, 8>(p, s);
         return hipGetLastError();
     }
-    const Tile* t = p.c_f32 ? FULL : FAST;
-    const Tile* end = p.c_f32 ? FULL + sizeof(FULL) / sizeof(Tile) : FAST + sizeof(FAST) / sizeof(Tile);
+    const bool exact = p.c_f32 || p.whole;
+    const Tile* t = exact ? FULL : FAST;
+    const Tile* end = exact ? FULL + sizeof(FULL) / sizeof(Tile) : FAST + sizeof(FAST) / sizeof(Tile);
     for (const Tile* x = t + 1; x < end; x++)
         if (tile_cost(p, *x, cus) < tile_cost(p, *t, cus)) t = x;
     p.n_tiles = (p.N + 32 * t->nw * t->ni - 1) / (32 * t->nw * t->ni);
@@ -889,28 +892,30 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     // two-stage forms: a workgroup per CU walks its tiles
     const long tiles = (long)p.n_tiles * p.m_tiles;
     const dim3 grid(xcd_grid(t->ns == 2 && t->kg == 1 && tiles > cus ? cus : tiles)), block(128 * t->nw * t->kg);
-#define TILE(E, NI, MJ, NS, KG, NW)                                                        \
-    if (p.c_f32 == E && t->ni == NI && t->mj == MJ && t->ns == NS && t->kg == KG && t->nw == NW) { \
-        hipLaunchKernelGGL((gemm_fp8_kernel<E, NI, MJ, NS, KG, NW>), grid, block, 0, s, p); \
-        return hipGetLastError();                                                       \
+#define TILE(E, F, NI, MJ, NS, KG, NW)                                                               \
+    if (exact == E && p.c_f32 == F && t->ni == NI && t->mj == MJ && t->ns == NS && t->kg == KG && t->nw == NW) { \
+        hipLaunchKernelGGL((gemm_fp8_kernel<E, F, NI, MJ, NS, KG, NW>), grid, block, 0, s, p);         \
+        return hipGetLastError();                                                                    \
     }
-    if (!p.c_f32 && t->ni == 4 && t->mj == 4) {
+#define FULL_TILE(NI, MJ, NS, KG, NW) TILE(1, 1, NI, MJ, NS, KG, NW) TILE(1, 0, NI, MJ, NS, KG, NW)
+    if (!exact && t->ni == 4 && t->mj == 4) {
         hipLaunchKernelGGL(gemm_fp8_wide_kernel, grid, block, 0, s, p);
         return hipGetLastError();
     }
-    TILE(0, 4, 3, 2, 1, 2)
-    TILE(0, 2, 3, 3, 1, 2)
-    TILE(0, 2, 2, 4, 1, 2)
-    TILE(0, 2, 1, 3, 2, 2)
-    TILE(0, 1, 1, 4, 2, 2)
-    TILE(1, 4, 4, 2, 1, 2)
-    TILE(1, 4, 3, 2, 1, 2)
-    TILE(1, 4, 2, 2, 1, 2)
-    TILE(1, 2, 2, 2, 2, 2)
-    TILE(1, 2, 1, 3, 2, 2)
-    TILE(1, 1, 1, 2, 4, 2)
-    TILE(0, 1, 1, 3, 4, 1)
-    TILE(1, 1, 1, 3, 4, 1)
+    TILE(0, 0, 4, 3, 2, 1, 2)
+    TILE(0, 0, 2, 3, 3, 1, 2)
+    TILE(0, 0, 2, 2, 4, 1, 2)
+    TILE(0, 0, 2, 1, 3, 2, 2)
+    TILE(0, 0, 1, 1, 4, 2, 2)
+    TILE(0, 0, 1, 1, 3, 4, 1)
+    FULL_TILE(4, 4, 2, 1, 2)
+    FULL_TILE(4, 3, 2, 1, 2)
+    FULL_TILE(4, 2, 2, 1, 2)
+    FULL_TILE(2, 2, 2, 2, 2)
+    FULL_TILE(2, 1, 3, 2, 2)
+    FULL_TILE(1, 1, 2, 4, 2)
+    FULL_TILE(1, 1, 3, 4, 1)
+#undef FULL_TILE
 #undef TILE
     return hipErrorInvalidValue;
 }

@@ -115,6 +115,8 @@ int dit_gemm_fp8(awa_ctx* ctx, const uint8_t* d_a, const uint32_t* d_as, int64_t
                  const uint32_t* d_ws, int64_t ld_ws, const float* d_bias, int dtype_c, void* d_c, int64_t ldc,
                  int M, int N, int K, awa_stream_t stream) {
     if (!ctx) return AWA_EARG;
+    const bool whole = dtype_c == (AWA_F32 | DIT_FP8_WHOLE) || dtype_c == (AWA_BF16 | DIT_FP8_WHOLE);
+    if (whole) dtype_c &= ~DIT_FP8_WHOLE;
     if (!d_a || !d_as || !d_w || !d_ws || !d_c || !dtype_ok(dtype_c) || M < 0 || M > DIT_OPS_ROWS_MAX || N < 1 ||
         N > DIT_OPS_COLS_MAX || K < DIT_FP8_BLOCK || K % DIT_FP8_BLOCK || K > DIT_OPS_COLS_MAX) {
         set_err(ctx, "dit_gemm_fp8: bad argument dtype=%d M=%d N=%d K=%d (M <= %d, N, K <= %d, K %% %d == 0)", dtype_c, M,
@@ -141,6 +143,7 @@ int dit_gemm_fp8(awa_ctx* ctx, const uint8_t* d_a, const uint32_t* d_as, int64_t
     p.C = d_c; p.ldc = M > 1 ? ldc : N;
     p.M = M; p.N = N; p.K = K;
     p.c_f32 = dtype_c == AWA_F32;
+    p.whole = whole;
     p.c_vec = aligned(d_c, 16) && p.ldc * elem(dtype_c) % 16 == 0;
     const size_t cb = span(M, p.ldc, N, elem(dtype_c));
     const int64_t g = groups_of(K);

@@ -29,6 +29,7 @@ struct Fp8Gemm {
     int64_t ldc;
     int M, N, K;
     int c_f32;           // C fp32, else bf16
+    int whole;           // bf16 C: every product enters the sums whole
     int c_vec;           // C's rows allow 16-byte stores
     int n_tiles, m_tiles;
 };

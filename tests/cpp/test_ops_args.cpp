@@ -88,6 +88,12 @@ int main() {
     check("gemm no rows", gemm(Q, S, 0, W, SW, 2, nullptr, AWA_BF16, C, 200, 0, 200, 256), ok, 0);
     check("gemm one row, any stride", gemm(Q, S, 1, W, SW, 2, nullptr, AWA_F32, C, 0, 1, 200, 256), ok);
     check("gemm unaligned C", gemm(Q, S, 5, W, SW, 2, X, AWA_BF16, C + 2, 201, 5, 200, 256), ok);
+    check("gemm whole", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16 | DIT_FP8_WHOLE, C, 200, 5, 200, 256), ok);
+    check("gemm whole fp32", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_F32 | DIT_FP8_WHOLE, C, 200, 5, 200, 256), ok);
+    check("gemm whole dtype", gemm(Q, S, 5, W, SW, 2, nullptr, 7 | DIT_FP8_WHOLE, C, 200, 5, 200, 256), bad);
+    check("gemm other flag", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16 | 2 * DIT_FP8_WHOLE, C, 200, 5, 200, 256), bad);
+    check("gemm whole and other flag", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_BF16 | 3 * DIT_FP8_WHOLE, C, 200, 5, 200, 256), bad);
+    check("gemm whole c alignment", gemm(Q, S, 5, W, SW, 2, nullptr, AWA_F32 | DIT_FP8_WHOLE, C + 2, 200, 5, 200, 256), bad);
     check("gemm null a", gemm(nullptr, S, 5, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);
     check("gemm null as", gemm(Q, nullptr, 5, W, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);
     check("gemm null w", gemm(Q, S, 5, nullptr, SW, 2, nullptr, AWA_BF16, C, 200, 5, 200, 256), bad);

@@ -224,6 +224,46 @@ def test_gemm_loses_no_more_than_stated(awa, ctx, m, times, k):
     assert math.sqrt(float((e ** 2).mean())) <= rms * (1 + 2.0 ** -8)
 
 
+# each form of whole products, some walking over several tiles (the last three), with and without whole chunks
+@pytest.mark.parametrize("m,n,k", [(5, 300, 384), (17, 2560, 384), (300, 2560, 512), (120, 9001, 896), (700, 3000, 256),
+                                   (671, 7601, 640), (1793, 8244, 640), (2305, 6673, 640), (3467, 6679, 640)])
+def test_gemm_whole(awa, ctx, m, n, k):
+    """bf16 C with whole products: the bits of the fp32 C, rounded; rows wider than C keep their other values."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    a, sa, _ = fp8_matrix(awa, ctx, m, k, False, g, spread=6)
+    w, sw, _ = fp8_matrix(awa, ctx, n, k, True, g, spread=3)
+    for bias in (None, torch.randn(n, generator=g, device="cuda") * 100):
+        want = ctx.gemm_fp8(a, sa, w, sw, bias=bias, dtype=torch.float32)
+        assert torch.equal(ctx.gemm_fp8(a, sa, w, sw, bias=bias, dtype=torch.float32, whole=True), want)
+        assert torch.equal(ctx.gemm_fp8(a, sa, w, sw, bias=bias, whole=True), want.bfloat16())
+        buf = torch.full((m + 2, n + 9), 7.0, dtype=torch.bfloat16, device="cuda")
+        ctx.gemm_fp8(a, sa, w, sw, bias=bias, out=buf[1:-1, :n], whole=True)
+        assert torch.equal(buf[1:-1, :n], want.bfloat16())
+        assert bool((buf[0] == 7).all()) and bool((buf[-1] == 7).all()) and bool((buf[:, n:] == 7).all())
+
+
+@pytest.mark.parametrize("m", [16, 17, 700, 6000])
+def test_gemm_whole_cancels(awa, ctx, m):
+    """Sums that cancel keep their bits with whole products, whatever the number of rows: the difference to a bias of
+    minus the exact result is within what an fp32 sum may lose (gemm_bar's first part and the addition's 2^-24), where
+    one column in eight is 2048 times the others."""
+    import torch
+    k, n = 1280, 1000
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn((1, k), generator=g, device="cuda")
+    x[:, ::8] *= 2048
+    a, w = ctx.quant_fp8(x), ctx.quant_fp8(torch.randn((n, k), generator=g, device="cuda"), blocks=True)
+    va, vw = awa.fp8_values(*a).double(), awa.fp8_values(*w).double()
+    exact = (va @ vw.T)[0]
+    bias = -exact.float()
+    out = ctx.gemm_fp8(a[0].view(torch.uint8).expand(m, -1).contiguous(), a[1].view(torch.uint8).expand(-1, m, -1).contiguous(),
+                       *w, bias=bias, whole=True)
+    e = exact + bias.double()
+    bar = (4 * k / 128 + 16) * 2.0 ** -24 * (va.abs() @ vw.abs().T)[0] + 2.0 ** -24 * exact.abs()
+    within(out, e.expand(m, -1), (bar + 2.0 ** -8 * (e.abs() + bar)).expand(m, -1))
+
+
 def test_gemm_misaligned_output(awa, ctx):
     """An output that begins at an odd element: no 16-byte stores."""
     import torch
