@@ -224,6 +224,59 @@ def test_gemm_loses_no_more_than_stated(awa, ctx, m, times, k):
     assert math.sqrt(float((e ** 2).mean())) <= rms * (1 + 2.0 ** -8)
 
 
+# tiles of 256 rows or features, more of them than CUs, over two to six scale words of odd strides: for fp32 C (1793 x
+# 8244 and 2093 x 7582) 256 x 128, 495 and 510 of them, (2305 x 6673) 256 x 192, 351, (3501 x 7000) 256 x 256, 392; for
+# bf16 C 256 x 192 and (3501 x 7000) 256 x 256
+WALKS = [(1793, 8244, 640), (2305, 6673, 640), (3501, 7000, 1664), (2093, 7582, 2688)]
+
+
+@pytest.mark.parametrize("m,n,k", WALKS)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gemm_walks(awa, ctx, m, n, k, dtype):
+    test_gemm(awa, ctx, m, n, k, dtype)
+
+
+@pytest.mark.parametrize("m,n", [(40, 600), (250, 2600), (500, 2600), (700, 3300), (671, 8001), (2400, 7000), (3501, 7000)])
+@pytest.mark.parametrize("ld", [0, 1, 2, 3])
+def test_gemm_scales_at_any_word(awa, ctx, m, n, ld):
+    """Scale words that begin 4, 8 and 12 bytes off 16, at strides of any remainder, in every form: rows cut at 1, 2 and
+    3 give the bits of their copies."""
+    import torch
+    k = 1664  # four words a row
+    g = torch.Generator(device="cuda").manual_seed(m + ld)
+    a, sa, _ = fp8_matrix(awa, ctx, m + 4 + ld, k, False, g, spread=6)
+    w, sw, _ = fp8_matrix(awa, ctx, n + 128 * ld, k, True, g, spread=3)
+    for r in (1, 2, 3):
+        ca, csa = a[r:r + m], sa[:, r:r + m]
+        cw, csw = w[128 * (r % (ld + 1)):][:n], sw[:, r % (ld + 1):][:, :-(-n // 128)]
+        for t in (BF16, F32):
+            want = ctx.gemm_fp8(ca.clone(), csa.contiguous(), cw.clone(), csw.contiguous(), dtype=dt(t))
+            assert torch.equal(ctx.gemm_fp8(ca, csa, cw, csw, dtype=dt(t)), want)
+
+
+@pytest.mark.parametrize("m,n", [(1, 300), (16, 300), (20, 300), (250, 2600), (700, 2560), (700, 7601), (2500, 7681), (6000, 4104)])
+@pytest.mark.parametrize("side", ["rows", "weights"])
+def test_gemm_least_scale(awa, ctx, m, n, side):
+    """Scale byte 0 is 2^-127 like any other: values of 2 to 448 times it, against scales of 2^60."""
+    import torch
+    k = 768
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+
+    def matrix(rows, blocks, byte):
+        v = torch.rand((rows, k), generator=g, device="cuda") * 446 + 2
+        q = torch.where(torch.rand((rows, k), generator=g, device="cuda") < 0.5, v, -v).to(torch.float8_e4m3fn)
+        s = torch.full((2, -(-rows // 128) if blocks else rows, 4), byte, dtype=torch.uint8, device="cuda")
+        return q, s.view(torch.float8_e8m0fnu), q.double() * 2.0 ** (byte - 127)
+
+    a, sa, va = matrix(m, False, 0 if side == "rows" else 187)
+    w, sw, vw = matrix(n, True, 187 if side == "rows" else 0)
+    ref = va @ vw.T
+    for t in (BF16, F32):
+        within(ctx.gemm_fp8(a, sa, w, sw, dtype=dt(t)), ref, gemm_bar(va, vw, ref, dt(t), k))
+    for q, s, v, per in ((a, sa, va, 1), (w, sw, vw, 128)):
+        assert torch.equal(awa.fp8_values(q, s).double(), v)
+
+
 # each form of whole products, some walking over several tiles (the last three), with and without whole chunks
 @pytest.mark.parametrize("m,n,k", [(5, 300, 384), (17, 2560, 384), (300, 2560, 512), (120, 9001, 896), (700, 3000, 256),
                                    (671, 7601, 640), (1793, 8244, 640), (2305, 6673, 640), (3467, 6679, 640)])
