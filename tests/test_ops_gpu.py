@@ -89,6 +89,42 @@ def test_quant(ctx, dtype, rows, cols, ld, blocks):
     check_quant(q, s, x, 128 if blocks else 1)
 
 
+# rows times groups of 512 columns from 16384 on: two rows a wave, eight a workgroup, here with 1 to 7 left over
+@pytest.mark.parametrize("rows,cols,ld", [(16387, 130, 131), (5499, 1537, 1540), (27259, 200, 200), (16385, 1, 1),
+                                          (8198, 600, 611), (4100, 2048, 2048), (3282, 2560, 2561)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quant_two_rows_a_wave(ctx, awa, dtype, rows, cols, ld):
+    """Against the definition, and with guard rows and words after the last row."""
+    import torch
+    groups, kp = -(-cols // 512), -(-cols // 128) * 128
+    assert rows * groups >= 16384 and rows % 8
+    test_quant(ctx, dtype, rows, cols, ld, False)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, cols), generator=g, device="cuda").to(dt(dtype))
+    q = torch.full((rows + 9, kp), 99, dtype=torch.uint8, device="cuda")
+    s = torch.full((groups + 1, rows + 9), 77, dtype=torch.int32, device="cuda")
+    ctx.check(awa.lib().dit_quant_fp8(ctx.ptr, awa.AWA_F32 if dtype == F32 else awa.AWA_BF16, x.data_ptr(), cols, rows,
+                                      cols, 1, q.data_ptr(), s.data_ptr(), rows + 9,
+                                      torch.cuda.current_stream().cuda_stream), "dit_quant_fp8")
+    check_quant(q[:rows], s[:-1, :rows].contiguous().view(torch.uint8).reshape(groups, rows, 4), x, 1)
+    assert bool((q[rows:] == 99).all()) and bool((s[-1] == 77).all()) and bool((s[:, rows:] == 77).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quant_two_rows_a_wave_special_values(ctx, dtype):
+    """Zeros, infinities, NaN, subnormals and the type's largest value in either row of a wave."""
+    import torch
+    t = dt(dtype)
+    x = torch.randn((16391, 256), device="cuda").to(t)
+    for r, v in enumerate((0.0, math.inf, -math.inf, math.nan, torch.finfo(t).max, torch.finfo(t).tiny,
+                           torch.finfo(t).smallest_normal * 2.0 ** -7, 448.0, 449.0, 452.0)):
+        for at in (r, 8000 + 11 * r, 16390 - r):
+            x[at, 128:] = v
+            x[at, r] = v
+    q, s = ctx.quant_fp8(x)
+    check_quant(q, s, x, 1)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("blocks", [False, True])
 def test_quant_special_values(ctx, dtype, blocks):
