@@ -502,6 +502,70 @@ def test_rope(awa, ctx, tokens, heads, head_d, pairs, layout, extra, dtype):
     assert torch.equal(x, out) and torch.equal(buf[:, heads * head_d:], rest)
 
 
+def rope_heads_a_thread(tokens, heads, head_d, pairs, layout, size, copy):
+    """(threads per token and piece, heads of the first of them, heads in flight) by the launcher's rule: 8 workgroups of
+    256 per CU, pieces of up to 16 bytes that the pairs and the head are whole numbers of."""
+    half, v = layout == "half", 16 // size // (1 if layout == "half" else 2)
+    while v > 1 and (pairs % v or head_d % v if half else head_d % (2 * v)):
+        v //= 2
+    w, turning = v if half else 2 * v, -(-pairs // v)
+    passing = max(0, head_d - (2 * pairs if half else w * turning))
+    units = turning + (-(-passing // w) if copy else 0)
+    lanes = min(heads, -(-2048 * 256 // (tokens * units)))
+    return lanes, -(-heads // lanes), 2 if half and v == 8 else 4
+
+
+# several heads a thread, whole numbers of those in flight and not, with channels that pass and without
+ROPES_LONG = [
+    (5440, 40, 128, (21, 21, 21), "interleaved", 2560), (5440, 40, 128, (21, 21, 21), "half", 2560),
+    (5440, 40, 128, (64,), "half", 2560), (20000, 12, 96, (32,), "half", 0), (20000, 12, 96, (32,), "interleaved", 0),
+    (9000, 37, 80, (20,), "half", 3), (9000, 37, 80, (20,), "interleaved", 3), (30000, 8, 80, (40,), "half", 16),
+    (30011, 7, 96, (8, 24), "half", 1), (70001, 9, 64, (30,), "interleaved", 0), (300000, 2, 64, (32,), "half", 0),
+    (150001, 5, 16, (8,), "interleaved", 8), (100003, 3, 33, (13,), "half", 0),
+]
+
+
+@pytest.mark.parametrize("tokens,heads,head_d,pairs,layout,extra", ROPES_LONG)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rope_heads_in_turn(awa, ctx, tokens, heads, head_d, pairs, layout, extra, dtype):
+    size = 2 if dtype == BF16 else 4
+    lanes, most, _ = rope_heads_a_thread(tokens, heads, head_d, sum(pairs), layout, size, True)
+    assert lanes < heads and most > 1
+    test_rope(awa, ctx, tokens, heads, head_d, pairs, layout, extra, dtype)
+
+
+def test_rope_heads_in_turn_reach_every_remainder():
+    """ROPES_LONG has threads whose heads fit those in flight once, and more than once with and without a remainder."""
+    for flight in (2, 4):
+        seen = set()
+        for tokens, heads, head_d, pairs, layout, _ in ROPES_LONG:
+            for size in (2, 4):
+                for copy in (False, True):
+                    lanes, most, r = rope_heads_a_thread(tokens, heads, head_d, sum(pairs), layout, size, copy)
+                    if r == flight:
+                        seen |= {(most > r, (-(-(heads - i) // lanes)) % r != 0) for i in range(lanes)}
+        assert seen >= {(False, False), (True, False), (True, True)}, (flight, seen)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_heads_of_two_tensors(awa, ctx, layout, dtype):
+    """Queries and keys of different numbers of heads, several a thread, in place inside qkv rows."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(9)
+    tok, hq, hk, d = 20001, 14, 3, 64
+    buf = torch.randn((tok, (hq + 2 * hk) * d), generator=g, device="cuda").to(dt(dtype))
+    was = buf.clone()
+    q, k = buf[:, :hq * d].unflatten(1, (hq, d)), buf[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d))
+    pos = torch.arange(tok, dtype=torch.int32, device="cuda")
+    f = awa.rope_freqs(32)
+    want = [plain_rope(t, pos, f, (32,), layout, 1.0, False) for t in (q, k)]
+    ctx.rope((q, k), pos, f, layout=layout, out=(q, k))
+    for t, (ref, bar) in zip((q, k), want):
+        within(t, ref, bar + half_step(dt(dtype)) * ref.abs())
+    assert torch.equal(buf[:, (hq + hk) * d:], was[:, (hq + hk) * d:])
+
+
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 def test_rope_far_positions(awa, ctx, layout):
     import torch
