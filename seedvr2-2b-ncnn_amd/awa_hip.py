@@ -282,8 +282,11 @@ def plan_windows(t, h, w, num_windows, shifted):
 def rope_freqs(n, base=10000.0, kind="plain", factor=1.0, trained=0.0, low=1.0, high=32.0):
     """dit_rope_freqs: the radians per position of n channel pairs (float64 [n]), for a
     context stretched by `factor` over a trained length where kind is not "plain"."""
-    out = np.empty(max(int(n), 1), np.float64)
-    rc = lib().dit_rope_freqs(ROPE_KINDS[kind], int(n), float(base), float(factor), float(trained), float(low),
+    if kind not in ROPE_KINDS:
+        raise ValueError(f"rope_freqs: kind must be one of {list(ROPE_KINDS)}")
+    n = min(max(int(n), 0), ROPE_MAX_PAIRS + 1)  # what is out of range stays so
+    out = np.empty(n, np.float64)
+    rc = lib().dit_rope_freqs(ROPE_KINDS[kind], n, float(base), float(factor), float(trained), float(low),
                               float(high), out.ctypes.data)
     if rc != AWA_OK:
         raise AwaError(rc, "dit_rope_freqs rejected the arguments")

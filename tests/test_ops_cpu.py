@@ -149,6 +149,15 @@ def test_tensors_of_another_stream_are_marked(awa, monkeypatch):
     assert len(calls) == 7
 
 
+def test_freqs_refused_by_the_binding(awa):
+    """Numbers of pairs whose low 32 bits are allowed, and kinds that are none."""
+    for n in (2 ** 32 + 8, -2 ** 32 + 8):
+        with pytest.raises(awa.AwaError):
+            awa.rope_freqs(n)
+    with pytest.raises(ValueError, match="kind must be one of"):
+        awa.rope_freqs(8, kind="cubic")
+
+
 def test_product_reads_sums_after_their_wait_states(tmp_path):
     """The static check of the other matrix kernels over the 8-bit product's: its sums pass through empty asm
     statements, which the compiler does not wait before."""
