@@ -149,6 +149,109 @@ def test_tensors_of_another_stream_are_marked(awa, monkeypatch):
     assert len(calls) == 7
 
 
+def test_binding_refusals_by_message(awa, monkeypatch):
+    """Each check of the binding by its own message; no call of them reaches the library."""
+    import torch
+    ctx, calls = meta_context(awa, monkeypatch)
+    bf16, f32, i32, u8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+
+    def empty(*shape, dtype=bf16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    def refused(match, call, error=ValueError):
+        with pytest.raises(error, match=match):
+            call()
+
+    # rows
+    x = empty(6, 300)
+    q, s = ctx.quant_fp8(x)
+    calls.clear()
+    refused("contiguous columns", lambda: ctx.quant_fp8(empty(300, 6).T))
+    refused("contiguous columns", lambda: ctx.quant_fp8(empty(6, 600)[:, ::2]))
+    refused("contiguous columns", lambda: ctx.quant_fp8(empty(300)))
+    refused("contiguous columns", lambda: ctx.quant_fp8(empty(2, 6, 300)))
+    refused("contiguous columns", lambda: ctx.quant_fp8(empty(6, 0)))
+    refused("unsupported dtype", lambda: ctx.quant_fp8(empty(6, 300, dtype=torch.float16)), TypeError)
+    for t in (empty(6, 300, dtype=u8), empty(5, 384, dtype=u8), empty(6, 384), empty(6, 400, dtype=u8)[:, :384]):
+        refused("q must be", lambda: ctx.quant_fp8(x, q=t, scale=s))
+    for t in (empty(1, 5, 4, dtype=u8), empty(2, 6, 4, dtype=u8), empty(1, 6, dtype=i32), empty(1, 6, 8, dtype=u8)[..., :4]):
+        refused("scale must be", lambda: ctx.quant_fp8(x, q=q, scale=t))
+    refused("scale must be", lambda: ctx.quant_fp8(x, blocks=True, q=q, scale=s))
+
+    # the product: 6 x 384 by 130 x 384
+    w, ws = empty(130, 384, dtype=u8), empty(1, 2, 4, dtype=u8)
+    gemm = ctx.gemm_fp8
+    refused(r"a \[M, K\] and w", lambda: gemm(q[0], s, w, ws))
+    refused(r"a \[M, K\] and w", lambda: gemm(q, s, w[0], ws))
+    refused("a must be", lambda: gemm(empty(6, 384), s, w, ws))
+    refused("a must be", lambda: gemm(empty(12, 384, dtype=u8)[::2], s, w, ws))
+    refused("w must be", lambda: gemm(q, s, empty(130, 256, dtype=u8), ws))
+    refused("w must be", lambda: gemm(q, s, empty(130, 400, dtype=u8)[:, :384], ws))
+    refused("w must be", lambda: gemm(q, s, empty(130, 384), ws))
+    for t in (empty(1, 5, 4, dtype=u8), empty(2, 6, 4, dtype=u8), empty(1, 6, 4), empty(1, 6, dtype=i32)):
+        refused("a_scale must be a", lambda: gemm(q, t, w, ws))
+    for t in (empty(1, 6, 8, dtype=u8)[..., :4], empty(1, 12, 4, dtype=u8)[:, ::2], empty(1, 4, 6, dtype=u8).transpose(1, 2)):
+        refused("a_scale must be whole words", lambda: gemm(q, t, w, ws))
+    refused("w_scale must be a", lambda: gemm(q, s, w, empty(1, 130, 4, dtype=u8)))
+    refused("w_scale must be whole words", lambda: gemm(q, s, w, empty(1, 4, 4, dtype=u8)[:, ::2]))
+    wide = empty(6, 640, dtype=u8), empty(130, 640, dtype=u8), empty(2, 2, 4, dtype=u8)
+    for t in (torch.empty_strided((2, 6, 4), (26, 4, 1), dtype=u8, device="meta"),
+              torch.empty_strided((2, 6, 4), (20, 4, 1), dtype=u8, device="meta")):  # no whole words, groups that overlap
+        refused("a_scale must be whole words", lambda: gemm(wide[0], t, *wide[1:]))
+    for t in (empty(130), empty(129, dtype=f32), empty(1, 130, dtype=f32), empty(260, dtype=f32)[::2]):
+        refused("bias must be", lambda: gemm(q, s, w, ws, bias=t))
+    for t in (empty(6, 129), empty(5, 130), empty(130, 6).T, empty(6, 260)[:, ::2], empty(780)):
+        refused("out must be", lambda: gemm(q, s, w, ws, out=t))
+    refused("out must be", lambda: gemm(q, s, w, ws, out=empty(6, 130), dtype=f32))
+    refused("unsupported dtype", lambda: gemm(q, s, w, ws, out=empty(6, 130, dtype=torch.float16)), TypeError)
+    refused("unsupported dtype", lambda: gemm(q, s, w, ws, dtype=torch.float16), TypeError)
+
+    # rotation: 6 tokens of 3 heads of 64
+    x, pos, f = empty(6, 3, 64), empty(6, dtype=i32), [1.0] * 32
+
+    def rope(x=x, pos=pos, f=f, **args):
+        return lambda: ctx.rope(x, pos, f, **args)
+
+    refused("one or two tensors", rope((x, x, x)))
+    refused("one or two tensors", rope(()))
+    refused("one or two tensors", rope((x, x), out=x))
+    refused("one or two tensors", rope(x, out=(x, x)))
+    refused(r"must be \[tokens, heads, head_d\]", rope(x[0]))
+    refused(r"must be \[tokens, heads, head_d\] of one dtype", rope(empty(6, 3, 128)[..., ::2]))
+    for t in (empty(5, 3, 64), empty(6, 3, 32), empty(6, 3, 64, dtype=f32), empty(6, 192), empty(6, 64, 3).transpose(1, 2)):
+        refused(r"must be \[tokens, heads, head_d\] of one dtype", rope((x, t)))
+    for t in (empty(6, dtype=torch.int64), empty(5, dtype=i32), empty(12, dtype=i32)[::2], empty(6, 1, 1, dtype=i32),
+              empty(1, 6, dtype=i32).T.expand(6, 2)):
+        refused("positions must be", rope(pos=t))
+    refused("must name each axis", rope(pairs=(16, 16)))
+    refused("must name each axis", rope(pairs=(31,)))
+    refused("must name each axis", rope(pos=empty(6, 3, dtype=i32), pairs=(16, 16)))
+    refused("must name each axis", rope(pos=empty(6, 5, dtype=i32), pairs=(8, 8, 8, 4, 4)))
+    refused("must name each axis", rope(empty(6, 3, 258), f=[1.0] * 129))
+    refused("layout must be", rope(layout="split"))
+    for t in (empty(6, 3, 63), empty(6, 3, 64, dtype=f32), empty(6, 3, 128)[..., ::2]):
+        refused("out must have", rope(out=t))
+    refused("unsupported dtype", rope(empty(6, 3, 64, dtype=torch.float16)), TypeError)
+
+    # each tensor elsewhere than the context's device
+    elsewhere = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 3 if any(t is e for e in elsewhere) else -1)
+    bias, out, turned = empty(130, dtype=f32), empty(6, 130), empty(6, 3, 64)
+    rows = empty(6, 300)
+    for call, tensors in ((lambda: ctx.quant_fp8(rows, q=q, scale=s), (rows, q, s)),
+                          (lambda: gemm(q, s, w, ws, bias=bias, out=out), (q, s, w, ws, bias, out)),
+                          (rope(out=turned), (x, pos, turned)), (rope((turned, x)), (x, turned))):
+        calls.clear()
+        call()
+        assert len(calls) == 1
+        calls.clear()
+        for t in tensors:
+            elsewhere[:] = [t]
+            refused("must be on device -1", call)
+        elsewhere.clear()
+    assert not calls
+
+
 def test_freqs_refused_by_the_binding(awa):
     """Numbers of pairs whose low 32 bits are allowed, and kinds that are none."""
     for n in (2 ** 32 + 8, -2 ** 32 + 8):
