@@ -189,8 +189,8 @@ int dit_rope(awa_ctx* ctx, int dtype, const dit_rope_rows* rows, int n_rows, int
         a.quarters[i] = plan->freq[i] / (0.5 * M_PI);
     }
     a.axes = plan->axes;
-    a.cos_scale = (float)plan->scale;
-    a.sin_scale = (float)(plan->inverse ? -plan->scale : plan->scale);
+    a.cos_scale = plan->scale;
+    a.sin_scale = plan->inverse ? -plan->scale : plan->scale;
     a.tokens = n_tokens;
     a.head_d = head_d;
     a.pos = d_pos;

@@ -47,7 +47,7 @@ struct RopeArgs {
     int rot_units, units;    // pieces of a head that turn, and all; filled by launch_rope
     int lanes[2];            // threads per token and piece, each with every lanes-th head; likewise
     const int32_t* pos;
-    float cos_scale, sin_scale;
+    double cos_scale, sin_scale;
     double quarters[DIT_ROPE_MAX_PAIRS];  // quarter turns per position
 };
 hipError_t launch_rope(int dtype, int layout, RopeArgs& a, hipStream_t s);

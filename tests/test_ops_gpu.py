@@ -577,6 +577,28 @@ def test_rope_far_positions(awa, ctx, layout):
 
 
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("scale", [1.0, 1.3465735902799727])
+def test_rope_sines_are_rounded_once(awa, ctx, layout, scale):
+    """Pairs (1, 0) turn to scale (cos, sin) alone: half a step, what the series leaves out (under 2^-28) and rounds
+    (the terms from x^4 / 24 <= 2^-5.9 on in fp32, at most four half steps of 2^-24 of them: under 2^-27.9), and the
+    angle's own error."""
+    import torch
+    tokens, pairs = 20000, 32
+    g = torch.Generator(device="cuda").manual_seed(12)
+    pos = torch.randint(0, 1 << 20, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    pos[:4000] = torch.arange(4000)
+    freqs = np.concatenate([awa.rope_freqs(pairs - 2), [2 * np.pi / 4000, -0.5 * np.pi / 4000]])
+    x = torch.zeros((tokens, 1, 2 * pairs), device="cuda")
+    first = slice(0, pairs) if layout == "half" else slice(0, None, 2)
+    second = slice(pairs, None) if layout == "half" else slice(1, None, 2)
+    x[..., first] = 1.0
+    out = ctx.rope(x, pos, freqs, layout=layout, scale=scale)
+    angle = pos.double()[:, None, None] * torch.from_numpy(freqs).cuda()
+    for part, ref in ((first, scale * angle.cos()), (second, scale * angle.sin())):
+        within(out[..., part], ref, 2.0 ** -24 * ref.abs() + scale * (2.0 ** -28 + 2.0 ** -27.9 + angle.abs() * 2.0 ** -51))
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
 def test_rope_quarter_turns(awa, ctx, layout):
     """Angles at and around the borders of the reduction: multiples of a sixteenth turn."""
     import torch
