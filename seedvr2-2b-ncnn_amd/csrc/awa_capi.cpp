@@ -70,16 +70,6 @@ hipError_t event_mark(awa_ctx* ctx, std::vector<hipEvent_t>& list, hipStream_t s
 
 namespace {
 
-#define HIPCK(ctx, expr)                                                                     \
-    do {                                                                                     \
-        hipError_t e_ = (expr);                                                              \
-        if (e_ != hipSuccess) {                                                              \
-            set_err(ctx, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__,    \
-                    __LINE__);                                                               \
-            return AWA_EHIP;                                                                 \
-        }                                                                                    \
-    } while (0)
-
 template <typename T>
 hipError_t dalloc(T** p, size_t n) {
     *p = nullptr;

@@ -291,6 +291,16 @@ namespace awa {
 
 // Host helpers shared by the C ABI translation units (awa_capi.cpp).
 void set_err(awa_ctx* ctx, const char* fmt, ...);
+// a HIP call of an entry point: its failure is the entry's
+#define HIPCK(ctx, expr)                                                                     \
+    do {                                                                                     \
+        hipError_t e_ = (expr);                                                              \
+        if (e_ != hipSuccess) {                                                              \
+            set_err(ctx, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__,    \
+                    __LINE__);                                                               \
+            return AWA_EHIP;                                                                 \
+        }                                                                                    \
+    } while (0)
 struct DeviceGuard {
     int prev = -1;
     bool ok = false;

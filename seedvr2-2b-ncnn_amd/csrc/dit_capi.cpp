@@ -11,16 +11,6 @@ using namespace awa;
 
 namespace {
 
-#define HIPCK(ctx, expr)                                                                     \
-    do {                                                                                     \
-        hipError_t e_ = (expr);                                                              \
-        if (e_ != hipSuccess) {                                                              \
-            set_err(ctx, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__,    \
-                    __LINE__);                                                               \
-            return AWA_EHIP;                                                                 \
-        }                                                                                    \
-    } while (0)
-
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 bool branch_ok(const dit_branch* b) {

@@ -17,6 +17,7 @@
 // others, 8.4e-5 and 8.9e-5 with 256 and 2048 times: a 260th to a 43rd of bf16's step,
 // and taken for bf16 C.  bf16 holds every e4m3 value, times any power of two, and the
 // bf16 instructions keep fp32's bits, at half the rate.
+#include "dit_device.hpp"
 #include "dit_ops_internal.hpp"
 
 namespace awa {
@@ -148,19 +149,14 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 // 1999 x 2816 24.1, 679 x 2560 x 6912 32.5, 5498 x 13824 x 2560 305.
 constexpr int ROW = 128;  // bytes of a block's row
 
-// A buffer resource with wave-uniform fields (as in dit_gemm.hip): loads past
-// `bytes` read zeros and stores past it are dropped.
-__device__ inline __amdgpu_buffer_rsrc_t uniform_rsrc(const void* p, uint32_t bytes) {
-    const uint64_t a = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
-                                             __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
-}
-// Waits until at most N vector memory operations and no LDS operation are outstanding.
-template <int N>
-__device__ inline void wait_vmem_lds() {
-    asm volatile("s_waitcnt vmcnt(%c0) lgkmcnt(0)" ::"n"(N) : "memory");
+// Where tile t of the walk begins: four m-tiles per group, n advancing across the group
+template <int BN, int BM>
+__device__ inline void place(const Fp8Gemm& p, int t, int& m0, int& n0) {
+    constexpr int GM = 4;
+    const int group = t / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
+    const int in_group = t - group * (GM * p.n_tiles);
+    m0 = (first_m + in_group % gm) * BM;
+    n0 = in_group / gm * BN;
 }
 
 // Lane (c = lane % 32, g = lane / 32) of accumulator (i, j): row 32 j + c, features
@@ -275,14 +271,6 @@ __global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     const int end = min(((int)blockIdx.x & 7) * per + per, total);
     int tile = ((int)blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (tile >= end) return;
-    auto place = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
-        // four m-tiles per group, n advancing across the group
-        constexpr int GM = 4;
-        const int group = t / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
-        const int in_group = t - group * (GM * p.n_tiles);
-        m0 = (first_m + in_group % gm) * BM;
-        n0 = in_group / gm * BN;
-    };
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int kg = __builtin_amdgcn_readfirstlane(tid / GT), wave = __builtin_amdgcn_readfirstlane((tid >> 6) % GW);
@@ -321,7 +309,7 @@ __global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
     auto fetch_from = [&](int t) __attribute__((always_inline)) {
         int m0 = 0, n0 = 0, wrows = 0, arows = 0;
         if (t < end) {
-            place(t, m0, n0);
+            place<BN, BM>(p, t, m0, n0);
             wrows = min(BN, p.N - n0);
             arows = min(BM, p.M - m0);
         }
@@ -502,7 +490,7 @@ __global__ __launch_bounds__(128 * NW * KG, 1) void gemm_fp8_kernel(Fp8Gemm p) {
             }
             half(1, slot, 0, false, NP, NP, 0, false);
         }
-        place(tile, m0, n0);
+        place<BN, BM>(p, tile, m0, n0);
         if constexpr (!WALK) {  // the slots are free once every DMA (of nothing, by now) and read is done
             wait_vmem_lds<0>();
             __builtin_amdgcn_s_barrier();
@@ -645,13 +633,6 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
     const int end = min(((int)blockIdx.x & 7) * per + per, total);
     int tile = ((int)blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (tile >= end) return;
-    auto place = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
-        constexpr int GM = 4;
-        const int group = t / (GM * p.n_tiles), first_m = group * GM, gm = min(p.m_tiles - first_m, GM);
-        const int in_group = t - group * (GM * p.n_tiles);
-        m0 = (first_m + in_group % gm) * BM;
-        n0 = in_group / gm * BN;
-    };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave >> 1, wm = wave & 1;
     const int nk = p.K >> 7;
@@ -676,7 +657,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
     auto fetch_from = [&](int t) __attribute__((always_inline)) {
         int m0 = 0, n0 = 0, wrows = 0, arows = 0;
         if (t < end) {
-            place(t, m0, n0);
+            place<BN, BM>(p, t, m0, n0);
             wrows = min(BN, p.N - n0);
             arows = min(BM, p.M - m0);
         }
@@ -817,7 +798,7 @@ __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
             for (int i = 0; i < 4; i++) af[i] = af[4 + i];
         }
         int m0, n0;
-        place(tile, m0, n0);
+        place<BN, BM>(p, tile, m0, n0);
         int l = 0;  // the lane anew: see the other tiles
         asm volatile("" : "+v"(l));
         l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, l));

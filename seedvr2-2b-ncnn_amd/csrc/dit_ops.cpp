@@ -8,16 +8,6 @@ using namespace awa;
 
 namespace {
 
-#define HIPCK(ctx, expr)                                                                     \
-    do {                                                                                     \
-        hipError_t e_ = (expr);                                                              \
-        if (e_ != hipSuccess) {                                                              \
-            set_err(ctx, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__,    \
-                    __LINE__);                                                               \
-            return AWA_EHIP;                                                                 \
-        }                                                                                    \
-    } while (0)
-
 size_t elem(int dtype) { return dtype == AWA_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == AWA_F32 || dtype == AWA_BF16; }
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
