@@ -534,9 +534,8 @@ class Context:
             if t is not None:
                 t.record_stream(stream)
 
-    def _sizes(self, what, rows, *cols):
-        if rows > OPS_ROWS_MAX or max(cols, default=0) > OPS_COLS_MAX:
-            raise ValueError(f"{what}: at most {OPS_ROWS_MAX} rows and {OPS_COLS_MAX} columns, got {[rows, *cols]}")
+    def _too_large(self, what, *sizes):
+        return ValueError(f"{what}: at most {OPS_ROWS_MAX} rows and {OPS_COLS_MAX} columns, got {list(sizes)}")
 
     def _elsewhere(self, what, t):
         return ValueError(f"{what}: tensors must be on device {self.device}, got {t.device}")
@@ -573,7 +572,8 @@ class Context:
         rows, cols = shape if len(shape) == 2 else (0, 0)
         if cols < 1 or (cols > 1 and st[1] != 1):
             raise ValueError("quant_fp8: x must be [rows, cols] with contiguous columns")
-        self._sizes("quant_fp8", rows, cols)
+        if rows > OPS_ROWS_MAX or cols > OPS_COLS_MAX:
+            raise self._too_large("quant_fp8", rows, cols)
         if x.get_device() != self.device:
             raise self._elsewhere("quant_fp8", x)
         kp, groups, srows = (cols + 127) // 128 * 128, (cols + 511) // 512, (rows + 127) // 128 if blocks else rows
@@ -605,7 +605,8 @@ class Context:
             raise ValueError("gemm_fp8: a [M, K] and w [N, K]")
         M, K = shape
         N = wshape[0]
-        self._sizes("gemm_fp8", M, N, K)
+        if M > OPS_ROWS_MAX or N > OPS_COLS_MAX or K > OPS_COLS_MAX:
+            raise self._too_large("gemm_fp8", M, N, K)
         groups, nb = (K + 511) // 512, (N + 127) // 128
         dev = self.device
         if not (a.dtype in _e4m3 and w.dtype in _e4m3 and wshape[1] == K and a.is_contiguous() and w.is_contiguous() and
@@ -654,7 +655,8 @@ class Context:
         if len(shape) != 3:
             raise ValueError("rope: tensors must be [tokens, heads, head_d]")
         tokens, _, head_d = shape
-        self._sizes("rope", tokens)
+        if tokens > OPS_ROWS_MAX:
+            raise self._too_large("rope", tokens)
         f = np.ascontiguousarray(freqs, np.float64)
         n, at = f.size, positions.shape
         axes = at[1] if len(at) == 2 else 1
