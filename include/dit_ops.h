@@ -11,6 +11,10 @@
  *   qkv    = product(q, s, w, sw)
  *   rope(q and k columns of qkv, positions)
  *
+ * (awa_forward normalises and rotates queries and keys itself and takes qkv as the
+ * product leaves it; the rotation here is for attention of the caller's own, after
+ * whatever norm its model has.)
+ *
  * Conventions as awa_capi.h: device pointers, stream-ordered and asynchronous,
  * 0 / AWA_EARG / AWA_EHIP, messages through awa_last_error of the context.
  * These calls allocate nothing and use no scratch of the context, so they may

@@ -50,8 +50,8 @@ __device__ inline bf16x8 widen(int lo, int hi, float scale) {
 // Up to 16 rows: 16 NI features per workgroup, the blocks of K in turn over its waves,
 // whose sums meet in LDS (in the waves' order).  Bound by W, which is read once,
 // straight into registers; A comes from the L2 again for every workgroup.  One row of
-// 7680 x 2560 takes 5.4 us (19.7 MB of W: 3.6 TB/s), of 2560 x 6912 6.4, of 4096 x 11008 10.0
-// (4.5 TB/s), 16 rows of 7680 x 2560 6.1, of which a launch and the fill of the chip are 2 to
+// 7680 x 2560 takes 5.4 us (19.7 MB of W: 3.6 TB/s), of 2560 x 6912 6.4, of 4096 x 11008 10.2
+// (4.4 TB/s), 16 rows of 7680 x 2560 6.0, of which a launch and the fill of the chip are 2 to
 // 3.  Widened to bf16: an 8-bit instruction would save nothing where W's bytes bound.
 template <int NI, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
@@ -142,11 +142,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_fp8_few_kernel(Fp8Gemm p) {
 //
 // Bound by what a tile's operands take from the L2 where the tiles are small, and by the
 // chip's power where they are large (a loop of 8-bit instructions alone reaches 4.0 to 4.1
-// PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 6.1 us, 679 x 2560 x 6912 19.7 (1.22
-// PFLOP/s), 1237 x 1999 x 2816 15.3, 1400 x 13824 x 2560 50 to 53 (1.9).  fp32 C: 679 x
-// 2560 x 6912 32 to 34 us (0.72), 5498 x 13824 x 2560 322 (1.21), 8192^3 752 (1.46; the
-// library's bf16 product 1.31).  bf16 C of whole products: 58 x 7680 x 2560 7.6 us, 1237 x
-// 1999 x 2816 24.1, 679 x 2560 x 6912 32.5, 5498 x 13824 x 2560 305.
+// PFLOP/s, at 1.9 GHz).  bf16 C: 58 x 7680 x 2560 6.3 us, 679 x 2560 x 6912 19 to 21 (1.2
+// PFLOP/s), 1237 x 1999 x 2816 14.6 to 15.1, 1400 x 13824 x 2560 52 (1.9).  fp32 C: 679 x
+// 2560 x 6912 32 to 34 us (0.73), 5498 x 13824 x 2560 294 to 322 (1.2 to 1.3), 8192^3 728 to
+// 752 (1.5; the library's bf16 product 1.31).  bf16 C of whole products: 58 x 7680 x 2560
+// 7.4 us, 1237 x 1999 x 2816 22 to 24, 679 x 2560 x 6912 32, 5498 x 13824 x 2560 278 to 305.
 constexpr int ROW = 128;  // bytes of a block's row
 
 // Where tile t of the walk begins: four m-tiles per group, n advancing across the group
@@ -619,8 +619,8 @@ __device__ inline void wide_epilogue(const Fp8Gemm& p, const f32x4 (&acc)[8][8],
 // this one's s: they change places from stage to stage), and each half of a slot is
 // refilled as soon as every wave has read it: two barriers a stage, fragment reads and
 // DMA even over all of it, and a whole stage for a refill to land, with two stages of
-// LDS.  5498 x 13824 x 2560 takes 160 us (2.43 PFLOP/s; tiles as above 165), 8192^3 354 to
-// 366 (3.0 to 3.1; 374), the matrix cores busy for 60 % of the cycles.  Bound by power: the
+// LDS.  5498 x 13824 x 2560 takes 151 to 161 us (2.4 to 2.6 PFLOP/s; tiles as above 5 more), 8192^3
+// 350 to 366 (3.0 to 3.1; 374), the matrix cores busy for 60 % of the cycles.  Bound by power: the
 // first stages of a tile without a wait for the stores of the tile before, and LDS reads
 // without bank conflicts, changed neither.
 __global__ __launch_bounds__(256, 1) void gemm_fp8_wide_kernel(Fp8Gemm p) {
@@ -832,9 +832,9 @@ constexpr Tile FULL[] = {{4, 4, 2, 1, 2, 2.16f, 2.50f, 9.0f}, {4, 3, 2, 1, 2, 1.
                          {1, 1, 3, 4, 1, 0.13f, 0.165f, 4.3f}};
 
 // Estimated time with tiles t: rounds of one tile per CU, the last one at 0.7 of a full
-// round plus 0.3 of its share (as for the bf16 GEMM).  All seven forms were timed on 36 products
-// of 17 to 5498 rows with either C: it takes the fastest of each but one, there a form 5 %
-// behind it (58 x 7680 x 512, bf16 C: 4.5 us, 4.3).
+// round plus 0.3 of its share (as for the bf16 GEMM).  All seven forms were timed on 38
+// products of 17 to 5498 rows with either C, and with bf16 C of whole products: it takes the
+// fastest of each but one, there a form 2 % behind it (512 x 512 x 512, bf16 C: 4.3 us, 4.2).
 float tile_cost(const Fp8Gemm& p, const Tile& t, int cus) {
     const long tiles = ((long)p.N + 32 * t.nw * t.ni - 1) / (32 * t.nw * t.ni) * (((long)p.M + 64 * t.mj - 1) / (64 * t.mj));
     const float r = (float)tiles / cus, share = r < 1.f ? r : 1.f;
@@ -854,8 +854,9 @@ hipError_t launch_gemm_fp8(Fp8Gemm& p, hipStream_t s) {
     if (p.M <= 16) {
         // 16, 32 or 64 features a workgroup, by what the busiest CU fetches: its features, and for
         // each of its workgroups A, as much as 4 + 3/4 M features (1 row: 4096 x 11008 10.0 us with
-        // 16, 14.4 with 32; 8000 x 5120 9.2 with 32 and 16; 24000 x 2560 12.5, 11.8 and 13.9; 16
-        // rows of 13824 x 2560 12.4, 10.2 and 9.3)
+        // 16, 14.4 with 32; 8000 x 5120 9.2 with 32 and 16; 24000 x 2560 12.5, 11.8 and 14.0; 16
+        // rows of 13824 x 2560 12.4, 10.3 and 9.3; of nine products it takes the fastest, or one 2 %
+        // behind it, but 14.7 us for 12.7 at 4 x 16000 x 4096)
         auto fetched = [&](int ni) { return ((p.N + 16 * ni - 1) / (16 * ni) + cus - 1) / cus * (64 * ni + 16 + 3 * p.M); };
         const int f1 = fetched(1), f2 = fetched(2), f4 = fetched(4);
         if (f4 < f1 && f4 < f2) few_launch<4, 4>(p, s);

@@ -7,9 +7,10 @@
 // conversion's, to nearest even.
 //
 // HBM-bound: each value is read once (2 or 4 bytes) and a byte written.  Rows of 27258 x
-// 2560 bf16 take 36.9 us (5.7 TB/s), 5498 x 6912 fp32 34.0 (5.6), weights of 13824 x 2560
-// bf16 17.6 (6.0) and 2560 x 6912 fp32 14.9 (5.9), where device copies of 50 to 100 MiB
-// reach 4.8 to 5.1 TB/s; rows of 58 x 2560 2.3 us, of 679 x 2560 2.9.
+// 2560 bf16 take 36 us (5.85 TB/s), 5498 x 6912 fp32 28 (6.8, in part from the memory-side
+// cache), weights of 13824 x 2560 bf16 17.6 (6.0) and 2560 x 6912 fp32 15.0 (5.9), where
+// device copies of 50 to 100 MiB reach 4.8 to 5.1 TB/s; rows of 58 x 2560 2.5 us, of 679 x
+// 2560 3.1.
 #include "dit_ops_internal.hpp"
 
 namespace awa {

@@ -3,8 +3,8 @@
 // A thread owns a piece of the head (V pairs, 16 bytes a load where the sizes allow)
 // of one token: it forms the V sines and cosines once and turns that piece of
 // every head of its part.  HBM-bound: each channel is read and written once: 5440 x 40 x
-// 128 bf16 inside rows of 7680 18.9 us (5.9 TB/s), 20000 x 12 x 96 fp32 35.6 (5.2), 4096 x
-// 40 x 128 fp32 25.9 (6.5); one token of 40 heads 3.1 us.
+// 128 bf16 inside rows of 7680 19.2 us (5.8 TB/s), 20000 x 12 x 96 fp32 30 (6.2; 35 with other
+// tensors each time), 4096 x 40 x 128 fp32 26.1 (6.4); one token of 40 heads 3.3 us.
 //
 // Angles: position times quarter turns per position in fp64, less the nearest whole
 // number of quarters (exact): far positions lose only what fp64 loses on the angle
