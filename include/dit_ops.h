@@ -87,7 +87,8 @@ enum { DIT_FP8_WHOLE = 256 };
  * normal data, 9e-5 where one column in eight is 256 or 2048 times the others, a
  * 260th and a 43rd of bf16's step.  A sum that cancels keeps its error whole.
  * dtype_c AWA_BF16 | DIT_FP8_WHOLE lets products enter whole for any number of rows,
- * at the time of fp32 C: the bits are those of the fp32 C, rounded.
+ * at the time of fp32 C: the bits are those of the fp32 C, rounded (AWA_F32 takes the
+ * flag too and is whole without it).
  * The result of a row does not depend on the other rows of A, but on their number
  * in the order of its sums (and, past 16 with bf16 C, in what enters them); the same
  * call gives the same bits.

@@ -850,3 +850,32 @@ def test_inputs_dropped_before_another_stream_has_read_them(awa, ctx):
     torch.cuda.synchronize()
     for g, r in zip(got, want):
         assert torch.equal(g.view(torch.uint8), r.view(torch.uint8))
+
+
+def test_captured_on_a_given_stream(awa, ctx):
+    """The run captured with stream= naming the capture's own stream, temporaries dropped inside it; whole products and
+    fp32 rotation too.  Inputs changed between replays, and given back after them."""
+    import torch
+    x, wt, bias, pos, freqs = layer_inputs(awa, ctx, 130, 21)
+    w = ctx.quant_fp8(wt, blocks=True)
+
+    def run(stream=None):
+        q, s = ctx.quant_fp8(x, stream=stream)
+        c = ctx.gemm_fp8(q, s, *w, dtype=torch.float32, stream=stream)
+        turned = ctx.rope(c.unflatten(1, (12, 128)), pos, freqs, pairs=(21, 21, 21), stream=stream)
+        return layer(ctx, x, w, bias, pos, freqs, stream), turned, ctx.gemm_fp8(q, s, *w, bias=bias, whole=True, stream=stream)
+
+    run()
+    torch.cuda.synchronize()
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        outs = run(st)
+    x0 = x.clone()
+    for k in range(4):
+        x.copy_(x0.roll(k, 0) * (k + 1))
+        eager = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+    del graph, outs
+    torch.cuda.synchronize()
