@@ -272,6 +272,64 @@ def test_gemm_walks(awa, ctx, m, n, k, dtype):
     test_gemm(awa, ctx, m, n, k, dtype)
 
 
+@pytest.mark.parametrize("m", [16, 17, 65, 300, 2000, 20000])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 31, 33])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gemm_few_features(awa, ctx, m, n, dtype):
+    test_gemm(awa, ctx, m, n, 384, dtype)
+
+
+def test_gemm_most_rows(awa, ctx):
+    """2^24 rows and, the other way round, 2^20 features: every row a multiple of one of 64, times exact values."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def some(rows):
+        return torch.randint(-1, 2, (rows, 128), generator=g, device="cuda").float()
+
+    def scales(rows):
+        return torch.full((1, rows, 4), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+
+    few, w = some(64), some(130)
+    m = 1 << 24
+    a = few.to(torch.float8_e4m3fn).view(torch.uint8).repeat(m // 64, 1)
+    for n in (3, 130):  # sums of at most 128 products of 1: exact in every form and type
+        for t in (BF16, F32):
+            out = ctx.gemm_fp8(a, scales(m), w[:n].to(torch.float8_e4m3fn), scales(-(-n // 128)), dtype=dt(t))
+            want = (few @ w[:n].T).to(dt(t))
+            assert bool((out.view(-1, 64, n) == want).all())
+            del out
+    del a
+    n = 1 << 20
+    wide = few.to(torch.float8_e4m3fn).view(torch.uint8).repeat(n // 64, 1)
+    for rows in (3, 130):
+        for t in (BF16, F32):
+            out = ctx.gemm_fp8(w[:rows].to(torch.float8_e4m3fn), scales(rows), wide, scales(n // 128), dtype=dt(t))
+            want = (w[:rows] @ few.T).to(dt(t))
+            assert bool((out.view(rows, -1, 64) == want[:, None]).all())
+
+
+@pytest.mark.parametrize("m,n", [(5, 300), (20, 300), (300, 520), (700, 2600), (1300, 3301), (2304, 4096)])
+def test_gemm_most_columns(awa, ctx, m, n):
+    """2^20 columns, 1024 of them repeated: sums of at most 2^20, exact in every form; the quantiser on as many."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m)
+    small = [torch.randint(-1, 2, (rows, 1024), generator=g, device="cuda").float() for rows in (m, n)]
+    a, w = (t.to(torch.float8_e4m3fn).view(torch.uint8).repeat(1, 1024) for t in small)
+
+    def scales(rows):
+        return torch.full((2048, rows, 4), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+
+    want = small[0] @ small[1].T * 1024.0
+    for t in (BF16, F32):
+        out = ctx.gemm_fp8(a, scales(m), w, scales(-(-n // 128)), dtype=dt(t))
+        assert torch.equal(out, want.to(dt(t)))
+    if m <= 300:  # quantised, a block's largest value 1 becomes 256 and its scale 2^-8
+        for blocks in (False, True):
+            q, s = ctx.quant_fp8(small[0].bfloat16().repeat(1, 1024), blocks=blocks)
+            assert torch.equal(q.float(), 256 * small[0].repeat(1, 1024)) and bool((s.view(torch.uint8) == 119).all())
+
+
 @pytest.mark.parametrize("m,n", [(40, 600), (250, 2600), (500, 2600), (700, 3300), (671, 8001), (2400, 7000), (3501, 7000)])
 @pytest.mark.parametrize("ld", [0, 1, 2, 3])
 def test_gemm_scales_at_any_word(awa, ctx, m, n, ld):
