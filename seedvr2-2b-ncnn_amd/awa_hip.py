@@ -530,6 +530,7 @@ class Context:
 
     def _used(self, stream, *tensors):
         """Keeps the memory of a call's tensors from other use until the given stream has passed the call."""
+        self._stream(stream)
         for t in tensors:
             if t is not None:
                 t.record_stream(stream)

@@ -149,6 +149,30 @@ def test_tensors_of_another_stream_are_marked(awa, monkeypatch):
     assert len(calls) == 7
 
 
+def test_stream_of_another_device_marks_nothing(awa, monkeypatch):
+    """A stream that the call refuses leaves no mark on the tensors given to it."""
+    import torch
+    own_stream = awa.Context._stream
+    ctx, calls = meta_context(awa, monkeypatch)
+    monkeypatch.setattr(awa.Context, "_stream", own_stream)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: pytest.fail("marked"))
+
+    class Stream:
+        device_index, device, cuda_stream = 5, "cuda:5", 0
+
+    def empty(*shape, dtype=torch.uint8):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    x, q, s = empty(5, 128, dtype=torch.bfloat16), empty(5, 128), empty(1, 5, 4)
+    heads = empty(5, 1, 64, dtype=torch.bfloat16)
+    for call in (lambda: ctx.quant_fp8(x, q=q, scale=s, stream=Stream()),
+                 lambda: ctx.gemm_fp8(q, s, empty(7, 128), empty(1, 1, 4), out=empty(5, 7, dtype=torch.bfloat16), stream=Stream()),
+                 lambda: ctx.rope(heads, empty(5, dtype=torch.int32), [1.0], out=heads, stream=Stream())):
+        with pytest.raises(ValueError, match="stream must be of device"):
+            call()
+    assert not calls
+
+
 def test_binding_refusals_by_message(awa, monkeypatch):
     """Each check of the binding by its own message; no call of them reaches the library."""
     import torch
