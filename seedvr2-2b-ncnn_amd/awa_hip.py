@@ -19,6 +19,7 @@ HEADER_DIR = os.path.join(os.path.dirname(HERE), "include")
 
 AWA_OK, AWA_EARG, AWA_EHIP = 0, -1, -2
 AWA_F32, AWA_BF16 = 0, 1
+DIT_FP8 = 2
 DIT_FP8_WHOLE = 256
 HEADS, HEAD_D, DIM, QKV, ROPE_ROT = 20, 128, 2560, 7680, 126
 
@@ -63,11 +64,15 @@ ROPE_MAX_PAIRS, ROPE_MAX_AXES = 128, 4
 ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "bands": 3}
 
+# and include/dit_train.h
+NORM_COLS_MAX, CROSS_SEQ_MAX, CROSS_HEADS_MAX, CROSS_HEAD_D_MAX = 16384, 65536, 1024, 128
+
 
 # dit_rope_plan of include/dit_ops.h up to its frequencies, and dit_rope_rows
 _PLAN = struct.Struct("@7i4xd")
 _NO_PAIRS, _NO_FREQS = (0,) * ROPE_MAX_AXES, bytes(8 * ROPE_MAX_PAIRS)
 _ROWS = struct.Struct("@PPi4x4q")
+_HEADS = struct.Struct("@Pqq")  # dit_heads of include/dit_train.h
 
 
 class GeomInfo(C.Structure):
@@ -170,6 +175,23 @@ def lib():
         L.dit_gemm_fp8.argtypes = [vp, vp, vp, C.c_int64, vp, vp, C.c_int64, vp, C.c_int, vp, C.c_int64, C.c_int,
                                    C.c_int, C.c_int, vp]
         L.dit_rope.argtypes = [vp, C.c_int, C.c_char_p, C.c_int, C.c_int, C.c_int, C.c_char_p, vp, vp]
+        i64, i64p = C.c_int64, C.POINTER(C.c_int64)
+        L.dit_layer_norm.argtypes = [vp, C.c_int, vp, i64, vp, vp, C.c_float, C.c_int, vp, i64, vp, C.c_int, C.c_int, vp]
+        L.dit_layer_norm_grad_work.argtypes = [C.c_int, C.c_int]
+        L.dit_layer_norm_grad.argtypes = [vp, C.c_int, vp, i64, C.c_int, vp, i64, vp, i64, vp, vp, C.c_int, vp, i64, vp, vp,
+                                          vp, i64, C.c_int, C.c_int, vp]
+        L.dit_grad_weight_work.argtypes = 5 * [C.c_int]
+        L.dit_grad_weight_fp8.argtypes = [vp, C.c_int, vp, i64, vp, vp, i64, C.c_int, vp, i64, vp, C.c_int, vp, i64, C.c_int,
+                                          C.c_int, C.c_int, vp]
+        L.dit_cross_create.argtypes = [vp, C.c_int, i64p, i64p, i64p, i64p, C.c_int, C.c_int, C.c_int, C.POINTER(vp)]
+        L.dit_cross_destroy.argtypes = [vp]
+        L.dit_cross_destroy.restype = None
+        L.dit_cross_work.argtypes = [vp, C.c_int, C.c_int]
+        L.dit_cross_forward.argtypes = [vp, vp, C.c_int] + 3 * [C.c_char_p] + [vp, C.c_float, C.c_char_p, vp, i64, vp, i64, vp]
+        L.dit_cross_grad.argtypes = [vp, vp, C.c_int] + 5 * [C.c_char_p] + [vp, i64, vp, C.c_float] + 3 * [C.c_char_p] + [
+            vp, i64, vp]
+        for fn in (L.dit_layer_norm_grad_work, L.dit_grad_weight_work, L.dit_cross_work):
+            fn.restype = i64
         L.dit_rope_freqs.argtypes = [C.c_int, C.c_int] + 5 * [C.c_double] + [vp]
         _torch, _storage = torch, {torch.float32: AWA_F32, torch.bfloat16: AWA_BF16}
         _e4m3, _e8m0 = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
@@ -301,6 +323,15 @@ def fp8_values(q, scale, cols=None):
     s = s if s.shape[0] == rows else s.repeat_interleave(128, 0)[:rows]
     v = torch.ldexp(q.view(torch.float8_e4m3fn).float().unflatten(1, (-1, 128)), s[:, :, None]).flatten(1)
     return v if cols is None else v[:, :cols]
+
+
+def _address(*tensors):
+    return [t.data_ptr() if t is not None else None for t in tensors]
+
+
+def _work_of(t):
+    """Address and bytes of a call's workspace."""
+    return (t.data_ptr(), t.numel()) if t is not None else (None, 0)
 
 
 def _stream_ptr(stream=None):
@@ -697,6 +728,234 @@ class Context:
             self.check(rc, "dit_rope")
         return tuple(res) if many else res[0]
 
+    # ---- operators that train a layer (include/dit_train.h); streams as above
+    def _rows_of(self, what, t, name, rows=None, cols=None):
+        """(dtype, elements from row to row) of t [rows, cols] with contiguous columns on the context's device."""
+        dtype, shape, st = _dtype_of(what, t), t.shape, t.stride()
+        if len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and st[1] != 1) or (
+                rows is not None and (shape[0] != rows or shape[1] != cols)):
+            raise ValueError(f"{what}: {name} must be [{'rows' if rows is None else rows}, {'cols' if cols is None else cols}] "
+                             f"with contiguous columns, got {list(shape)} with strides {st}")
+        if t.get_device() != self.device:
+            raise self._elsewhere(what, t)
+        return dtype, st[0]
+
+    def _vector(self, what, t, name, *shape):
+        """The address of a contiguous fp32 tensor of this shape, or None."""
+        if t is None:
+            return None
+        if t.dtype != _torch.float32 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous fp32 tensor {list(shape)}")
+        if t.get_device() != self.device:
+            raise self._elsewhere(what, t)
+        return t.data_ptr()
+
+    def layer_norm(self, x, weight=None, bias=None, eps=1e-5, dtype=None, out=None, stats=False, stream=None):
+        """dit_layer_norm: each row of x [rows, cols] (bf16 or fp32, columns contiguous) normalised, times weight plus bias
+        (fp32 [cols]); `dtype` of the result (default x's), or that of `out` (x itself: in place).  stats=True: (y, stats),
+        each row's mean and rstd (fp32 [rows, 2]), which layer_norm_grad takes; a tensor is written."""
+        lib_ = lib()
+        dx, ldx = self._rows_of("layer_norm", x, "x")
+        rows, cols = x.shape
+        if rows > OPS_ROWS_MAX or cols > NORM_COLS_MAX:
+            raise ValueError(f"layer_norm: at most {OPS_ROWS_MAX} rows and {NORM_COLS_MAX} columns, got {[rows, cols]}")
+        w, b = self._vector("layer_norm", weight, "weight", cols), self._vector("layer_norm", bias, "bias", cols)
+        if out is None:
+            out = self._empty(dtype or x.dtype, stream, rows, cols)
+        elif (dtype or out.dtype) != out.dtype:
+            raise ValueError(f"layer_norm: out must be of dtype {dtype}")
+        dy, ldy = self._rows_of("layer_norm", out, "out", rows, cols)
+        st = self._empty(_torch.float32, stream, rows, 2) if stats is True else stats if stats is not False else None
+        sp = self._vector("layer_norm", st, "stats", rows, 2)
+        if rows:
+            if stream is not None:
+                self._used(stream, x, weight, bias, out, st)
+            rc = lib_.dit_layer_norm(self.ptr, dx, x.data_ptr(), ldx, w, b, eps, dy, out.data_ptr(), ldy, sp, rows, cols,
+                                     self._stream(stream))
+            if rc:
+                self.check(rc, "dit_layer_norm")
+        return out if st is None else (out, st)
+
+    def layer_norm_grad(self, dy, x, stats, weight=None, x_scale=None, params=True, dtype=None, dx=None, stream=None):
+        """dit_layer_norm_grad: (dx, dweight, dbias) for the gradient dy [rows, cols] of layer_norm's result, its input x
+        (bf16, fp32, or 8-bit rows and x_scale as quant_fp8 returns them) and stats.  params=False: dx alone, the others
+        None.  `dtype` of dx (default x's, bf16 for 8-bit rows), or that of the given `dx` (dy or x itself: in place)."""
+        lib_ = lib()
+        what = "layer_norm_grad"
+        ddy, lddy = self._rows_of(what, dy, "dy")
+        rows, cols = dy.shape
+        if rows > OPS_ROWS_MAX or cols > NORM_COLS_MAX:
+            raise ValueError(f"{what}: at most {OPS_ROWS_MAX} rows and {NORM_COLS_MAX} columns, got {[rows, cols]}")
+        if x_scale is None:
+            dtx, ldx = self._rows_of(what, x, "x", rows, cols)
+            xs, ld_xs = None, 0
+        else:
+            self._bytes_of(what, x, "x", _e4m3, rows, (cols + 127) // 128 * 128)
+            dtx, ldx = DIT_FP8, 0
+            xs, ld_xs = x_scale.data_ptr(), self._scale_ld(what, x_scale, "x_scale", (cols + 511) // 512, rows)
+        sp, w = self._vector(what, stats, "stats", rows, 2), self._vector(what, weight, "weight", cols)
+        if sp is None:
+            raise ValueError(f"{what}: stats must be a contiguous fp32 tensor [{rows}, 2]")
+        if dx is None:
+            dx = self._empty(dtype or (x.dtype if x_scale is None else _torch.bfloat16), stream, rows, cols)
+        elif (dtype or dx.dtype) != dx.dtype:
+            raise ValueError(f"{what}: dx must be of dtype {dtype}")
+        dtd, lddx = self._rows_of(what, dx, "dx", rows, cols)
+        dw = db = work = None
+        if params:
+            dw, db = self._empty(_torch.float32, stream, cols), self._empty(_torch.float32, stream, cols)
+            work = self._work(stream, lib_.dit_layer_norm_grad_work(rows, cols))
+        if rows or params:
+            if stream is not None:
+                self._used(stream, dy, x, x_scale, stats, weight, dx, dw, db)
+            rc = lib_.dit_layer_norm_grad(self.ptr, ddy, dy.data_ptr(), lddy, dtx, x.data_ptr(), ldx, xs, ld_xs, sp, w, dtd,
+                                          dx.data_ptr(), lddx, *_address(dw, db), *_work_of(work), rows, cols,
+                                          self._stream(stream))
+            if rc:
+                self.check(rc, "dit_layer_norm_grad")
+        return dx, dw, db
+
+    def grad_weight_fp8(self, dy, x, x_scale, cols=None, bias=False, dtype=None, out=None, add=False, stream=None):
+        """dit_grad_weight_fp8: dW [N, cols] = dy^T X for the gradient dy [M, N] (bf16 or fp32) of X W^T and X [M, cols] in
+        8-bit rows as quant_fp8 returns them (cols: X's columns, default all that x holds).  `dtype` fp32 (default) or bf16,
+        or that of `out` (rows may be strided).  bias=True: (dW, db), dy's sums over the rows (fp32 [N]); a tensor is
+        written.  add=True: added to what `out` (fp32) and a given bias hold."""
+        lib_ = lib()
+        what = "grad_weight_fp8"
+        ddy, lddy = self._rows_of(what, dy, "dy")
+        M, N = dy.shape
+        shape = x.shape
+        if len(shape) != 2:
+            raise ValueError(f"{what}: x must be [M, K]")
+        K = shape[1] if cols is None else cols
+        if K < 1 or (K + 127) // 128 * 128 != shape[1]:
+            raise ValueError(f"{what}: x of {shape[1]} columns does not hold {K} padded to 128")
+        if M > OPS_ROWS_MAX or N > OPS_COLS_MAX or K > OPS_COLS_MAX:
+            raise self._too_large(what, M, N, K)
+        self._bytes_of(what, x, "x", _e4m3, M, shape[1])
+        ld_s = self._scale_ld(what, x_scale, "x_scale", (K + 511) // 512, M)
+        if add and (out is None or bias is True):
+            raise ValueError(f"{what}: add needs an out, and a tensor for bias, to add to")
+        if out is None:
+            out = self._empty(dtype or _torch.float32, stream, N, K)
+        elif (dtype or out.dtype) != out.dtype:
+            raise ValueError(f"{what}: out must be of dtype {dtype}")
+        dtw, ldw = self._rows_of(what, out, "out", N, K)
+        db = self._empty(_torch.float32, stream, N) if bias is True else bias if bias is not False else None
+        bp = self._vector(what, db, "bias", N)
+        work = self._work(stream, lib_.dit_grad_weight_work(ddy, dtw, M, N, K))
+        if stream is not None:
+            self._used(stream, dy, x, x_scale, out, db)
+        rc = lib_.dit_grad_weight_fp8(self.ptr, ddy, dy.data_ptr(), lddy, x.data_ptr(), x_scale.data_ptr(), ld_s, dtw,
+                                      out.data_ptr(), ldw, bp, 1 if add else 0, *_work_of(work), M, N, K, self._stream(stream))
+        if rc:
+            self.check(rc, "dit_grad_weight_fp8")
+        return out if db is None else (out, db)
+
+    def cross_plan(self, heads, head_d, q_len, k_len, kv_heads=None, q_at=None, k_at=None):
+        """dit_cross_create: the lengths of a batch for cross_attn, of each sequence its query rows q_at .. q_at + q_len and key
+        rows k_at .. k_at + k_len (host integers; without q_at or k_at sequences follow one another).  Sequences may share
+        the same key rows.  Made once for a batch, with a copy to the device (not while a stream is captured)."""
+        return CrossPlan(self, heads, head_d, q_len, k_len, kv_heads, q_at, k_at)
+
+    def _heads_of(self, what, plan, t, name, rows, heads, like=None):
+        """t as a dit_heads: [rows or more, heads, head_d] with contiguous channels, of like's dtype and shape."""
+        shape, st = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != plan.head_d or shape[0] < rows or st[2] != 1:
+            raise ValueError(f"{what}: {name} must be [{rows} rows or more, {heads}, {plan.head_d}] with contiguous channels, got "
+                             f"{list(shape)} with strides {st}")
+        if like is not None and (t.dtype != like.dtype or shape[0] != like.shape[0]):
+            raise ValueError(f"{what}: {name} must have {like.shape[0]} rows of {like.dtype}, got {shape[0]} of {t.dtype}")
+        if t.get_device() != self.device:
+            raise self._elsewhere(what, t)
+        # a stride of one thing only does not matter
+        return _HEADS.pack(t.data_ptr(), st[0] if shape[0] > 1 else 0, st[1] if heads > 1 else 0)
+
+    def _cross_inputs(self, what, plan, q, k, v, mask, scale):
+        dtype = _dtype_of(what, q)
+        if plan.device != self.device or not plan.ptr:
+            raise ValueError(f"{what}: the plan is of device {plan.device}, or closed; the context is of device {self.device}")
+        if k.dtype != q.dtype:
+            raise ValueError(f"{what}: q, k and v must have one dtype, got {q.dtype} and {k.dtype}")
+        qkv = (self._heads_of(what, plan, q, "q", plan.q_rows, plan.heads),
+               self._heads_of(what, plan, k, "k", plan.k_rows, plan.kv_heads),
+               self._heads_of(what, plan, v, "v", plan.k_rows, plan.kv_heads, k))
+        if mask is not None:
+            if mask.dtype not in (_torch.bool, _torch.uint8) or mask.shape != k.shape[:1] or not mask.is_contiguous():
+                raise ValueError(f"{what}: mask must be a contiguous bool tensor [{k.shape[0]}]")
+            if mask.get_device() != self.device:
+                raise self._elsewhere(what, mask)
+        return dtype, qkv, mask.data_ptr() if mask is not None else None, plan.head_d ** -0.5 if scale is None else scale
+
+    def cross_attn(self, plan, q, k, v, mask=None, scale=None, out=None, lse=False, stream=None):
+        """dit_cross_forward: softmax(scale q k^T) v by the plan's sequences, q [rows, heads, head_d] and k, v [rows, kv_heads,
+        head_d] (bf16 or fp32, channels contiguous); mask: bool [key rows], False keys take no part; scale: default
+        head_d^-0.5.  lse=True: (out, lse), fp32 [heads, query rows], which cross_attn_grad takes; a tensor is written.  Rows of
+        no sequence are zeros in results made here and stay as they are in given ones."""
+        lib_ = lib()
+        what = "cross_attn"
+        dtype, qkv, mp, scale = self._cross_inputs(what, plan, q, k, v, mask, scale)
+        if out is None:
+            out = self._made(q.dtype, stream, plan.q_whole(q.shape[0]), *q.shape)
+        op = self._heads_of(what, plan, out, "out", plan.q_rows, plan.heads, q)
+        l = lse if lse is not True and lse is not False else None
+        if lse is True:
+            l = self._made(_torch.float32, stream, plan.q_whole(q.shape[0]), plan.heads, q.shape[0])
+        lp = self._vector(what, l, "lse", plan.heads, q.shape[0])
+        work = self._work(stream, plan.work(dtype, 0))
+        if stream is not None:
+            self._used(stream, q, k, v, mask, out, l)
+        rc = lib_.dit_cross_forward(self.ptr, plan.ptr, dtype, *qkv, mp, scale, op, lp, q.shape[0], *_work_of(work),
+                                    self._stream(stream))
+        if rc:
+            self.check(rc, "dit_cross_forward")
+        return out if l is None else (out, l)
+
+    def cross_attn_grad(self, plan, dout, q, k, v, out, lse, mask=None, scale=None, dq=None, dk=None, dv=None, stream=None):
+        """dit_cross_grad: (dq, dk, dv) for the gradient dout of cross_attn's result, from its inputs and results.  Gradients
+        of keys are summed over the heads and sequences that share them; rows of no sequence as in cross_attn."""
+        lib_ = lib()
+        what = "cross_attn_grad"
+        dtype, qkv, mp, scale = self._cross_inputs(what, plan, q, k, v, mask, scale)
+        dop = self._heads_of(what, plan, dout, "dout", plan.q_rows, plan.heads, q)
+        op = self._heads_of(what, plan, out, "out", plan.q_rows, plan.heads, q)
+        lp = self._vector(what, lse, "lse", plan.heads, q.shape[0])
+        if lp is None:
+            raise ValueError(f"{what}: lse must be a contiguous fp32 tensor [{plan.heads}, {q.shape[0]}]")
+        if dq is None:
+            dq = self._made(q.dtype, stream, plan.q_whole(q.shape[0]), *q.shape)
+        whole = plan.k_whole(k.shape[0])
+        dk = self._made(k.dtype, stream, whole, *k.shape) if dk is None else dk
+        dv = self._made(v.dtype, stream, whole, *v.shape) if dv is None else dv
+        grads = (self._heads_of(what, plan, dq, "dq", plan.q_rows, plan.heads, q),
+                 self._heads_of(what, plan, dk, "dk", plan.k_rows, plan.kv_heads, k),
+                 self._heads_of(what, plan, dv, "dv", plan.k_rows, plan.kv_heads, k))
+        work = self._work(stream, plan.work(dtype, 1))
+        if stream is not None:
+            self._used(stream, dout, q, k, v, out, lse, mask, dq, dk, dv)
+        rc = lib_.dit_cross_grad(self.ptr, plan.ptr, dtype, dop, *qkv, op, lp, q.shape[0], mp, scale, *grads, *_work_of(work),
+                                 self._stream(stream))
+        if rc:
+            self.check(rc, "dit_cross_grad")
+        return dq, dk, dv
+
+    def _work(self, stream, size):
+        """A call's workspace, from the memory of the stream that uses it."""
+        if size < 0:
+            raise AwaError(AWA_EARG, "workspace of sizes out of range")
+        return self._empty(_torch.uint8, stream, size) if size else None
+
+    def _made(self, dtype, stream, whole, *shape):
+        """A result; zeros where not every row of it is written."""
+        if whole:
+            return self._empty(dtype, stream, *shape)
+        if stream is None:
+            return _torch.zeros(*shape, dtype=dtype, device=self._on)
+        t = self._empty(dtype, stream, *shape)
+        with _torch.cuda.stream(stream):
+            t.zero_()
+        return t
+
     def reserve(self, geom, dtype="bf16"):
         """awa_reserve: size the op's scratch for geom in this storage dtype."""
         self.check(lib().awa_reserve(self.ptr, geom.ptr, AWA_BF16 if dtype == "bf16" else AWA_F32), "awa_reserve")
@@ -851,6 +1110,64 @@ class Context:
                                     float(eps), P(vo), P(to))
         self.check(rc, "awa_forward_host")
         return vo, to
+
+
+class CrossPlan:
+    """dit_cross: the lengths of a batch (see Context.cross_plan); keep it until the calls that use it have finished."""
+
+    def __init__(self, ctx, heads, head_d, q_len, k_len, kv_heads=None, q_at=None, k_at=None):
+        def integers(v, name):
+            a = np.asarray(v)
+            if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+                raise ValueError(f"cross_plan: {name} must be a list of integers")
+            return np.ascontiguousarray(a, np.int64)
+
+        self.ptr = C.c_void_p()
+        ql, kl = integers(q_len, "q_len"), integers(k_len, "k_len")
+        qa = np.cumsum(ql) - ql if q_at is None else integers(q_at, "q_at")
+        ka = np.cumsum(kl) - kl if k_at is None else integers(k_at, "k_at")
+        n = ql.size
+        if not n == kl.size == qa.size == ka.size:
+            raise ValueError("cross_plan: one length and one place of queries and keys for each sequence")
+        kv_heads = heads if kv_heads is None else kv_heads
+        if n > CROSS_SEQ_MAX or not (0 < kv_heads <= heads <= CROSS_HEADS_MAX) or not 0 < head_d <= CROSS_HEAD_D_MAX:
+            raise ValueError(f"cross_plan: at most {CROSS_SEQ_MAX} sequences, {CROSS_HEADS_MAX} heads of {CROSS_HEAD_D_MAX} "
+                             f"channels, got {n}, {heads} ({kv_heads} of keys) of {head_d}")
+        rc = lib().dit_cross_create(ctx.ptr, n, *[a.ctypes.data_as(C.POINTER(C.c_int64)) for a in (qa, ql, ka, kl)], heads,
+                                    kv_heads, head_d, C.byref(self.ptr))
+        ctx.check(rc, "dit_cross_create")
+        self.device, self.heads, self.kv_heads, self.head_d = ctx.device, heads, kv_heads, head_d
+        self.q_rows = int((qa + ql)[ql > 0].max(initial=0))
+        self.k_rows = int((ka + kl)[kl > 0].max(initial=0))
+        # rows that belong to a sequence (shared keys counted once)
+        self._q_count = int(ql.sum())
+        self._k_count = int(sum(dict(zip(ka[kl > 0].tolist(), kl[kl > 0].tolist())).values()))
+        self._work = {}
+
+    def q_whole(self, rows):
+        """Whether every one of so many query rows belongs to a sequence."""
+        return self._q_count == rows
+
+    def k_whole(self, rows):
+        return self._k_count == rows
+
+    def work(self, dtype, grad):
+        """dit_cross_work, asked once."""
+        n = self._work.get((dtype, grad))
+        if n is None:
+            n = self._work[dtype, grad] = lib().dit_cross_work(self.ptr, dtype, grad)
+        return n
+
+    def close(self):
+        if self.ptr:
+            lib().dit_cross_destroy(self.ptr)
+            self.ptr = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Geometry:

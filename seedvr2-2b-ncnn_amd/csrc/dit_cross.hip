@@ -1,0 +1,343 @@
+// dit_cross.hip — attention to states of another length: the forward pass and the gradient of the queries.
+//
+// A workgroup takes a block of columns (queries of one head, or of the heads that share a key head: see
+// CrossItem) over a run of keys.  Scores are formed transposed, S^T = K Q^T, so that a lane owns one column: its
+// softmax needs two lane exchanges a tile, and the probabilities leave the accumulator as the operand of
+// O^T += V^T P^T (dit_cross_device.hpp).  Keys and values reach LDS by DMA, the next tile's during this one's
+// products; masked keys and rows past the end are fetched from past the buffer and so become zeros, whatever memory
+// holds there, and their scores -infinity.  The gradient of the queries is the same walk with P from the kept
+// lse: dP^T = V dO^T, dS = P (dP - D), dQ^T += K^T dS^T.
+//
+// Two shapes: blocks of 128 columns, four waves of 32 that share the tiles; and for few columns (tokens being
+// generated) blocks of 16 or 32, waves that take tiles of their own in turn and add their results in LDS.
+// Runs of keys of one block that go to different workgroups leave fp32 partial results, which a second kernel joins.
+#include "dit_cross_device.hpp"
+
+namespace awa {
+
+using namespace cross;
+
+namespace {
+
+template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD>
+__global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p) {
+    using Frag = typename T::Frag;
+    using L = Tile<T, DP>;
+    constexpr int KS = DP / 32, DB = DP / 16, KB = KT / 16, WAVES = WQ * WK;
+    constexpr int TILE_B = KT * L::ROW, STAGE = 2 * TILE_B;  // K, then V
+    constexpr int JOIN = WK > 1 ? WAVES * NQ * 16 * (DP + 2) * 4 : 0;
+    constexpr int LDS = WK * 2 * STAGE > JOIN ? WK * 2 * STAGE : JOIN;
+    static_assert(LDS <= 160 * 1024 && (WQ == 1 || WK == 1), "LDS");
+    __shared__ __align__(16) char lds[LDS];
+    const int groups = p.heads / p.qs.pack, total = p.qs.n_items * groups;
+    const int wg = xcd_remap(total);
+    if (wg >= total) return;
+    const int hb = wg / p.qs.n_items;
+    const CrossItem it = p.qs.items[wg - hb * p.qs.n_items];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wq = wave % WQ, wk = wave / WQ, g = lane >> 4;
+    const int head0 = hb * p.qs.pack, kv_head = head0 / (p.heads / p.kv_heads);
+    const int width = p.head_d * T::SIZE;
+
+    // the wave's columns
+    int row[NQ], head[NQ];
+    bool there[NQ];
+    Frag q[NQ][KS], dout[GRAD ? NQ : 1][KS];
+    float lse2[NQ], dsum[NQ];  // GRAD: lse in powers of two, rowsum(dout out)
+#pragma unroll
+    for (int j = 0; j < NQ; j++) {
+        const int c = (wq * NQ + j) * 16 + (lane & 15);
+        there[j] = c < it.cols;
+        row[j] = it.q0 + c / p.qs.pack;
+        head[j] = head0 + c % p.qs.pack;
+        const char* at = p.q + row[j] * p.q_row + head[j] * p.q_head;
+        const char* dat = p.dout + row[j] * p.dout_row + head[j] * p.dout_head;
+        const char* oat = p.out + row[j] * p.out_row + head[j] * p.out_head;
+        lse2[j] = dsum[j] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int d = 32 * ks + 8 * g;
+            const bool in = there[j] && d < p.head_d;
+            q[j][ks] = T::zero();
+            if (in) q[j][ks] = T::load(at + d * T::SIZE);
+            if constexpr (GRAD) {
+                dout[j][ks] = T::zero();
+                if (in) {
+                    dout[j][ks] = T::load(dat + d * T::SIZE);
+                    dsum[j] += T::dot(dout[j][ks], T::load(oat + d * T::SIZE));
+                }
+            }
+        }
+        if constexpr (GRAD) {
+            dsum[j] = sum4(dsum[j]);
+            if (there[j]) {
+                const float l = p.lse[head[j] * p.ld_lse + row[j]];
+                lse2[j] = l == -INFINITY ? INFINITY : l * LOG2E;  // a row without keys: P = 0
+                if (it.first && wk == 0 && g == 0) p.dsum[head[j] * p.ld_dsum + row[j]] = dsum[j];
+            }
+        }
+    }
+
+    f32x4 acc[DB][NQ];
+    float top[NQ], sum[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; j++) {
+        top[j] = -INFINITY;
+        sum[j] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; db++) acc[db][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int tiles = (it.kn + KT - 1) / KT;
+    const uint8_t* mask = p.mask ? p.mask + it.k0 : nullptr;
+    auto mask_byte = [&](int t) __attribute__((always_inline)) {
+        const int key = t * KT + lane;
+        return mask && lane < KT && key < it.kn ? (int)mask[key] : 1;
+    };
+    auto valid_of = [&](int t, int byte) __attribute__((always_inline)) {
+        return __builtin_amdgcn_ballot_w64(lane < KT && t * KT + lane < it.kn && byte);
+    };
+    char* ring = lds + wk * 2 * STAGE;
+    auto fetch = [&](int t, int slot, uint64_t valid) __attribute__((always_inline)) {
+        const int64_t first = it.k0 + (int64_t)t * KT;
+        const __amdgpu_buffer_rsrc_t kr = uniform_rsrc(p.k + kv_head * p.k_head + first * p.k_row, 0x7fffffffu);
+        const __amdgpu_buffer_rsrc_t vr = uniform_rsrc(p.v + kv_head * p.v_head + first * p.v_row, 0x7fffffffu);
+        char* st = ring + slot * STAGE;
+        constexpr int N = TILE_B / 1024;
+#pragma unroll
+        for (int i = 0; i < N / WQ; i++) {
+            L::dma(st, wq * (N / WQ) + i, kr, p.k_row, valid, width, lane);
+            L::dma(st + TILE_B, wq * (N / WQ) + i, vr, p.v_row, valid, width, lane);
+        }
+    };
+    uint64_t valid = 0;
+    int byte = 1;
+    if (wk < tiles) {
+        valid = valid_of(wk, mask_byte(wk));
+        byte = mask_byte(wk + WK);
+        fetch(wk, 0, valid);
+    }
+    int slot = 0;
+    for (int t = wk; t < tiles; t += WK, slot ^= 1) {
+        wait_vmem_lds<0>();  // this tile has landed (and what was read of the other slot has arrived)
+        if constexpr (WQ > 1) __syncthreads();
+        const uint64_t next = valid_of(t + WK, byte);
+        byte = mask_byte(t + 2 * WK);
+        if (t + WK < tiles) fetch(t + WK, slot ^ 1, next);
+        const char* kt = ring + slot * STAGE;
+        const char* vt = kt + TILE_B;
+
+        f32x4 s[KB][NQ], dp[GRAD ? KB : 1][NQ];
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const Frag kf = L::row_frag(kt, 16 * b + (lane & 15), ks, g);
+#pragma unroll
+                for (int j = 0; j < NQ; j++) s[b][j] = T::mma(kf, q[j][ks], ks ? s[b][j] : (f32x4){0.f, 0.f, 0.f, 0.f});
+                if constexpr (GRAD) {
+                    const Frag vf = L::row_frag(vt, 16 * b + (lane & 15), ks, g);
+#pragma unroll
+                    for (int j = 0; j < NQ; j++)
+                        dp[b][j] = T::mma(vf, dout[j][ks], ks ? dp[b][j] : (f32x4){0.f, 0.f, 0.f, 0.f});
+                }
+            }
+        constexpr uint64_t ALL = KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1;
+        if (valid != ALL) {
+            const uint64_t mine = valid >> (4 * g);
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (!((mine >> (16 * b + r)) & 1))
+#pragma unroll
+                        for (int j = 0; j < NQ; j++) s[b][j][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; j++) {
+            if constexpr (GRAD) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float e = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -lse2[j]));
+                        s[b][j][r] = e * (dp[b][j][r] - dsum[j]);
+                    }
+                if (valid != ALL) {  // what a masked key's products hold is no number to multiply by zero
+                    const uint64_t mine = valid >> (4 * g);
+#pragma unroll
+                    for (int b = 0; b < KB; b++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (!((mine >> (16 * b + r)) & 1)) s[b][j][r] = 0.f;
+                }
+            } else {
+                float m = s[0][j][0];
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) m = fmaxf(m, s[b][j][r]);
+                m = fmaxf(max4(m), top[j]);
+                const float ref = m == -INFINITY ? 0.f : m * p.c;
+                const float fade = exp2_of(top[j] * p.c - ref);
+                top[j] = m;
+                float add = 0.f;
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        s[b][j][r] = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -ref));
+                        add += s[b][j][r];
+                    }
+                sum[j] = sum[j] * fade + add;
+#pragma unroll
+                for (int db = 0; db < DB; db++) acc[db][j] *= fade;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < KB / 2; h++) {
+            Frag pf[NQ];
+#pragma unroll
+            for (int j = 0; j < NQ; j++) pf[j] = T::pack(s[2 * h][j], s[2 * h + 1][j]);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const Frag f = L::column_frag(GRAD ? kt : vt, 32 * h, db, lane);
+#pragma unroll
+                for (int j = 0; j < NQ; j++) acc[db][j] = T::mma(f, pf[j], acc[db][j]);
+            }
+        }
+        valid = next;
+    }
+
+    const int d = p.head_d;
+    char* const to = GRAD ? p.dq : p.o;
+    const int64_t to_row = GRAD ? p.dq_row : p.o_row, to_head = GRAD ? p.dq_head : p.o_head;
+    float* const part = it.part < 0 ? nullptr : p.qpart + ((int64_t)it.part * groups + hb) * cross_query_part(p.qs.block, d);
+#pragma unroll
+    for (int j = 0; j < NQ; j++) sum[j] = sum4(sum[j]);
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int j = 0; j < NQ; j++) {
+            if (!there[j]) continue;
+            const int c = (wq * NQ + j) * 16 + (lane & 15);
+            const float f = part ? 1.f : GRAD ? p.scale : sum[j] > 0.f || sum[j] != sum[j] ? 1.f / sum[j] : 0.f;
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const int ch = 16 * db + 4 * g;
+                if (ch >= d) continue;
+                if (part) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = acc[db][j];
+                else T::store4(to + row[j] * to_row + head[j] * to_head + ch * T::SIZE, acc[db][j] * f);
+            }
+            if (!GRAD && g == 0) {
+                if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){top[j], sum[j]};
+                else if (p.lse) p.lse[head[j] * p.ld_lse + row[j]] = top[j] == -INFINITY ? -INFINITY : top[j] * p.scale + LN2 * __builtin_amdgcn_logf(sum[j]);
+            }
+        }
+    } else {
+        // the waves' results, in their order
+        constexpr int COLS = 16 * NQ;
+        float* all = reinterpret_cast<float*>(lds);
+        float* ml = all + WAVES * COLS * DP;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NQ; j++) {
+            const int c = 16 * j + (lane & 15);
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+                *reinterpret_cast<f32x4*>(all + (wave * COLS + c) * DP + 16 * db + 4 * g) = acc[db][j];
+            if (g == 0) *reinterpret_cast<f32x2*>(ml + 2 * (wave * COLS + c)) = (f32x2){top[j], sum[j]};
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < COLS * (DP / 4); e += 64 * WAVES) {
+            const int c = e / (DP / 4), ch = e % (DP / 4) * 4;
+            if (c >= it.cols || ch >= d) continue;
+            float m = -INFINITY, l = 0.f;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (!GRAD) {
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) m = fmaxf(m, ml[2 * (w * COLS + c)]);
+            }
+            const float ref = m == -INFINITY ? 0.f : m * p.c;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float f = GRAD ? 1.f : exp2_of(ml[2 * (w * COLS + c)] * p.c - ref);
+                v += *reinterpret_cast<const f32x4*>(all + (w * COLS + c) * DP + ch) * f;
+                if constexpr (!GRAD) l += ml[2 * (w * COLS + c) + 1] * f;
+            }
+            const int r = it.q0 + c / p.qs.pack, h = head0 + c % p.qs.pack;
+            const float f = part ? 1.f : GRAD ? p.scale : l > 0.f || l != l ? 1.f / l : 0.f;
+            if (part) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = v;
+            else T::store4(to + r * to_row + h * to_head + ch * T::SIZE, v * f);
+            if (!GRAD && ch == 0) {
+                if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){m, l};
+                else if (p.lse) p.lse[h * p.ld_lse + r] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+            }
+        }
+    }
+}
+
+// Blocks whose keys went to several workgroups: the parts in their order, a piece of four channels a thread.
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
+    const int groups = p.heads / p.qs.pack, hb = blockIdx.x / p.qs.n_joins;
+    const CrossJoin it = p.qs.joins[blockIdx.x - hb * p.qs.n_joins];
+    const int d = p.head_d, pieces = d / 4;
+    const int64_t stride = (int64_t)groups * cross_query_part(p.qs.block, d);
+    const float* first = p.qpart + ((int64_t)it.part0 * groups + hb) * cross_query_part(p.qs.block, d);
+    for (int e = threadIdx.x; e < it.cols * pieces; e += 256) {
+        const int c = e / pieces, ch = e % pieces * 4;
+        const float* o = first + (int64_t)c * d + ch;
+        const float* ml = first + (int64_t)p.qs.block * d + 2 * c;
+        float m = -INFINITY, l = 0.f;
+        if constexpr (!GRAD)
+            for (int i = 0; i < it.parts; i++) m = fmaxf(m, ml[i * stride]);
+        const float ref = m == -INFINITY ? 0.f : m * p.c;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < it.parts; i++) {
+            const float f = GRAD ? 1.f : exp2_of(ml[i * stride] * p.c - ref);
+            v += *reinterpret_cast<const f32x4*>(o + i * stride) * f;
+            if constexpr (!GRAD) l += ml[i * stride + 1] * f;
+        }
+        const int r = it.q0 + c / p.qs.pack, h = hb * p.qs.pack + c % p.qs.pack;
+        const float f = GRAD ? p.scale : l > 0.f || l != l ? 1.f / l : 0.f;
+        char* to = GRAD ? p.dq + r * p.dq_row + h * p.dq_head : p.o + r * p.o_row + h * p.o_head;
+        T::store4(to + ch * T::SIZE, v * f);
+        if (!GRAD && ch == 0 && p.lse)
+            p.lse[h * p.ld_lse + r] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+    }
+}
+
+template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD>
+void run(const CrossArgs& a, hipStream_t s) {
+    const long total = (long)a.qs.n_items * (a.heads / a.qs.pack);
+    hipLaunchKernelGGL((cross_queries_kernel<T, DP, NQ, WQ, WK, KT, GRAD>), dim3(xcd_grid(total)), dim3(64 * WQ * WK), 0, s, a);
+}
+template <typename T, int DP, bool GRAD>
+void run_block(const CrossArgs& a, hipStream_t s) {
+    constexpr int WK = T::SIZE == 2 ? 4 : 2;
+    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 ? 64 : 32, GRAD>(a, s);
+    else if (a.qs.block == 32) run<T, DP, 2, 1, WK, 32, GRAD>(a, s);
+    else run<T, DP, 1, 1, WK, 32, GRAD>(a, s);
+}
+template <typename T, bool GRAD>
+hipError_t run_all(const CrossArgs& a, hipStream_t s) {
+    if (a.qs.n_items == 0) return hipSuccess;
+    if (a.head_d <= 64) run_block<T, 64, GRAD>(a, s);
+    else if (a.head_d <= 96) run_block<T, 96, GRAD>(a, s);
+    else run_block<T, 128, GRAD>(a, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.qs.n_joins == 0) return e;
+    hipLaunchKernelGGL((cross_join_kernel<T, GRAD>), dim3((unsigned)(a.qs.n_joins * (a.heads / a.qs.pack))), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cross_forward(int dtype, const CrossArgs& a, hipStream_t s) {
+    return dtype == AWA_F32 ? run_all<F32, false>(a, s) : run_all<Bf16, false>(a, s);
+}
+hipError_t launch_cross_grad_queries(int dtype, const CrossArgs& a, hipStream_t s) {
+    return dtype == AWA_F32 ? run_all<F32, true>(a, s) : run_all<Bf16, true>(a, s);
+}
+
+}  // namespace awa

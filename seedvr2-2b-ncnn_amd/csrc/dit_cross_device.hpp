@@ -1,0 +1,142 @@
+// dit_cross_device.hpp — fragments, LDS tiles and reductions of the attention kernels of dit_train.h.
+//
+// All products are 16 x 16 x 32 with eight values of the summed axis a lane: lane 16 g + i holds values
+// 8 g .. 8 g + 7 of row (column) i.  For bf16 that is one matrix instruction; for fp32 it is eight of
+// 16 x 16 x 4, the j-th on the lanes' j-th values.  A result's lane 16 g + i holds rows 4 g .. 4 g + 3 of
+// column i.  So where 32 rows of a result (two blocks of 16) are the summed axis of the next product, a lane
+// already holds eight of them, {4 g + j, 16 + 4 g + j}, and the other operand is read in that order.
+#pragma once
+
+#include "dit_device.hpp"
+#include "dit_train_internal.hpp"
+
+namespace awa {
+namespace cross {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) bf16x4 lbf16x4_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+struct Bf16 {
+    static constexpr int SIZE = 2;
+    using Frag = bf16x8;
+    static __device__ inline Frag zero() { return (bf16x8)(__bf16)0.f; }
+    static __device__ inline f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    // two blocks of a result as the next product's operand
+    static __device__ inline Frag pack(const f32x4& lo, const f32x4& hi) {
+        const f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_convertvector(v, bf16x8);
+    }
+    static __device__ inline float dot(const Frag& a, const Frag& b) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = __builtin_fmaf((float)a[i], (float)b[i], s);
+        return s;
+    }
+    static __device__ inline Frag load(const char* p) { return __builtin_bit_cast(Frag, *reinterpret_cast<const u32x4*>(p)); }
+    // four consecutive channels
+    static __device__ inline void store4(char* p, const f32x4& v) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
+    }
+};
+struct F32 {
+    static constexpr int SIZE = 4;
+    using Frag = f32x8;
+    static __device__ inline Frag zero() { return (f32x8)0.f; }
+    static __device__ inline f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
+        f32x4 r = c;
+#pragma unroll
+        for (int j = 0; j < 8; j++) r = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], r, 0, 0, 0);
+        return r;
+    }
+    static __device__ inline Frag pack(const f32x4& lo, const f32x4& hi) {
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ inline float dot(const Frag& a, const Frag& b) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = __builtin_fmaf(a[i], b[i], s);
+        return s;
+    }
+    static __device__ inline Frag load(const char* p) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 16);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ inline void store4(char* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+};
+
+// An LDS tile: rows of 64 or 128 channels (DP = 96 has rows of 128, whose last channels nothing reads), 16-byte
+// chunk c of row r at chunk c ^ swizzle(r): eight neighbouring rows, and the four rows of a transposed read's 16
+// lanes, begin at different banks.
+__device__ inline int swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+template <typename T, int DP>
+struct Tile {
+    static constexpr int ROW = (DP == 64 ? 64 : 128) * T::SIZE, CHUNKS = ROW / 16, PER = 1024 / ROW;  // PER: rows of an instruction
+    // eight channels 32 ks + 8 g .. of row `row`
+    static __device__ inline typename T::Frag row_frag(const char* t, int row, int ks, int g) {
+        const char* at = t + row * ROW;
+        const int s = swizzle(row);
+        if constexpr (T::SIZE == 2) {
+            return __builtin_bit_cast(typename T::Frag, *reinterpret_cast<const u32x4*>(at + (((4 * ks + g) ^ s) << 4)));
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(at + (((8 * ks + 2 * g) ^ s) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(at + (((8 * ks + 2 * g + 1) ^ s) << 4));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // channel 16 db + lane % 16 of rows base + {4 g + j, 16 + 4 g + j}; base a multiple of 16
+    static __device__ inline typename T::Frag column_frag(const char* t, int base, int db, int lane) {
+        const int g = lane >> 4;
+        if constexpr (T::SIZE == 2) {
+            // lane 16 g + 4 i + a of a transposed read addresses row 4 g + i, channels 4 a .. 4 a + 3, and receives its
+            // own channel's rows 4 g .. 4 g + 3
+            const int r = 4 * g + ((lane >> 2) & 3), a = lane & 3;
+            const char* at = t + (base + r) * ROW + (((2 * db + (a >> 1)) ^ swizzle(r)) << 4) + ((a & 1) << 3);
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lbf16x4_t*)at);
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lbf16x4_t*)(at + 16 * ROW));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            typename T::Frag f;
+            const int c = 4 * db + ((lane >> 2) & 3);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = 4 * g + j;
+                const char* at = t + (base + r) * ROW + ((c ^ swizzle(r)) << 4) + ((lane & 3) << 2);
+                f[j] = *reinterpret_cast<const float*>(at);
+                f[4 + j] = *reinterpret_cast<const float*>(at + 16 * ROW);
+            }
+            return f;
+        }
+    }
+    // DMA instruction i of a tile: rows PER i .. of it, one 16-byte chunk a lane.  Rows that are not in `valid` (a bit
+    // per row) and channels past head_d lie past the resource and become zeros.
+    static __device__ inline void dma(char* t, int i, __amdgpu_buffer_rsrc_t from, int64_t row_bytes, uint64_t valid, int width,
+                                      int lane) {
+        const int row = i * PER + lane / CHUNKS, c = ((lane % CHUNKS) ^ swizzle(row)) << 4;
+        const bool in = ((valid >> row) & 1) && c < width;
+        const uint32_t at = in ? (uint32_t)(row * (uint32_t)row_bytes + c) : 0x80000000u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(t + i * 1024), 16, at, 0, 0, 0);
+    }
+};
+
+// Over the four lanes l % 16 + 16 i
+__device__ inline float sum4(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+}  // namespace cross
+}  // namespace awa

@@ -1,0 +1,240 @@
+// dit_cross_keys.hip — attention to states of another length: the gradient of keys and values.
+//
+// A workgroup takes a block of keys of one key head over a run of units, up to 64 query rows of one head each, of
+// all sequences that attend to these keys and all heads that share the key head.  Here keys are the columns: with K
+// and V as operands in registers, S = Q K^T and dP = dO V^T come out with a key per lane, P and dS leave the
+// accumulators as operands of dV^T += dO^T P and dK^T += Q^T dS (dit_cross_device.hpp), and the sums stay in registers
+// over the run.  Q and dO reach LDS by DMA, the next unit's during this one's products.
+//
+// Keys are few where queries are many, so the units are divided over workgroups, whose fp32 partial sums a second
+// kernel adds in their order.
+#include "dit_cross_device.hpp"
+
+namespace awa {
+
+using namespace cross;
+
+namespace {
+
+// NK blocks of 16 keys a wave, WKEY waves over the keys; where WKEY is 2 the other two take the second 32 rows of a
+// unit, and the two halves' sums meet in LDS at the end.
+template <typename T, int DP, int NK, int WKEY>
+__global__ __launch_bounds__(256) void cross_keys_kernel(CrossArgs p) {
+    using Frag = typename T::Frag;
+    using L = Tile<T, DP>;
+    constexpr int KS = DP / 32, DB = DP / 16, QT = CROSS_QT, SUBS = 4 / WKEY;
+    constexpr int TILE_B = QT * L::ROW, STAGE = 2 * TILE_B + 2 * QT * 4;  // Q, dO, lse, dsum
+    constexpr int JOIN = SUBS > 1 ? 2 * 64 * WKEY * NK * DB * 16 : 0;
+    constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __align__(16) char lds[LDS];
+    const int total = p.ks.n_items * p.kv_heads;
+    const int wg = xcd_remap(total);
+    if (wg >= total) return;
+    const int kv_head = wg / p.ks.n_items;
+    const CrossKeys it = p.ks.items[wg - kv_head * p.ks.n_items];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wk = wave % WKEY, sub0 = wave / WKEY, g = lane >> 4;
+    const int width = p.head_d * T::SIZE;
+
+    // the wave's keys
+    Frag k[NK][KS], v[NK][KS];
+    bool in[NK];  // takes part
+#pragma unroll
+    for (int j = 0; j < NK; j++) {
+        const int c = (wk * NK + j) * 16 + (lane & 15);
+        in[j] = c < it.kn && (!p.mask || p.mask[it.k0 + c]);
+        const char* kp = p.k + (int64_t)(it.k0 + c) * p.k_row + kv_head * p.k_head;
+        const char* vp = p.v + (int64_t)(it.k0 + c) * p.v_row + kv_head * p.v_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int d = 32 * ks + 8 * g;
+            k[j][ks] = v[j][ks] = T::zero();
+            if (in[j] && d < p.head_d) {
+                k[j][ks] = T::load(kp + d * T::SIZE);
+                v[j][ks] = T::load(vp + d * T::SIZE);
+            }
+        }
+    }
+    f32x4 dk[DB][NK], dv[DB][NK];
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int j = 0; j < NK; j++) dk[db][j] = dv[db][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int heads_per = p.heads / p.kv_heads;
+    auto fetch = [&](int u, int slot) __attribute__((always_inline)) {
+        const int head = kv_head * heads_per + u / it.units;
+        const CrossUnit un = p.ks.units[it.unit0 + u % it.units];
+        const uint64_t valid = un.rows == 64 ? ~(uint64_t)0 : ((uint64_t)1 << un.rows) - 1;
+        const __amdgpu_buffer_rsrc_t qr = uniform_rsrc(p.q + un.q0 * p.q_row + head * p.q_head, 0x7fffffffu);
+        const __amdgpu_buffer_rsrc_t dr = uniform_rsrc(p.dout + un.q0 * p.dout_row + head * p.dout_head, 0x7fffffffu);
+        char* st = lds + slot * STAGE;
+        constexpr int N = TILE_B / 1024 / 4;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            L::dma(st, wave * N + i, qr, p.q_row, valid, width, lane);
+            L::dma(st + TILE_B, wave * N + i, dr, p.dout_row, valid, width, lane);
+        }
+        if (wave < 2) {
+            const float* from = wave ? p.dsum + head * p.ld_dsum : p.lse + head * p.ld_lse;
+            const __amdgpu_buffer_rsrc_t r = uniform_rsrc(from + un.q0, (uint32_t)un.rows * 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)(st + 2 * TILE_B + wave * QT * 4), 4, 4 * lane, 0, 0, 0);
+        }
+    };
+    if (it.count > 0) fetch(it.first, 0);
+    for (int n = 0; n < it.count; n++) {
+        wait_vmem_lds<0>();
+        __syncthreads();
+        const int u = it.first + n;
+        if (n + 1 < it.count) fetch(u + 1, (n + 1) & 1);
+        const char* qt = lds + (n & 1) * STAGE;
+        const char* dt = qt + TILE_B;
+        const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE_B);
+        const int rows = p.ks.units[it.unit0 + u % it.units].rows;
+#pragma unroll
+        for (int s0 = 0; s0 < QT / 32; s0 += SUBS) {
+            const int sub = s0 + (SUBS > 1 ? sub0 : 0), base = 32 * sub;
+            if (base >= rows) continue;
+            f32x4 s[2][NK], dp[2][NK];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const Frag qf = L::row_frag(qt, base + 16 * b + (lane & 15), ks, g);
+                    const Frag df = L::row_frag(dt, base + 16 * b + (lane & 15), ks, g);
+#pragma unroll
+                    for (int j = 0; j < NK; j++) {
+                        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                        s[b][j] = T::mma(qf, k[j][ks], ks ? s[b][j] : z);
+                        dp[b][j] = T::mma(df, v[j][ks], ks ? dp[b][j] : z);
+                    }
+                }
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int r0 = base + 16 * b + 4 * g;
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + r0), d4 = *reinterpret_cast<const f32x4*>(lse + QT + r0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float l2 = l4[r] == -INFINITY ? INFINITY : l4[r] * LOG2E;  // a row without keys: P = 0
+#pragma unroll
+                    for (int j = 0; j < NK; j++) {
+                        float e = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -l2));
+                        float ds = e * (dp[b][j][r] - d4[r]);
+                        if (r0 + r >= rows) e = ds = 0.f;  // rows past the end are zeros, but infinite keys times zero are not
+                        s[b][j][r] = e;
+                        dp[b][j][r] = ds;
+                    }
+                }
+            }
+            Frag pf[NK], sf[NK];
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                pf[j] = T::pack(s[0][j], s[1][j]);
+                sf[j] = T::pack(dp[0][j], dp[1][j]);
+            }
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const Frag df = L::column_frag(dt, base, db, lane);
+#pragma unroll
+                for (int j = 0; j < NK; j++) dv[db][j] = T::mma(df, pf[j], dv[db][j]);
+                const Frag qf = L::column_frag(qt, base, db, lane);
+#pragma unroll
+                for (int j = 0; j < NK; j++) dk[db][j] = T::mma(qf, sf[j], dk[db][j]);
+            }
+        }
+    }
+    if constexpr (SUBS > 1) {
+        // the second halves' sums, to the first's
+        __syncthreads();
+        f32x4* at = reinterpret_cast<f32x4*>(lds) + (wk * 64 + lane);
+        constexpr int STEP = 64 * WKEY;
+        if (sub0) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int j = 0; j < NK; j++) {
+                    at[(2 * (db * NK + j)) * STEP] = dk[db][j];
+                    at[(2 * (db * NK + j) + 1) * STEP] = dv[db][j];
+                }
+        }
+        __syncthreads();
+        if (sub0) return;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                dk[db][j] += at[(2 * (db * NK + j)) * STEP];
+                dv[db][j] += at[(2 * (db * NK + j) + 1) * STEP];
+            }
+    }
+    const int d = p.head_d;
+    float* const part = it.part < 0 ? nullptr : p.kpart + ((int64_t)it.part * p.kv_heads + kv_head) * cross_key_part(p.ks.block, d);
+#pragma unroll
+    for (int j = 0; j < NK; j++) {
+        const int c = (wk * NK + j) * 16 + (lane & 15);
+        if (c >= it.kn) continue;
+        char* kp = p.dk + (int64_t)(it.k0 + c) * p.dk_row + kv_head * p.dk_head;
+        char* vp = p.dv + (int64_t)(it.k0 + c) * p.dv_row + kv_head * p.dv_head;
+#pragma unroll
+        for (int db = 0; db < DB; db++) {
+            const int ch = 16 * db + 4 * g;
+            if (ch >= d) continue;
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 a = in[j] ? dk[db][j] * p.scale : z, b = in[j] ? dv[db][j] : z;
+            if (part) {
+                *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = a;
+                *reinterpret_cast<f32x4*>(part + (int64_t)(p.ks.block + c) * d + ch) = b;
+            } else {
+                T::store4(kp + ch * T::SIZE, a);
+                T::store4(vp + ch * T::SIZE, b);
+            }
+        }
+    }
+}
+
+// Blocks of keys whose units went to several workgroups: the parts in their order, four channels a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
+    const int kv_head = blockIdx.x / p.ks.n_joins;
+    const CrossKeyJoin it = p.ks.joins[blockIdx.x - kv_head * p.ks.n_joins];
+    const int d = p.head_d, pieces = d / 4, e = blockIdx.y * 256 + threadIdx.x;
+    if (e >= 2 * it.kn * pieces) return;
+    const int64_t size = cross_key_part(p.ks.block, d), stride = p.kv_heads * size;
+    const int which = e / (it.kn * pieces), c = e / pieces % it.kn, ch = e % pieces * 4;
+    const float* from = p.kpart + ((int64_t)it.part0 * p.kv_heads + kv_head) * size + (int64_t)(which * p.ks.block + c) * d + ch;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < it.parts; i++) v += *reinterpret_cast<const f32x4*>(from + i * stride);
+    char* to = which ? p.dv + (int64_t)(it.k0 + c) * p.dv_row + kv_head * p.dv_head
+                     : p.dk + (int64_t)(it.k0 + c) * p.dk_row + kv_head * p.dk_head;
+    T::store4(to + ch * T::SIZE, v);
+}
+
+template <typename T, int DP>
+void run(const CrossArgs& a, hipStream_t s) {
+    const dim3 grid(xcd_grid((long)a.ks.n_items * a.kv_heads));
+    if (a.ks.block == 128) hipLaunchKernelGGL((cross_keys_kernel<T, DP, 2, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((cross_keys_kernel<T, DP, 2, 2>), grid, dim3(256), 0, s, a);
+}
+template <typename T>
+hipError_t run_all(const CrossArgs& a, hipStream_t s) {
+    if (a.ks.n_items == 0) return hipSuccess;
+    if (a.head_d <= 64) run<T, 64>(a, s);
+    else if (a.head_d <= 96) run<T, 96>(a, s);
+    else run<T, 128>(a, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.ks.n_joins == 0) return e;
+    const int pieces = 2 * a.ks.block * (a.head_d / 4);
+    hipLaunchKernelGGL((cross_keys_join_kernel<T>), dim3((unsigned)(a.ks.n_joins * a.kv_heads), (unsigned)((pieces + 255) / 256)),
+                       dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cross_grad_keys(int dtype, const CrossArgs& a, hipStream_t s) {
+    return dtype == AWA_F32 ? run_all<F32>(a, s) : run_all<Bf16>(a, s);
+}
+
+}  // namespace awa

@@ -1,0 +1,418 @@
+// dit_norm.hip — layer norm of rows and its gradient.
+//
+// Forward.  A row stays in registers: its sum gives a first mean, a second pass over the
+// registers the mean of what is left and the squares of it, so that neither a large common
+// value nor the first sum's rounding reaches the variance:
+//   d = x - m0,  r = sum d / K,  mean = m0 + r,  var = sum d^2 / K - r^2.
+// Backward.  With h = (x - mean) rstd and a = dy w a row needs sum a and sum a h, and every
+// column sum dy h and sum dy over the rows: lanes keep their columns' sums in registers over
+// all rows of their wave, waves add theirs in LDS in a fixed order, workgroups leave a row of
+// partial sums each, which a second kernel adds in their order.
+//
+// Both are bound by HBM: each value is read once and written once.
+#include <algorithm>
+
+#include "dit_train_internal.hpp"
+
+namespace awa {
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// rows are only known to be aligned to their elements
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+
+struct Fp8 {
+    uint8_t v;
+};
+
+// A lane's piece: four consecutive columns, 256 between the pieces of a lane.
+constexpr int V = 4, STEP = 64 * V;
+
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    f32x4 v;
+    __device__ void load(const float* p) { v = *reinterpret_cast<const f32x4_4*>(p); }
+    __device__ void load_some(const float* p, int n) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = i < n ? p[i] : 0.f;
+    }
+    __device__ float get(int i) const { return v[i]; }
+};
+template <> struct Raw<uint16_t> {
+    u32x2 v;
+    __device__ void load(const uint16_t* p) { v = *reinterpret_cast<const u32x2_2*>(p); }
+    __device__ void load_some(const uint16_t* p, int n) {
+        v = (u32x2){0, 0};
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    }
+    __device__ float get(int i) const { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
+};
+// columns past K are zeros in memory, up to whole blocks of 128
+template <> struct Raw<Fp8> {
+    uint32_t v;
+    __device__ void load(const Fp8* p) { v = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ void load_some(const Fp8* p, int) { load(p); }
+    __device__ float get(int i) const {
+        const f32x2 f = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false);
+        return f[i & 1];
+    }
+};
+
+template <typename T>
+__device__ inline void load_piece(Raw<T>& r, const T* row, int col, int K) {
+    if (col + V <= K) r.load(row + col);
+    else r.load_some(row + col, max(K - col, 0));
+}
+template <>
+__device__ inline void load_piece<Fp8>(Raw<Fp8>& r, const Fp8* row, int col, int K) {
+    if (col < K) r.load(row + col);
+    else r.v = 0;
+}
+
+__device__ inline void store_piece(float* p, const f32x4& v, int n) {
+    if (n >= V) {
+        __builtin_nontemporal_store(v, reinterpret_cast<f32x4_4*>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) p[i] = v[i];
+    }
+}
+__device__ inline void store_piece(uint16_t* p, const f32x4& v, int n) {
+    const u32x2 w = {bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3])};
+    if (n >= V) {
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x2_2*>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+}
+
+template <int CTRL>
+__device__ inline float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+// over the 64 lanes, the same bits in each
+__device__ inline float wave_sum(float v) {
+    v = dpp_add<0xB1>(v);   // lane ^ 1
+    v = dpp_add<0x4E>(v);   // lane ^ 2
+    v = dpp_add<0x141>(v);  // mirrored in 8: the other four
+    v = dpp_add<0x140>(v);  // mirrored in 16
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// two sums over the WPR waves of a row, in the waves' order; `at`: LDS that no other call of the row's
+// uses (a wave may run ahead by one call)
+template <int WPR>
+__device__ inline void row_sums(float& a, float& b, float2* at, int wave) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) at[wave] = make_float2(a, b);
+        __syncthreads();
+        a = 0.f;
+        b = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; i++) {
+            a += at[i].x;
+            b += at[i].y;
+        }
+    }
+}
+
+// R pieces a lane; WPR waves a row, 4 waves a workgroup.
+template <typename TX, typename TY, int R, int WPR>
+__global__ __launch_bounds__(256) void layer_norm_kernel(NormFwd a) {
+    constexpr int WAVES = 4, ROWS = WAVES / WPR;
+    __shared__ float2 part[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR;
+    if (row >= a.M) return;  // whole workgroups where waves share a row
+    const int col0 = (wave % WPR) * (R * STEP) + lane * V;
+    const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
+    Raw<TX> v[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) load_piece(v[i], x, col0 + i * STEP, a.K);
+    const float inv = 1.f / (float)a.K;
+    float s = 0.f, none = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; i++) s += (v[i].get(0) + v[i].get(1)) + (v[i].get(2) + v[i].get(3));
+    row_sums<WPR>(s, none, part[0], wave);
+    const float m0 = s * inv;
+    float sd = 0.f, ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float d = col0 + i * STEP + j < a.K ? v[i].get(j) - m0 : 0.f;
+            sd += d;
+            ss += d * d;
+        }
+    row_sums<WPR>(sd, ss, part[1], wave);
+    const float r = sd * inv, var = fmaxf(ss * inv - r * r, 0.f);
+    // fmaxf takes a NaN's other operand
+    const float rstd = 1.f / sqrtf((ss == ss ? var : ss) + a.eps);
+    if (a.stats && lane == 0 && wave % WPR == 0) a.stats[row] = make_float2(m0 + r, rstd);
+    TY* y = reinterpret_cast<TY*>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int col = col0 + i * STEP;
+        if (col >= a.K) continue;
+        f32x4 w = {1.f, 1.f, 1.f, 1.f}, b = {0.f, 0.f, 0.f, 0.f};
+        if (a.w) {
+            Raw<float> t;
+            load_piece(t, a.w, col, a.K);
+            w = t.v;
+        }
+        if (a.b) {
+            Raw<float> t;
+            load_piece(t, a.b, col, a.K);
+            b = t.v;
+        }
+        f32x4 o;
+#pragma unroll
+        for (int j = 0; j < V; j++) o[j] = ((v[i].get(j) - m0) - r) * rstd * w[j] + b[j];
+        store_piece(y + col, o, a.K - col);
+    }
+}
+
+// Rows in turn over the workgroups; eight waves a workgroup.  w stays in LDS: with x, dy and both
+// columns' sums in registers it would be the part that does not fit.
+template <typename TD, typename TX, int R, int WPR>
+__global__ __launch_bounds__(512) void layer_norm_grad_kernel(NormGrad a) {
+    constexpr int WAVES = 8, ROWS = WAVES / WPR, COLS = WPR * R * STEP;
+    constexpr int BUFS = ROWS > 1 ? ROWS / 2 : 1;  // half of the rows' sums of columns at a time
+    __shared__ float2 part[2][WAVES];
+    __shared__ __align__(16) float ws[COLS];
+    __shared__ __align__(16) float cols[ROWS > 1 ? BUFS * 2 * COLS : 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sub = wave / WPR, col0 = (wave % WPR) * (R * STEP) + lane * V;
+    const float inv = 1.f / (float)a.K;
+    for (int c = tid; c < COLS; c += 512) ws[c] = c >= a.K ? 0.f : a.w ? a.w[c] : 1.f;
+    __syncthreads();
+    f32x4 dw[R], db[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) dw[i] = db[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int turn = 0;
+    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.M; row0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = row0 + sub;
+        if (ROWS > 1 && row >= a.M) {
+            if constexpr (WPR > 1) {  // meets the barrier of the other rows' waves
+                float z0 = 0.f, z1 = 0.f;
+                row_sums<WPR>(z0, z1, part[turn & 1] + sub * WPR, wave % WPR);
+                turn++;
+            }
+            continue;
+        }
+        const TD* dy = reinterpret_cast<const TD*>(a.dy) + row * a.lddy;
+        const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
+        Raw<TD> d[R];
+        Raw<TX> v[R];
+        float sc[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            load_piece(d[i], dy, col0 + i * STEP, a.K);
+            load_piece(v[i], x, col0 + i * STEP, a.K);
+            sc[i] = 1.f;
+            if constexpr (sizeof(TX) == 1) {
+                const int block = (col0 + i * STEP) >> 7;
+                if (col0 + i * STEP < a.K) {
+                    const uint32_t b = a.xs[(block >> 2) * a.ld_xs + row] >> (8 * (block & 3)) & 0xff;
+                    sc[i] = __uint_as_float(b ? b << 23 : 0x400000u);  // 2^(b - 127)
+                }
+            }
+        }
+        const float2 st = a.stats[row];
+        auto hat = [&](int i, int j) __attribute__((always_inline)) {
+            return ((sizeof(TX) == 1 ? v[i].get(j) * sc[i] : v[i].get(j)) - st.x) * st.y;
+        };
+        float sa = 0.f, sah = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(ws + col0 + i * STEP);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float g = d[i].get(j), h = col0 + i * STEP + j < a.K ? hat(i, j) : 0.f;
+                const float aw = g * w[j];
+                dw[i][j] += g * h;
+                db[i][j] += g;
+                sa += aw;
+                sah += aw * h;
+            }
+        }
+        row_sums<WPR>(sa, sah, part[turn & 1] + sub * WPR, wave % WPR);
+        turn++;
+        if (a.dx) {
+            const float ma = sa * inv, mah = sah * inv;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int col = col0 + i * STEP;
+                if (col >= a.K) continue;
+                const f32x4 w = *reinterpret_cast<const f32x4*>(ws + col);
+                f32x4 o;
+#pragma unroll
+                for (int j = 0; j < V; j++) o[j] = st.y * (d[i].get(j) * w[j] - ma - hat(i, j) * mah);
+                if (a.dx_f32) store_piece(reinterpret_cast<float*>(a.dx) + row * a.lddx + col, o, a.K - col);
+                else store_piece(reinterpret_cast<uint16_t*>(a.dx) + row * a.lddx + col, o, a.K - col);
+            }
+        }
+    }
+    if (!a.part) return;
+    // the rows' column sums: the upper half's to the lower half, and again
+#pragma unroll
+    for (int n = ROWS; n > 1; n >>= 1) {
+        __syncthreads();
+        float* at = cols + (sub % (n / 2)) * (2 * COLS) + col0;
+        if (sub >= n / 2 && sub < n) {
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                *reinterpret_cast<f32x4*>(at + i * STEP) = dw[i];
+                *reinterpret_cast<f32x4*>(at + COLS + i * STEP) = db[i];
+            }
+        }
+        __syncthreads();
+        if (sub < n / 2) {
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                dw[i] += *reinterpret_cast<const f32x4*>(at + i * STEP);
+                db[i] += *reinterpret_cast<const f32x4*>(at + COLS + i * STEP);
+            }
+        }
+    }
+    if (sub) return;
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.K;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int col = col0 + i * STEP;
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (col + j < a.K) {
+                out[col + j] = dw[i][j];
+                out[a.K + col + j] = db[i][j];
+            }
+    }
+}
+
+// dw and db from the workgroups' partial sums: 64 of the 2 K columns a workgroup, its four waves
+// a quarter of the rows each.
+__global__ __launch_bounds__(256) void norm_params_kernel(const float* part, int groups, int K, float* dw, float* db) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (c < 2 * K) {
+        const int per = (groups + 3) / 4, end = min((wave + 1) * per, groups);
+#pragma unroll 8
+        for (int g = wave * per; g < end; g++) s += part[(int64_t)g * 2 * K + c];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= 2 * K) return;
+    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (c < K) {
+        if (dw) dw[c] = s;
+    } else if (db) {
+        db[c - K] = s;
+    }
+}
+
+__global__ __launch_bounds__(256) void norm_zero_kernel(int K, float* dw, float* db) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= K) return;
+    if (dw) dw[c] = 0.f;
+    if (db) db[c] = 0.f;
+}
+
+template <typename TX, typename TY, int R, int WPR>
+void fwd(const NormFwd& a, hipStream_t s) {
+    constexpr int rows = 4 / WPR;
+    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, R, WPR>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(256), 0, s, a);
+}
+template <typename TX, typename TY>
+void fwd_any(const NormFwd& a, hipStream_t s) {
+    const int n = (a.K + STEP - 1) / STEP;  // pieces of a row, by 64 lanes
+    if (n <= 2) fwd<TX, TY, 2, 1>(a, s);
+    else if (n <= 4) fwd<TX, TY, 4, 1>(a, s);
+    else if (n <= 6) fwd<TX, TY, 6, 1>(a, s);
+    else if (n <= 8) fwd<TX, TY, 8, 1>(a, s);
+    else if (n <= 10) fwd<TX, TY, 10, 1>(a, s);
+    else if (n <= 12) fwd<TX, TY, 12, 1>(a, s);
+    else if (n <= 16) fwd<TX, TY, 16, 1>(a, s);
+    else if (n <= 32) fwd<TX, TY, 8, 4>(a, s);
+    else fwd<TX, TY, 16, 4>(a, s);
+}
+
+template <typename TD, typename TX, int R, int WPR>
+void grad(const NormGrad& a, hipStream_t s) {
+    hipLaunchKernelGGL((layer_norm_grad_kernel<TD, TX, R, WPR>), dim3((unsigned)a.groups), dim3(512), 0, s, a);
+}
+template <typename TD, typename TX>
+void grad_any(const NormGrad& a, hipStream_t s) {
+    const int n = (a.K + STEP - 1) / STEP;
+    if (n <= 2) grad<TD, TX, 2, 1>(a, s);
+    else if (n <= 4) grad<TD, TX, 4, 1>(a, s);
+    else if (n <= 6) grad<TD, TX, 3, 2>(a, s);
+    else if (n <= 8) grad<TD, TX, 4, 2>(a, s);
+    else if (n <= 10) grad<TD, TX, 5, 2>(a, s);
+    else if (n <= 12) grad<TD, TX, 6, 2>(a, s);
+    else if (n <= 16) grad<TD, TX, 4, 4>(a, s);
+    else if (n <= 24) grad<TD, TX, 6, 4>(a, s);
+    else if (n <= 32) grad<TD, TX, 8, 4>(a, s);
+    else if (n <= 48) grad<TD, TX, 6, 8>(a, s);
+    else grad<TD, TX, 8, 8>(a, s);
+}
+template <typename TD>
+void grad_in(int dtype_x, const NormGrad& a, hipStream_t s) {
+    if (dtype_x == AWA_F32) grad_any<TD, float>(a, s);
+    else if (dtype_x == AWA_BF16) grad_any<TD, uint16_t>(a, s);
+    else grad_any<TD, Fp8>(a, s);
+}
+
+// rows that a workgroup of the gradient takes at once
+int rows_at_once(int K) {
+    const int n = (K + STEP - 1) / STEP;
+    return n <= 4 ? 8 : n <= 12 ? 4 : n <= 32 ? 2 : 1;
+}
+
+}  // namespace
+
+int norm_grad_groups(int M, int K) {
+    const int rows = rows_at_once(K);
+    return std::min((M + rows - 1) / rows, 256);
+}
+
+hipError_t launch_layer_norm(int dtype_x, int dtype_y, const NormFwd& a, hipStream_t s) {
+    if (dtype_x == AWA_F32) {
+        if (dtype_y == AWA_F32) fwd_any<float, float>(a, s);
+        else fwd_any<float, uint16_t>(a, s);
+    } else {
+        if (dtype_y == AWA_F32) fwd_any<uint16_t, float>(a, s);
+        else fwd_any<uint16_t, uint16_t>(a, s);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_layer_norm_grad(int dtype_dy, int dtype_x, const NormGrad& a, hipStream_t s) {
+    if (a.M == 0) {
+        hipLaunchKernelGGL(norm_zero_kernel, dim3((unsigned)((a.K + 255) / 256)), dim3(256), 0, s, a.K, a.dw, a.db);
+        return hipGetLastError();
+    }
+    if (dtype_dy == AWA_F32) grad_in<float>(dtype_x, a, s);
+    else grad_in<uint16_t>(dtype_x, a, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.part) return e;
+    hipLaunchKernelGGL(norm_params_kernel, dim3((unsigned)((2 * a.K + 63) / 64)), dim3(256), 0, s, a.part, a.groups, a.K, a.dw, a.db);
+    return hipGetLastError();
+}
+
+}  // namespace awa

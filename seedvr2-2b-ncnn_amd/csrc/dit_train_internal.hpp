@@ -1,0 +1,132 @@
+// dit_train_internal.hpp — shared definitions of the operators of dit_train.h.
+#pragma once
+
+#include "dit_internal.hpp"
+#include "dit_train.h"
+
+namespace awa {
+
+struct NormFwd {
+    const void* x;
+    int64_t ldx;
+    const float *w, *b;  // [K] or null
+    float eps;
+    void* y;
+    int64_t ldy;
+    float2* stats;  // [M] or null
+    int M, K;
+};
+hipError_t launch_layer_norm(int dtype_x, int dtype_y, const NormFwd& a, hipStream_t s);
+
+struct NormGrad {
+    const void* dy;
+    int64_t lddy;
+    const void* x;
+    int64_t ldx;
+    const uint32_t* xs;  // scale words of 8-bit rows
+    int64_t ld_xs;
+    const float2* stats;
+    const float* w;  // [K] or null
+    void* dx;        // or null
+    int64_t lddx;
+    int dx_f32;      // dx fp32, else bf16
+    float *dw, *db;  // [K] or null
+    float* part;     // [groups][2][K], or null where neither is wanted
+    int groups;      // workgroups
+    int M, K;
+};
+// workgroups of the gradient's kernel, each of which leaves a row of partial sums
+int norm_grad_groups(int M, int K);
+hipError_t launch_layer_norm_grad(int dtype_dy, int dtype_x, const NormGrad& a, hipStream_t s);
+
+struct GradWeight {
+    const void* dy;  // [M][N]
+    int64_t lddy;
+    const uint8_t* q;  // [M][kp] e4m3
+    const uint32_t* s;
+    int64_t ld_s;
+    void* dw;  // [N][K]
+    int64_t ldw;
+    float* db;  // [N] or null
+    int add, w_f32;
+    float* part;  // [splits][N][K] and [splits][N] where splits > 1
+    int splits, rows_per;  // rows of a split, a multiple of the kernel's stage
+    int M, N, K, kp;
+    int n_tiles, k_tiles;
+};
+// splits of the rows, for the workspace and the launch alike
+int grad_weight_splits(int dtype_dy, int dtype_w, int M, int N, int K);
+hipError_t launch_grad_weight(int dtype_dy, GradWeight& a, hipStream_t s);
+
+// ---- attention to states of another length
+
+// A block of queries and the keys that a workgroup takes it over: columns c = 0 .. of a block are
+// query rows q0 + c / pack of the heads head0 + c % pack (head0 the work item's; pack 1: a head's rows).
+struct CrossItem {
+    int q0, cols;  // first query row, columns
+    int k0, kn;    // first key row, keys
+    int part;      // slot of the partial results, -1: the only part, written in place
+    int first;     // 1: the block's first run of keys
+};
+// A block whose keys are split: its parts are slots part0 .. part0 + parts - 1.
+struct CrossJoin {
+    int q0, cols, part0, parts;
+};
+// Queries of the gradient of keys: up to CROSS_QT rows of a sequence.
+constexpr int CROSS_QT = 64;
+struct CrossUnit {
+    int q0, rows;
+};
+// A block of keys and the run of its units (of every head that shares the key head: units ahead of
+// heads) that a workgroup takes.
+struct CrossKeys {
+    int k0, kn;              // first key row, keys
+    int unit0, units;        // of its sequences, in the units' table
+    int first, count;        // the run, among units x shared heads
+    int part;                // slot of partial sums, -1: the only one
+    int pad;
+};
+struct CrossKeyJoin {
+    int k0, kn, part0, parts;
+};
+
+// One of the two forms of a plan's query side.
+struct CrossQueries {
+    int pack = 1, block = 0;  // heads in a block, columns of a block
+    int n_items = 0, n_joins = 0, n_parts = 0;
+    const CrossItem* items = nullptr;
+    const CrossJoin* joins = nullptr;
+};
+struct CrossKeySide {
+    int block = 0;
+    int n_items = 0, n_joins = 0, n_parts = 0;
+    const CrossKeys* items = nullptr;
+    const CrossKeyJoin* joins = nullptr;
+    const CrossUnit* units = nullptr;
+};
+
+struct CrossArgs {
+    const char *q, *k, *v, *out, *dout;
+    char *o, *dq, *dk, *dv;
+    // strides in bytes
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, dout_row, dout_head;
+    int64_t o_row, o_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+    const uint8_t* mask;
+    float scale, c;  // c = scale log2(e)
+    float* lse;
+    int64_t ld_lse;
+    int heads, kv_heads, head_d;
+    CrossQueries qs;
+    CrossKeySide ks;
+    float *qpart, *kpart;  // partial results
+    float* dsum;           // rowsum(dout out), [heads][ld_dsum]
+    int64_t ld_dsum;
+};
+hipError_t launch_cross_forward(int dtype, const CrossArgs& a, hipStream_t s);
+hipError_t launch_cross_grad_queries(int dtype, const CrossArgs& a, hipStream_t s);  // first: it leaves dsum
+hipError_t launch_cross_grad_keys(int dtype, const CrossArgs& a, hipStream_t s);
+// floats of a partial block of queries (of a head group) and of keys (of a key head)
+__host__ __device__ inline int64_t cross_query_part(int block, int head_d) { return (int64_t)block * (head_d + 2); }
+__host__ __device__ inline int64_t cross_key_part(int block, int head_d) { return (int64_t)block * 2 * head_d; }
+
+}  // namespace awa
