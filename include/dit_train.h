@@ -77,7 +77,7 @@ int dit_layer_norm_grad(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
  *   dW[n][k] = sum over m of dy[m][n] x[m][k]   (+ dW[n][k] before, with add)
  *   db[n]    = sum over m of dy[m][n]           (+ db[n] before, with add)
  *
- * dy [M][N] of type dtype_dy (AWA_F32 or AWA_BF16), rows lddy apart; x [M][K] in 8-bit
+ * dy [M][N] of type dtype_dy (AWA_F32 or AWA_BF16), rows lddy (at most DIT_OPS_COLS_MAX) apart; x [M][K] in 8-bit
  * rows (d_q [M][K padded to 128], 16-byte aligned, d_s words, ld_s from group to group).
  * dW [N][K] of type dtype_w, rows ldw apart; db fp32 [N], may be NULL.  add needs fp32 dW.
  * Every product enters the sums whole, for fp32 dy too (as three bf16 parts: values of x

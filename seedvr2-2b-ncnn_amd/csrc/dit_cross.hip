@@ -20,7 +20,7 @@ using namespace cross;
 namespace {
 
 template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD>
-__global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p) {
+__global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) void cross_queries_kernel(CrossArgs p) {
     using Frag = typename T::Frag;
     using L = Tile<T, DP>;
     constexpr int KS = DP / 32, DB = DP / 16, KB = KT / 16, WAVES = WQ * WK;
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p
     const int wg = xcd_remap(total);
     if (wg >= total) return;
     const int hb = wg / p.qs.n_items;
-    const CrossItem it = p.qs.items[wg - hb * p.qs.n_items];
+    const CrossItem it = table_entry(p.qs.items, wg - hb * p.qs.n_items);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wq = wave % WQ, wk = wave / WQ, g = lane >> 4;
     const int head0 = hb * p.qs.pack, kv_head = head0 / (p.heads / p.kv_heads);
@@ -72,8 +72,17 @@ __global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p
             dsum[j] = sum4(dsum[j]);
             if (there[j]) {
                 const float l = p.lse[head[j] * p.ld_lse + row[j]];
-                lse2[j] = l == -INFINITY ? INFINITY : l * LOG2E;  // a row without keys: P = 0
-                if (it.first && wk == 0 && g == 0) p.dsum[head[j] * p.ld_dsum + row[j]] = dsum[j];
+                lse2[j] = l * LOG2E;
+                if (l == -INFINITY) {  // a row without keys: P = 0, and nothing that comes back counts
+                    lse2[j] = INFINITY;
+                    dsum[j] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) dout[j][ks] = T::zero();
+                }
+                if (it.first && wk == 0 && g == 0) {
+                    p.dsum[head[j] * p.ld_dsum + row[j]] = dsum[j];
+                    p.lse2[head[j] * p.ld_dsum + row[j]] = lse2[j];
+                }
             }
         }
     }
@@ -163,24 +172,24 @@ __global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p
                         const float e = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -lse2[j]));
                         s[b][j][r] = e * (dp[b][j][r] - dsum[j]);
                     }
-                if (valid != ALL) {  // what a masked key's products hold is no number to multiply by zero
-                    const uint64_t mine = valid >> (4 * g);
-#pragma unroll
-                    for (int b = 0; b < KB; b++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            if (!((mine >> (16 * b + r)) & 1)) s[b][j][r] = 0.f;
-                }
             } else {
                 float m = s[0][j][0];
 #pragma unroll
                 for (int b = 0; b < KB; b++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) m = fmaxf(m, s[b][j][r]);
-                m = fmaxf(max4(m), top[j]);
-                const float ref = m == -INFINITY ? 0.f : m * p.c;
-                const float fade = exp2_of(top[j] * p.c - ref);
-                top[j] = m;
+                m = max4(m);
+                // the maximum that exponents refer to stays until one exceeds it 2^8 times: sums and results
+                // are as exact for it, and are scaled anew in few tiles
+                if (__builtin_amdgcn_ballot_w64((m - top[j]) * p.c > 8.f)) {
+                    m = fmaxf(m, top[j]);
+                    const float fade = exp2_of(top[j] * p.c - (m == -INFINITY ? 0.f : m * p.c));
+                    top[j] = m;
+                    sum[j] *= fade;
+#pragma unroll
+                    for (int db = 0; db < DB; db++) acc[db][j] *= fade;
+                }
+                const float ref = top[j] == -INFINITY ? 0.f : top[j] * p.c;
                 float add = 0.f;
 #pragma unroll
                 for (int b = 0; b < KB; b++)
@@ -189,9 +198,7 @@ __global__ __launch_bounds__(64 * WQ * WK) void cross_queries_kernel(CrossArgs p
                         s[b][j][r] = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -ref));
                         add += s[b][j][r];
                     }
-                sum[j] = sum[j] * fade + add;
-#pragma unroll
-                for (int db = 0; db < DB; db++) acc[db][j] *= fade;
+                sum[j] += add;
             }
         }
 #pragma unroll
@@ -315,7 +322,7 @@ void run(const CrossArgs& a, hipStream_t s) {
 template <typename T, int DP, bool GRAD>
 void run_block(const CrossArgs& a, hipStream_t s) {
     constexpr int WK = T::SIZE == 2 ? 4 : 2;
-    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 ? 64 : 32, GRAD>(a, s);
+    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 && !GRAD ? 64 : 32, GRAD>(a, s);
     else if (a.qs.block == 32) run<T, DP, 2, 1, WK, 32, GRAD>(a, s);
     else run<T, DP, 1, 1, WK, 32, GRAD>(a, s);
 }

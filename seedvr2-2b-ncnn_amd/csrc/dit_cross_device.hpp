@@ -21,7 +21,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) bf16x4 lbf16x4_t;
-typedef __attribute__((address_space(3))) void* lptr_t;
 
 struct Bf16 {
     static constexpr int SIZE = 2;
@@ -73,13 +72,40 @@ struct F32 {
     static __device__ inline void store4(char* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
 };
 
+// One LDS DMA instruction, 16 (4) bytes a lane to LDS at `to` + 16 (4) x lane from byte offset `at` of the resource.  From
+// asm, because the compiler lets every transposed read wait for all DMA that it knows of; the kernels wait by themselves
+// (wait_vmem_lds and a barrier) before anything reads the tile.  M0, the LDS address, is not used otherwise here.
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(size_t)(const __attribute__((address_space(3))) char*)p);
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ inline void dma16(const void* to, __amdgpu_buffer_rsrc_t from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tbuffer_load_dwordx4 %[v], %[r], 0 offen lds"
+                 :
+                 : [v] "v"(at), [r] "s"(from), [m] "s"(lds_address(to))
+                 : "memory", "m0");
+}
+__device__ inline void dma4(const void* to, __amdgpu_buffer_rsrc_t from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tbuffer_load_dword %[v], %[r], 0 offen lds"
+                 :
+                 : [v] "v"(at), [r] "s"(from), [m] "s"(lds_address(to))
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // An LDS tile: rows of 64 or 128 channels (DP = 96 has rows of 128, whose last channels nothing reads), 16-byte
-// chunk c of row r at chunk c ^ swizzle(r): eight neighbouring rows, and the four rows of a transposed read's 16
-// lanes, begin at different banks.
-__device__ inline int swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// chunk c of row r at chunk c ^ swizzle(r).  LDS answers 256 bytes a cycle from 64 banks, so the 16 rows that read one
+// chunk together, and the eight rows that 32 lanes of a transposed read (four rows that 64 lanes of fp32 columns) take two
+// (four) neighbouring chunks of, have to begin at different ones.
 template <typename T, int DP>
 struct Tile {
     static constexpr int ROW = (DP == 64 ? 64 : 128) * T::SIZE, CHUNKS = ROW / 16, PER = 1024 / ROW;  // PER: rows of an instruction
+    static __device__ inline int swizzle(int r) {
+        if constexpr (T::SIZE == 4) return r & 15;
+        if constexpr (DP == 64) r >>= 1;  // rows of half the banks
+        return DP == 64 ? ((r & 3) << 1) | ((r >> 2) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+    }
     // eight channels 32 ks + 8 g .. of row `row`
     static __device__ inline typename T::Frag row_frag(const char* t, int row, int ks, int g) {
         const char* at = t + row * ROW;
@@ -123,9 +149,24 @@ struct Tile {
         const int row = i * PER + lane / CHUNKS, c = ((lane % CHUNKS) ^ swizzle(row)) << 4;
         const bool in = ((valid >> row) & 1) && c < width;
         const uint32_t at = in ? (uint32_t)(row * (uint32_t)row_bytes + c) : 0x80000000u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(t + i * 1024), 16, at, 0, 0, 0);
+        dma16(t + i * 1024, from, at);
     }
 };
+
+// An entry of a plan's table by the scalar cache (read-only memory at a wave-uniform index: as a vector load it would be
+// waited for together with the tiles on their way)
+template <typename S>
+__device__ inline S table_entry(const S* table, int i) {
+    constexpr int N = sizeof(S) / 4;
+    typedef const __attribute__((address_space(4))) uint32_t* constant_t;
+    const constant_t from = (constant_t)table + (size_t)__builtin_amdgcn_readfirstlane(i) * N;
+    uint32_t w[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) w[k] = from[k];
+    S s;
+    __builtin_memcpy(&s, w, sizeof(S));
+    return s;
+}
 
 // Over the four lanes l % 16 + 16 i
 __device__ inline float sum4(float v) {

@@ -16,13 +16,13 @@ using namespace cross;
 
 namespace {
 
-// NK blocks of 16 keys a wave, WKEY waves over the keys; where WKEY is 2 the other two take the second 32 rows of a
+// NK blocks of 16 keys a wave, WKEY waves over the keys; where SUBS is 2 as many more take the second 32 rows of a
 // unit, and the two halves' sums meet in LDS at the end.
-template <typename T, int DP, int NK, int WKEY>
-__global__ __launch_bounds__(256) void cross_keys_kernel(CrossArgs p) {
+template <typename T, int DP, int NK, int WKEY, int SUBS>
+__global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs p) {
     using Frag = typename T::Frag;
     using L = Tile<T, DP>;
-    constexpr int KS = DP / 32, DB = DP / 16, QT = CROSS_QT, SUBS = 4 / WKEY;
+    constexpr int KS = DP / 32, DB = DP / 16, QT = CROSS_QT, WAVES = WKEY * SUBS;
     constexpr int TILE_B = QT * L::ROW, STAGE = 2 * TILE_B + 2 * QT * 4;  // Q, dO, lse, dsum
     constexpr int JOIN = SUBS > 1 ? 2 * 64 * WKEY * NK * DB * 16 : 0;
     constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void cross_keys_kernel(CrossArgs p) {
     const int wg = xcd_remap(total);
     if (wg >= total) return;
     const int kv_head = wg / p.ks.n_items;
-    const CrossKeys it = p.ks.items[wg - kv_head * p.ks.n_items];
+    const CrossKeys it = table_entry(p.ks.items, wg - kv_head * p.ks.n_items);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = wave % WKEY, sub0 = wave / WKEY, g = lane >> 4;
     const int width = p.head_d * T::SIZE;
@@ -62,36 +62,40 @@ __global__ __launch_bounds__(256) void cross_keys_kernel(CrossArgs p) {
 #pragma unroll
         for (int j = 0; j < NK; j++) dk[db][j] = dv[db][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    const int heads_per = p.heads / p.kv_heads;
-    auto fetch = [&](int u, int slot) __attribute__((always_inline)) {
-        const int head = kv_head * heads_per + u / it.units;
-        const CrossUnit un = p.ks.units[it.unit0 + u % it.units];
-        const uint64_t valid = un.rows == 64 ? ~(uint64_t)0 : ((uint64_t)1 << un.rows) - 1;
-        const __amdgpu_buffer_rsrc_t qr = uniform_rsrc(p.q + un.q0 * p.q_row + head * p.q_head, 0x7fffffffu);
-        const __amdgpu_buffer_rsrc_t dr = uniform_rsrc(p.dout + un.q0 * p.dout_row + head * p.dout_head, 0x7fffffffu);
+    // the run's units, one ahead of the tiles that are fetched
+    int at = it.first % it.units, head = kv_head * (p.heads / p.kv_heads) + it.first / it.units;
+    CrossUnit next = table_entry(p.ks.units, it.unit0 + at);
+    auto fetch = [&](int slot) __attribute__((always_inline)) {
+        const uint64_t valid = next.rows == 64 ? ~(uint64_t)0 : ((uint64_t)1 << next.rows) - 1;
+        const __amdgpu_buffer_rsrc_t qr = uniform_rsrc(p.q + next.q0 * p.q_row + head * p.q_head, 0x7fffffffu);
+        const __amdgpu_buffer_rsrc_t dr = uniform_rsrc(p.dout + next.q0 * p.dout_row + head * p.dout_head, 0x7fffffffu);
         char* st = lds + slot * STAGE;
-        constexpr int N = TILE_B / 1024 / 4;
+        constexpr int N = TILE_B / 1024 / WAVES;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             L::dma(st, wave * N + i, qr, p.q_row, valid, width, lane);
             L::dma(st + TILE_B, wave * N + i, dr, p.dout_row, valid, width, lane);
         }
         if (wave < 2) {
-            const float* from = wave ? p.dsum + head * p.ld_dsum : p.lse + head * p.ld_lse;
-            const __amdgpu_buffer_rsrc_t r = uniform_rsrc(from + un.q0, (uint32_t)un.rows * 4);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)(st + 2 * TILE_B + wave * QT * 4), 4, 4 * lane, 0, 0, 0);
+            const float* from = (wave ? p.dsum : p.lse2) + head * p.ld_dsum + next.q0;
+            const __amdgpu_buffer_rsrc_t r = uniform_rsrc(from, (uint32_t)next.rows * 4);
+            dma4(st + 2 * TILE_B + wave * QT * 4, r, 4 * lane);
+        }
+        if (++at == it.units) {
+            at = 0;
+            head++;
         }
     };
-    if (it.count > 0) fetch(it.first, 0);
+    if (it.count > 0) fetch(0);
     for (int n = 0; n < it.count; n++) {
+        const int rows = next.rows;
+        if (n + 1 < it.count) next = table_entry(p.ks.units, it.unit0 + at);
         wait_vmem_lds<0>();
         __syncthreads();
-        const int u = it.first + n;
-        if (n + 1 < it.count) fetch(u + 1, (n + 1) & 1);
+        if (n + 1 < it.count) fetch((n + 1) & 1);
         const char* qt = lds + (n & 1) * STAGE;
         const char* dt = qt + TILE_B;
         const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE_B);
-        const int rows = p.ks.units[it.unit0 + u % it.units].rows;
 #pragma unroll
         for (int s0 = 0; s0 < QT / 32; s0 += SUBS) {
             const int sub = s0 + (SUBS > 1 ? sub0 : 0), base = 32 * sub;
@@ -115,17 +119,22 @@ __global__ __launch_bounds__(256) void cross_keys_kernel(CrossArgs p) {
                 const int r0 = base + 16 * b + 4 * g;
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + r0), d4 = *reinterpret_cast<const f32x4*>(lse + QT + r0);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float l2 = l4[r] == -INFINITY ? INFINITY : l4[r] * LOG2E;  // a row without keys: P = 0
+                for (int r = 0; r < 4; r++)
 #pragma unroll
                     for (int j = 0; j < NK; j++) {
-                        float e = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -l2));
-                        float ds = e * (dp[b][j][r] - d4[r]);
-                        if (r0 + r >= rows) e = ds = 0.f;  // rows past the end are zeros, but infinite keys times zero are not
+                        const float e = exp2_of(__builtin_fmaf(s[b][j][r], p.c, -l4[r]));
+                        dp[b][j][r] = e * (dp[b][j][r] - d4[r]);
                         s[b][j][r] = e;
-                        dp[b][j][r] = ds;
                     }
-                }
+            }
+            if (rows < base + 32) {  // rows past the end hold zeros, but infinite keys times zero are not
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (base + 16 * b + 4 * g + r >= rows)
+#pragma unroll
+                            for (int j = 0; j < NK; j++) s[b][j][r] = dp[b][j][r] = 0.f;
             }
             Frag pf[NK], sf[NK];
 #pragma unroll
@@ -214,8 +223,8 @@ __global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
 template <typename T, int DP>
 void run(const CrossArgs& a, hipStream_t s) {
     const dim3 grid(xcd_grid((long)a.ks.n_items * a.kv_heads));
-    if (a.ks.block == 128) hipLaunchKernelGGL((cross_keys_kernel<T, DP, 2, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((cross_keys_kernel<T, DP, 2, 2>), grid, dim3(256), 0, s, a);
+    if (a.ks.block == 128) hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, 8, 1>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, 4, 2>), grid, dim3(512), 0, s, a);
 }
 template <typename T>
 hipError_t run_all(const CrossArgs& a, hipStream_t s) {

@@ -32,10 +32,12 @@ constexpr int MS = 32;  // rows of a stage: one instruction's
 __device__ inline float scale_of(uint32_t b) { return __uint_as_float(b ? b << 23 : 0x400000u); }  // 2^(b - 127)
 __device__ inline uint32_t pk(bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
 // upper halves of a and b as one word
-__device__ inline uint32_t upper(float a, float b) { return (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u); }
+__device__ inline uint32_t upper(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
 __device__ inline float truncated(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 
-// Eight columns of a row of dy as PARTS words of bf16 pairs
+// Eight columns of a row of dy, and the bf16 parts that they are the sum of
 template <int PARTS> struct DyPiece;
 template <> struct DyPiece<1> {
     using T = uint16_t;
@@ -48,7 +50,7 @@ template <> struct DyPiece<1> {
             if (i < n) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
     }
     __device__ void zero() { v = (u32x4){0, 0, 0, 0}; }
-    __device__ u32x4 part(int) const { return v; }
+    __device__ void parts(u32x4 (&out)[1]) const { out[0] = v; }
 };
 template <> struct DyPiece<3> {
     using T = float;
@@ -62,101 +64,177 @@ template <> struct DyPiece<3> {
         for (int i = 0; i < 8; i++) v[i >> 2][i & 3] = i < n ? p[i] : 0.f;
     }
     __device__ void zero() { v[0] = v[1] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
-    // part x: the bits that the parts before it leave; an infinity is all in the first
-    __device__ u32x4 part(int x) const {
-        float r[8];
+    // each part the upper 16 bits of what the parts before it leave: 8 + 8 + 8 bits
+    __device__ void parts(u32x4 (&out)[3]) const {
+        float r[8], top = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             r[i] = v[i >> 2][i & 3];
-            for (int k = 0; k < x; k++) {
-                const float h = truncated(r[i]);
-                r[i] = h == r[i] ? 0.f : r[i] - h;
+            top = fmaxf(top, fabsf(r[i]));
+        }
+        const bool infinite = __builtin_amdgcn_ballot_w64(top == INFINITY) != 0;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            out[k] = (u32x4){upper(r[0], r[1]), upper(r[2], r[3]), upper(r[4], r[5]), upper(r[6], r[7])};
+#pragma unroll
+            for (int i = 0; i < 8 && k < 2; i++) r[i] -= truncated(r[i]);
+            if (k == 0 && infinite) {  // an infinity is all in the first part
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (fabsf(v[i >> 2][i & 3]) == INFINITY) r[i] = 0.f;
             }
         }
-        return (u32x4){upper(r[0], r[1]), upper(r[2], r[3]), upper(r[4], r[5]), upper(r[6], r[7])};
     }
 };
 
-// Chunk c (16 bytes) of row m lies at chunk c ^ sw(m): the four rows that 16 lanes of a transposed read
-// touch begin at different banks.
-__device__ inline int sw(int m) { return (m & 3) << 1; }
+// Chunk c (16 bytes) of row m lies at chunk c ^ sw(m): the eight rows of which 32 lanes of a transposed read
+// take two neighbouring chunks, and the every other chunk of two rows that 16 lanes write, are in different banks.
+__device__ inline int sw(int m) { return ((m & 7) << 1) | (m & 1); }
 
-// TN x TK accumulators of 16 x 16 a wave, WN x WK waves.
-template <int PARTS, int TN, int TK, int WN, int WK>
-__global__ __launch_bounds__(64 * WN * WK) void grad_weight_kernel(GradWeight p) {
+// Four columns of a row of dW, of which `left` are there
+__device__ inline void put(const GradWeight& p, int row, int col, int left, f32x4 v) {
+    if (p.w_f32) {
+        float* to = reinterpret_cast<float*>(p.dw) + row * p.ldw + col;
+        if (left >= 4) {
+            if (p.add) v += *reinterpret_cast<const f32x4_4*>(to);
+            *reinterpret_cast<f32x4_4*>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < left) to[e] = p.add ? to[e] + v[e] : v[e];
+        }
+    } else {
+        typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+        uint16_t* to = reinterpret_cast<uint16_t*>(p.dw) + row * p.ldw + col;
+        const u32x2_2 w = {bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3])};
+        if (left >= 4) {
+            *reinterpret_cast<u32x2_2*>(to) = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < left) to[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+}
+
+// Tile t: four n tiles side by side, k advancing
+template <int BN, int BK>
+__device__ inline void place(const GradWeight& p, int t, int& n0, int& k0) {
+    constexpr int GN = 4;
+    const int group = t / (GN * p.k_tiles), first = group * GN, gn = min(p.n_tiles - first, GN);
+    const int in = t - group * (GN * p.k_tiles);
+    n0 = (first + in % gn) * BN;
+    k0 = in / gn * BK;
+}
+
+// TN x TK accumulators of 16 x 16 a wave, WN x WK waves; at least two waves a SIMD.
+template <int PARTS, int TN, int TK, int WN, int WK, int DEPTH>
+__global__ __launch_bounds__(64 * WN * WK, 2) void grad_weight_kernel(GradWeight p) {
     constexpr int BN = 16 * TN * WN, BK = 16 * TK * WK, THREADS = 64 * WN * WK;
     constexpr int CN = BN / 8, CK = BK / 8;  // chunks of a row
-    constexpr int NR = MS * CN / THREADS, KR = MS * CK / 2 / THREADS;  // a thread's pieces: 8 columns of dy, 16 of x
-    static_assert(NR >= 1 && KR >= 1 && MS * CN % THREADS == 0 && MS * CK / 2 % THREADS == 0, "pieces");
+    // a thread's pieces: 8 columns of dy, 16 of x (8 where there are more threads)
+    constexpr int XC = MS * CK / 2 >= THREADS ? 2 : 1, XR = CK / XC;
+    constexpr int NR = MS * CN / THREADS, KR = MS * XR / THREADS;
+    static_assert(NR >= 1 && KR >= 1 && MS * CN % THREADS == 0 && MS * XR % THREADS == 0, "pieces");
+    typedef uint32_t xpiece __attribute__((ext_vector_type(2 * XC)));
     constexpr int PART = MS * BN * 2, STAGE = PARTS * PART + MS * BK * 2;
     __shared__ __align__(16) uint8_t lds[2 * STAGE];
-    const int total = p.n_tiles * p.k_tiles * p.splits;
-    const int wg = xcd_remap(total);
-    if (wg >= total) return;
-    const int per_split = p.n_tiles * p.k_tiles, split = wg / per_split;
-    int n0, k0;
-    {  // four n tiles side by side, k advancing
-        constexpr int GN = 4;
-        const int t = wg - split * per_split, group = t / (GN * p.k_tiles), first = group * GN, gn = min(p.n_tiles - first, GN);
-        const int in = t - group * (GN * p.k_tiles);
-        n0 = (first + in % gn) * BN;
-        k0 = in / gn * BK;
+    // whole tiles, then those whose rows are divided
+    int tile, split = -1;
+    if ((int)blockIdx.x < p.whole) {
+        // the XCD's contiguous range; the few past a multiple of 8 are the last ones
+        const int per = p.whole >> 3, b = (int)blockIdx.x;
+        tile = b < 8 * per ? (b & 7) * per + (b >> 3) : b;
+    } else {
+        const int b = (int)blockIdx.x - p.whole, rest = p.n_tiles * p.k_tiles - p.whole, per = (rest * p.splits + 7) >> 3;
+        const int i = (b & 7) * per + (b >> 3);
+        if (i >= rest * p.splits) return;
+        split = i / rest;
+        tile = p.whole + i - split * rest;
     }
-    const int m_first = split * p.rows_per, m_end = min(m_first + p.rows_per, p.M);
+    int n0, k0;
+    place<BN, BK>(p, tile, n0, k0);
+    const int m_first = max(split, 0) * p.rows_per, m_end = split < 0 ? p.M : min(m_first + p.rows_per, p.M);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave / WK, wk = wave % WK;
 
     // pieces: the same columns in every stage
-    const int nc = tid % CN, nr = tid / CN, kc = tid % (CK / 2), kr = tid / (CK / 2);
+    const int nc = tid % CN, nr = tid / CN, kc = tid % XR, kr = tid / XR;
     using TD = typename DyPiece<PARTS>::T;
-    const int n = n0 + 8 * nc, k = k0 + 16 * kc, block = k >> 7;
-    const TD* dy = reinterpret_cast<const TD*>(p.dy) + n;
-    const uint8_t* q = p.q + k;
-    const uint32_t* words = p.s + (int64_t)(block >> 2) * p.ld_s;
-    DyPiece<PARTS> d[NR];
-    u32x4 x[KR];
-    uint32_t xs[KR];
-    auto load = [&](int m0) __attribute__((always_inline)) {
+    const int n = n0 + 8 * nc, k = k0 + 8 * XC * kc, block = k >> 7;
+    struct Pieces {
+        DyPiece<PARTS> d[NR];
+        xpiece x[KR];
+        uint32_t xs[KR];
+    };
+    // A lane's offsets inside a stage are the same for all (32 bits: rows are at most 2^20 elements), its rows' address is
+    // the wave's.  Columns past N or K only reach results past them, so only rows past the end have to be zeros: pieces past
+    // the last column are read from the tile's first, and one across it goes on into the next row, where there is one.
+    // Stages for which that holds are loaded without a branch, so that the loads of several are on their way at once.
+    const uint32_t dy_of = (uint32_t)nr * (uint32_t)p.lddy + (n < p.N ? 8 * nc : 0);
+    const uint32_t q_of = (uint32_t)kr * (uint32_t)p.kp + (k < p.kp ? 8 * XC * kc : 0);
+    const TD* const dy0 = reinterpret_cast<const TD*>(p.dy) + n0;
+    const uint8_t* const q0 = p.q + k0;
+    const uint32_t* const s0 = p.s + (int64_t)(k0 >> 9) * p.ld_s;  // a tile's columns have one word a row
+    const int plain = p.N < 8 ? 0 : (n0 + BN <= p.N || m_end < p.M ? m_end - m_first : m_end - m_first - 1) / MS;
+    auto load = [&](Pieces& r, int st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NR; j++) r.d[j].load(dy0 + (m_first + st * MS + j * (THREADS / CN)) * p.lddy + dy_of);
+#pragma unroll
+        for (int j = 0; j < KR; j++) {
+            const int m = m_first + st * MS + j * (THREADS / XR);
+            r.x[j] = *reinterpret_cast<const xpiece*>(q0 + (int64_t)m * p.kp + q_of);
+            r.xs[j] = (s0 + m)[kr];
+        }
+    };
+    // any stage
+    auto load_any = [&](Pieces& r, int st) __attribute__((always_inline)) {
+        if (st < plain) {
+            load(r, st);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < NR; j++) {
-            const int m = m0 + nr + j * (THREADS / CN);
-            if (m < m_end && n + 8 <= p.N) d[j].load(dy + (int64_t)m * p.lddy);
-            else if (m < m_end && n < p.N) d[j].load_some(dy + (int64_t)m * p.lddy, p.N - n);
-            else d[j].zero();
+            const int m = m_first + st * MS + j * (THREADS / CN);
+            r.d[j].zero();
+            if (m + nr < m_end && n + 8 <= p.N) r.d[j].load(dy0 + m * p.lddy + dy_of);
+            else if (m + nr < m_end && n < p.N) r.d[j].load_some(dy0 + m * p.lddy + dy_of, p.N - n);
         }
 #pragma unroll
         for (int j = 0; j < KR; j++) {
-            const int m = m0 + kr + j * (THREADS / (CK / 2));
-            x[j] = (u32x4){0, 0, 0, 0};
-            xs[j] = 0;
-            if (m < m_end && k < p.kp) {
-                x[j] = *reinterpret_cast<const u32x4*>(q + (int64_t)m * p.kp);
-                xs[j] = words[m];
+            const int m = m_first + st * MS + j * (THREADS / XR);
+            r.x[j] = (xpiece)0u;
+            r.xs[j] = 0;
+            if (m + kr < m_end) {
+                r.x[j] = *reinterpret_cast<const xpiece*>(q0 + (int64_t)m * p.kp + q_of);
+                r.xs[j] = (s0 + m)[kr];
             }
         }
     };
-    auto store = [&](uint8_t* st) __attribute__((always_inline)) {
+    auto store = [&](const Pieces& r, uint8_t* st) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NR; j++) {
             const int m = nr + j * (THREADS / CN);
+            u32x4 part[PARTS];
+            r.d[j].parts(part);
 #pragma unroll
             for (int i = 0; i < PARTS; i++)
-                *reinterpret_cast<u32x4*>(st + i * PART + m * (2 * BN) + ((nc ^ sw(m)) << 4)) = d[j].part(i);
+                *reinterpret_cast<u32x4*>(st + i * PART + m * (2 * BN) + ((nc ^ sw(m)) << 4)) = part[i];
         }
 #pragma unroll
         for (int j = 0; j < KR; j++) {
-            const int m = kr + j * (THREADS / (CK / 2));
-            const float sc = scale_of(xs[j] >> (8 * (block & 3)) & 0xff);
+            const int m = kr + j * (THREADS / XR);
+            const float sc = scale_of(r.xs[j] >> (8 * (block & 3)) & 0xff);
             uint8_t* row = st + PARTS * PART + m * (2 * BK);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < XC; h++) {
                 u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    w[2 * i] = pk(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[j][2 * h + i], sc, false));
-                    w[2 * i + 1] = pk(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[j][2 * h + i], sc, true));
+                    w[2 * i] = pk(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[j][2 * h + i], sc, false));
+                    w[2 * i + 1] = pk(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[j][2 * h + i], sc, true));
                 }
-                *reinterpret_cast<u32x4*>(row + (((2 * kc + h) ^ sw(m)) << 4)) = w;
+                *reinterpret_cast<u32x4*>(row + (((XC * kc + h) ^ sw(m)) << 4)) = w;
             }
         }
     };
@@ -181,19 +259,10 @@ __global__ __launch_bounds__(64 * WN * WK) void grad_weight_kernel(GradWeight p)
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
+    // a stage's loads have DEPTH stages to arrive
     const int stages = (m_end - m_first + MS - 1) / MS;
-    if (stages > 0) {
-        load(m_first);
-        store(lds);
-        load(m_first + MS);
-    }
-    for (int st = 0; st < stages; st++) {
-        __syncthreads();
-        const uint8_t* now = lds + (st & 1) * STAGE;
-        if (st + 1 < stages) {
-            store(lds + ((st + 1) & 1) * STAGE);
-            load(m_first + (st + 2) * MS);
-        }
+    Pieces r0, r1;
+    auto products = [&](const uint8_t* now) __attribute__((always_inline)) {
         bf16x8 b[PARTS][TN];
 #pragma unroll
         for (int i = 0; i < PARTS; i++)
@@ -203,124 +272,139 @@ __global__ __launch_bounds__(64 * WN * WK) void grad_weight_kernel(GradWeight p)
         for (int i = 0; i < TK; i++) {
             const bf16x8 a = frag(now + PARTS * PART, 2 * BK, wk * TK + i);
 #pragma unroll
-            for (int j = 0; j < TN; j++)
+            for (int h = PARTS - 1; h >= 0; h--)
 #pragma unroll
-                for (int h = PARTS - 1; h >= 0; h--)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[h][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[h][j], acc[i][j], 0, 0, 0);
         }
         if (sums) {
 #pragma unroll
-            for (int j = 0; j < TN; j++)
+            for (int h = PARTS - 1; h >= 0; h--)
 #pragma unroll
-                for (int h = PARTS - 1; h >= 0; h--)
-                    sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b[h][j], sum[j], 0, 0, 0);
+                for (int j = 0; j < TN; j++) sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b[h][j], sum[j], 0, 0, 0);
         }
+    };
+    // stage st, while the next one goes to LDS and the DEPTH-th after that is fetched
+    auto step = [&](int st, Pieces& r) __attribute__((always_inline)) {
+        __syncthreads();
+        store(r, lds + ((st + 1) & 1) * STAGE);
+        load(r, st + 1 + DEPTH);
+        products(lds + (st & 1) * STAGE);
+    };
+    auto step_any = [&](int st, Pieces& r) __attribute__((always_inline)) {
+        __syncthreads();
+        if (st + 1 < stages) {
+            store(r, lds + ((st + 1) & 1) * STAGE);
+            load_any(r, st + 1 + DEPTH);
+        }
+        products(lds + (st & 1) * STAGE);
+    };
+    int st = 0;
+    if (stages > 0) {
+        load_any(r0, 0);
+        if constexpr (DEPTH == 2) load_any(r1, 1);
+        store(r0, lds);
+        load_any(r0, DEPTH);
+    }
+    Pieces& odd = DEPTH == 2 ? r1 : r0;  // of stage 1
+    for (; st + 2 + DEPTH < plain; st += 2) {
+        step(st, odd);
+        step(st + 1, r0);
+    }
+#pragma unroll 1
+    for (; st < stages; st += 2) {
+        step_any(st, odd);
+        if (st + 1 < stages) step_any(st + 1, r0);
     }
 
-    const bool whole = p.splits == 1;
-    float* part = whole ? nullptr : p.part + (int64_t)split * ((int64_t)p.N * p.K + p.N);
+    const bool whole = split < 0;
+    // a part of a divided tile: [BN][BK], then db's [BN]
+    float* part = whole ? nullptr : p.part + ((int64_t)(tile - p.whole) * p.splits + split) * ((int64_t)BN * BK + BN);
 #pragma unroll
     for (int j = 0; j < TN; j++) {
         const int row = n0 + (wn * TN + j) * 16 + (lane & 15);
         if (row >= p.N) continue;
         if (sums && lane < 16) {
-            if (!whole) part[(int64_t)p.N * p.K + row] = sum[j][0];
+            if (!whole) part[BN * BK + row - n0] = sum[j][0];
             else p.db[row] = p.add ? p.db[row] + sum[j][0] : sum[j][0];
         }
 #pragma unroll
         for (int i = 0; i < TK; i++) {
             const int col = k0 + (wk * TK + i) * 16 + 4 * (lane >> 4), left = p.K - col;
             if (left <= 0) continue;
-            f32x4 v = acc[i][j];
-            if (!whole || p.w_f32) {
-                float* to = whole ? reinterpret_cast<float*>(p.dw) + row * p.ldw + col : part + (int64_t)row * p.K + col;
-                if (whole && p.add) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e < left) v[e] += to[e];
-                }
-                if (left >= 4) {
-                    *reinterpret_cast<f32x4_4*>(to) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e < left) to[e] = v[e];
-                }
-            } else {
-                typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
-                uint16_t* to = reinterpret_cast<uint16_t*>(p.dw) + row * p.ldw + col;
-                const u32x2_2 w = {bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3])};
-                if (left >= 4) {
-                    *reinterpret_cast<u32x2_2*>(to) = w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e < left) to[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                }
-            }
+            if (whole) put(p, row, col, left, acc[i][j]);
+            else *reinterpret_cast<f32x4*>(part + (row - n0) * BK + (col - k0)) = acc[i][j];
         }
     }
 }
 
-// The splits' sums, in their order: four columns a thread, rows over the grid's second dimension
+// The divided tiles' parts, in their order: four columns a thread, a tile's rows over the grid's second dimension
+template <int BN, int BK>
 __global__ __launch_bounds__(256) void grad_weight_join_kernel(GradWeight p) {
-    const int64_t stride = (int64_t)p.N * p.K + p.N;
-    for (int64_t row = blockIdx.y; row < p.N; row += gridDim.y) {
-        if (p.db && blockIdx.x == 0 && threadIdx.x == 0) {
-            float s = p.add ? p.db[row] : 0.f, t = 0.f;
-            for (int i = 0; i < p.splits; i++) t += p.part[i * stride + (int64_t)p.N * p.K + row];
-            p.db[row] = s + t;
-        }
-        const int col = (blockIdx.x * 256 + threadIdx.x) * 4, left = p.K - col;
-        if (left <= 0) continue;
-        const float* from = p.part + row * p.K + col;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (left >= 4) {
-            for (int i = 0; i < p.splits; i++) v += *reinterpret_cast<const f32x4_4*>(from + i * stride);
-        } else {
-            for (int i = 0; i < p.splits; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (e < left) v[e] += from[i * stride + e];
-        }
-        const int count = min(left, 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (e >= count) continue;
-            if (p.w_f32) {
-                float* to = reinterpret_cast<float*>(p.dw) + row * p.ldw + col + e;
-                *to = p.add ? *to + v[e] : v[e];
-            } else {
-                reinterpret_cast<uint16_t*>(p.dw)[row * p.ldw + col + e] = (uint16_t)bf16x2_rne(v[e], v[e]);
-            }
-        }
+    constexpr int ROWS = 1024 / BK;  // of a workgroup
+    constexpr int64_t SIZE = (int64_t)BN * BK + BN;
+    int n0, k0;
+    place<BN, BK>(p, p.whole + blockIdx.x, n0, k0);
+    const float* part = p.part + (int64_t)blockIdx.x * p.splits * SIZE;
+    const int r = blockIdx.y * ROWS + threadIdx.x / (BK / 4), c = threadIdx.x % (BK / 4) * 4;
+    const int row = n0 + r, col = k0 + c, left = p.K - col;
+    if (row >= p.N) return;
+    if (p.db && k0 == 0 && c == 0) {
+        float s = 0.f;
+        for (int i = 0; i < p.splits; i++) s += part[i * SIZE + BN * BK + r];
+        p.db[row] = p.add ? p.db[row] + s : s;
     }
+    if (left <= 0) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < p.splits; i++) v += *reinterpret_cast<const f32x4*>(part + i * SIZE + r * BK + c);
+    put(p, row, col, left, v);
 }
 
-template <int PARTS, int TN, int TK, int WN, int WK>
-void run(GradWeight& a, hipStream_t s) {
-    a.n_tiles = (a.N + 16 * TN * WN - 1) / (16 * TN * WN);
-    a.k_tiles = (a.K + 16 * TK * WK - 1) / (16 * TK * WK);
-    hipLaunchKernelGGL((grad_weight_kernel<PARTS, TN, TK, WN, WK>), dim3(xcd_grid((long)a.n_tiles * a.k_tiles * a.splits)),
+template <int PARTS, int TN, int TK, int WN, int WK, int DEPTH>
+hipError_t run(const GradWeight& a, hipStream_t s) {
+    constexpr int BN = 16 * TN * WN, BK = 16 * TK * WK;
+    const int rest = a.n_tiles * a.k_tiles - a.whole;
+    hipLaunchKernelGGL((grad_weight_kernel<PARTS, TN, TK, WN, WK, DEPTH>), dim3((unsigned)a.whole + xcd_grid((long)rest * a.splits)),
                        dim3(64 * WN * WK), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || rest == 0) return e;
+    hipLaunchKernelGGL((grad_weight_join_kernel<BN, BK>), dim3((unsigned)rest, BN * BK / 1024), dim3(256), 0, s, a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int grad_weight_splits(int dtype_dy, int dtype_w, int M, int N, int K) {
-    const int64_t tiles = (int64_t)((N + 127) / 128) * ((K + 127) / 128);
-    const int64_t fill = 512 / std::max<int64_t>(tiles, 1);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({fill, M / 256, 16}));
+// Tiles of 256 x 256 (a workgroup per CU) or 128 x 128 (two).  Tiles fill the chip in whole rounds; those that are
+// left over (all, of a small dW) have their rows divided so that they fill one more.
+GradWeightPlan grad_weight_plan(int dtype_dy, int M, int N, int K) {
+    GradWeightPlan p{};
+    auto tiles = [&](int b) { return (int64_t)((N + b - 1) / b) * ((K + b - 1) / b); };
+    p.tile = dtype_dy == AWA_F32 || M < 512 || tiles(256) < 128 ? 128 : 256;
+    const int64_t all = tiles(p.tile), slots = p.tile == 256 ? 256 : 512, rest = all % slots;
+    const int64_t least = 256;  // rows of a part at least
+    const int64_t s = rest ? std::min<int64_t>(slots / rest, M / least) : 1;
+    if (s > 1) {
+        p.splits = (int)s;
+        p.whole = (int)(all - rest);
+        p.rows_per = (int)((((M + s - 1) / s) + MS - 1) / MS * MS);
+    } else {
+        p.splits = 1;
+        p.whole = (int)all;
+        p.rows_per = M;
+    }
+    p.work = s > 1 ? rest * s * ((int64_t)p.tile * p.tile + p.tile) * 4 : 0;
+    return p;
 }
 
 hipError_t launch_grad_weight(int dtype_dy, GradWeight& a, hipStream_t s) {
-    a.rows_per = ((a.M + a.splits - 1) / a.splits + MS - 1) / MS * MS;
-    if (dtype_dy == AWA_F32) run<3, 4, 4, 2, 2>(a, s);
-    else run<1, 4, 4, 2, 2>(a, s);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL(grad_weight_join_kernel, dim3((unsigned)((a.K + 1023) / 1024), (unsigned)std::min(a.N, 65535)), dim3(256), 0, s, a);
-    return hipGetLastError();
+    const GradWeightPlan p = grad_weight_plan(dtype_dy, a.M, a.N, a.K);
+    a.n_tiles = (a.N + p.tile - 1) / p.tile;
+    a.k_tiles = (a.K + p.tile - 1) / p.tile;
+    a.whole = p.whole;
+    a.splits = p.splits;
+    a.rows_per = p.rows_per;
+    if (dtype_dy == AWA_F32) return run<3, 4, 4, 2, 2, 2>(a, s);
+    return p.tile == 256 ? run<1, 8, 4, 2, 4, 1>(a, s) : run<1, 4, 4, 2, 2, 2>(a, s);
 }
 
 }  // namespace awa

@@ -64,10 +64,7 @@ bool norm_sizes_ok(int M, int K) { return M >= 0 && M <= DIT_OPS_ROWS_MAX && K >
 bool weight_sizes_ok(int M, int N, int K) {
     return M >= 0 && M <= DIT_OPS_ROWS_MAX && N >= 1 && N <= DIT_OPS_COLS_MAX && K >= 1 && K <= DIT_OPS_COLS_MAX;
 }
-int64_t weight_work(int dtype_dy, int dtype_w, int M, int N, int K) {
-    const int splits = grad_weight_splits(dtype_dy, dtype_w, M, N, K);
-    return splits > 1 ? align_up((int64_t)splits * ((int64_t)N * K + N) * 4) : 0;
-}
+int64_t weight_work(int dtype_dy, int M, int N, int K) { return align_up(grad_weight_plan(dtype_dy, M, N, K).work); }
 
 // ---- the attention's plan
 
@@ -259,7 +256,7 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
 
 // the parts of the workspace, each aligned
 struct CrossWork {
-    int64_t qpart, kpart, dsum, total;
+    int64_t qpart, kpart, dsum, lse2, total;
 };
 CrossWork cross_work(const dit_cross& c, bool grad) {
     CrossWork w{};
@@ -273,6 +270,7 @@ CrossWork cross_work(const dit_cross& c, bool grad) {
     if (grad) {
         w.kpart = take((int64_t)c.ks.n_parts * c.kv_heads * cross_key_part(c.ks.block, c.head_d));
         w.dsum = take((int64_t)c.heads * c.q_rows);
+        w.lse2 = take((int64_t)c.heads * c.q_rows);
     }
     w.total = at;
     return w;
@@ -446,7 +444,7 @@ int dit_layer_norm_grad(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
 
 int64_t dit_grad_weight_work(int dtype_dy, int dtype_w, int M, int N, int K) {
     if (!dtype_ok(dtype_dy) || !dtype_ok(dtype_w) || !weight_sizes_ok(M, N, K)) return AWA_EARG;
-    return weight_work(dtype_dy, dtype_w, M, N, K);
+    return weight_work(dtype_dy, M, N, K);
 }
 
 int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t lddy, const uint8_t* d_q, const uint32_t* d_s,
@@ -463,12 +461,12 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
         set_err(ctx, "dit_grad_weight_fp8: null or misaligned pointer (d_q 16 bytes, words and db 4, others their elements)");
         return AWA_EARG;
     }
-    if (!stride_ok(M, lddy, N) || !stride_ok(N, ldw, K) || ld_s < M || ld_s > STRIDE_MAX) {
-        set_err(ctx, "dit_grad_weight_fp8: lddy=%lld (at least %d), ldw=%lld (at least %d), ld_s=%lld (at least %d; all at most 2^36)",
-                (long long)lddy, N, (long long)ldw, K, (long long)ld_s, M);
+    if (!stride_ok(M, lddy, N) || (M > 1 && lddy > DIT_OPS_COLS_MAX) || !stride_ok(N, ldw, K) || ld_s < M || ld_s > STRIDE_MAX) {
+        set_err(ctx, "dit_grad_weight_fp8: lddy=%lld (%d .. %d), ldw=%lld (at least %d), ld_s=%lld (at least %d; both at most 2^36)",
+                (long long)lddy, N, DIT_OPS_COLS_MAX, (long long)ldw, K, (long long)ld_s, M);
         return AWA_EARG;
     }
-    const int64_t need = weight_work(dtype_dy, dtype_w, M, N, K);
+    const int64_t need = weight_work(dtype_dy, M, N, K);
     if (int rc = work_ok(ctx, "dit_grad_weight_fp8", d_work, work_bytes, need)) return rc;
     GradWeight a{};
     a.dy = d_dy; a.lddy = M > 1 ? lddy : N;
@@ -477,7 +475,6 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
     a.db = d_db;
     a.add = add != 0; a.w_f32 = dtype_w == AWA_F32;
     a.part = static_cast<float*>(d_work);
-    a.splits = grad_weight_splits(dtype_dy, dtype_w, M, N, K);
     a.M = M; a.N = N; a.K = K; a.kp = padded(K);
     const Extent dy{d_dy, span(M, a.lddy, N, elem(dtype_dy))}, q{d_q, (size_t)M * a.kp}, s{d_s, span(groups_of(K), ld_s, M, 4)};
     const Extent dw{d_dw, span(N, a.ldw, K, elem(dtype_w))}, db{d_db, (size_t)N * 4}, wk{d_work, (size_t)need};
@@ -623,6 +620,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
     a.qpart = reinterpret_cast<float*>(base + w.qpart);
     a.kpart = reinterpret_cast<float*>(base + w.kpart);
     a.dsum = reinterpret_cast<float*>(base + w.dsum);
+    a.lse2 = reinterpret_cast<float*>(base + w.lse2);
     a.ld_dsum = qr;
     DeviceGuard dg(ctx->device);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

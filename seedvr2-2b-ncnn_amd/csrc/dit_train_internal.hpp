@@ -49,13 +49,17 @@ struct GradWeight {
     int64_t ldw;
     float* db;  // [N] or null
     int add, w_f32;
-    float* part;  // [splits][N][K] and [splits][N] where splits > 1
-    int splits, rows_per;  // rows of a split, a multiple of the kernel's stage
+    float* part;  // of the divided tiles: [tile][split] of a tile's sums and db's
+    // filled by launch_grad_weight: tiles, how many of them are whole, the others' parts and the rows of one
+    int n_tiles, k_tiles, whole, splits, rows_per;
     int M, N, K, kp;
-    int n_tiles, k_tiles;
 };
-// splits of the rows, for the workspace and the launch alike
-int grad_weight_splits(int dtype_dy, int dtype_w, int M, int N, int K);
+// how the work is divided, for the workspace and the launch alike
+struct GradWeightPlan {
+    int tile, whole, splits, rows_per;
+    int64_t work;  // bytes
+};
+GradWeightPlan grad_weight_plan(int dtype_dy, int M, int N, int K);
 hipError_t launch_grad_weight(int dtype_dy, GradWeight& a, hipStream_t s);
 
 // ---- attention to states of another length
@@ -119,7 +123,9 @@ struct CrossArgs {
     CrossQueries qs;
     CrossKeySide ks;
     float *qpart, *kpart;  // partial results
-    float* dsum;           // rowsum(dout out), [heads][ld_dsum]
+    // left by the gradient of the queries for that of the keys, [heads][ld_dsum]: rowsum(dout out), and lse in
+    // powers of two (infinite for a row without keys, so that its probabilities are 0)
+    float *dsum, *lse2;
     int64_t ld_dsum;
 };
 hipError_t launch_cross_forward(int dtype, const CrossArgs& a, hipStream_t s);

@@ -26,7 +26,7 @@ DeviceGuard::~DeviceGuard() {}
 hipError_t launch_layer_norm(int, int, const NormFwd&, hipStream_t) { launches++; return hipSuccess; }
 hipError_t launch_layer_norm_grad(int, int, const NormGrad&, hipStream_t) { launches++; return hipSuccess; }
 int norm_grad_groups(int M, int) { return std::min(M, 256); }
-int grad_weight_splits(int, int, int M, int, int) { return M >= 1024 ? 4 : 1; }
+GradWeightPlan grad_weight_plan(int, int M, int, int) { return {128, 1, 1, M, M >= 1024 ? 1 << 20 : 0}; }
 hipError_t launch_grad_weight(int, GradWeight&, hipStream_t) { launches++; return hipSuccess; }
 hipError_t launch_cross_forward(int, const CrossArgs&, hipStream_t) { launches++; return hipSuccess; }
 hipError_t launch_cross_grad_queries(int, const CrossArgs&, hipStream_t) { launches++; return hipSuccess; }
@@ -276,6 +276,7 @@ int main() {
     check("weight misaligned q", weight([&](D& d) { d.q = Y + 8; }), bad);
     check("weight misaligned dy", weight([&](D& d) { d.dy = X + 1; }), bad);
     check("weight lddy", weight([](D& d) { d.lddy = 49; }), bad);
+    check("weight far lddy", weight([](D& d) { d.lddy = DIT_OPS_COLS_MAX + 1; }), bad);
     check("weight ldw", weight([](D& d) { d.ldw = 99; }), bad);
     check("weight ld_s", weight([](D& d) { d.ld_s = 6; }), bad);
     check("weight N", weight([](D& d) { d.N = 0; }), bad);

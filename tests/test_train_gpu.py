@@ -247,7 +247,8 @@ def check_weight(dw, db, dy, x, before=None, db_before=None):
 @pytest.mark.parametrize("tdy,tw", [(BF16, F32), (BF16, BF16), (F32, F32), (F32, BF16)])
 @pytest.mark.parametrize("M,N,K,ld", [(1, 1, 1, 1), (2, 3, 5, 3), (31, 64, 128, 64), (32, 65, 129, 70), (33, 127, 100, 127),
                                       (58, 300, 640, 300), (257, 128, 128, 128), (700, 130, 513, 131), (1237, 199, 269, 199),
-                                      (2100, 256, 384, 512), (5498, 96, 160, 96), (64, 1000, 2693, 1001)])
+                                      (2100, 256, 384, 512), (5498, 96, 160, 96), (64, 1000, 2693, 1001),
+                                      (600, 4100, 2090, 4103), (1000, 4353, 4090, 4353), (70, 4, 300, 4), (77, 9, 300, 9)])
 def test_grad_weight(ctx, awa, tdy, tw, M, N, K, ld):
     import torch
     g = gen(M + N + K)
