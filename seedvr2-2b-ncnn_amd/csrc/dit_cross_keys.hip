@@ -8,6 +8,8 @@
 //
 // Keys are few where queries are many, so the units are divided over workgroups, whose fp32 partial sums a second
 // kernel adds in their order.
+#include <type_traits>
+
 #include "dit_cross_device.hpp"
 
 namespace awa {
@@ -19,7 +21,7 @@ namespace {
 // NK blocks of 16 keys a wave, WKEY waves over the keys; where SUBS is 2 as many more take the second 32 rows of a
 // unit, and the two halves' sums meet in LDS at the end.
 template <typename T, int DP, int NK, int WKEY, int SUBS>
-__global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs p) {
+__global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossArgs p) {
     using Frag = typename T::Frag;
     using L = Tile<T, DP>;
     constexpr int KS = DP / 32, DB = DP / 16, QT = CROSS_QT, WAVES = WKEY * SUBS;
@@ -96,13 +98,12 @@ __global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs 
         const char* qt = lds + (n & 1) * STAGE;
         const char* dt = qt + TILE_B;
         const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE_B);
+        // 32 HALVES rows from base on (64 at once where registers allow: more products that do not wait for each other)
+        auto take = [&](auto halves, int base) __attribute__((always_inline)) {
+            constexpr int HALVES = decltype(halves)::value, NB = 2 * HALVES;
+            f32x4 s[NB][NK], dp[NB][NK];
 #pragma unroll
-        for (int s0 = 0; s0 < QT / 32; s0 += SUBS) {
-            const int sub = s0 + (SUBS > 1 ? sub0 : 0), base = 32 * sub;
-            if (base >= rows) continue;
-            f32x4 s[2][NK], dp[2][NK];
-#pragma unroll
-            for (int b = 0; b < 2; b++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     const Frag qf = L::row_frag(qt, base + 16 * b + (lane & 15), ks, g);
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs 
                     }
                 }
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < NB; b++) {
                 const int r0 = base + 16 * b + 4 * g;
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + r0), d4 = *reinterpret_cast<const f32x4*>(lse + QT + r0);
 #pragma unroll
@@ -127,30 +128,41 @@ __global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs 
                         s[b][j][r] = e;
                     }
             }
-            if (rows < base + 32) {  // rows past the end hold zeros, but infinite keys times zero are not
+            if (rows < base + 32 * HALVES) {  // rows past the end hold zeros, but infinite keys times zero are not
 #pragma unroll
-                for (int b = 0; b < 2; b++)
+                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if (base + 16 * b + 4 * g + r >= rows)
 #pragma unroll
                             for (int j = 0; j < NK; j++) s[b][j][r] = dp[b][j][r] = 0.f;
             }
-            Frag pf[NK], sf[NK];
 #pragma unroll
-            for (int j = 0; j < NK; j++) {
-                pf[j] = T::pack(s[0][j], s[1][j]);
-                sf[j] = T::pack(dp[0][j], dp[1][j]);
+            for (int h = 0; h < HALVES; h++) {
+                if (h) __builtin_amdgcn_sched_barrier(0xf);  // arithmetic may pass: reads that move further up spill registers
+                Frag pf[NK], sf[NK];
+#pragma unroll
+                for (int j = 0; j < NK; j++) {
+                    pf[j] = T::pack(s[2 * h][j], s[2 * h + 1][j]);
+                    sf[j] = T::pack(dp[2 * h][j], dp[2 * h + 1][j]);
+                }
+#pragma unroll
+                for (int db = 0; db < DB; db++) {
+                    const Frag df = L::column_frag(dt, base + 32 * h, db, lane);
+#pragma unroll
+                    for (int j = 0; j < NK; j++) dv[db][j] = T::mma(df, pf[j], dv[db][j]);
+                    const Frag qf = L::column_frag(qt, base + 32 * h, db, lane);
+#pragma unroll
+                    for (int j = 0; j < NK; j++) dk[db][j] = T::mma(qf, sf[j], dk[db][j]);
+                }
             }
-#pragma unroll
-            for (int db = 0; db < DB; db++) {
-                const Frag df = L::column_frag(dt, base, db, lane);
-#pragma unroll
-                for (int j = 0; j < NK; j++) dv[db][j] = T::mma(df, pf[j], dv[db][j]);
-                const Frag qf = L::column_frag(qt, base, db, lane);
-#pragma unroll
-                for (int j = 0; j < NK; j++) dk[db][j] = T::mma(qf, sf[j], dk[db][j]);
-            }
+        };
+        typedef std::integral_constant<int, 1> One;
+        typedef std::integral_constant<int, 2> Two;
+        if constexpr (SUBS == 2) {
+            if (32 * sub0 < rows) take(One(), 32 * sub0);
+        } else {
+            take(Two(), 0);
         }
     }
     if constexpr (SUBS > 1) {
@@ -178,22 +190,24 @@ __global__ __launch_bounds__(64 * WKEY * SUBS) void cross_keys_kernel(CrossArgs 
             }
     }
     const int d = p.head_d;
-    float* const part = it.part < 0 ? nullptr : p.kpart + ((int64_t)it.part * p.kv_heads + kv_head) * cross_key_part(p.ks.block, d);
+    float* const part = it.part < 0 ? nullptr : p.kpart + ((int64_t)it.part * p.kv_heads + kv_head) * cross_key_part(CROSS_KEYS, d);
 #pragma unroll
     for (int j = 0; j < NK; j++) {
-        const int c = (wk * NK + j) * 16 + (lane & 15);
+        // the lane counted anew: kept over the loop, what follows from it would cost registers there
+        const int own = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+        const int c = (wk * NK + j) * 16 + (own & 15), ch0 = 4 * (own >> 4);
         if (c >= it.kn) continue;
         char* kp = p.dk + (int64_t)(it.k0 + c) * p.dk_row + kv_head * p.dk_head;
         char* vp = p.dv + (int64_t)(it.k0 + c) * p.dv_row + kv_head * p.dv_head;
 #pragma unroll
         for (int db = 0; db < DB; db++) {
-            const int ch = 16 * db + 4 * g;
+            const int ch = 16 * db + ch0;
             if (ch >= d) continue;
             const f32x4 z = {0.f, 0.f, 0.f, 0.f};
             const f32x4 a = in[j] ? dk[db][j] * p.scale : z, b = in[j] ? dv[db][j] : z;
             if (part) {
                 *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = a;
-                *reinterpret_cast<f32x4*>(part + (int64_t)(p.ks.block + c) * d + ch) = b;
+                *reinterpret_cast<f32x4*>(part + (int64_t)(CROSS_KEYS + c) * d + ch) = b;
             } else {
                 T::store4(kp + ch * T::SIZE, a);
                 T::store4(vp + ch * T::SIZE, b);
@@ -209,9 +223,9 @@ __global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
     const CrossKeyJoin it = p.ks.joins[blockIdx.x - kv_head * p.ks.n_joins];
     const int d = p.head_d, pieces = d / 4, e = blockIdx.y * 256 + threadIdx.x;
     if (e >= 2 * it.kn * pieces) return;
-    const int64_t size = cross_key_part(p.ks.block, d), stride = p.kv_heads * size;
+    const int64_t size = cross_key_part(CROSS_KEYS, d), stride = p.kv_heads * size;
     const int which = e / (it.kn * pieces), c = e / pieces % it.kn, ch = e % pieces * 4;
-    const float* from = p.kpart + ((int64_t)it.part0 * p.kv_heads + kv_head) * size + (int64_t)(which * p.ks.block + c) * d + ch;
+    const float* from = p.kpart + ((int64_t)it.part0 * p.kv_heads + kv_head) * size + (int64_t)(which * CROSS_KEYS + c) * d + ch;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < it.parts; i++) v += *reinterpret_cast<const f32x4*>(from + i * stride);
@@ -223,8 +237,9 @@ __global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
 template <typename T, int DP>
 void run(const CrossArgs& a, hipStream_t s) {
     const dim3 grid(xcd_grid((long)a.ks.n_items * a.kv_heads));
-    if (a.ks.block == 128) hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, 8, 1>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, 4, 2>), grid, dim3(512), 0, s, a);
+    // fp32: tiles are twice as large, so that one workgroup fills a CU's LDS; twice the waves on them
+    constexpr int SUBS = T::SIZE == 2 ? 1 : 2;
+    hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, CROSS_KEYS / 16, SUBS>), grid, dim3(4 * CROSS_KEYS * SUBS), 0, s, a);
 }
 template <typename T>
 hipError_t run_all(const CrossArgs& a, hipStream_t s) {
@@ -234,7 +249,7 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
     else run<T, 128>(a, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.ks.n_joins == 0) return e;
-    const int pieces = 2 * a.ks.block * (a.head_d / 4);
+    const int pieces = 2 * CROSS_KEYS * (a.head_d / 4);
     hipLaunchKernelGGL((cross_keys_join_kernel<T>), dim3((unsigned)(a.ks.n_joins * a.kv_heads), (unsigned)((pieces + 255) / 256)),
                        dim3(256), 0, s, a);
     return hipGetLastError();

@@ -76,25 +76,55 @@ struct Plan {
     std::vector<CrossUnit> units;
 };
 
-// Workgroups wanted before work is divided further: two for each of the 256 compute units.
-constexpr int64_t WANTED = 512;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How far to divide the long axis of each block's work: the number of runs with the least estimated time, of a chip that
+// takes `slots` workgroups at once, each t0 and t1 a step of its run, and then joins `part` bytes of each run (written and
+// read).  `blocks`: how many blocks have how many steps.
+struct Cost {
+    int64_t slots;
+    double t0, t1, join, part;  // us, us, us, bytes
+};
+int64_t runs_of(const std::map<int64_t, int64_t>& blocks, const Cost& c) {
+    int64_t most = 0, best = 1;
+    for (const auto& b : blocks) most = std::max(most, b.first);
+    double least = 0;
+    for (int64_t runs = 1; runs <= std::min<int64_t>(most, 64); runs++) {
+        const int64_t run = ceil_div(most, runs);
+        int64_t total = 0, parts = 0;
+        for (const auto& b : blocks) {
+            const int64_t n = std::max<int64_t>(1, ceil_div(b.first, run));
+            total += b.second * n;
+            if (n > 1) parts += b.second * n;
+        }
+        const double t = (double)ceil_div(total, c.slots) * (c.t0 + c.t1 * (double)run) +
+                         (parts ? c.join + 2.0 * c.part * (double)parts / 4e6 : 0.0);
+        if (runs == 1 || t < least) {
+            least = t;
+            best = runs;
+        }
+    }
+    return most > 0 ? ceil_div(most, best) : 1;  // steps of a run
+}
 
 void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
-                  const std::vector<int64_t>& kl, int heads, int kv_heads, CrossQueries& s, Plan& p) {
+                  const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, CrossQueries& s, Plan& p) {
     const int per = heads / kv_heads;
-    int64_t most = per, blocks = 0;
+    int64_t most = per;
     for (int64_t n : ql) most = std::max(most, n * per);
     // Few columns: the heads that share a key head in one block, so that its keys are read once.
     s.block = most <= 16 ? 16 : most <= 32 ? 32 : 128;
     s.pack = s.block < 128 ? per : 1;
     const int rows = s.block / s.pack;
-    for (int64_t n : ql) blocks += (n + rows - 1) / rows;
-    const int64_t groups = heads / s.pack, made = std::max<int64_t>(blocks * groups, 1);
-    // keys of a run: whole rounds of the block's waves
-    const int64_t least = 128, want = (WANTED + made - 1) / made;
+    // A step is 64 keys, or 128 for the four waves of a block of few columns.  Measured, heads of 128 channels in bf16: a
+    // block of 128 columns takes 6 us and 1.6 a step where two share a CU; one of few columns 4 us and 1.5 a step.
+    const int64_t groups = heads / s.pack, step = s.block < 128 ? 128 : 64;
+    std::map<int64_t, int64_t> made;
+    for (size_t i = 0; i < ql.size(); i++)
+        if (ql[i]) made[ceil_div(kl[i], step)] += ceil_div(ql[i], rows) * groups;
+    const Cost cost{s.block < 128 ? 256 : 512, s.block < 128 ? 4.0 : 6.0, s.block < 128 ? 1.5 : 1.6, 5.0, 4.0 * s.block * head_d};
+    const int64_t run = runs_of(made, cost) * step;
     for (size_t i = 0; i < ql.size(); i++) {
-        const int64_t runs = std::max<int64_t>(1, std::min(want, (kl[i] + least - 1) / least));
-        const int64_t run = std::max<int64_t>((((kl[i] + runs - 1) / runs) + least - 1) / least * least, least);
         for (int64_t r = 0; r < ql[i]; r += rows) {
             const int n = (int)std::min<int64_t>(rows, ql[i] - r) * s.pack;
             const int parts = (int)std::max<int64_t>(1, (kl[i] + run - 1) / run), first = s.n_parts;
@@ -119,31 +149,29 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
 }
 
 void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
-               const std::vector<int64_t>& kl, int heads, int kv_heads, CrossKeySide& s, Plan& p) {
+               const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, CrossKeySide& s, Plan& p) {
     const int per = heads / kv_heads;
     // sequences by their keys
     std::map<int64_t, std::vector<size_t>> shared;
-    int64_t most = 0;
     for (size_t i = 0; i < kl.size(); i++)
-        if (kl[i]) {
-            shared[ka[i]].push_back(i);
-            most = std::max(most, kl[i]);
-        }
-    s.block = most <= 64 ? 64 : 128;
-    int64_t blocks = 0;
-    for (auto& e : shared) blocks += (kl[e.second[0]] + s.block - 1) / s.block;
-    const int64_t made = std::max<int64_t>(blocks * kv_heads, 1), want = (WANTED + made - 1) / made;
+        if (kl[i]) shared[ka[i]].push_back(i);
+    // A step is a unit.  Measured as above: a block takes 5 us and 2 a unit where two share a CU.
+    std::map<int64_t, int64_t> made;
+    for (auto& e : shared) {
+        int64_t units = 0;
+        for (size_t i : e.second) units += ceil_div(ql[i], CROSS_QT);
+        made[units * per] += ceil_div(kl[e.second[0]], CROSS_KEYS) * kv_heads;
+    }
+    const int64_t run = runs_of(made, {512, 5.0, 2.0, 5.0, 8.0 * CROSS_KEYS * head_d});
     for (auto& e : shared) {
         const int unit0 = (int)p.units.size();
         for (size_t i : e.second)
             for (int64_t r = 0; r < ql[i]; r += CROSS_QT)
                 p.units.push_back({(int)(qa[i] + r), (int)std::min<int64_t>(CROSS_QT, ql[i] - r)});
         const int units = (int)p.units.size() - unit0;
-        const int64_t all = (int64_t)units * per, runs = std::max<int64_t>(1, std::min(want, all));
-        const int64_t run = std::max<int64_t>((all + runs - 1) / runs, 1);
-        const int64_t n = kl[e.second[0]];
-        for (int64_t c = 0; c < n; c += s.block) {
-            const int kn = (int)std::min<int64_t>(s.block, n - c), k0 = (int)(e.first + c);
+        const int64_t all = (int64_t)units * per, n = kl[e.second[0]];
+        for (int64_t c = 0; c < n; c += CROSS_KEYS) {
+            const int kn = (int)std::min<int64_t>(CROSS_KEYS, n - c), k0 = (int)(e.first + c);
             const int parts = (int)std::max<int64_t>(1, (all + run - 1) / run), first = s.n_parts;
             for (int i = 0; i < parts; i++) {
                 CrossKeys it{};
@@ -213,8 +241,8 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
     c.head_d = head_d;
     c.q_rows = q_rows;
     c.k_rows = k_rows;
-    plan_queries(qa, ql, ka, kl, heads, kv_heads, c.qs, p);
-    plan_keys(qa, ql, ka, kl, heads, kv_heads, c.ks, p);
+    plan_queries(qa, ql, ka, kl, heads, kv_heads, head_d, c.qs, p);
+    plan_keys(qa, ql, ka, kl, heads, kv_heads, head_d, c.ks, p);
     // grids are a workgroup per item and head
     if ((int64_t)c.qs.n_items * heads > 0x7fffff00 || (int64_t)c.ks.n_items * heads > 0x7fffff00) {
         set_err(ctx, "dit_cross_create: too many blocks for one launch");
@@ -268,7 +296,7 @@ CrossWork cross_work(const dit_cross& c, bool grad) {
     };
     w.qpart = take((int64_t)c.qs.n_parts * (c.heads / c.qs.pack) * cross_query_part(c.qs.block, c.head_d));
     if (grad) {
-        w.kpart = take((int64_t)c.ks.n_parts * c.kv_heads * cross_key_part(c.ks.block, c.head_d));
+        w.kpart = take((int64_t)c.ks.n_parts * c.kv_heads * cross_key_part(CROSS_KEYS, c.head_d));
         w.dsum = take((int64_t)c.heads * c.q_rows);
         w.lse2 = take((int64_t)c.heads * c.q_rows);
     }

@@ -81,6 +81,10 @@ constexpr int CROSS_QT = 64;
 struct CrossUnit {
     int q0, rows;
 };
+// Keys of a block: with 64, and their four waves' tiles, two workgroups share a CU, so that one's products fill the
+// other's waits (gradients of 16384 queries x 384 keys x 20 heads 304 us with 128 keys in eight waves, 292 so; of four clips
+// of up to 5440 x 512 363 and 308).
+constexpr int CROSS_KEYS = 64;
 // A block of keys and the run of its units (of every head that shares the key head: units ahead of
 // heads) that a workgroup takes.
 struct CrossKeys {
@@ -102,7 +106,6 @@ struct CrossQueries {
     const CrossJoin* joins = nullptr;
 };
 struct CrossKeySide {
-    int block = 0;
     int n_items = 0, n_joins = 0, n_parts = 0;
     const CrossKeys* items = nullptr;
     const CrossKeyJoin* joins = nullptr;

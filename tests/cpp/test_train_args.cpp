@@ -60,8 +60,8 @@ static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t
     Plan p;
     CrossQueries qs;
     CrossKeySide ks;
-    plan_queries(qa, ql, ka, kl, heads, kv_heads, qs, p);
-    plan_keys(qa, ql, ka, kl, heads, kv_heads, ks, p);
+    plan_queries(qa, ql, ka, kl, heads, kv_heads, 64, qs, p);
+    plan_keys(qa, ql, ka, kl, heads, kv_heads, 64, ks, p);
     const int per = heads / kv_heads, n = (int)ql.size();
     bool ok = (qs.block == 16 || qs.block == 32 || qs.block == 128) && (qs.pack == 1 || qs.pack == per) && qs.pack <= qs.block &&
               heads % qs.pack == 0 && qs.n_items == (int)p.items.size() && qs.n_joins == (int)p.joins.size();
@@ -103,7 +103,7 @@ static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t
             w.first = kl[i];
             if (ql[i]) w.second.insert({qa[i], ql[i]});
         }
-    ok = ks.block == 64 || ks.block == 128;
+    ok = true;
     std::set<int> kslots;
     size_t kat = 0, kjoin = 0;
     for (auto& w : want) {
@@ -115,7 +115,7 @@ static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t
             bool empty = w.second.second.empty();
             while (kat < p.kitems.size() && p.kitems[kat].k0 == f.k0) {
                 const CrossKeys& it = p.kitems[kat++];
-                ok = ok && it.k0 == w.first + c && it.kn == f.kn && it.kn > 0 && it.kn <= ks.block && it.unit0 == f.unit0 &&
+                ok = ok && it.k0 == w.first + c && it.kn == f.kn && it.kn > 0 && it.kn <= CROSS_KEYS && it.unit0 == f.unit0 &&
                      it.units == f.units && it.count >= 0 && (empty ? it.count == 0 : it.count > 0);
                 for (int u = it.first; ok && u < it.first + it.count; u++) {
                     if (u >= (int)seen.size() || seen[u]++) ok = false;
@@ -317,7 +317,6 @@ int main() {
     dit_cross c;
     c.heads = 4; c.kv_heads = 2; c.head_d = 64; c.q_rows = 100; c.k_rows = 50;
     c.qs.block = 128;
-    c.ks.block = 64;
     const int64_t row = 4 * 64;
     struct A {
         int t = AWA_BF16; dit_heads q, k, v, o, dout, dq, dk, dv; const void* mask = nullptr; float scale = 0.125f; void* lse;
