@@ -186,85 +186,158 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(NormFwd a) {
     }
 }
 
-// Rows in turn over the workgroups; eight waves a workgroup.  w stays in LDS: with x, dy and both
-// columns' sums in registers it would be the part that does not fit.
-template <typename TD, typename TX, int R, int WPR>
-__global__ __launch_bounds__(512) void layer_norm_grad_kernel(NormGrad a) {
-    constexpr int WAVES = 8, ROWS = WAVES / WPR, COLS = WPR * R * STEP;
+// A lane's piece of a row for the gradient: W consecutive columns (4; 1 for rows of fewer than four), read without a branch
+// so that the next row's pieces are on their way while this row's are worked on.
+template <typename T, int W> struct Bits;
+template <> struct Bits<float, 4> {
+    f32x4 v;
+    __device__ void load(const float* p) { v = *reinterpret_cast<const f32x4_4*>(p); }
+    __device__ float get(int i) const { return v[i]; }
+};
+template <> struct Bits<uint16_t, 4> {
+    u32x2 v;
+    __device__ void load(const uint16_t* p) { v = *reinterpret_cast<const u32x2_2*>(p); }
+    __device__ float get(int i) const { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
+};
+template <> struct Bits<Fp8, 4> {
+    uint32_t v;
+    __device__ void load(const Fp8* p) {
+        typedef uint32_t u32_1 __attribute__((aligned(1)));
+        v = *reinterpret_cast<const u32_1*>(p);
+    }
+    __device__ float get(int i) const {
+        const f32x2 f = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false);
+        return f[i & 1];
+    }
+};
+template <> struct Bits<float, 1> {
+    float v;
+    __device__ void load(const float* p) { v = *p; }
+    __device__ float get(int) const { return v; }
+};
+template <> struct Bits<uint16_t, 1> {
+    uint32_t v;
+    __device__ void load(const uint16_t* p) { v = *p; }
+    __device__ float get(int) const { return __uint_as_float(v << 16); }
+};
+template <> struct Bits<Fp8, 1> {
+    uint32_t v;
+    __device__ void load(const Fp8* p) { v = p->v; }
+    __device__ float get(int) const { return __builtin_amdgcn_cvt_f32_fp8((int)v, 0); }
+};
+
+// Rows in turn over the workgroups, WPR of the eight waves a row, R pieces a lane; the next row's loads are in flight over
+// each row.  w stays in LDS: with two rows and the columns' sums in registers it would be the part that does not fit.
+// A piece past the last column is read at the last whole one's place; its elements before `skip` belong to another lane.
+template <typename TD, typename TX, int R, int WPR, int W>
+__global__ __launch_bounds__(512, 2) void layer_norm_grad_kernel(NormGrad a) {
+    constexpr int WAVES = 8, ROWS = WAVES / WPR, PIECES = 64 * W, COLS = WPR * R * PIECES;
     constexpr int BUFS = ROWS > 1 ? ROWS / 2 : 1;  // half of the rows' sums of columns at a time
     __shared__ float2 part[2][WAVES];
     __shared__ __align__(16) float ws[COLS];
     __shared__ __align__(16) float cols[ROWS > 1 ? BUFS * 2 * COLS : 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int sub = wave / WPR, col0 = (wave % WPR) * (R * STEP) + lane * V;
+    const int sub = wave / WPR, first = (wave % WPR) * (R * PIECES), col0 = first + lane * W;
     const float inv = 1.f / (float)a.K;
     for (int c = tid; c < COLS; c += 512) ws[c] = c >= a.K ? 0.f : a.w ? a.w[c] : 1.f;
     __syncthreads();
+    struct Row {
+        Bits<TD, W> d[R];
+        Bits<TX, W> v[R];
+        uint32_t word[R];
+        float2 st;
+    };
+    auto place = [&](int i) __attribute__((always_inline)) { return min(col0 + i * PIECES, a.K - W); };
+    auto load = [&](Row& r, int64_t row) __attribute__((always_inline)) {
+        row = min(row, (int64_t)a.M - 1);
+        const TD* dy = reinterpret_cast<const TD*>(a.dy) + row * a.lddy;
+        const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            r.d[i].load(dy + place(i));
+            r.v[i].load(x + place(i));
+            if constexpr (sizeof(TX) == 1) {  // a wave's piece lies in one word's 512 columns
+                typedef const __attribute__((address_space(4))) uint32_t* constant_t;
+                const int group = min(first + i * PIECES, a.K - 1) >> 9;
+                r.word[i] = *((constant_t)a.xs + group * a.ld_xs + row);
+            }
+        }
+        r.st = a.stats[row];
+    };
     f32x4 dw[R], db[R];
 #pragma unroll
     for (int i = 0; i < R; i++) dw[i] = db[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int64_t step = (int64_t)gridDim.x * ROWS;
     int turn = 0;
-    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.M; row0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = row0 + sub;
+    auto work = [&](const Row& r, int64_t row) __attribute__((always_inline)) {
+        float2* at = part[turn & 1] + sub * WPR;
+        turn++;
         if (ROWS > 1 && row >= a.M) {
-            if constexpr (WPR > 1) {  // meets the barrier of the other rows' waves
-                float z0 = 0.f, z1 = 0.f;
-                row_sums<WPR>(z0, z1, part[turn & 1] + sub * WPR, wave % WPR);
-                turn++;
-            }
-            continue;
+            float z0 = 0.f, z1 = 0.f;
+            if constexpr (WPR > 1) row_sums<WPR>(z0, z1, at, wave % WPR);  // meets the barrier of the other rows' waves
+            return;
         }
-        const TD* dy = reinterpret_cast<const TD*>(a.dy) + row * a.lddy;
-        const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
-        Raw<TD> d[R];
-        Raw<TX> v[R];
-        float sc[R];
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            load_piece(d[i], dy, col0 + i * STEP, a.K);
-            load_piece(v[i], x, col0 + i * STEP, a.K);
-            sc[i] = 1.f;
-            if constexpr (sizeof(TX) == 1) {
-                const int block = (col0 + i * STEP) >> 7;
-                if (col0 + i * STEP < a.K) {
-                    const uint32_t b = a.xs[(block >> 2) * a.ld_xs + row] >> (8 * (block & 3)) & 0xff;
-                    sc[i] = __uint_as_float(b ? b << 23 : 0x400000u);  // 2^(b - 127)
-                }
-            }
-        }
-        const float2 st = a.stats[row];
-        auto hat = [&](int i, int j) __attribute__((always_inline)) {
-            return ((sizeof(TX) == 1 ? v[i].get(j) * sc[i] : v[i].get(j)) - st.x) * st.y;
-        };
+        float h[R][W], g[R][W];
         float sa = 0.f, sah = 0.f;
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(ws + col0 + i * STEP);
+            const int col = col0 + i * PIECES, skip = col - place(i);
+            float sc = 1.f;
+            if constexpr (sizeof(TX) == 1) {
+                const uint32_t b = r.word[i] >> (8 * ((min(col, a.K - 1) >> 7) & 3)) & 0xff;
+                sc = __uint_as_float(b ? b << 23 : 0x400000u);  // 2^(b - 127)
+            }
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float g = d[i].get(j), h = col0 + i * STEP + j < a.K ? hat(i, j) : 0.f;
-                const float aw = g * w[j];
-                dw[i][j] += g * h;
-                db[i][j] += g;
-                sa += aw;
-                sah += aw * h;
+            for (int j = 0; j < W; j++) {
+                const float xv = sizeof(TX) == 1 ? r.v[i].get(j) * sc : r.v[i].get(j);
+                h[i][j] = (xv - r.st.x) * r.st.y;
+                g[i][j] = r.d[i].get(j);
+                if (first + (i + 1) * PIECES > a.K && j < skip) h[i][j] = g[i][j] = 0.f;
+                dw[i][j] += g[i][j] * h[i][j];
+                db[i][j] += g[i][j];
+                g[i][j] *= ws[place(i) + j];
+                sa += g[i][j];
+                sah += g[i][j] * h[i][j];
             }
         }
-        row_sums<WPR>(sa, sah, part[turn & 1] + sub * WPR, wave % WPR);
-        turn++;
-        if (a.dx) {
-            const float ma = sa * inv, mah = sah * inv;
+        row_sums<WPR>(sa, sah, at, wave % WPR);
+        if (!a.dx) return;
+        const float ma = sa * inv, mah = sah * inv;
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int col = col0 + i * STEP;
-                if (col >= a.K) continue;
-                const f32x4 w = *reinterpret_cast<const f32x4*>(ws + col);
-                f32x4 o;
+        for (int i = 0; i < R; i++) {
+            const int col = col0 + i * PIECES, at = place(i);
+            f32x4 o;
 #pragma unroll
-                for (int j = 0; j < V; j++) o[j] = st.y * (d[i].get(j) * w[j] - ma - hat(i, j) * mah);
-                if (a.dx_f32) store_piece(reinterpret_cast<float*>(a.dx) + row * a.lddx + col, o, a.K - col);
-                else store_piece(reinterpret_cast<uint16_t*>(a.dx) + row * a.lddx + col, o, a.K - col);
+            for (int j = 0; j < W; j++) o[j] = r.st.y * (g[i][j] - ma - h[i][j] * mah);
+            if (W == 4 && col + W <= a.K) {
+                if (a.dx_f32) store_piece(reinterpret_cast<float*>(a.dx) + row * a.lddx + col, o, 4);
+                else store_piece(reinterpret_cast<uint16_t*>(a.dx) + row * a.lddx + col, o, 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    if (col >= a.K || at + j < col) continue;
+                    if (a.dx_f32) reinterpret_cast<float*>(a.dx)[row * a.lddx + at + j] = o[j];
+                    else reinterpret_cast<uint16_t*>(a.dx)[row * a.lddx + at + j] = (uint16_t)bf16x2_rne(o[j], o[j]);
+                }
             }
+        }
+    };
+    const int64_t row0 = (int64_t)blockIdx.x * ROWS;
+    if constexpr (R > 4) {  // the widest rows: one is all that registers hold
+        for (int64_t row = row0; row < a.M; row += step) {
+            Row r;
+            load(r, row + sub);
+            work(r, row + sub);
+        }
+    } else {
+        Row r0, r1;
+        load(r0, row0 + sub);
+        for (int64_t row = row0; row < a.M; row += 2 * step) {
+            load(r1, row + step + sub);
+            work(r0, row + sub);
+            if (row + step >= a.M) break;
+            load(r0, row + 2 * step + sub);
+            work(r1, row + step + sub);
         }
     }
     if (!a.part) return;
@@ -272,53 +345,57 @@ __global__ __launch_bounds__(512) void layer_norm_grad_kernel(NormGrad a) {
 #pragma unroll
     for (int n = ROWS; n > 1; n >>= 1) {
         __syncthreads();
-        float* at = cols + (sub % (n / 2)) * (2 * COLS) + col0;
+        float* at = cols + (sub % (n / 2)) * (2 * COLS) + (wave % WPR) * (R * PIECES);
         if (sub >= n / 2 && sub < n) {
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                *reinterpret_cast<f32x4*>(at + i * STEP) = dw[i];
-                *reinterpret_cast<f32x4*>(at + COLS + i * STEP) = db[i];
-            }
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    at[i * PIECES + j * 64 + lane] = dw[i][j];
+                    at[COLS + i * PIECES + j * 64 + lane] = db[i][j];
+                }
         }
         __syncthreads();
         if (sub < n / 2) {
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                dw[i] += *reinterpret_cast<const f32x4*>(at + i * STEP);
-                db[i] += *reinterpret_cast<const f32x4*>(at + COLS + i * STEP);
-            }
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    dw[i][j] += at[i * PIECES + j * 64 + lane];
+                    db[i][j] += at[COLS + i * PIECES + j * 64 + lane];
+                }
         }
     }
     if (sub) return;
     float* out = a.part + (int64_t)blockIdx.x * 2 * a.K;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int col = col0 + i * STEP;
+        const int col = col0 + i * PIECES;
 #pragma unroll
-        for (int j = 0; j < V; j++)
-            if (col + j < a.K) {
-                out[col + j] = dw[i][j];
-                out[a.K + col + j] = db[i][j];
+        for (int j = 0; j < W; j++)
+            if (col < a.K && place(i) + j >= col) {
+                out[place(i) + j] = dw[i][j];
+                out[a.K + place(i) + j] = db[i][j];
             }
     }
 }
 
-// dw and db from the workgroups' partial sums: 64 of the 2 K columns a workgroup, its four waves
-// a quarter of the rows each.
-__global__ __launch_bounds__(256) void norm_params_kernel(const float* part, int groups, int K, float* dw, float* db) {
-    __shared__ float sums[4][64];
+// dw and db from the workgroups' partial sums: 64 of the 2 K columns a workgroup, a part of the rows each of its 16 waves.
+__global__ __launch_bounds__(1024) void norm_params_kernel(const float* part, int groups, int K, float* dw, float* db) {
+    __shared__ float sums[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;
     float s = 0.f;
     if (c < 2 * K) {
-        const int per = (groups + 3) / 4, end = min((wave + 1) * per, groups);
+        const int per = (groups + 15) / 16, end = min((wave + 1) * per, groups);
 #pragma unroll 8
         for (int g = wave * per; g < end; g++) s += part[(int64_t)g * 2 * K + c];
     }
     sums[wave][lane] = s;
     __syncthreads();
     if (wave || c >= 2 * K) return;
-    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+#pragma unroll
+    for (int w = 1; w < 16; w++) s += sums[w][lane];
     if (c < K) {
         if (dw) dw[c] = s;
     } else if (db) {
@@ -352,22 +429,22 @@ void fwd_any(const NormFwd& a, hipStream_t s) {
     else fwd<TX, TY, 16, 4>(a, s);
 }
 
-template <typename TD, typename TX, int R, int WPR>
+template <typename TD, typename TX, int R, int WPR, int W = 4>
 void grad(const NormGrad& a, hipStream_t s) {
-    hipLaunchKernelGGL((layer_norm_grad_kernel<TD, TX, R, WPR>), dim3((unsigned)a.groups), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((layer_norm_grad_kernel<TD, TX, R, WPR, W>), dim3((unsigned)a.groups), dim3(512), 0, s, a);
 }
 template <typename TD, typename TX>
 void grad_any(const NormGrad& a, hipStream_t s) {
     const int n = (a.K + STEP - 1) / STEP;
-    if (n <= 2) grad<TD, TX, 2, 1>(a, s);
+    if (a.K < 4) grad<TD, TX, 1, 1, 1>(a, s);
+    else if (n <= 2) grad<TD, TX, 2, 1>(a, s);
     else if (n <= 4) grad<TD, TX, 4, 1>(a, s);
     else if (n <= 6) grad<TD, TX, 3, 2>(a, s);
     else if (n <= 8) grad<TD, TX, 4, 2>(a, s);
-    else if (n <= 10) grad<TD, TX, 5, 2>(a, s);
-    else if (n <= 12) grad<TD, TX, 6, 2>(a, s);
+    else if (n <= 12) grad<TD, TX, 3, 4>(a, s);
     else if (n <= 16) grad<TD, TX, 4, 4>(a, s);
-    else if (n <= 24) grad<TD, TX, 6, 4>(a, s);
-    else if (n <= 32) grad<TD, TX, 8, 4>(a, s);
+    else if (n <= 24) grad<TD, TX, 3, 8>(a, s);
+    else if (n <= 32) grad<TD, TX, 4, 8>(a, s);
     else if (n <= 48) grad<TD, TX, 6, 8>(a, s);
     else grad<TD, TX, 8, 8>(a, s);
 }
@@ -381,7 +458,7 @@ void grad_in(int dtype_x, const NormGrad& a, hipStream_t s) {
 // rows that a workgroup of the gradient takes at once
 int rows_at_once(int K) {
     const int n = (K + STEP - 1) / STEP;
-    return n <= 4 ? 8 : n <= 12 ? 4 : n <= 32 ? 2 : 1;
+    return n <= 4 ? 8 : n <= 8 ? 4 : n <= 16 ? 2 : 1;
 }
 
 }  // namespace
@@ -411,7 +488,7 @@ hipError_t launch_layer_norm_grad(int dtype_dy, int dtype_x, const NormGrad& a, 
     else grad_in<uint16_t>(dtype_x, a, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.part) return e;
-    hipLaunchKernelGGL(norm_params_kernel, dim3((unsigned)((2 * a.K + 63) / 64)), dim3(256), 0, s, a.part, a.groups, a.K, a.dw, a.db);
+    hipLaunchKernelGGL(norm_params_kernel, dim3((unsigned)((2 * a.K + 63) / 64)), dim3(1024), 0, s, a.part, a.groups, a.K, a.dw, a.db);
     return hipGetLastError();
 }
 
