@@ -19,14 +19,14 @@ using namespace cross;
 
 namespace {
 
-template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD>
-__global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) void cross_queries_kernel(CrossArgs p) {
+template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD, bool ONE>
+__global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 : 2) : 1)) void cross_queries_kernel(CrossArgs p) {
     using Frag = typename T::Frag;
     using L = Tile<T, DP>;
     constexpr int KS = DP / 32, DB = DP / 16, KB = KT / 16, WAVES = WQ * WK;
     constexpr int TILE_B = KT * L::ROW, STAGE = 2 * TILE_B;  // K, then V
     constexpr int JOIN = WK > 1 ? WAVES * NQ * 16 * (DP + 2) * 4 : 0;
-    constexpr int LDS = WK * 2 * STAGE > JOIN ? WK * 2 * STAGE : JOIN;
+    constexpr int RING = WK * (ONE ? 1 : 2) * STAGE, LDS = RING > JOIN ? RING : JOIN;
     static_assert(LDS <= 160 * 1024 && (WQ == 1 || WK == 1), "LDS");
     __shared__ __align__(16) char lds[LDS];
     const int groups = p.heads / p.qs.pack, total = p.qs.n_items * groups;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) vo
     auto valid_of = [&](int t, int byte) __attribute__((always_inline)) {
         return __builtin_amdgcn_ballot_w64(lane < KT && t * KT + lane < it.kn && byte);
     };
-    char* ring = lds + wk * 2 * STAGE;
+    char* ring = lds + wk * (ONE ? 1 : 2) * STAGE;
     auto fetch = [&](int t, int slot, uint64_t valid) __attribute__((always_inline)) {
         const int64_t first = it.k0 + (int64_t)t * KT;
         const __amdgpu_buffer_rsrc_t kr = uniform_rsrc(p.k + kv_head * p.k_head + first * p.k_row, 0x7fffffffu);
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) vo
         if constexpr (WQ > 1) __syncthreads();
         const uint64_t next = valid_of(t + WK, byte);
         byte = mask_byte(t + 2 * WK);
-        if (t + WK < tiles) fetch(t + WK, slot ^ 1, next);
+        if (!ONE && t + WK < tiles) fetch(t + WK, slot ^ 1, next);
         const char* kt = ring + slot * STAGE;
         const char* vt = kt + TILE_B;
 
@@ -214,6 +214,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) vo
             }
         }
         valid = next;
+        if constexpr (ONE) break;
     }
 
     const int d = p.head_d;
@@ -225,15 +226,19 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? 2 : 1)) vo
     if constexpr (WK == 1) {
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
-            if (!there[j]) continue;
             const int c = (wq * NQ + j) * 16 + (lane & 15);
-            const float f = part ? 1.f : GRAD ? p.scale : sum[j] > 0.f || sum[j] != sum[j] ? 1.f / sum[j] : 0.f;
+            if (part) {
+                if (!there[j]) continue;
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                const int ch = 16 * db + 4 * g;
-                if (ch >= d) continue;
-                if (part) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = acc[db][j];
-                else T::store4(to + row[j] * to_row + head[j] * to_head + ch * T::SIZE, acc[db][j] * f);
+                for (int db = 0; db < DB; db++)
+                    if (16 * db + 4 * g < d) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + 16 * db + 4 * g) = acc[db][j];
+            } else {
+                const float f = GRAD ? p.scale : sum[j] > 0.f || sum[j] != sum[j] ? 1.f / sum[j] : 0.f;
+                // lanes exchange channels before the ones of no column drop out
+#pragma unroll
+                for (int db = 0; db < DB; db += 2)
+                    T::store_blocks(to + row[j] * to_row + head[j] * to_head, db, g, there[j] ? d : 0, acc[db][j] * f, acc[db + 1][j] * f);
+                if (!there[j]) continue;
             }
             if (!GRAD && g == 0) {
                 if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){top[j], sum[j]};
@@ -314,15 +319,16 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
     }
 }
 
-template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD>
+template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD, bool ONE = false>
 void run(const CrossArgs& a, hipStream_t s) {
     const long total = (long)a.qs.n_items * (a.heads / a.qs.pack);
-    hipLaunchKernelGGL((cross_queries_kernel<T, DP, NQ, WQ, WK, KT, GRAD>), dim3(xcd_grid(total)), dim3(64 * WQ * WK), 0, s, a);
+    hipLaunchKernelGGL((cross_queries_kernel<T, DP, NQ, WQ, WK, KT, GRAD, ONE>), dim3(xcd_grid(total)), dim3(64 * WQ * WK), 0, s, a);
 }
 template <typename T, int DP, bool GRAD>
 void run_block(const CrossArgs& a, hipStream_t s) {
     constexpr int WK = T::SIZE == 2 ? 4 : 2;
-    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 && !GRAD ? 64 : 32, GRAD>(a, s);
+    if (a.qs.block == 128 && T::SIZE == 2 && a.qs.most_keys <= 64) run<T, DP, 2, 4, 1, 64, GRAD, true>(a, s);
+    else if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 && !GRAD ? 64 : 32, GRAD>(a, s);
     else if (a.qs.block == 32) run<T, DP, 2, 1, WK, 32, GRAD>(a, s);
     else run<T, DP, 1, 1, WK, 32, GRAD>(a, s);
 }

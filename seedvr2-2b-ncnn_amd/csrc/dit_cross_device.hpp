@@ -45,6 +45,15 @@ struct Bf16 {
     static __device__ inline void store4(char* p, const f32x4& v) {
         *reinterpret_cast<uint2*>(p) = make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
     }
+    // Two neighbouring blocks of 16 channels of a row whose lane 16 g + i holds channels 4 g .. 4 g + 3 of both: neighbouring
+    // lane groups exchange halves, so that each stores 16 bytes and the four 64 in a row (one after the other at 8 bytes
+    // a lane, 16384 queries x 128 keys x 20 heads take 52 us, so 46).
+    static __device__ inline void store_blocks(char* row, int db, int g, int d, const f32x4& a, const f32x4& b) {
+        const auto x = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[0], a[1]), bf16x2_rne(b[0], b[1]), false, false);
+        const auto y = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[2], a[3]), bf16x2_rne(b[2], b[3]), false, false);
+        const int ch = 16 * (db + (g & 1)) + 8 * (g >> 1);
+        if (ch < d) *reinterpret_cast<u32x4*>(row + 2 * ch) = (u32x4){x[0], y[0], x[1], y[1]};
+    }
 };
 struct F32 {
     static constexpr int SIZE = 4;
@@ -70,6 +79,11 @@ struct F32 {
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     static __device__ inline void store4(char* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+    static __device__ inline void store_blocks(char* row, int db, int g, int d, const f32x4& a, const f32x4& b) {
+        const int ch = 16 * db + 4 * g;
+        if (ch < d) store4(row + 4 * ch, a);
+        if (ch + 16 < d) store4(row + 4 * (ch + 16), b);
+    }
 };
 
 // One LDS DMA instruction, 16 (4) bytes a lane to LDS at `to` + 16 (4) x lane from byte offset `at` of the resource.  From

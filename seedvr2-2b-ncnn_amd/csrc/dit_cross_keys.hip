@@ -196,22 +196,25 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
         // the lane counted anew: kept over the loop, what follows from it would cost registers there
         const int own = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
         const int c = (wk * NK + j) * 16 + (own & 15), ch0 = 4 * (own >> 4);
-        if (c >= it.kn) continue;
+        const bool there = c < it.kn;
         char* kp = p.dk + (int64_t)(it.k0 + c) * p.dk_row + kv_head * p.dk_head;
         char* vp = p.dv + (int64_t)(it.k0 + c) * p.dv_row + kv_head * p.dv_head;
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int db = 0; db < DB; db++) {
+            dk[db][j] = in[j] ? dk[db][j] * p.scale : z;
+            dv[db][j] = in[j] ? dv[db][j] : z;
             const int ch = 16 * db + ch0;
-            if (ch >= d) continue;
-            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            const f32x4 a = in[j] ? dk[db][j] * p.scale : z, b = in[j] ? dv[db][j] : z;
-            if (part) {
-                *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = a;
-                *reinterpret_cast<f32x4*>(part + (int64_t)(CROSS_KEYS + c) * d + ch) = b;
-            } else {
-                T::store4(kp + ch * T::SIZE, a);
-                T::store4(vp + ch * T::SIZE, b);
+            if (part && there && ch < d) {
+                *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = dk[db][j];
+                *reinterpret_cast<f32x4*>(part + (int64_t)(CROSS_KEYS + c) * d + ch) = dv[db][j];
             }
+        }
+        if (part) continue;
+#pragma unroll
+        for (int db = 0; db < DB; db += 2) {
+            T::store_blocks(kp, db, own >> 4, there ? d : 0, dk[db][j], dk[db + 1][j]);
+            T::store_blocks(vp, db, own >> 4, there ? d : 0, dv[db][j], dv[db + 1][j]);
         }
     }
 }

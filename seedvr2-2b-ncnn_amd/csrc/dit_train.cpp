@@ -136,6 +136,7 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
                 it.kn = (int)std::min(run, kl[i] - c * run);
                 it.part = parts > 1 ? first + c : -1;
                 it.first = c == 0;
+                s.most_keys = std::max(s.most_keys, it.kn);
                 p.items.push_back(it);
             }
             if (parts > 1) {

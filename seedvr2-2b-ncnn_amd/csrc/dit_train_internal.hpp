@@ -101,6 +101,7 @@ struct CrossKeyJoin {
 // One of the two forms of a plan's query side.
 struct CrossQueries {
     int pack = 1, block = 0;  // heads in a block, columns of a block
+    int most_keys = 0;        // of an item
     int n_items = 0, n_joins = 0, n_parts = 0;
     const CrossItem* items = nullptr;
     const CrossJoin* joins = nullptr;
