@@ -39,6 +39,36 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
     const int head0 = hb * p.qs.pack, kv_head = head0 / (p.heads / p.kv_heads);
     const int width = p.head_d * T::SIZE;
 
+    const int tiles = (it.kn + KT - 1) / KT;
+    const uint8_t* mask = p.mask ? p.mask + it.k0 : nullptr;
+    auto mask_byte = [&](int t) __attribute__((always_inline)) {
+        const int key = t * KT + lane;
+        return mask && lane < KT && key < it.kn ? (int)mask[key] : 1;
+    };
+    auto valid_of = [&](int t, int byte) __attribute__((always_inline)) {
+        return __builtin_amdgcn_ballot_w64(lane < KT && t * KT + lane < it.kn && byte);
+    };
+    char* ring = lds + wk * (ONE ? 1 : 2) * STAGE;
+    auto fetch = [&](int t, int slot, uint64_t valid) __attribute__((always_inline)) {
+        const int64_t first = it.k0 + (int64_t)t * KT;
+        const __amdgpu_buffer_rsrc_t kr = uniform_rsrc(p.k + kv_head * p.k_head + first * p.k_row, 0x7fffffffu);
+        const __amdgpu_buffer_rsrc_t vr = uniform_rsrc(p.v + kv_head * p.v_head + first * p.v_row, 0x7fffffffu);
+        char* st = ring + slot * STAGE;
+        constexpr int N = TILE_B / 1024;
+#pragma unroll
+        for (int i = 0; i < N / WQ; i++) {
+            L::dma(st, wq * (N / WQ) + i, kr, p.k_row, valid, width, lane);
+            L::dma(st + TILE_B, wq * (N / WQ) + i, vr, p.v_row, valid, width, lane);
+        }
+    };
+    // the first tile is on its way before the queries are asked for
+    uint64_t valid = 0;
+    int byte = 1;
+    if (wk < tiles) {
+        valid = valid_of(wk, mask_byte(wk));
+        byte = mask_byte(wk + WK);
+        fetch(wk, 0, valid);
+    }
     // the wave's columns
     int row[NQ], head[NQ];
     bool there[NQ];
@@ -48,23 +78,48 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
     for (int j = 0; j < NQ; j++) {
         const int c = (wq * NQ + j) * 16 + (lane & 15);
         there[j] = c < it.cols;
-        row[j] = it.q0 + c / p.qs.pack;
-        head[j] = head0 + c % p.qs.pack;
-        const char* at = p.q + row[j] * p.q_row + head[j] * p.q_head;
-        const char* dat = p.dout + row[j] * p.dout_row + head[j] * p.dout_head;
-        const char* oat = p.out + row[j] * p.out_row + head[j] * p.out_head;
+        row[j] = it.q0 + c;
+        head[j] = head0;
+        if constexpr (WQ == 1) {  // heads that share their keys
+            row[j] = it.q0 + c / p.qs.pack;
+            head[j] = head0 + c % p.qs.pack;
+        }
         lse2[j] = dsum[j] = 0.f;
+        // One head's rows: columns and channels that are not there lie past resources, without branches (16384 queries x 64
+        // keys: gradients 112 us with them, 109 so; the forward pass, which loads a third, gains nothing).
+        if constexpr (WQ > 1 && GRAD) {
+            const __amdgpu_buffer_rsrc_t qr = uniform_rsrc(p.q + it.q0 * p.q_row + head0 * p.q_head, 0x7fffffffu);
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int d = 32 * ks + 8 * g;
-            const bool in = there[j] && d < p.head_d;
-            q[j][ks] = T::zero();
-            if (in) q[j][ks] = T::load(at + d * T::SIZE);
-            if constexpr (GRAD) {
-                dout[j][ks] = T::zero();
-                if (in) {
-                    dout[j][ks] = T::load(dat + d * T::SIZE);
-                    dsum[j] += T::dot(dout[j][ks], T::load(oat + d * T::SIZE));
+            for (int ks = 0; ks < KS; ks++) {
+                const int d = 32 * ks + 8 * g;
+                const bool in = there[j] && d < p.head_d;
+                q[j][ks] = buffer_frag<T>(qr, in ? (uint32_t)c * (uint32_t)p.q_row + d * T::SIZE : 0x80000000u);
+            }
+            const __amdgpu_buffer_rsrc_t dr = uniform_rsrc(p.dout + it.q0 * p.dout_row + head0 * p.dout_head, 0x7fffffffu);
+            const __amdgpu_buffer_rsrc_t orr = uniform_rsrc(p.out + it.q0 * p.out_row + head0 * p.out_head, 0x7fffffffu);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const int d = 32 * ks + 8 * g;
+                const bool in = there[j] && d < p.head_d;
+                dout[j][ks] = buffer_frag<T>(dr, in ? (uint32_t)c * (uint32_t)p.dout_row + d * T::SIZE : 0x80000000u);
+                dsum[j] += T::dot(dout[j][ks], buffer_frag<T>(orr, in ? (uint32_t)c * (uint32_t)p.out_row + d * T::SIZE : 0x80000000u));
+            }
+        } else {
+            const char* at = p.q + row[j] * p.q_row + head[j] * p.q_head;
+            const char* dat = p.dout + row[j] * p.dout_row + head[j] * p.dout_head;
+            const char* oat = p.out + row[j] * p.out_row + head[j] * p.out_head;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const int d = 32 * ks + 8 * g;
+                const bool in = there[j] && d < p.head_d;
+                q[j][ks] = T::zero();
+                if (in) q[j][ks] = T::load(at + d * T::SIZE);
+                if constexpr (GRAD) {
+                    dout[j][ks] = T::zero();
+                    if (in) {
+                        dout[j][ks] = T::load(dat + d * T::SIZE);
+                        dsum[j] += T::dot(dout[j][ks], T::load(oat + d * T::SIZE));
+                    }
                 }
             }
         }
@@ -97,35 +152,6 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
         for (int db = 0; db < DB; db++) acc[db][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
 
-    const int tiles = (it.kn + KT - 1) / KT;
-    const uint8_t* mask = p.mask ? p.mask + it.k0 : nullptr;
-    auto mask_byte = [&](int t) __attribute__((always_inline)) {
-        const int key = t * KT + lane;
-        return mask && lane < KT && key < it.kn ? (int)mask[key] : 1;
-    };
-    auto valid_of = [&](int t, int byte) __attribute__((always_inline)) {
-        return __builtin_amdgcn_ballot_w64(lane < KT && t * KT + lane < it.kn && byte);
-    };
-    char* ring = lds + wk * (ONE ? 1 : 2) * STAGE;
-    auto fetch = [&](int t, int slot, uint64_t valid) __attribute__((always_inline)) {
-        const int64_t first = it.k0 + (int64_t)t * KT;
-        const __amdgpu_buffer_rsrc_t kr = uniform_rsrc(p.k + kv_head * p.k_head + first * p.k_row, 0x7fffffffu);
-        const __amdgpu_buffer_rsrc_t vr = uniform_rsrc(p.v + kv_head * p.v_head + first * p.v_row, 0x7fffffffu);
-        char* st = ring + slot * STAGE;
-        constexpr int N = TILE_B / 1024;
-#pragma unroll
-        for (int i = 0; i < N / WQ; i++) {
-            L::dma(st, wq * (N / WQ) + i, kr, p.k_row, valid, width, lane);
-            L::dma(st + TILE_B, wq * (N / WQ) + i, vr, p.v_row, valid, width, lane);
-        }
-    };
-    uint64_t valid = 0;
-    int byte = 1;
-    if (wk < tiles) {
-        valid = valid_of(wk, mask_byte(wk));
-        byte = mask_byte(wk + WK);
-        fetch(wk, 0, valid);
-    }
     int slot = 0;
     for (int t = wk; t < tiles; t += WK, slot ^= 1) {
         wait_vmem_lds<0>();  // this tile has landed (and what was read of the other slot has arrived)
@@ -186,8 +212,10 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
                     const float fade = exp2_of(top[j] * p.c - (m == -INFINITY ? 0.f : m * p.c));
                     top[j] = m;
                     sum[j] *= fade;
+                    if constexpr (!ONE) {
 #pragma unroll
-                    for (int db = 0; db < DB; db++) acc[db][j] *= fade;
+                        for (int db = 0; db < DB; db++) acc[db][j] *= fade;
+                    }
                 }
                 const float ref = top[j] == -INFINITY ? 0.f : top[j] * p.c;
                 float add = 0.f;

@@ -108,6 +108,18 @@ __device__ inline void dma4(const void* to, __amdgpu_buffer_rsrc_t from, uint32_
 }
 #pragma clang diagnostic pop
 
+// Eight channels at byte offset `at` of a resource (zeros past it)
+template <typename T>
+__device__ inline typename T::Frag buffer_frag(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+    const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+    if constexpr (T::SIZE == 2) {
+        return __builtin_bit_cast(typename T::Frag, lo);
+    } else {
+        const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(from, at + 16, 0, 0);
+        return __builtin_shufflevector(__builtin_bit_cast(f32x4, lo), __builtin_bit_cast(f32x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
 // An LDS tile: rows of 64 or 128 channels (DP = 96 has rows of 128, whose last channels nothing reads), 16-byte
 // chunk c of row r at chunk c ^ swizzle(r).  LDS answers 256 bytes a cycle from 64 banks, so the 16 rows that read one
 // chunk together, and the eight rows that 32 lanes of a transposed read (four rows that 64 lanes of fp32 columns) take two
