@@ -320,11 +320,12 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
     const int groups = p.heads / p.qs.pack, hb = blockIdx.x / p.qs.n_joins;
-    const CrossJoin it = p.qs.joins[blockIdx.x - hb * p.qs.n_joins];
+    const CrossJoin it = table_entry(p.qs.joins, blockIdx.x - hb * p.qs.n_joins);
     const int d = p.head_d, pieces = d / 4;
     const int64_t stride = (int64_t)groups * cross_query_part(p.qs.block, d);
     const float* first = p.qpart + ((int64_t)it.part0 * groups + hb) * cross_query_part(p.qs.block, d);
-    for (int e = threadIdx.x; e < it.cols * pieces; e += 256) {
+    const int e = blockIdx.y * 256 + threadIdx.x;
+    if (e < it.cols * pieces) {
         const int c = e / pieces, ch = e % pieces * 4;
         const float* o = first + (int64_t)c * d + ch;
         const float* ml = first + (int64_t)p.qs.block * d + 2 * c;
@@ -333,6 +334,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
             for (int i = 0; i < it.parts; i++) m = fmaxf(m, ml[i * stride]);
         const float ref = m == -INFINITY ? 0.f : m * p.c;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int i = 0; i < it.parts; i++) {
             const float f = GRAD ? 1.f : exp2_of(ml[i * stride] * p.c - ref);
             v += *reinterpret_cast<const f32x4*>(o + i * stride) * f;
@@ -368,7 +370,8 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
     else run_block<T, 128, GRAD>(a, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.qs.n_joins == 0) return e;
-    hipLaunchKernelGGL((cross_join_kernel<T, GRAD>), dim3((unsigned)(a.qs.n_joins * (a.heads / a.qs.pack))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((cross_join_kernel<T, GRAD>), dim3((unsigned)(a.qs.n_joins * (a.heads / a.qs.pack)), (unsigned)((a.qs.block * (a.head_d / 4) + 255) / 256)),
+                       dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

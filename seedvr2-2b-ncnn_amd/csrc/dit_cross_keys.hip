@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
 template <typename T>
 __global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
     const int kv_head = blockIdx.x / p.ks.n_joins;
-    const CrossKeyJoin it = p.ks.joins[blockIdx.x - kv_head * p.ks.n_joins];
+    const CrossKeyJoin it = table_entry(p.ks.joins, blockIdx.x - kv_head * p.ks.n_joins);
     const int d = p.head_d, pieces = d / 4, e = blockIdx.y * 256 + threadIdx.x;
     if (e >= 2 * it.kn * pieces) return;
     const int64_t size = cross_key_part(CROSS_KEYS, d), stride = p.kv_heads * size;

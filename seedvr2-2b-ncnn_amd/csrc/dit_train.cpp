@@ -15,8 +15,9 @@ struct dit_cross {
     int heads = 0, kv_heads = 0, head_d = 0;
     int64_t q_rows = 0, k_rows = 0;  // past the last row of any sequence
     void* tables = nullptr;
-    CrossQueries qs;
-    CrossKeySide ks;
+    // for AWA_F32 and AWA_BF16, whose work is worth dividing differently
+    CrossQueries qs[2];
+    CrossKeySide ks[2];
 };
 
 namespace {
@@ -108,7 +109,7 @@ int64_t runs_of(const std::map<int64_t, int64_t>& blocks, const Cost& c) {
 }
 
 void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
-                  const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, CrossQueries& s, Plan& p) {
+                  const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, int dtype, CrossQueries& s, Plan& p) {
     const int per = heads / kv_heads;
     int64_t most = per;
     for (int64_t n : ql) most = std::max(most, n * per);
@@ -116,13 +117,16 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
     s.block = most <= 16 ? 16 : most <= 32 ? 32 : 128;
     s.pack = s.block < 128 ? per : 1;
     const int rows = s.block / s.pack;
-    // A step is 64 keys, or 128 for the four waves of a block of few columns.  Measured, heads of 128 channels in bf16: a
-    // block of 128 columns takes 6 us and 1.6 a step where two share a CU; one of few columns 4 us and 1.5 a step.
+    // A step is 64 keys, or 128 for the waves of a block of few columns.  Measured with heads of 128 channels: in bf16 a
+    // block of 128 columns takes 6 us and 1.6 a step where two share a CU, one of few columns 4 us and 1.5 a step; in fp32,
+    // one workgroup a CU, 8 us and 8 a step, and 4 us and 3.
     const int64_t groups = heads / s.pack, step = s.block < 128 ? 128 : 64;
     std::map<int64_t, int64_t> made;
     for (size_t i = 0; i < ql.size(); i++)
         if (ql[i]) made[ceil_div(kl[i], step)] += ceil_div(ql[i], rows) * groups;
-    const Cost cost{s.block < 128 ? 256 : 512, s.block < 128 ? 4.0 : 6.0, s.block < 128 ? 1.5 : 1.6, 5.0, 4.0 * s.block * head_d};
+    const bool few = s.block < 128, f32 = dtype == AWA_F32;
+    const Cost cost{few || f32 ? 256 : 512, few ? 4.0 : f32 ? 8.0 : 6.0, few ? (f32 ? 3.0 : 1.5) : f32 ? 8.0 : 1.6, 5.0,
+                    4.0 * s.block * head_d};
     const int64_t run = runs_of(made, cost) * step;
     for (size_t i = 0; i < ql.size(); i++) {
         for (int64_t r = 0; r < ql[i]; r += rows) {
@@ -150,20 +154,21 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
 }
 
 void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
-               const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, CrossKeySide& s, Plan& p) {
+               const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, int dtype, CrossKeySide& s, Plan& p) {
     const int per = heads / kv_heads;
     // sequences by their keys
     std::map<int64_t, std::vector<size_t>> shared;
     for (size_t i = 0; i < kl.size(); i++)
         if (kl[i]) shared[ka[i]].push_back(i);
-    // A step is a unit.  Measured as above: a block takes 5 us and 2 a unit where two share a CU.
+    // A step is a unit.  Measured as above: in bf16 a block takes 5 us and 2 a unit where two share a CU, in fp32 8 and 8.
     std::map<int64_t, int64_t> made;
     for (auto& e : shared) {
         int64_t units = 0;
         for (size_t i : e.second) units += ceil_div(ql[i], CROSS_QT);
         made[units * per] += ceil_div(kl[e.second[0]], CROSS_KEYS) * kv_heads;
     }
-    const int64_t run = runs_of(made, {512, 5.0, 2.0, 5.0, 8.0 * CROSS_KEYS * head_d});
+    const int64_t run = runs_of(made, dtype == AWA_F32 ? Cost{256, 8.0, 8.0, 5.0, 8.0 * CROSS_KEYS * head_d}
+                                                        : Cost{512, 5.0, 2.0, 5.0, 8.0 * CROSS_KEYS * head_d});
     for (auto& e : shared) {
         const int unit0 = (int)p.units.size();
         for (size_t i : e.second)
@@ -234,7 +239,6 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
         set_err(ctx, "dit_cross_create: query rows of two sequences overlap, or key rows do and are not the same");
         return AWA_EARG;
     }
-    Plan p;
     dit_cross c;
     c.device = ctx->device;
     c.heads = heads;
@@ -242,25 +246,29 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
     c.head_d = head_d;
     c.q_rows = q_rows;
     c.k_rows = k_rows;
-    plan_queries(qa, ql, ka, kl, heads, kv_heads, head_d, c.qs, p);
-    plan_keys(qa, ql, ka, kl, heads, kv_heads, head_d, c.ks, p);
-    // grids are a workgroup per item and head
-    if ((int64_t)c.qs.n_items * heads > 0x7fffff00 || (int64_t)c.ks.n_items * heads > 0x7fffff00) {
-        set_err(ctx, "dit_cross_create: too many blocks for one launch");
-        return AWA_EARG;
-    }
     std::vector<char> host;
+    size_t at[2][5];
     auto add = [&](const void* from, size_t bytes) {
-        const size_t at = host.size();
-        host.resize(at + (bytes + 15) / 16 * 16);
-        if (bytes) std::copy_n(static_cast<const char*>(from), bytes, host.data() + at);
-        return at;
+        const size_t to = host.size();
+        host.resize(to + (bytes + 15) / 16 * 16);
+        if (bytes) std::copy_n(static_cast<const char*>(from), bytes, host.data() + to);
+        return to;
     };
-    const size_t items = add(p.items.data(), p.items.size() * sizeof(CrossItem));
-    const size_t joins = add(p.joins.data(), p.joins.size() * sizeof(CrossJoin));
-    const size_t kitems = add(p.kitems.data(), p.kitems.size() * sizeof(CrossKeys));
-    const size_t kjoins = add(p.kjoins.data(), p.kjoins.size() * sizeof(CrossKeyJoin));
-    const size_t units = add(p.units.data(), p.units.size() * sizeof(CrossUnit));
+    for (int t = 0; t < 2; t++) {
+        Plan p;
+        plan_queries(qa, ql, ka, kl, heads, kv_heads, head_d, t, c.qs[t], p);
+        plan_keys(qa, ql, ka, kl, heads, kv_heads, head_d, t, c.ks[t], p);
+        // grids are a workgroup per item and head
+        if ((int64_t)c.qs[t].n_items * heads > 0x7fffff00 || (int64_t)c.ks[t].n_items * heads > 0x7fffff00) {
+            set_err(ctx, "dit_cross_create: too many blocks for one launch");
+            return AWA_EARG;
+        }
+        at[t][0] = add(p.items.data(), p.items.size() * sizeof(CrossItem));
+        at[t][1] = add(p.joins.data(), p.joins.size() * sizeof(CrossJoin));
+        at[t][2] = add(p.kitems.data(), p.kitems.size() * sizeof(CrossKeys));
+        at[t][3] = add(p.kjoins.data(), p.kjoins.size() * sizeof(CrossKeyJoin));
+        at[t][4] = add(p.units.data(), p.units.size() * sizeof(CrossUnit));
+    }
     dit_cross* made = new dit_cross(c);
     if (!host.empty()) {
         DeviceGuard dg(ctx->device);
@@ -274,11 +282,13 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
         }
     }
     const char* base = static_cast<const char*>(made->tables);
-    made->qs.items = reinterpret_cast<const CrossItem*>(base + items);
-    made->qs.joins = reinterpret_cast<const CrossJoin*>(base + joins);
-    made->ks.items = reinterpret_cast<const CrossKeys*>(base + kitems);
-    made->ks.joins = reinterpret_cast<const CrossKeyJoin*>(base + kjoins);
-    made->ks.units = reinterpret_cast<const CrossUnit*>(base + units);
+    for (int t = 0; t < 2; t++) {
+        made->qs[t].items = reinterpret_cast<const CrossItem*>(base + at[t][0]);
+        made->qs[t].joins = reinterpret_cast<const CrossJoin*>(base + at[t][1]);
+        made->ks[t].items = reinterpret_cast<const CrossKeys*>(base + at[t][2]);
+        made->ks[t].joins = reinterpret_cast<const CrossKeyJoin*>(base + at[t][3]);
+        made->ks[t].units = reinterpret_cast<const CrossUnit*>(base + at[t][4]);
+    }
     *out = made;
     return AWA_OK;
 }
@@ -287,7 +297,9 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
 struct CrossWork {
     int64_t qpart, kpart, dsum, lse2, total;
 };
-CrossWork cross_work(const dit_cross& c, bool grad) {
+CrossWork cross_work(const dit_cross& c, int dtype, bool grad) {
+    const CrossQueries& qs = c.qs[dtype];
+    const CrossKeySide& ks = c.ks[dtype];
     CrossWork w{};
     int64_t at = 0;
     auto take = [&](int64_t floats) {
@@ -295,9 +307,9 @@ CrossWork cross_work(const dit_cross& c, bool grad) {
         at += align_up(4 * floats);
         return p;
     };
-    w.qpart = take((int64_t)c.qs.n_parts * (c.heads / c.qs.pack) * cross_query_part(c.qs.block, c.head_d));
+    w.qpart = take((int64_t)qs.n_parts * (c.heads / qs.pack) * cross_query_part(qs.block, c.head_d));
     if (grad) {
-        w.kpart = take((int64_t)c.ks.n_parts * c.kv_heads * cross_key_part(CROSS_KEYS, c.head_d));
+        w.kpart = take((int64_t)ks.n_parts * c.kv_heads * cross_key_part(CROSS_KEYS, c.head_d));
         w.dsum = take((int64_t)c.heads * c.q_rows);
         w.lse2 = take((int64_t)c.heads * c.q_rows);
     }
@@ -539,7 +551,7 @@ void dit_cross_destroy(dit_cross* plan) {
 
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad) {
     if (!plan || !dtype_ok(dtype)) return AWA_EARG;
-    return cross_work(*plan, grad != 0).total;
+    return cross_work(*plan, dtype, grad != 0).total;
 }
 
 int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_heads* q, const dit_heads* k,
@@ -561,7 +573,7 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
         set_err(ctx, "%s: d_lse must be 4-byte aligned", who);
         return AWA_EARG;
     }
-    const CrossWork w = cross_work(*plan, false);
+    const CrossWork w = cross_work(*plan, dtype, false);
     if (int rc = work_ok(ctx, who, d_work, work_bytes, w.total)) return rc;
     const Extent lse{d_lse, d_lse ? span(h, ld_lse, qr, 4) : 0}, wk{d_work, (size_t)w.total}, mask{d_mask, (size_t)kr};
     const Extent eo = extent(out, dtype, qr, h, d), eq = extent(q, dtype, qr, h, d), ek = extent(k, dtype, kr, hk, d),
@@ -582,7 +594,7 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
     a.lse = d_lse;
     a.ld_lse = ld_lse;
     a.heads = h; a.kv_heads = hk; a.head_d = d;
-    a.qs = plan->qs; a.ks = plan->ks;
+    a.qs = plan->qs[dtype]; a.ks = plan->ks[dtype];
     a.qpart = reinterpret_cast<float*>(static_cast<char*>(d_work) + w.qpart);
     DeviceGuard dg(ctx->device);
     HIPCK(ctx, launch_cross_forward(dtype, a, reinterpret_cast<hipStream_t>(stream)));
@@ -613,7 +625,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
         set_err(ctx, "%s: d_lse must not be NULL, and 4-byte aligned", who);
         return AWA_EARG;
     }
-    const CrossWork w = cross_work(*plan, true);
+    const CrossWork w = cross_work(*plan, dtype, true);
     if (int rc = work_ok(ctx, who, d_work, work_bytes, w.total)) return rc;
     const Extent lse{d_lse, qr ? span(h, ld_lse, qr, 4) : 0}, wk{d_work, (size_t)w.total}, mask{d_mask, (size_t)kr};
     bool bad = touches(wk, lse) || touches(wk, mask);
@@ -644,7 +656,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
     a.lse = const_cast<float*>(d_lse);
     a.ld_lse = ld_lse;
     a.heads = h; a.kv_heads = hk; a.head_d = d;
-    a.qs = plan->qs; a.ks = plan->ks;
+    a.qs = plan->qs[dtype]; a.ks = plan->ks[dtype];
     char* base = static_cast<char*>(d_work);
     a.qpart = reinterpret_cast<float*>(base + w.qpart);
     a.kpart = reinterpret_cast<float*>(base + w.kpart);

@@ -56,12 +56,12 @@ static void hold(const char* what, bool ok) {
 
 // The tables of a batch against its lengths.
 static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
-                       const std::vector<int64_t>& kl, int heads, int kv_heads) {
+                       const std::vector<int64_t>& kl, int heads, int kv_heads, int dtype) {
     Plan p;
     CrossQueries qs;
     CrossKeySide ks;
-    plan_queries(qa, ql, ka, kl, heads, kv_heads, 64, qs, p);
-    plan_keys(qa, ql, ka, kl, heads, kv_heads, 64, ks, p);
+    plan_queries(qa, ql, ka, kl, heads, kv_heads, 64, dtype, qs, p);
+    plan_keys(qa, ql, ka, kl, heads, kv_heads, 64, dtype, ks, p);
     const int per = heads / kv_heads, n = (int)ql.size();
     bool ok = (qs.block == 16 || qs.block == 32 || qs.block == 128) && (qs.pack == 1 || qs.pack == per) && qs.pack <= qs.block &&
               heads % qs.pack == 0 && qs.n_items == (int)p.items.size() && qs.n_joins == (int)p.joins.size();
@@ -316,7 +316,7 @@ int main() {
     // ---- the attention's calls, on a plan whose tables nothing reads
     dit_cross c;
     c.heads = 4; c.kv_heads = 2; c.head_d = 64; c.q_rows = 100; c.k_rows = 50;
-    c.qs.block = 128;
+    for (int t = 0; t < 2; t++) c.qs[t].block = 128;
     const int64_t row = 4 * 64;
     struct A {
         int t = AWA_BF16; dit_heads q, k, v, o, dout, dq, dk, dv; const void* mask = nullptr; float scale = 0.125f; void* lse;
@@ -362,7 +362,7 @@ int main() {
     check("cross lse over out", fwd([&](A& a) { a.lse = W; }), bad);
     check("cross misaligned lse", fwd([&](A& a) { a.lse = S + 2; }), bad);
     check("cross out over mask", fwd([&](A& a) { a.mask = W + 5; }), bad);
-    c.qs.n_parts = 3;
+    c.qs[AWA_BF16].n_parts = 3;
     check("cross work", fwd([&](A& a) { a.bytes = dit_cross_work(&c, AWA_BF16, 0); }), ok);
     check("cross little work", fwd([&](A& a) { a.bytes = dit_cross_work(&c, AWA_BF16, 0) - 1; }), bad);
     check("cross no work", fwd([](A& a) { a.work = nullptr; }), bad);
@@ -412,10 +412,10 @@ int main() {
                 k += kl.back() + upto(3);
             }
         }
-        check_plan(qa, ql, ka, kl, h, hk);
+        check_plan(qa, ql, ka, kl, h, hk, t & 1);
     }
-    check_plan({0}, {1 << 24}, {0}, {200}, 4, 1);
-    check_plan({0}, {1}, {0}, {1 << 24}, 1024, 1);
+    check_plan({0}, {1 << 24}, {0}, {200}, 4, 1, AWA_BF16);
+    check_plan({0}, {1}, {0}, {1 << 24}, 1024, 1, AWA_F32);
 
     printf("checks=%d failures=%d\n", checks, failures);
     return failures != 0;
