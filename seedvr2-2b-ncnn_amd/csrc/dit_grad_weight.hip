@@ -322,17 +322,42 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void grad_weight_kernel(GradWeight
 #pragma unroll
     for (int j = 0; j < TN; j++) {
         const int row = n0 + (wn * TN + j) * 16 + (lane & 15);
-        if (row >= p.N) continue;
-        if (sums && lane < 16) {
+        const bool there = row < p.N;
+        if (sums && there && lane < 16) {
             if (!whole) part[BN * BK + row - n0] = sum[j][0];
             else p.db[row] = p.add ? p.db[row] + sum[j][0] : sum[j][0];
         }
+        const int g = lane >> 4, col0 = k0 + wk * TK * 16;
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < TK; i++) {
-            const int col = k0 + (wk * TK + i) * 16 + 4 * (lane >> 4), left = p.K - col;
-            if (left <= 0) continue;
-            if (whole) put(p, row, col, left, acc[i][j]);
-            else *reinterpret_cast<f32x4*>(part + (row - n0) * BK + (col - k0)) = acc[i][j];
+            for (int i = 0; i < TK; i++) {
+                const int col = col0 + 16 * i + 4 * g;
+                if (there && col < p.K) *reinterpret_cast<f32x4*>(part + (row - n0) * BK + (col - k0)) = acc[i][j];
+            }
+        } else if (p.w_f32) {
+#pragma unroll
+            for (int i = 0; i < TK; i++) {
+                const int col = col0 + 16 * i + 4 * g;
+                if (there && col < p.K) put(p, row, col, p.K - col, acc[i][j]);
+            }
+        } else {
+            // neighbouring lane groups exchange halves of two blocks, so that each stores 16 bytes
+#pragma unroll
+            for (int i = 0; i < TK; i += 2) {
+                const f32x4 a = acc[i][j], b = acc[i + 1][j];
+                const auto x = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[0], a[1]), bf16x2_rne(b[0], b[1]), false, false);
+                const auto y = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[2], a[3]), bf16x2_rne(b[2], b[3]), false, false);
+                const u32x4_2 w = {x[0], y[0], x[1], y[1]};
+                const int col = col0 + 16 * (i + (g & 1)) + 8 * (g >> 1), left = there ? p.K - col : 0;
+                uint16_t* to = reinterpret_cast<uint16_t*>(p.dw) + row * p.ldw + col;
+                if (left >= 8) {
+                    *reinterpret_cast<u32x4_2*>(to) = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (e < left) to[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                }
+            }
         }
     }
 }
@@ -374,26 +399,35 @@ hipError_t run(const GradWeight& a, hipStream_t s) {
 
 }  // namespace
 
-// Tiles of 256 x 256 (a workgroup per CU) or 128 x 128 (two).  Tiles fill the chip in whole rounds; those that are
-// left over (all, of a small dW) have their rows divided so that they fill one more.
+// Tiles of 256 x 256 (a workgroup per CU; not for fp32 dy) or 128 x 128 (two).  Tiles fill the chip in whole rounds; the
+// rows of those that are left over (all, of a small dW) may be divided so that they fill one more.  Tile and parts are
+// those with the least estimated time: a stage of 32 rows takes 0.9 us and a tile's ends 9 for 256 x 256, 0.58 and 5 for two
+// of 128 x 128 (fp32 dy 1.1 and 6), the parts' sums 5 and their bytes, written and read, at 8 TB/s (from the caches).
 GradWeightPlan grad_weight_plan(int dtype_dy, int M, int N, int K) {
-    GradWeightPlan p{};
-    auto tiles = [&](int b) { return (int64_t)((N + b - 1) / b) * ((K + b - 1) / b); };
-    p.tile = dtype_dy == AWA_F32 || M < 512 || tiles(256) < 128 ? 128 : 256;
-    const int64_t all = tiles(p.tile), slots = p.tile == 256 ? 256 : 512, rest = all % slots;
-    const int64_t least = 256;  // rows of a part at least
-    const int64_t s = rest ? std::min<int64_t>(slots / rest, M / least) : 1;
-    if (s > 1) {
-        p.splits = (int)s;
-        p.whole = (int)(all - rest);
-        p.rows_per = (int)((((M + s - 1) / s) + MS - 1) / MS * MS);
-    } else {
-        p.splits = 1;
-        p.whole = (int)all;
-        p.rows_per = M;
+    GradWeightPlan best{};
+    double least = 0;
+    for (int tile : {128, 256}) {
+        if (tile == 256 && dtype_dy == AWA_F32) continue;
+        const int64_t all = (int64_t)((N + tile - 1) / tile) * ((K + tile - 1) / tile), slots = tile == 256 ? 256 : 512;
+        const int64_t rest = all % slots, stages = (M + MS - 1) / MS;
+        const double ts = tile == 256 ? 0.9 : dtype_dy == AWA_F32 ? 1.1 : 0.58, t0 = tile == 256 ? 9 : dtype_dy == AWA_F32 ? 6 : 5;
+        const int64_t most = rest ? std::max<int64_t>(std::min<int64_t>({slots / rest, stages / 4, 64}), 1) : 1;
+        for (int64_t s = 1; s <= most; s++) {
+            const int64_t per = (stages + s - 1) / s;
+            const double bytes = (double)(rest * s) * tile * tile * 8;
+            const double alone = slots == 512 && rest * s <= 256 ? 0.6 : 1.0;  // one workgroup a CU
+            const double t = (double)(all / slots) * ((double)stages * ts + t0) + (rest ? (double)per * ts * alone + t0 : 0.0) +
+                             (s > 1 ? 5.0 + bytes / 8e6 : 0.0);
+            if (best.tile && t >= least) continue;
+            least = t;
+            best.tile = tile;
+            best.splits = (int)s;
+            best.whole = (int)(s > 1 ? all - rest : all);
+            best.rows_per = s > 1 ? (int)per * MS : M;
+            best.work = s > 1 ? rest * s * ((int64_t)tile * tile + tile) * 4 : 0;
+        }
     }
-    p.work = s > 1 ? rest * s * ((int64_t)p.tile * p.tile + p.tile) * 4 : 0;
-    return p;
+    return best;
 }
 
 hipError_t launch_grad_weight(int dtype_dy, GradWeight& a, hipStream_t s) {
