@@ -1113,7 +1113,8 @@ class Context:
 
 
 class CrossPlan:
-    """dit_cross: the lengths of a batch (see Context.cross_plan); keep it until the calls that use it have finished."""
+    """dit_cross: the lengths of a batch (see Context.cross_plan); keep it until the calls that use it have finished, and as
+    long as a graph that captured them is replayed."""
 
     def __init__(self, ctx, heads, head_d, q_len, k_len, kv_heads=None, q_at=None, k_at=None):
         def integers(v, name):

@@ -29,11 +29,19 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
     constexpr int RING = WK * (ONE ? 1 : 2) * STAGE, LDS = RING > JOIN ? RING : JOIN;
     static_assert(LDS <= 160 * 1024 && (WQ == 1 || WK == 1), "LDS");
     __shared__ __align__(16) char lds[LDS];
-    const int groups = p.heads / p.qs.pack, total = p.qs.n_items * groups;
-    const int wg = xcd_remap(total);
-    if (wg >= total) return;
-    const int hb = wg / p.qs.n_items;
-    const CrossItem it = table_entry(p.qs.items, wg - hb * p.qs.n_items);
+    const int groups = p.heads / p.qs.pack;
+    CrossItem it;
+    int hb;
+    if (p.qs.n_listed) {
+        it = table_entry(p.qs.items, (int)blockIdx.x);
+        if (it.cols == 0) return;
+        hb = it.group;
+    } else {
+        const int total = p.qs.n_items * groups, wg = xcd_remap(total);
+        if (wg >= total) return;
+        hb = wg / p.qs.n_items;
+        it = table_entry(p.qs.items, wg - hb * p.qs.n_items);
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wq = wave % WQ, wk = wave / WQ, g = lane >> 4;
     const int head0 = hb * p.qs.pack, kv_head = head0 / (p.heads / p.kv_heads);
@@ -351,8 +359,8 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
 
 template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD, bool ONE = false>
 void run(const CrossArgs& a, hipStream_t s) {
-    const long total = (long)a.qs.n_items * (a.heads / a.qs.pack);
-    hipLaunchKernelGGL((cross_queries_kernel<T, DP, NQ, WQ, WK, KT, GRAD, ONE>), dim3(xcd_grid(total)), dim3(64 * WQ * WK), 0, s, a);
+    const unsigned grid = a.qs.n_listed ? (unsigned)a.qs.n_listed : xcd_grid((long)a.qs.n_items * (a.heads / a.qs.pack));
+    hipLaunchKernelGGL((cross_queries_kernel<T, DP, NQ, WQ, WK, KT, GRAD, ONE>), dim3(grid), dim3(64 * WQ * WK), 0, s, a);
 }
 template <typename T, int DP, bool GRAD>
 void run_block(const CrossArgs& a, hipStream_t s) {

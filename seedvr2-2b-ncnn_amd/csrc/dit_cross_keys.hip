@@ -30,11 +30,18 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
     constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
     static_assert(LDS <= 160 * 1024, "LDS");
     __shared__ __align__(16) char lds[LDS];
-    const int total = p.ks.n_items * p.kv_heads;
-    const int wg = xcd_remap(total);
-    if (wg >= total) return;
-    const int kv_head = wg / p.ks.n_items;
-    const CrossKeys it = table_entry(p.ks.items, wg - kv_head * p.ks.n_items);
+    CrossKeys it;
+    int kv_head;
+    if (p.ks.n_listed) {
+        it = table_entry(p.ks.items, (int)blockIdx.x);
+        if (it.kn == 0) return;
+        kv_head = it.group;
+    } else {
+        const int total = p.ks.n_items * p.kv_heads, wg = xcd_remap(total);
+        if (wg >= total) return;
+        kv_head = wg / p.ks.n_items;
+        it = table_entry(p.ks.items, wg - kv_head * p.ks.n_items);
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = wave % WKEY, sub0 = wave / WKEY, g = lane >> 4;
     const int width = p.head_d * T::SIZE;
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(256) void cross_keys_join_kernel(CrossArgs p) {
 
 template <typename T, int DP>
 void run(const CrossArgs& a, hipStream_t s) {
-    const dim3 grid(xcd_grid((long)a.ks.n_items * a.kv_heads));
+    const dim3 grid(a.ks.n_listed ? (unsigned)a.ks.n_listed : xcd_grid((long)a.ks.n_items * a.kv_heads));
     // fp32: tiles are twice as large, so that one workgroup fills a CU's LDS; twice the waves on them
     constexpr int SUBS = T::SIZE == 2 ? 1 : 2;
     hipLaunchKernelGGL((cross_keys_kernel<T, DP, 1, CROSS_KEYS / 16, SUBS>), grid, dim3(4 * CROSS_KEYS * SUBS), 0, s, a);

@@ -1,8 +1,8 @@
 // dit_train.cpp — C ABI of the operators of dit_train.h: argument checks, the attention's plan, launches.
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <map>
-#include <new>
 #include <vector>
 
 #include "dit_train_internal.hpp"
@@ -108,6 +108,15 @@ int64_t runs_of(const std::map<int64_t, int64_t>& blocks, const Cost& c) {
     return most > 0 ? ceil_div(most, best) : 1;  // steps of a run
 }
 
+// A step is 64 keys, or 128 for the waves of a block of few columns.  Measured with heads of 128 channels: in bf16 a
+// block of 128 columns takes 6 us and 1.6 a step where two share a CU, one of few columns 4 us and 1.5 a step; in fp32,
+// one workgroup a CU, 8 us and 8 a step, and 4 us and 3.
+int64_t query_step(int block) { return block < 128 ? 128 : 64; }
+Cost query_cost(int block, int dtype, int head_d) {
+    const bool few = block < 128, f32 = dtype == AWA_F32;
+    return {few || f32 ? 256 : 512, few ? 4.0 : f32 ? 8.0 : 6.0, few ? (f32 ? 3.0 : 1.5) : f32 ? 8.0 : 1.6, 5.0, 4.0 * block * head_d};
+}
+
 void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
                   const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, int dtype, CrossQueries& s, Plan& p) {
     const int per = heads / kv_heads;
@@ -117,16 +126,11 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
     s.block = most <= 16 ? 16 : most <= 32 ? 32 : 128;
     s.pack = s.block < 128 ? per : 1;
     const int rows = s.block / s.pack;
-    // A step is 64 keys, or 128 for the waves of a block of few columns.  Measured with heads of 128 channels: in bf16 a
-    // block of 128 columns takes 6 us and 1.6 a step where two share a CU, one of few columns 4 us and 1.5 a step; in fp32,
-    // one workgroup a CU, 8 us and 8 a step, and 4 us and 3.
-    const int64_t groups = heads / s.pack, step = s.block < 128 ? 128 : 64;
+    const int64_t groups = heads / s.pack, step = query_step(s.block);
     std::map<int64_t, int64_t> made;
     for (size_t i = 0; i < ql.size(); i++)
         if (ql[i]) made[ceil_div(kl[i], step)] += ceil_div(ql[i], rows) * groups;
-    const bool few = s.block < 128, f32 = dtype == AWA_F32;
-    const Cost cost{few || f32 ? 256 : 512, few ? 4.0 : f32 ? 8.0 : 6.0, few ? (f32 ? 3.0 : 1.5) : f32 ? 8.0 : 1.6, 5.0,
-                    4.0 * s.block * head_d};
+    const Cost cost = query_cost(s.block, dtype, head_d);
     const int64_t run = runs_of(made, cost) * step;
     for (size_t i = 0; i < ql.size(); i++) {
         for (int64_t r = 0; r < ql[i]; r += rows) {
@@ -153,6 +157,11 @@ void plan_queries(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql
     s.n_joins = (int)p.joins.size();
 }
 
+// A step is a unit.  Measured as above: in bf16 a block takes 5 us and 2 a unit where two share a CU, in fp32 8 and 8.
+Cost key_cost(int dtype, int head_d) {
+    return dtype == AWA_F32 ? Cost{256, 8.0, 8.0, 5.0, 8.0 * CROSS_KEYS * head_d} : Cost{512, 5.0, 2.0, 5.0, 8.0 * CROSS_KEYS * head_d};
+}
+
 void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, const std::vector<int64_t>& ka,
                const std::vector<int64_t>& kl, int heads, int kv_heads, int head_d, int dtype, CrossKeySide& s, Plan& p) {
     const int per = heads / kv_heads;
@@ -160,15 +169,13 @@ void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, c
     std::map<int64_t, std::vector<size_t>> shared;
     for (size_t i = 0; i < kl.size(); i++)
         if (kl[i]) shared[ka[i]].push_back(i);
-    // A step is a unit.  Measured as above: in bf16 a block takes 5 us and 2 a unit where two share a CU, in fp32 8 and 8.
     std::map<int64_t, int64_t> made;
     for (auto& e : shared) {
         int64_t units = 0;
         for (size_t i : e.second) units += ceil_div(ql[i], CROSS_QT);
         made[units * per] += ceil_div(kl[e.second[0]], CROSS_KEYS) * kv_heads;
     }
-    const int64_t run = runs_of(made, dtype == AWA_F32 ? Cost{256, 8.0, 8.0, 5.0, 8.0 * CROSS_KEYS * head_d}
-                                                        : Cost{512, 5.0, 2.0, 5.0, 8.0 * CROSS_KEYS * head_d});
+    const int64_t run = runs_of(made, key_cost(dtype, head_d));
     for (auto& e : shared) {
         const int unit0 = (int)p.units.size();
         for (size_t i : e.second)
@@ -198,6 +205,33 @@ void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, c
     }
     s.n_items = (int)p.kitems.size();
     s.n_joins = (int)p.kjoins.size();
+}
+
+// Items as a table by workgroup (see CrossQueries), or as they are.  steps(item): its run's; an entry without work is Item{}.
+template <typename Item, typename Steps>
+int spread(std::vector<Item>& items, int groups, const Cost& c, Steps steps) {
+    const int64_t n = (int64_t)items.size() * groups;
+    if (n == 0 || n > CROSS_LISTED) return 0;
+    auto cost = [&](const Item& it) { return c.t0 + c.t1 * (double)steps(it); };
+    double all = 0, at = 0;
+    for (const Item& it : items) all += cost(it) * groups;
+    std::vector<Item> lists[8];
+    for (int g = 0; g < groups; g++)
+        for (const Item& it : items) {
+            const double w = cost(it);
+            lists[std::min(7, (int)((at + 0.5 * w) / all * 8.0))].push_back(it);
+            lists[std::min(7, (int)((at + 0.5 * w) / all * 8.0))].back().group = g;
+            at += w;
+        }
+    size_t longest = 0;
+    for (auto& l : lists) {
+        std::stable_sort(l.begin(), l.end(), [&](const Item& a, const Item& b) { return steps(a) > steps(b); });
+        longest = std::max(longest, l.size());
+    }
+    items.assign(8 * longest, Item{});
+    for (int x = 0; x < 8; x++)
+        for (size_t i = 0; i < lists[x].size(); i++) items[8 * i + x] = lists[x][i];
+    return (int)items.size();
 }
 
 // Whether ranges [at, at + len) of which `same` may coincide, but not overlap otherwise, do so; empty ones do not count.
@@ -263,6 +297,10 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
             set_err(ctx, "dit_cross_create: too many blocks for one launch");
             return AWA_EARG;
         }
+        const int64_t step = query_step(c.qs[t].block);
+        c.qs[t].n_listed = spread(p.items, heads / c.qs[t].pack, query_cost(c.qs[t].block, t, head_d),
+                                  [&](const CrossItem& it) { return ceil_div(it.kn, step); });
+        c.ks[t].n_listed = spread(p.kitems, kv_heads, key_cost(t, head_d), [](const CrossKeys& it) { return (int64_t)it.count; });
         at[t][0] = add(p.items.data(), p.items.size() * sizeof(CrossItem));
         at[t][1] = add(p.joins.data(), p.joins.size() * sizeof(CrossJoin));
         at[t][2] = add(p.kitems.data(), p.kitems.size() * sizeof(CrossKeys));
@@ -534,8 +572,11 @@ int dit_cross_create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64
     if (out) *out = nullptr;
     try {
         return create(ctx, n_seq, h_q_at, h_q_len, h_k_at, h_k_len, heads, kv_heads, head_d, out);
-    } catch (const std::bad_alloc&) {
-        set_err(ctx, "dit_cross_create: out of host memory");
+    } catch (const std::exception& e) {  // memory: no exception leaves a C entry
+        try {
+            set_err(ctx, "dit_cross_create: %s", e.what());
+        } catch (...) {
+        }
         return AWA_EHIP;
     }
 }

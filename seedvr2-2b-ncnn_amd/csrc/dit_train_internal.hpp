@@ -71,6 +71,8 @@ struct CrossItem {
     int k0, kn;    // first key row, keys
     int part;      // slot of the partial results, -1: the only part, written in place
     int first;     // 1: the block's first run of keys
+    int group;     // head group, in a table by workgroup (below)
+    int pad;
 };
 // A block whose keys are split: its parts are slots part0 .. part0 + parts - 1.
 struct CrossJoin {
@@ -92,22 +94,28 @@ struct CrossKeys {
     int unit0, units;        // of its sequences, in the units' table
     int first, count;        // the run, among units x shared heads
     int part;                // slot of partial sums, -1: the only one
-    int pad;
+    int group;               // key head, in a table by workgroup
 };
 struct CrossKeyJoin {
     int k0, kn, part0, parts;
 };
 
-// One of the two forms of a plan's query side.
+// The items are a table by workgroup, with entries for every head group and in the order that they should start, where that
+// is not too long (CROSS_LISTED), or else one for all head groups.  By workgroup: the XCDs, which take workgroups in turn, get
+// lists of equal work, each of neighbouring heads and sequences (whose keys one L2 then holds), the longest first; entries
+// without columns (keys) fill the shorter lists.  Gradients of four clips of up to 5440 x 512 297 us by equal counts, 281 so.
+constexpr int CROSS_LISTED = 1 << 16;
 struct CrossQueries {
     int pack = 1, block = 0;  // heads in a block, columns of a block
     int most_keys = 0;        // of an item
     int n_items = 0, n_joins = 0, n_parts = 0;
+    int n_listed = 0;         // entries of a table by workgroup, 0: items is one for all head groups
     const CrossItem* items = nullptr;
     const CrossJoin* joins = nullptr;
 };
 struct CrossKeySide {
     int n_items = 0, n_joins = 0, n_parts = 0;
+    int n_listed = 0;
     const CrossKeys* items = nullptr;
     const CrossKeyJoin* joins = nullptr;
     const CrossUnit* units = nullptr;

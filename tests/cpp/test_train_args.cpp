@@ -152,6 +152,36 @@ static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t
             ok = ok && c <= w.second.first;
         }
     }
+    auto check_spread = [&](auto items, int groups, const Cost& c, auto steps, auto there) {
+        const size_t n = items.size() * groups;
+        auto list = items;
+        const int entries = spread(list, groups, c, steps);
+        if (n == 0 || n > CROSS_LISTED) return entries == 0 && list.size() == items.size();
+        if (entries != (int)list.size() || entries % 8) return false;
+        size_t seen = 0;
+        std::vector<int> per_group(groups, 0);
+        int64_t work = 0, want_work = 0;
+        for (int x = 0; x < 8; x++) {
+            int64_t before = INT64_MAX;
+            for (int i = x; i < entries; i += 8) {
+                if (!there(list[i])) continue;
+                if (steps(list[i]) > before || list[i].group < 0 || list[i].group >= groups) return false;
+                before = steps(list[i]);
+                seen++;
+                per_group[list[i].group]++;
+                work += steps(list[i]) * (list[i].group + 1) + list[i].k0;
+            }
+        }
+        for (int g = 0; g < groups; g++) {
+            if (per_group[g] != (int)items.size()) return false;
+            for (auto& it : items) want_work += steps(it) * (g + 1) + it.k0;
+        }
+        return seen == n && work == want_work;
+    };
+    hold("plan: queries by workgroup", check_spread(p.items, heads / qs.pack, query_cost(qs.block, dtype, 64),
+         [&](const CrossItem& it) { return ceil_div(it.kn, query_step(qs.block)); }, [](const CrossItem& it) { return it.cols > 0; }));
+    hold("plan: keys by workgroup", check_spread(p.kitems, kv_heads, key_cost(dtype, 64), [](const CrossKeys& it) { return (int64_t)it.count; },
+         [](const CrossKeys& it) { return it.kn > 0; }));
     hold("plan: keys", ok && kat == p.kitems.size() && kjoin == p.kjoins.size() && (int)kslots.size() == ks.n_parts);
 }
 

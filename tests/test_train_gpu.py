@@ -635,3 +635,150 @@ def test_two_calls_at_once(ctx):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_two_graphs_of_one_plan(ctx):
+    """Two captured graphs of one plan, replayed in turn and at once on two streams: each has a workspace of its own."""
+    import torch
+    g = gen(24)
+    plan = ctx.cross_plan(4, 64, [1] * 5, [1200] * 5, kv_heads=2)
+
+    def inputs():
+        return [randn(g, 5, 4, 64), randn(g, 6000, 2, 64), randn(g, 6000, 2, 64), randn(g, 5, 4, 64)]
+
+    def program(q, k, v, do):
+        out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+        return [out, lse, *ctx.cross_attn_grad(plan, do, q, k, v, out, lse)]
+
+    sets, graphs, results = [inputs(), inputs()], [], []
+    program(*sets[0])
+    torch.cuda.synchronize()
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(program(*s))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for s in sets:
+            for t, n in zip(s, inputs()):
+                t.copy_(n)
+        want = [program(*s) for s in sets]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ------------------------------------------------------------------ places past 32 bits, other devices
+
+def far_rows(rows, cols, ld, dtype, g):
+    """[rows, cols] random values in rows ld elements apart: only they are written."""
+    import torch
+    t = torch.empty((rows, ld), dtype=dtype, device="cuda")[:, ld - cols:]
+    t.copy_(randn(g, rows, cols))
+    return t
+
+
+def test_norm_places_past_32_bits(ctx):
+    import torch
+    g = gen(31)
+    x = far_rows(34000, 70, 1 << 16, torch.bfloat16, g)  # 4.5 GB, 2.2 G elements
+    y, st = ctx.layer_norm(x, stats=True)
+    check_norm(y, st, x, None, None, 1e-5)
+    out = torch.empty((34000, 1 << 16), dtype=torch.bfloat16, device="cuda")[:, :70]
+    dx, dw, db = ctx.layer_norm_grad(y, x, st, dx=out)
+    rx, bx, rw, bw, rb, bb = norm_grad_reference(y, x, st, None)
+    within(dx, rx, bx + half_step(dx.dtype) * rx.abs(), "dx")
+    within(dw, rw, bw, "dw")
+
+
+def test_weight_places_past_32_bits(ctx, awa):
+    import torch
+    g = gen(32)
+    dy = far_rows(2500, 90, 1 << 20, torch.bfloat16, g)  # 5.2 GB
+    q, s, v = saved(ctx, awa, randn(g, 2500, 200))
+    out = torch.empty((90, 1 << 26), dtype=torch.bfloat16, device="cuda")[:, :200]  # 12 GB
+    dw, db = ctx.grad_weight_fp8(dy, q, s, cols=200, out=out, bias=True)
+    check_weight(dw, db, dy, v)
+
+
+@pytest.mark.parametrize("nq", [1, 140])
+def test_cross_places_past_32_bits(ctx, nq):
+    """A long cache of wide rows, and heads far apart: the last sequences lie past 2^32 bytes."""
+    import torch
+    g = gen(33)
+    ql, kl, k_at = [nq, nq], [300, 130], [2100, 2400]
+    cache = torch.empty((2600, 1 << 20), dtype=torch.bfloat16, device="cuda")  # 5.4 GB
+    kv = cache[:, (1 << 20) - 256:].unflatten(1, (2, 2, 64))
+    kv[2000:].copy_(randn(g, 600, 2, 2, 64))
+    k, v = kv[:, 0], kv[:, 1]
+    wide = torch.empty((4, 1 << 30), dtype=torch.bfloat16, device="cuda")  # 8.6 GB: a head's rows 2 GB from the next's
+    q = wide[:, :2 * nq * 64].unflatten(1, (2 * nq, 64)).transpose(0, 1)
+    q.copy_(randn(g, 2 * nq, 4, 64))
+    do = randn(g, 2 * nq, 4, 64).to(torch.bfloat16)
+    plan = ctx.cross_plan(4, 64, ql, kl, kv_heads=2, k_at=k_at)
+    ref = reference([0, nq], ql, k_at, kl, q, k, v, None, 0.125, do)
+    out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+    within(out, *ref["out"], "out")
+    grads = torch.empty((2600, 1 << 20), dtype=torch.bfloat16, device="cuda")[:, :256].unflatten(1, (2, 2, 64))
+    dq, dk, dv = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, dk=grads[:, 0], dv=grads[:, 1])
+    within(dq, *ref["dq"], "dq")
+    for name, t in (("dk", dk), ("dv", dv)):
+        within(t[2100:2530], ref[name][0][2100:2530], ref[name][1][2100:2530], name)
+
+
+def test_host_tensors_are_refused(ctx, awa):
+    import torch
+    x, st = torch.randn(5, 128, device="cuda"), torch.zeros(5, 2, device="cuda")
+    w = torch.ones(128)
+    q8, s8 = ctx.quant_fp8(x)
+    plan = ctx.cross_plan(2, 64, [5], [7])
+    q, k = torch.randn(5, 2, 64, device="cuda"), torch.randn(7, 2, 64, device="cuda")
+    out, lse = ctx.cross_attn(plan, q, k, k, lse=True)
+    mask = torch.ones(7, dtype=torch.bool)
+    for call in (lambda: ctx.layer_norm(x.cpu()), lambda: ctx.layer_norm(x, w), lambda: ctx.layer_norm(x, out=x.cpu()),
+                 lambda: ctx.layer_norm(x, stats=st.cpu()), lambda: ctx.layer_norm_grad(x.cpu(), x, st),
+                 lambda: ctx.layer_norm_grad(x, x.cpu(), st), lambda: ctx.layer_norm_grad(x, x, st.cpu()),
+                 lambda: ctx.layer_norm_grad(x, x, st, w), lambda: ctx.layer_norm_grad(x, q8.cpu(), st, x_scale=s8),
+                 lambda: ctx.layer_norm_grad(x, q8, st, x_scale=s8.cpu()), lambda: ctx.layer_norm_grad(x, x, st, dx=x.cpu()),
+                 lambda: ctx.grad_weight_fp8(x.cpu(), q8, s8), lambda: ctx.grad_weight_fp8(x, q8.cpu(), s8),
+                 lambda: ctx.grad_weight_fp8(x, q8, s8.cpu()), lambda: ctx.grad_weight_fp8(x, q8, s8, out=torch.zeros(128, 128)),
+                 lambda: ctx.grad_weight_fp8(x, q8, s8, bias=torch.zeros(128)), lambda: ctx.cross_attn(plan, q.cpu(), k, k),
+                 lambda: ctx.cross_attn(plan, q, k.cpu(), k), lambda: ctx.cross_attn(plan, q, k, k.cpu()),
+                 lambda: ctx.cross_attn(plan, q, k, k, mask=mask), lambda: ctx.cross_attn(plan, q, k, k, out=q.cpu()),
+                 lambda: ctx.cross_attn_grad(plan, q, q, k, k, out.cpu(), lse), lambda: ctx.cross_attn_grad(plan, q, q, k, k, out, lse.cpu()),
+                 lambda: ctx.cross_attn_grad(plan, q, q, k, k, out, lse, dk=k.cpu())):
+        with pytest.raises(ValueError, match="device"):
+            call()
+
+
+def test_refusals_with_their_messages(ctx, awa):
+    """What the library itself refuses reaches the caller as AwaError with its message."""
+    import torch
+    x = torch.randn(6, 128, device="cuda")
+    y, st = ctx.layer_norm(x, stats=True)
+    q8, s8 = ctx.quant_fp8(x)
+    plan = ctx.cross_plan(2, 64, [5], [7])
+    buf = torch.randn(40, 2, 64, device="cuda")
+    q, k = buf[:5], buf[20:27]
+    out, lse = ctx.cross_attn(plan, q, k, k, lse=True)
+    big = torch.randn(2000, device="cuda")
+    for call, text in ((lambda: ctx.layer_norm(x, eps=-1.0), "eps"), (lambda: ctx.layer_norm(x[:5], out=x[1:]), "lie over"),
+                       (lambda: ctx.layer_norm_grad(y[:5], x[:5], st[:5], dx=x[1:]), "lie over"),
+                       (lambda: ctx.grad_weight_fp8(x, q8, s8, out=x[:1].expand(128, 128)), "ldw"),
+                       (lambda: ctx.cross_attn(plan, q, k, k, scale=0.0), "scale"),
+                       (lambda: ctx.cross_attn(plan, q, k, k, scale=math.nan), "scale"),
+                       (lambda: ctx.cross_attn(plan, q, k, k, out=q), "lie over"),
+                       (lambda: ctx.cross_attn(plan, big[1:1 + 640].view(5, 2, 64), k, k), "16-byte"),
+                       (lambda: ctx.cross_attn(plan, q, k, k, out=buf[:1].expand(5, 2, 64)), "coincide"),
+                       (lambda: ctx.cross_attn_grad(plan, q, q, k, k, out, lse, dk=k), "lie over"),
+                       (lambda: ctx.cross_plan(2, 60, [5], [7]), "head_d"), (lambda: ctx.cross_plan(3, 64, [5], [7], kv_heads=2), "kv_heads"),
+                       (lambda: ctx.cross_plan(2, 64, [5, 5], [7, 7], q_at=[0, 4]), "overlap"),
+                       (lambda: ctx.cross_plan(2, 64, [5, 5], [7, 7], k_at=[0, 3]), "overlap"),
+                       (lambda: ctx.cross_plan(2, 64, [-1], [7]), "rows")):
+        with pytest.raises(awa.AwaError, match=text):
+            call()
