@@ -8,6 +8,10 @@
 //
 // Keys are few where queries are many, so the units are divided over workgroups, whose fp32 partial sums a second
 // kernel adds in their order.
+//
+// Bound by LDS: a wave reads 64 KB of a unit, twice the cycles of its 64 matrix instructions.  Both gradients (this kernel a little
+// over half): 16384 queries x 384 keys x 20 heads 290 us (0.78 PFLOP/s of seven products), x 128 144, x 64 110; four clips of up to
+// 5440 x 512, masked, 280.  fp32, 10 heads of 80 on 2, 2 x up to 1237 x 300: 97.
 #include <type_traits>
 
 #include "dit_cross_device.hpp"

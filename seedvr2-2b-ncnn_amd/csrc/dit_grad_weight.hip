@@ -9,6 +9,11 @@
 // columns of x.
 //
 // Where dW has few tiles the rows are divided over workgroups, whose sums a second kernel adds in order.
+//
+// Bound by the matrix instructions where dW is large (a stage of a 256 x 256 tile takes 1.04 us of which they are 0.98), by
+// LDS in tiles of 128 x 128.  bf16 dy and dW: 5498 x 13824 x 2560 360 us (1.08 PFLOP/s), 5498 x 7680 x 2560 221 (0.98), 5498 x
+// 2560 x 2560 103, 679 x 7680 x 2560 45, 58 x 7680 x 2560 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a
+// product: 1.1 PFLOP/s of them), 1237 x 1999 x 2693 57.
 #include <algorithm>
 
 #include "dit_device.hpp"
