@@ -47,7 +47,7 @@ struct Bf16 {
     }
     // Two neighbouring blocks of 16 channels of a row whose lane 16 g + i holds channels 4 g .. 4 g + 3 of both: neighbouring
     // lane groups exchange halves, so that each stores 16 bytes and the four 64 in a row (one after the other at 8 bytes
-    // a lane, 16384 queries x 128 keys x 20 heads take 52 us, so 46).
+    // a lane, 16384 queries x 128 keys x 20 heads take 52 us, so 44).
     static __device__ inline void store_blocks(char* row, int db, int g, int d, const f32x4& a, const f32x4& b) {
         const auto x = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[0], a[1]), bf16x2_rne(b[0], b[1]), false, false);
         const auto y = __builtin_amdgcn_permlane16_swap(bf16x2_rne(a[2], a[3]), bf16x2_rne(b[2], b[3]), false, false);

@@ -10,10 +10,11 @@
 //
 // Where dW has few tiles the rows are divided over workgroups, whose sums a second kernel adds in order.
 //
-// Bound by the matrix instructions where dW is large (a stage of a 256 x 256 tile takes 1.04 us of which they are 0.98), by
-// LDS in tiles of 128 x 128.  bf16 dy and dW: 5498 x 13824 x 2560 360 us (1.08 PFLOP/s), 5498 x 7680 x 2560 221 (0.98), 5498 x
-// 2560 x 2560 103, 679 x 7680 x 2560 45, 58 x 7680 x 2560 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a
-// product: 1.1 PFLOP/s of them), 1237 x 1999 x 2693 57.
+// A stage of a 256 x 256 tile takes 0.8 us, its matrix instructions 0.5 and its 128 KB through LDS about as long: where dW is
+// large the two are bound together, as all waves of a workgroup pass a barrier a stage; tiles of 128 x 128 are bound by LDS.
+// bf16 dy and dW: 5498 x 13824 x 2560 327 us (1.19 PFLOP/s), 5498 x 7680 x 2560 210 (1.03), 5498 x 2560 x 2560 94, 679 x 7680 x
+// 2560 46, 58 x 7680 x 2560 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a product: 1.1 PFLOP/s of
+// them), 1237 x 1999 x 2693 57.
 #include <algorithm>
 
 #include "dit_device.hpp"
@@ -267,19 +268,35 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void grad_weight_kernel(GradWeight
     // a stage's loads have DEPTH stages to arrive
     const int stages = (m_end - m_first + MS - 1) / MS;
     Pieces r0, r1;
-    auto products = [&](const uint8_t* now) __attribute__((always_inline)) {
-        bf16x8 b[PARTS][TN];
+    // A stage's products, and `aside`, the next stage's way into LDS.  For bf16 dy fragments are asked for a block of x ahead
+    // of their use, with `aside` behind the first ones, and fences keep that order: without them each block's reads come right
+    // before its products, which wait for them (5498 x 13824 x 2560 327 us for 360).  With three parts the products hide the
+    // reads and the order costs (1237 x 1999 x 2693 61 us for 57).
+    auto products = [&](const uint8_t* now, auto aside) __attribute__((always_inline)) {
+        constexpr bool AHEAD = PARTS == 1;
+        if constexpr (!AHEAD) aside();
+        const uint8_t* const x = now + PARTS * PART;
+        bf16x8 b[PARTS][TN], a[2];
+        a[0] = frag(x, 2 * BK, wk * TK);
 #pragma unroll
-        for (int i = 0; i < PARTS; i++)
+        for (int h = 0; h < PARTS; h++)
 #pragma unroll
-            for (int j = 0; j < TN; j++) b[i][j] = frag(now + i * PART, 2 * BN, wn * TN + j);
+            for (int j = 0; j < TN; j++) b[h][j] = frag(now + h * PART, 2 * BN, wn * TN + j);
+        if constexpr (AHEAD) {
+            __builtin_amdgcn_sched_barrier(0);
+            aside();
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int i = 0; i < TK; i++) {
-            const bf16x8 a = frag(now + PARTS * PART, 2 * BK, wk * TK + i);
+            if (i + 1 < TK) a[(i + 1) & 1] = frag(x, 2 * BK, wk * TK + i + 1);
+            if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int h = PARTS - 1; h >= 0; h--)
 #pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[h][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i & 1], b[h][j], acc[i][j], 0, 0, 0);
+            if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
         }
         if (sums) {
 #pragma unroll
@@ -291,17 +308,18 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void grad_weight_kernel(GradWeight
     // stage st, while the next one goes to LDS and the DEPTH-th after that is fetched
     auto step = [&](int st, Pieces& r) __attribute__((always_inline)) {
         __syncthreads();
-        store(r, lds + ((st + 1) & 1) * STAGE);
-        load(r, st + 1 + DEPTH);
-        products(lds + (st & 1) * STAGE);
+        products(lds + (st & 1) * STAGE, [&]() __attribute__((always_inline)) {
+            store(r, lds + ((st + 1) & 1) * STAGE);
+            load(r, st + 1 + DEPTH);
+        });
     };
     auto step_any = [&](int st, Pieces& r) __attribute__((always_inline)) {
         __syncthreads();
-        if (st + 1 < stages) {
+        products(lds + (st & 1) * STAGE, [&]() __attribute__((always_inline)) {
+            if (st + 1 >= stages) return;
             store(r, lds + ((st + 1) & 1) * STAGE);
             load_any(r, st + 1 + DEPTH);
-        }
-        products(lds + (st & 1) * STAGE);
+        });
     };
     int st = 0;
     if (stages > 0) {
@@ -406,7 +424,7 @@ hipError_t run(const GradWeight& a, hipStream_t s) {
 
 // Tiles of 256 x 256 (a workgroup per CU; not for fp32 dy) or 128 x 128 (two).  Tiles fill the chip in whole rounds; the
 // rows of those that are left over (all, of a small dW) may be divided so that they fill one more.  Tile and parts are
-// those with the least estimated time: a stage of 32 rows takes 0.9 us and a tile's ends 9 for 256 x 256, 0.58 and 5 for two
+// those with the least estimated time: a stage of 32 rows takes 0.82 us and a tile's ends 9 for 256 x 256, 0.58 and 5 for two
 // of 128 x 128 (fp32 dy 1.1 and 6), the parts' sums 5 and their bytes, written and read, at 8 TB/s (from the caches).
 GradWeightPlan grad_weight_plan(int dtype_dy, int M, int N, int K) {
     GradWeightPlan best{};
@@ -415,7 +433,7 @@ GradWeightPlan grad_weight_plan(int dtype_dy, int M, int N, int K) {
         if (tile == 256 && dtype_dy == AWA_F32) continue;
         const int64_t all = (int64_t)((N + tile - 1) / tile) * ((K + tile - 1) / tile), slots = tile == 256 ? 256 : 512;
         const int64_t rest = all % slots, stages = (M + MS - 1) / MS;
-        const double ts = tile == 256 ? 0.9 : dtype_dy == AWA_F32 ? 1.1 : 0.58, t0 = tile == 256 ? 9 : dtype_dy == AWA_F32 ? 6 : 5;
+        const double ts = tile == 256 ? 0.82 : dtype_dy == AWA_F32 ? 1.1 : 0.58, t0 = tile == 256 ? 9 : dtype_dy == AWA_F32 ? 6 : 5;
         const int64_t most = rest ? std::max<int64_t>(std::min<int64_t>({slots / rest, stages / 4, 64}), 1) : 1;
         for (int64_t s = 1; s <= most; s++) {
             const int64_t per = (stages + s - 1) / s;
