@@ -676,9 +676,9 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
         if (!o.written || !o.rows) continue;
         bad = bad || touches(e, lse) || touches(e, mask);
         for (const auto& t : all)
-            if (t.t != o.t && t.rows) bad = bad || heads_collide(o.t, o.rows, o.heads, t.t, t.rows, t.heads, dtype, d);
+            if (&t != &o && t.rows) bad = bad || heads_collide(o.t, o.rows, o.heads, t.t, t.rows, t.heads, dtype, d);
     }
-    if (bad || (dk == dv && kr)) {
+    if (bad) {
         set_err(ctx, "%s: outputs or d_work lie over an input or each other", who);
         return AWA_EARG;
     }

@@ -408,6 +408,13 @@ int main() {
     check("cross_grad dk over k", bwd([&](A& a) { a.dk.p = Y; }), bad);
     check("cross_grad dq over lse", bwd([&](A& a) { a.dq.p = S; }), bad);
     check("cross_grad work over out", bwd([&](A& a) { a.work = W; }), bad);
+    // one description for an input and a gradient
+    check("cross_grad dq is q", dit_cross_grad(&ctx, &c, AWA_BF16, &a0.dout, &a0.q, &a0.k, &a0.v, &a0.o, (const float*)S, 100, nullptr, 1.f,
+                                               &a0.q, &a0.dk, &a0.dv, K, 1 << 30, nullptr), bad);
+    check("cross_grad dk is k", dit_cross_grad(&ctx, &c, AWA_BF16, &a0.dout, &a0.q, &a0.k, &a0.v, &a0.o, (const float*)S, 100, nullptr, 1.f,
+                                               &a0.dq, &a0.k, &a0.dv, K, 1 << 30, nullptr), bad);
+    check("cross_grad dv is dk", dit_cross_grad(&ctx, &c, AWA_BF16, &a0.dout, &a0.q, &a0.k, &a0.v, &a0.o, (const float*)S, 100, nullptr, 1.f,
+                                                &a0.dq, &a0.dk, &a0.dk, K, 1 << 30, nullptr), bad);
     check("cross_grad dv rows coincide", bwd([](A& a) { a.dv.row = 64; }), bad);
     check("cross_grad misaligned dout", bwd([&](A& a) { a.dout.p = X + 4; }), bad);
     ctx.device = 1;
