@@ -203,6 +203,8 @@ void plan_keys(const std::vector<int64_t>& qa, const std::vector<int64_t>& ql, c
             }
         }
     }
+    // a run without units still reads one: the table has one past the last
+    if (!p.kitems.empty()) p.units.push_back({0, 0});
     s.n_items = (int)p.kitems.size();
     s.n_joins = (int)p.kjoins.size();
 }

@@ -115,6 +115,8 @@ static void check_plan(const std::vector<int64_t>& qa, const std::vector<int64_t
             bool empty = w.second.second.empty();
             while (kat < p.kitems.size() && p.kitems[kat].k0 == f.k0) {
                 const CrossKeys& it = p.kitems[kat++];
+                // the kernel reads the run's first unit whether the run has any or not
+                ok = ok && it.unit0 + it.first % it.units < (int)p.units.size();
                 ok = ok && it.k0 == w.first + c && it.kn == f.kn && it.kn > 0 && it.kn <= CROSS_KEYS && it.unit0 == f.unit0 &&
                      it.units == f.units && it.count >= 0 && (empty ? it.count == 0 : it.count > 0);
                 for (int u = it.first; ok && u < it.first + it.count; u++) {
