@@ -100,16 +100,18 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
  *   S = scale q k^T over the sequence's keys whose mask byte is not 0 (all, without a mask)
  *   P = softmax of each row,  out = P v,  lse = log sum exp S
  *
- * A row for which no key is left gets zeros, lse -infinity, and no gradient; masked
- * keys (whatever they hold, NaN and infinities too) take no part and get gradients of
- * zero.  Rows of tensors that belong to no sequence are neither read nor written. */
+ * A row for which no key is left, or whose scores are all -infinity, gets zeros, lse
+ * -infinity, and no gradient; masked keys (whatever they hold, NaN and infinities too)
+ * take no part and get gradients of zero.  Rows of tensors that belong to no sequence are
+ * neither read nor written. */
 typedef struct dit_cross dit_cross;
 enum { DIT_CROSS_SEQ_MAX = 65536, DIT_CROSS_HEADS_MAX = 1024, DIT_CROSS_HEAD_D_MAX = 128 };
 /* Allocates on the context's device and waits for the copy of its tables: not while a
- * stream is captured.  Rows reach at most DIT_OPS_ROWS_MAX. */
+ * stream is captured.  Rows reach at most DIT_OPS_ROWS_MAX.  A batch of about 2^23 blocks
+ * of 64 keys (by key heads) or 2^24 of 128 query rows (by heads; a sequence's last ones count whole), or more, is rejected. */
 int dit_cross_create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_len, const int64_t* h_k_at,
                      const int64_t* h_k_len, int heads, int kv_heads, int head_d, dit_cross** out);
-/* Frees the tables; calls that use them must have finished (graphs too). */
+/* Frees the tables; calls that use them must have finished (graphs too), and no stream may be capturing. */
 void dit_cross_destroy(dit_cross* plan);
 /* Bytes of d_work of dit_cross_forward (grad 0) or dit_cross_grad (1); negative: bad arguments. */
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad);

@@ -294,8 +294,9 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
         Plan p;
         plan_queries(qa, ql, ka, kl, heads, kv_heads, head_d, t, c.qs[t], p);
         plan_keys(qa, ql, ka, kl, heads, kv_heads, head_d, t, c.ks[t], p);
-        // grids are a workgroup per item and head
-        if ((int64_t)c.qs[t].n_items * heads > 0x7fffff00 || (int64_t)c.ks[t].n_items * heads > 0x7fffff00) {
+        // a workgroup (of at most 256 threads; 512 for fp32 keys) per item and head group, in launches of less than 2^32 threads
+        const int64_t q_blocks = (int64_t)c.qs[t].n_items * (heads / c.qs[t].pack), k_blocks = (int64_t)c.ks[t].n_items * kv_heads;
+        if (q_blocks > (1 << 24) - 8 || k_blocks > (t == AWA_F32 ? 1 << 23 : 1 << 24) - 8) {  // grids are multiples of 8
             set_err(ctx, "dit_cross_create: too many blocks for one launch");
             return AWA_EARG;
         }

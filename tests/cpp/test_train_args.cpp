@@ -342,6 +342,12 @@ int main() {
     check("plan same queries", plan({0, 0}, {4, 4}, {0, 9}, {9, 9}, 4, 2, 64), bad);
     check("plan keys overlap", plan({0, 4}, {4, 4}, {0, 5}, {9, 9}, 4, 2, 64), bad);
     check("plan keys of one start", plan({0, 4}, {4, 4}, {0, 0}, {9, 8}, 4, 2, 64), bad);
+    {  // a launch has fewer than 2^32 threads
+        std::vector<int64_t> at(DIT_CROSS_SEQ_MAX), one(at.size(), 1), none(at.size(), 0);
+        for (size_t i = 0; i < at.size(); i++) at[i] = (int64_t)i;
+        check("plan blocks of queries", plan(at, one, none, none, 1024, 1024, 8), bad);
+        check("plan blocks of keys", plan(none, none, at, one, 1024, 1024, 8), bad);
+    }
     check("plan null out", dit_cross_create(&ctx, 0, nullptr, nullptr, nullptr, nullptr, 1, 1, 8, nullptr), bad);
     check("plan null lengths", plan({}, {}, {}, {}, 0, 1, 8), bad);
 
