@@ -57,26 +57,11 @@ template <> struct Raw<uint16_t> {
     }
     __device__ float get(int i) const { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
 };
-// columns past K are zeros in memory, up to whole blocks of 128
-template <> struct Raw<Fp8> {
-    uint32_t v;
-    __device__ void load(const Fp8* p) { v = *reinterpret_cast<const uint32_t*>(p); }
-    __device__ void load_some(const Fp8* p, int) { load(p); }
-    __device__ float get(int i) const {
-        const f32x2 f = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false);
-        return f[i & 1];
-    }
-};
 
 template <typename T>
 __device__ inline void load_piece(Raw<T>& r, const T* row, int col, int K) {
     if (col + V <= K) r.load(row + col);
     else r.load_some(row + col, max(K - col, 0));
-}
-template <>
-__device__ inline void load_piece<Fp8>(Raw<Fp8>& r, const Fp8* row, int col, int K) {
-    if (col < K) r.load(row + col);
-    else r.v = 0;
 }
 
 __device__ inline void store_piece(float* p, const f32x4& v, int n) {
@@ -139,7 +124,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(NormFwd a) {
     constexpr int WAVES = 4, ROWS = WAVES / WPR;
     __shared__ float2 part[2][WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR;
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + wave / WPR;
     if (row >= a.M) return;  // whole workgroups where waves share a row
     const int col0 = (wave % WPR) * (R * STEP) + lane * V;
     const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
@@ -415,8 +400,9 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(int K, float* dw, float*
 
 template <typename TX, typename TY, int R, int WPR>
 void fwd(const NormFwd& a, hipStream_t s) {
-    constexpr int rows = 4 / WPR;
-    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, R, WPR>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(256), 0, s, a);
+    // a dimension of a launch has fewer than 2^32 threads, which the most rows of four waves do not leave
+    const unsigned n = (unsigned)((a.M + 4 / WPR - 1) / (4 / WPR)), y = (n + 65535) / 65536;
+    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, R, WPR>), dim3((n + y - 1) / y, y), dim3(256), 0, s, a);
 }
 // A wave a row as long as its pieces fit its registers (the least that hold them), four waves beyond
 template <typename TX, typename TY>

@@ -127,6 +127,18 @@ def test_layer_norm_constant_rows_and_special_values(ctx):
     assert bool(y.isnan().all()) and bool((st[0, 1] == math.inf).all())
 
 
+@pytest.mark.parametrize("rows,cols", [(70001, 4100), (270003, 40)])
+def test_layer_norm_many_rows(ctx, rows, cols):
+    """More workgroups than one dimension of the launch takes, not a multiple of the dimensions."""
+    g = gen(11)
+    x = randn(g, rows, cols).to(dt(BF16))
+    y, st = ctx.layer_norm(x, stats=True)
+    at = list(range(9)) + list(range(rows // 2 - 9, rows // 2 + 9)) + list(range(65530, 65540)) + list(range(rows - 9, rows))
+    check_norm(y[at], st[at], x[at], None, None, 1e-5)
+    # every row: no row is left out
+    assert float(st[:, 1].min()) > 0.5 and float((y.float().pow(2).mean(1) - 1).abs().max()) < 0.02
+
+
 def test_layer_norm_in_place_and_rows_around(ctx):
     """y over x; rows and columns beside the result stay as they were."""
     import torch
