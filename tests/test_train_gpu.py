@@ -274,6 +274,57 @@ def test_grad_weight(ctx, awa, tdy, tw, M, N, K, ld):
     assert torch.equal(ctx.grad_weight_fp8(dy, q, s, cols=K, dtype=dt(tw)), dw)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (33, 7, 40), (64, 9, 130), (95, 130, 127), (700, 300, 513), (1300, 515, 700)])
+@pytest.mark.parametrize("tdy", [BF16, F32])
+def test_what_lies_around(ctx, awa, tdy, M, N, K):
+    """NaN beside and behind dy, x and its scales, and in the workspace's memory: nothing of it counts, and what lies beside and
+    behind the results stays.  (Columns of 8-bit rows past K reach columns past K only.)"""
+    import torch
+    g = gen(M + N)
+    nan = float("nan")
+
+    def middle(rows, cols, dtype, fill):
+        whole = torch.full((rows + 3, cols + 12), fill, device="cuda", dtype=dtype)
+        return whole, whole[1:rows + 1, 5:cols + 5]
+
+    def stays(whole, part, fill):
+        part.fill_(fill)
+        assert bool((whole.isnan() if fill != fill else whole == fill).all())
+
+    x = randn(g, M, K)
+    q, s, v = saved(ctx, awa, x)
+    q_all = torch.full((M + 5, q.shape[1]), 0x7f, device="cuda", dtype=torch.uint8)
+    q_all[:M] = q.view(torch.uint8)
+    if q.shape[1] > K:
+        q_all[:, K:] = 0x7f
+    s_all = torch.full((s.shape[0], M + 5, 4), 0xff, device="cuda", dtype=torch.uint8)
+    s_all[:, :M] = s.view(torch.uint8)
+    q2, s2 = q_all[:M].view(q.dtype), s_all.view(s.dtype)[:, :M]
+    dy = middle(M, N, dt(tdy), nan)[1]
+    dy.copy_(randn(g, M, N))
+    dw_all, dw = middle(N, K, dt(F32), 7.0)
+    junk = torch.full((1 << 23,), nan, device="cuda")
+    del junk
+    _, db = ctx.grad_weight_fp8(dy, q2, s2, cols=K, bias=True, out=dw)
+    check_weight(dw, db, dy, v)
+    stays(dw_all, dw, 7.0)
+
+    rows = middle(M, K, dt(tdy), nan)[1]
+    rows.copy_(randn(g, M, K))
+    y_all, y = middle(M, K, dt(tdy), 7.0)
+    w = 1 + 0.1 * randn(g, K)
+    _, st = ctx.layer_norm(rows, w, out=y, stats=True)
+    check_norm(y, st, rows, w, None, 1e-5)
+    want = ctx.layer_norm_grad(rows.contiguous(), v.to(dt(F32)), st, w, dtype=dt(tdy))
+    stays(y_all, y, 7.0)
+    junk = torch.full((1 << 23,), nan, device="cuda")
+    del junk
+    dx_all, dx = middle(M, K, dt(tdy), 7.0)
+    for a, b in zip(ctx.layer_norm_grad(rows, q2, st, w, x_scale=s2, dx=dx), want):
+        assert torch.equal(a, b)
+    stays(dx_all, dx, 7.0)
+
+
 @pytest.mark.parametrize("M", [0, 1, 600])
 @pytest.mark.parametrize("tdy", [BF16, F32])
 def test_grad_weight_added(ctx, awa, tdy, M):
