@@ -10,9 +10,9 @@
 //
 // Where dW has few tiles the rows are divided over workgroups, whose sums a second kernel adds in order.
 //
-// A stage of a 256 x 256 tile takes 0.8 us, its matrix instructions 0.5 and its 128 KB through LDS about as long: where dW is
-// large the two are bound together, as all waves of a workgroup pass a barrier a stage; tiles of 128 x 128 are bound by LDS.
-// bf16 dy and dW: 5498 x 13824 x 2560 327 us (1.19 PFLOP/s), 5498 x 7680 x 2560 210 (1.03), 5498 x 2560 x 2560 94, 679 x 7680 x
+// Bound by LDS: of the 1,930 cycles of a stage of a 256 x 256 tile its 192 transposed reads (6 cycles for 512 bytes, in any
+// layout) and the 32 KB that are written take 1,400, its matrix instructions 1,024; in tiles of 128 x 128 the share is larger.
+// bf16 dy and dW: 5498 x 13824 x 2560 327 to 346 us (1.16 PFLOP/s), 5498 x 7680 x 2560 210 (1.03), 5498 x 2560 x 2560 94, 679 x 7680 x
 // 2560 46, 58 x 7680 x 2560 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a product: 1.1 PFLOP/s of
 // them), 1237 x 1999 x 2693 57.
 #include <algorithm>
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void grad_weight_kernel(GradWeight
     Pieces r0, r1;
     // A stage's products, and `aside`, the next stage's way into LDS.  For bf16 dy fragments are asked for a block of x ahead
     // of their use, with `aside` behind the first ones, and fences keep that order: without them each block's reads come right
-    // before its products, which wait for them (5498 x 13824 x 2560 327 us for 360).  With three parts the products hide the
+    // before its products, which wait for them (5498 x 13824 x 2560 327 to 346 us for 360 to 390).  With three parts the products hide the
     // reads and the order costs (1237 x 1999 x 2693 61 us for 57).
     auto products = [&](const uint8_t* now, auto aside) __attribute__((always_inline)) {
         constexpr bool AHEAD = PARTS == 1;
