@@ -113,7 +113,8 @@ int dit_cross_create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64
                      const int64_t* h_k_len, int heads, int kv_heads, int head_d, dit_cross** out);
 /* Frees the tables; calls that use them must have finished (graphs too), and no stream may be capturing. */
 void dit_cross_destroy(dit_cross* plan);
-/* Bytes of d_work of dit_cross_forward (grad 0) or dit_cross_grad (1); negative: bad arguments. */
+enum { DIT_CROSS_WHOLE = 256 };
+/* Bytes of d_work of dit_cross_forward (grad 0) or dit_cross_grad (1), the same with DIT_CROSS_WHOLE; negative: bad arguments. */
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad);
 
 /* A tensor [rows][heads][head_d]; strides in elements, a head's channels contiguous.  The
@@ -126,7 +127,9 @@ typedef struct {
 
 /* d_mask: NULL, or a byte per key row; scale: 1e-30 .. 1e30; d_lse: NULL, or fp32 [heads][ld_lse],
  * ld_lse at least the plan's last query row + 1.  dtype AWA_F32 or AWA_BF16, of all tensors.
- * bf16: scores and sums are fp32, probabilities are rounded to bf16 before they meet v. */
+ * bf16: scores and sums are fp32, probabilities are rounded to bf16 before they meet v (2^-8 of each at most).  dtype
+ * AWA_BF16 | DIT_CROSS_WHOLE: they meet it with 16 bits (2^-16 of each), so that rounding the result is what is left
+ * (AWA_F32 takes the flag too, and rounds nothing without it). */
 int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_heads* q, const dit_heads* k,
                       const dit_heads* v, const uint8_t* d_mask, float scale, const dit_heads* out, float* d_lse,
                       int64_t ld_lse, void* d_work, int64_t work_bytes, awa_stream_t stream);
@@ -134,7 +137,7 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
 /* Gradients dq, dk, dv for d_out, given the forward's inputs and results (out and lse): all written, none
  * added to; keys of several heads, or sequences, get the sum over them.  With P and S as above,
  *   dv = P^T dout, dS = P (dout v^T - rowsum(dout out)), dq = scale dS k, dk = scale dS^T q
- * bf16: P and dS are rounded to bf16 before they meet the tensors. */
+ * bf16: P and dS are rounded to bf16 before they meet the tensors, or with DIT_CROSS_WHOLE have 16 bits, as above. */
 int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_heads* dout, const dit_heads* q,
                    const dit_heads* k, const dit_heads* v, const dit_heads* out, const float* d_lse, int64_t ld_lse,
                    const uint8_t* d_mask, float scale, const dit_heads* dq, const dit_heads* dk, const dit_heads* dv,

@@ -20,7 +20,7 @@ HEADER_DIR = os.path.join(os.path.dirname(HERE), "include")
 AWA_OK, AWA_EARG, AWA_EHIP = 0, -1, -2
 AWA_F32, AWA_BF16 = 0, 1
 DIT_FP8 = 2
-DIT_FP8_WHOLE = 256
+DIT_FP8_WHOLE = DIT_CROSS_WHOLE = 256
 HEADS, HEAD_D, DIM, QKV, ROPE_ROT = 20, 128, 2560, 7680, 126
 
 _lib = None
@@ -887,11 +887,12 @@ class Context:
                 raise self._elsewhere(what, mask)
         return dtype, qkv, mask.data_ptr() if mask is not None else None, plan.head_d ** -0.5 if scale is None else scale
 
-    def cross_attn(self, plan, q, k, v, mask=None, scale=None, out=None, lse=False, stream=None):
+    def cross_attn(self, plan, q, k, v, mask=None, scale=None, out=None, lse=False, stream=None, whole=False):
         """dit_cross_forward: softmax(scale q k^T) v by the plan's sequences, q [rows, heads, head_d] and k, v [rows, kv_heads,
         head_d] (bf16 or fp32, channels contiguous); mask: bool [key rows], False keys take no part; scale: default
         head_d^-0.5.  lse=True: (out, lse), fp32 [heads, query rows], which cross_attn_grad takes; a tensor is written.  Rows of
-        no sequence are zeros in results made here and stay as they are in given ones."""
+        no sequence are zeros in results made here and stay as they are in given ones.  whole=True (DIT_CROSS_WHOLE): bf16
+        probabilities meet v with 16 bits in place of 8."""
         lib_ = lib()
         what = "cross_attn"
         dtype, qkv, mp, scale = self._cross_inputs(what, plan, q, k, v, mask, scale)
@@ -905,15 +906,16 @@ class Context:
         work = self._work(stream, plan.work(dtype, 0))
         if stream is not None:
             self._used(stream, q, k, v, mask, out, l)
-        rc = lib_.dit_cross_forward(self.ptr, plan.ptr, dtype, *qkv, mp, scale, op, lp, q.shape[0], *_work_of(work),
-                                    self._stream(stream))
+        rc = lib_.dit_cross_forward(self.ptr, plan.ptr, dtype | DIT_CROSS_WHOLE if whole else dtype, *qkv, mp, scale, op, lp,
+                                    q.shape[0], *_work_of(work), self._stream(stream))
         if rc:
             self.check(rc, "dit_cross_forward")
         return out if l is None else (out, l)
 
-    def cross_attn_grad(self, plan, dout, q, k, v, out, lse, mask=None, scale=None, dq=None, dk=None, dv=None, stream=None):
+    def cross_attn_grad(self, plan, dout, q, k, v, out, lse, mask=None, scale=None, dq=None, dk=None, dv=None, stream=None,
+                        whole=False):
         """dit_cross_grad: (dq, dk, dv) for the gradient dout of cross_attn's result, from its inputs and results.  Gradients
-        of keys are summed over the heads and sequences that share them; rows of no sequence as in cross_attn."""
+        of keys are summed over the heads and sequences that share them; rows of no sequence, and whole, as in cross_attn."""
         lib_ = lib()
         what = "cross_attn_grad"
         dtype, qkv, mp, scale = self._cross_inputs(what, plan, q, k, v, mask, scale)
@@ -924,17 +926,17 @@ class Context:
             raise ValueError(f"{what}: lse must be a contiguous fp32 tensor [{plan.heads}, {q.shape[0]}]")
         if dq is None:
             dq = self._made(q.dtype, stream, plan.q_whole(q.shape[0]), *q.shape)
-        whole = plan.k_whole(k.shape[0])
-        dk = self._made(k.dtype, stream, whole, *k.shape) if dk is None else dk
-        dv = self._made(v.dtype, stream, whole, *v.shape) if dv is None else dv
+        filled = plan.k_whole(k.shape[0])
+        dk = self._made(k.dtype, stream, filled, *k.shape) if dk is None else dk
+        dv = self._made(v.dtype, stream, filled, *v.shape) if dv is None else dv
         grads = (self._heads_of(what, plan, dq, "dq", plan.q_rows, plan.heads, q),
                  self._heads_of(what, plan, dk, "dk", plan.k_rows, plan.kv_heads, k),
                  self._heads_of(what, plan, dv, "dv", plan.k_rows, plan.kv_heads, k))
         work = self._work(stream, plan.work(dtype, 1))
         if stream is not None:
             self._used(stream, dout, q, k, v, out, lse, mask, dq, dk, dv)
-        rc = lib_.dit_cross_grad(self.ptr, plan.ptr, dtype, dop, *qkv, op, lp, q.shape[0], mp, scale, *grads, *_work_of(work),
-                                 self._stream(stream))
+        rc = lib_.dit_cross_grad(self.ptr, plan.ptr, dtype | DIT_CROSS_WHOLE if whole else dtype, dop, *qkv, op, lp, q.shape[0],
+                                 mp, scale, *grads, *_work_of(work), self._stream(stream))
         if rc:
             self.check(rc, "dit_cross_grad")
         return dq, dk, dv

@@ -245,14 +245,14 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
         }
 #pragma unroll
         for (int h = 0; h < KB / 2; h++) {
-            Frag pf[NQ];
+            typename T::Packed pf[NQ];
 #pragma unroll
             for (int j = 0; j < NQ; j++) pf[j] = T::pack(s[2 * h][j], s[2 * h + 1][j]);
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 const Frag f = L::column_frag(GRAD ? kt : vt, 32 * h, db, lane);
 #pragma unroll
-                for (int j = 0; j < NQ; j++) acc[db][j] = T::mma(f, pf[j], acc[db][j]);
+                for (int j = 0; j < NQ; j++) acc[db][j] = T::mma_packed(f, pf[j], acc[db][j]);
             }
         }
         valid = next;
@@ -384,7 +384,7 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
     else run_block<T, 128, GRAD>(a, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.qs.n_joins == 0) return e;
-    hipLaunchKernelGGL((cross_join_kernel<T, GRAD>), dim3((unsigned)(a.qs.n_joins * (a.heads / a.qs.pack)), (unsigned)((a.qs.block * (a.head_d / 4) + 255) / 256)),
+    hipLaunchKernelGGL((cross_join_kernel<Rows<T>, GRAD>), dim3((unsigned)(a.qs.n_joins * (a.heads / a.qs.pack)), (unsigned)((a.qs.block * (a.head_d / 4) + 255) / 256)),
                        dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -392,10 +392,10 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_cross_forward(int dtype, const CrossArgs& a, hipStream_t s) {
-    return dtype == AWA_F32 ? run_all<F32, false>(a, s) : run_all<Bf16, false>(a, s);
+    return dtype == AWA_F32 ? run_all<F32, false>(a, s) : a.whole ? run_all<Bf16Whole, false>(a, s) : run_all<Bf16, false>(a, s);
 }
 hipError_t launch_cross_grad_queries(int dtype, const CrossArgs& a, hipStream_t s) {
-    return dtype == AWA_F32 ? run_all<F32, true>(a, s) : run_all<Bf16, true>(a, s);
+    return dtype == AWA_F32 ? run_all<F32, true>(a, s) : a.whole ? run_all<Bf16Whole, true>(a, s) : run_all<Bf16, true>(a, s);
 }
 
 }  // namespace awa

@@ -7,6 +7,8 @@
 // already holds eight of them, {4 g + j, 16 + 4 g + j}, and the other operand is read in that order.
 #pragma once
 
+#include <type_traits>
+
 #include "dit_device.hpp"
 #include "dit_train_internal.hpp"
 
@@ -29,11 +31,13 @@ struct Bf16 {
     static __device__ inline f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
-    // two blocks of a result as the next product's operand
-    static __device__ inline Frag pack(const f32x4& lo, const f32x4& hi) {
+    // two blocks of a result as the next product's operand (rounded: see Bf16Whole), and that product
+    using Packed = Frag;
+    static __device__ inline Packed pack(const f32x4& lo, const f32x4& hi) {
         const f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_convertvector(v, bf16x8);
     }
+    static __device__ inline f32x4 mma_packed(const Frag& a, const Packed& b, const f32x4& c) { return mma(a, b, c); }
     static __device__ inline float dot(const Frag& a, const Frag& b) {
         float s = 0.f;
 #pragma unroll
@@ -55,6 +59,24 @@ struct Bf16 {
         if (ch < d) *reinterpret_cast<u32x4*>(row + 2 * ch) = (u32x4){x[0], y[0], x[1], y[1]};
     }
 };
+// bf16 tensors whose probabilities (and dS) keep 16 bits, as the sum of two bf16 values and in two products (an infinity,
+// whose rest is none, becomes NaN).  Rounded to one value they cost a result as much again as its own rounding, at three
+// quarters of the time, so that a caller chooses.  2-norm of the error over the result's, heads of 128: results 2.32e-3 in one
+// product and 1.66e-3 (their rounding) in two, dq 2.37e-3 and 1.68e-3.  27200 queries x 1024 keys x 20 heads: forward 306 us and
+// 382, gradients 1137 and 1500; 16384 x 384 81 and 98, 297 and 378; 5440 x 58 15.4 and 15.8, 56 and 60.
+struct Bf16Whole : Bf16 {
+    struct Packed {
+        Frag top, rest;
+    };
+    static __device__ inline Packed pack(const f32x4& lo, const f32x4& hi) {
+        const f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const bf16x8 top = __builtin_convertvector(v, bf16x8);
+        return {top, __builtin_convertvector(v - __builtin_convertvector(top, f32x8), bf16x8)};
+    }
+    static __device__ inline f32x4 mma_packed(const Frag& a, const Packed& b, const f32x4& c) {
+        return mma(a, b.top, mma(a, b.rest, c));
+    }
+};
 struct F32 {
     static constexpr int SIZE = 4;
     using Frag = f32x8;
@@ -65,9 +87,11 @@ struct F32 {
         for (int j = 0; j < 8; j++) r = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], r, 0, 0, 0);
         return r;
     }
-    static __device__ inline Frag pack(const f32x4& lo, const f32x4& hi) {
+    using Packed = Frag;
+    static __device__ inline Packed pack(const f32x4& lo, const f32x4& hi) {
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    static __device__ inline f32x4 mma_packed(const Frag& a, const Packed& b, const f32x4& c) { return mma(a, b, c); }
     static __device__ inline float dot(const Frag& a, const Frag& b) {
         float s = 0.f;
 #pragma unroll
@@ -85,6 +109,10 @@ struct F32 {
         if (ch + 16 < d) store4(row + 4 * (ch + 16), b);
     }
 };
+
+// How T's tensors are stored
+template <typename T>
+using Rows = std::conditional_t<T::SIZE == 4, F32, Bf16>;
 
 // One LDS DMA instruction, 16 (4) bytes a lane to LDS at `to` + 16 (4) x lane from byte offset `at` of the resource.  From
 // asm, because the compiler lets every transposed read wait for all DMA that it knows of; the kernels wait by themselves

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
 #pragma unroll
             for (int h = 0; h < HALVES; h++) {
                 if (h) __builtin_amdgcn_sched_barrier(0xf);  // arithmetic may pass: reads that move further up spill registers
-                Frag pf[NK], sf[NK];
+                typename T::Packed pf[NK], sf[NK];
 #pragma unroll
                 for (int j = 0; j < NK; j++) {
                     pf[j] = T::pack(s[2 * h][j], s[2 * h + 1][j]);
@@ -161,10 +161,10 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
                 for (int db = 0; db < DB; db++) {
                     const Frag df = L::column_frag(dt, base + 32 * h, db, lane);
 #pragma unroll
-                    for (int j = 0; j < NK; j++) dv[db][j] = T::mma(df, pf[j], dv[db][j]);
+                    for (int j = 0; j < NK; j++) dv[db][j] = T::mma_packed(df, pf[j], dv[db][j]);
                     const Frag qf = L::column_frag(qt, base + 32 * h, db, lane);
 #pragma unroll
-                    for (int j = 0; j < NK; j++) dk[db][j] = T::mma(qf, sf[j], dk[db][j]);
+                    for (int j = 0; j < NK; j++) dk[db][j] = T::mma_packed(qf, sf[j], dk[db][j]);
                 }
             }
         };
@@ -264,7 +264,7 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.ks.n_joins == 0) return e;
     const int pieces = 2 * CROSS_KEYS * (a.head_d / 4);
-    hipLaunchKernelGGL((cross_keys_join_kernel<T>), dim3((unsigned)(a.ks.n_joins * a.kv_heads), (unsigned)((pieces + 255) / 256)),
+    hipLaunchKernelGGL((cross_keys_join_kernel<Rows<T>>), dim3((unsigned)(a.ks.n_joins * a.kv_heads), (unsigned)((pieces + 255) / 256)),
                        dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -272,7 +272,7 @@ hipError_t run_all(const CrossArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_cross_grad_keys(int dtype, const CrossArgs& a, hipStream_t s) {
-    return dtype == AWA_F32 ? run_all<F32>(a, s) : run_all<Bf16>(a, s);
+    return dtype == AWA_F32 ? run_all<F32>(a, s) : a.whole ? run_all<Bf16Whole>(a, s) : run_all<Bf16>(a, s);
 }
 
 }  // namespace awa

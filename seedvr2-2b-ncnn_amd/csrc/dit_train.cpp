@@ -406,6 +406,13 @@ void place(const dit_heads* t, int dtype, char*& p, int64_t& row, int64_t& head)
     head = t->head * (int64_t)elem(dtype);
 }
 
+// takes DIT_CROSS_WHOLE off a dtype that may have it
+bool take_whole(int& dtype) {
+    const bool whole = dtype == (AWA_F32 | DIT_CROSS_WHOLE) || dtype == (AWA_BF16 | DIT_CROSS_WHOLE);
+    if (whole) dtype &= ~DIT_CROSS_WHOLE;
+    return whole;
+}
+
 int cross_args_ok(awa_ctx* ctx, const char* who, const dit_cross* plan, int dtype, float scale, bool with_lse, int64_t ld_lse) {
     if (!plan || !dtype_ok(dtype) || !(scale >= 1e-30f && scale <= 1e30f)) {
         set_err(ctx, "%s: bad argument (plan, dtype=%d, scale=%g: 1e-30 .. 1e30)", who, dtype, (double)scale);
@@ -594,6 +601,7 @@ void dit_cross_destroy(dit_cross* plan) {
 }
 
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad) {
+    take_whole(dtype);
     if (!plan || !dtype_ok(dtype)) return AWA_EARG;
     return cross_work(*plan, dtype, grad != 0).total;
 }
@@ -603,6 +611,7 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
                       void* d_work, int64_t work_bytes, awa_stream_t stream) {
     const char* who = "dit_cross_forward";
     if (!ctx) return AWA_EARG;
+    const bool whole = take_whole(dtype);
     if (int rc = cross_args_ok(ctx, who, plan, dtype, scale, d_lse != nullptr, ld_lse)) return rc;
     if (plan->q_rows == 0) return AWA_OK;
     const int64_t qr = plan->q_rows, kr = plan->k_rows;
@@ -638,6 +647,7 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
     a.lse = d_lse;
     a.ld_lse = ld_lse;
     a.heads = h; a.kv_heads = hk; a.head_d = d;
+    a.whole = whole;
     a.qs = plan->qs[dtype]; a.ks = plan->ks[dtype];
     a.qpart = reinterpret_cast<float*>(static_cast<char*>(d_work) + w.qpart);
     DeviceGuard dg(ctx->device);
@@ -651,6 +661,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
                    void* d_work, int64_t work_bytes, awa_stream_t stream) {
     const char* who = "dit_cross_grad";
     if (!ctx) return AWA_EARG;
+    const bool whole = take_whole(dtype);
     if (int rc = cross_args_ok(ctx, who, plan, dtype, scale, true, ld_lse)) return rc;
     const int64_t qr = plan->q_rows, kr = plan->k_rows;
     const int h = plan->heads, hk = plan->kv_heads, d = plan->head_d;
@@ -700,6 +711,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
     a.lse = const_cast<float*>(d_lse);
     a.ld_lse = ld_lse;
     a.heads = h; a.kv_heads = hk; a.head_d = d;
+    a.whole = whole;
     a.qs = plan->qs[dtype]; a.ks = plan->ks[dtype];
     char* base = static_cast<char*>(d_work);
     a.qpart = reinterpret_cast<float*>(base + w.qpart);

@@ -132,6 +132,7 @@ struct CrossArgs {
     float* lse;
     int64_t ld_lse;
     int heads, kv_heads, head_d;
+    int whole;  // DIT_CROSS_WHOLE
     CrossQueries qs;
     CrossKeySide ks;
     float *qpart, *kpart;  // partial results
