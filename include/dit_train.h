@@ -102,7 +102,8 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
  *
  * A row for which no key is left, or whose scores are all -infinity, gets zeros, lse
  * -infinity, and no gradient; masked keys (whatever they hold, NaN and infinities too)
- * take no part and get gradients of zero.  Rows of tensors that belong to no sequence are
+ * take no part and get gradients of zero.  A row with a NaN or +infinity among its scores, or with its largest past
+ * fp32 once more times log2(e), is NaN, its lse too.  Rows of tensors that belong to no sequence are
  * neither read nor written. */
 typedef struct dit_cross dit_cross;
 enum { DIT_CROSS_SEQ_MAX = 65536, DIT_CROSS_HEADS_MAX = 1024, DIT_CROSS_HEAD_D_MAX = 128 };

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
                 for (int db = 0; db < DB; db++)
                     if (16 * db + 4 * g < d) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + 16 * db + 4 * g) = acc[db][j];
             } else {
-                const float f = GRAD ? p.scale : sum[j] > 0.f || sum[j] != sum[j] ? 1.f / sum[j] : 0.f;
+                const float f = GRAD ? p.scale : inverse_of(top[j], sum[j]);
                 // lanes exchange channels before the ones of no column drop out
 #pragma unroll
                 for (int db = 0; db < DB; db += 2)
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
             }
             if (!GRAD && g == 0) {
                 if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){top[j], sum[j]};
-                else if (p.lse) p.lse[head[j] * p.ld_lse + row[j]] = top[j] == -INFINITY ? -INFINITY : top[j] * p.scale + LN2 * __builtin_amdgcn_logf(sum[j]);
+                else if (p.lse) p.lse[head[j] * p.ld_lse + row[j]] = lse_of(top[j], sum[j], p.scale);
             }
         }
     } else {
@@ -319,12 +319,12 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
                 if constexpr (!GRAD) l += ml[2 * (w * COLS + c) + 1] * f;
             }
             const int r = it.q0 + c / p.qs.pack, h = head0 + c % p.qs.pack;
-            const float f = part ? 1.f : GRAD ? p.scale : l > 0.f || l != l ? 1.f / l : 0.f;
+            const float f = part ? 1.f : GRAD ? p.scale : inverse_of(m, l);
             if (part) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = v;
             else T::store4(to + r * to_row + h * to_head + ch * T::SIZE, v * f);
             if (!GRAD && ch == 0) {
                 if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){m, l};
-                else if (p.lse) p.lse[h * p.ld_lse + r] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+                else if (p.lse) p.lse[h * p.ld_lse + r] = lse_of(m, l, p.scale);
             }
         }
     }
@@ -355,11 +355,10 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
             if constexpr (!GRAD) l += ml[i * stride + 1] * f;
         }
         const int r = it.q0 + c / p.qs.pack, h = hb * p.qs.pack + c % p.qs.pack;
-        const float f = GRAD ? p.scale : l > 0.f || l != l ? 1.f / l : 0.f;
+        const float f = GRAD ? p.scale : inverse_of(m, l);
         char* to = GRAD ? p.dq + r * p.dq_row + h * p.dq_head : p.o + r * p.o_row + h * p.o_head;
         T::store4(to + ch * T::SIZE, v * f);
-        if (!GRAD && ch == 0 && p.lse)
-            p.lse[h * p.ld_lse + r] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+        if (!GRAD && ch == 0 && p.lse) p.lse[h * p.ld_lse + r] = lse_of(m, l, p.scale);
     }
 }
 

@@ -233,5 +233,15 @@ __device__ inline float sum4(float v) {
 __device__ inline float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// A row's results from its maximum and sum.  A row without keys, or with scores of -infinity alone, keeps the maximum and the sum
+// that it starts with; a NaN leaves no mark on the maximum (fmaxf takes the other operand), but the sum is one; and a sum
+// of 0 beside a maximum means that this passed fp32 on the way to a power of two.
+__device__ inline bool no_score(float top, float sum) { return top == -INFINITY && sum == 0.f; }
+__device__ inline float inverse_of(float top, float sum) { return no_score(top, sum) ? 0.f : 1.f / sum; }
+__device__ inline float lse_of(float top, float sum, float scale) {
+    if (no_score(top, sum)) return -INFINITY;
+    return sum > 0.f ? top * scale + LN2 * __builtin_amdgcn_logf(sum) : NAN;
+}
+
 }  // namespace cross
 }  // namespace awa

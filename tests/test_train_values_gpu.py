@@ -87,3 +87,63 @@ def test_whole_fp32(ctx):
     want = ctx.cross_attn_grad(plan, do, q, k, v, out, lse)
     got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, whole=True)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------ NaN and infinities that take part
+
+# few columns (undivided and divided keys), one tile, several tiles (undivided and divided)
+FORMS = [(1, 40), (3, 3000), (40, 50), (70, 200), (140, 2000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nk", FORMS)
+@pytest.mark.parametrize("where", ["query", "key", "only key"])
+def test_nan_among_scores(ctx, dtype, nq, nk, where):
+    """A row with a NaN among its scores is NaN, its lse too (it is no row without keys), and so is what follows from it; all else
+    is as it would be."""
+    import torch
+    g = gen(nq + nk)
+    q, k, v, do = (randn(g, n, h, 64).to(dt(dtype)) for n, h in ((nq, 4), (nk, 2), (nk, 2), (nq, 4)))
+    mask = torch.ones(nk, dtype=torch.bool, device="cuda")
+    if where == "query":
+        q[nq // 2, 1, 5] = math.nan
+    else:
+        k[nk - 3, 1, 60] = math.nan
+        if where == "only key":
+            mask[:] = False
+            mask[nk - 3] = True
+    plan = ctx.cross_plan(4, 64, [nq], [nk], kv_heads=2)
+    out, lse = ctx.cross_attn(plan, q, k, v, mask=mask, lse=True)
+    ref = attention(q, k, v, 0.125, do, half_step(q.dtype) if dtype == BF16 else 0.0, mask)
+    if where == "query":
+        assert bool(ref["lse"][0][1, nq // 2].isnan()) and int(ref["lse"][0].isnan().sum()) == 1
+    else:
+        assert bool(ref["lse"][0][2:].isnan().all()) and not bool(ref["lse"][0][:2].isnan().any())
+    within(out, *ref["out"], "out")
+    within(lse, *ref["lse"], "lse")
+    got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, mask=mask)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        if name != "dq":  # keys that take no part get zeros
+            ref[name][0][~mask] = 0.0
+        within(t, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nk", FORMS)
+def test_scores_past_fp32(ctx, dtype, nq, nk):
+    """Finite products that the scale takes past fp32 make their row NaN (not one without keys); the other rows stay as they are."""
+    import torch
+    g = gen(nq + nk)
+    q, k, v = (randn(g, n, h, 64) for n, h in ((nq, 2), (nk, 2), (nk, 2)))
+    q *= 1e-30  # scores of ordinary sizes
+    q[nq - 1, 1], k[:, 1] = 1e5, 1e5 * (1 + 0.01 * randn(g, nk, 64))
+    q[: nq - 1, 1] *= 1e-5
+    q, k, v = (t.to(dt(dtype)) for t in (q, k, v))
+    plan = ctx.cross_plan(2, 64, [nq], [nk])
+    out, lse = ctx.cross_attn(plan, q, k, v, scale=1e29, lse=True)
+    ref = attention(q, k, v, 1e29, hp=half_step(q.dtype) if dtype == BF16 else 0.0)
+    for name in ("out", "lse"):
+        for t in ref[name]:
+            (t[nq - 1, 1] if name == "out" else t[1, nq - 1:]).fill_(math.nan)
+    within(out, *ref["out"], "out")
+    within(lse, *ref["lse"], "lse")
