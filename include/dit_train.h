@@ -101,7 +101,8 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
  *   P = softmax of each row,  out = P v,  lse = log sum exp S
  *
  * A row for which no key is left, or whose scores are all -infinity, gets zeros, lse
- * -infinity, and no gradient; masked keys (whatever they hold, NaN and infinities too)
+ * -infinity, and no gradient, whatever it, its dout, and the keys and values that made it so, hold
+ * (a row whose given lse is -infinity, too); masked keys (whatever they hold, NaN and infinities too)
  * take no part and get gradients of zero.  A row with a NaN or +infinity among its scores, or with its largest past
  * fp32 once more times log2(e), is NaN, its lse too.  Rows of tensors that belong to no sequence are
  * neither read nor written. */

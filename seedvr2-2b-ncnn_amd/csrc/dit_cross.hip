@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
             if (there[j]) {
                 const float l = p.lse[head[j] * p.ld_lse + row[j]];
                 lse2[j] = l * LOG2E;
-                if (l == -INFINITY) {  // a row without keys: P = 0, and nothing that comes back counts
+                if (l == -INFINITY) {  // a row without scores: P = 0, and nothing that comes back counts
                     lse2[j] = INFINITY;
                     dsum[j] = 0.f;
 #pragma unroll
@@ -265,6 +265,17 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
     float* const part = it.part < 0 ? nullptr : p.qpart + ((int64_t)it.part * groups + hb) * cross_query_part(p.qs.block, d);
 #pragma unroll
     for (int j = 0; j < NQ; j++) sum[j] = sum4(sum[j]);
+    // a row without scores gets zeros: its probabilities are, but what they met may have been infinite
+#pragma unroll
+    for (int j = 0; j < NQ; j++) {
+        const bool none = GRAD ? lse2[j] == INFINITY : WK == 1 && !part && no_score(top[j], sum[j]);
+        if (__builtin_amdgcn_ballot_w64(none)) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[db][j][r] = none ? 0.f : acc[db][j][r];
+        }
+    }
     if constexpr (WK == 1) {
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
@@ -321,7 +332,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 :
             const int r = it.q0 + c / p.qs.pack, h = head0 + c % p.qs.pack;
             const float f = part ? 1.f : GRAD ? p.scale : inverse_of(m, l);
             if (part) *reinterpret_cast<f32x4*>(part + (int64_t)c * d + ch) = v;
-            else T::store4(to + r * to_row + h * to_head + ch * T::SIZE, v * f);
+            else T::store4(to + r * to_row + h * to_head + ch * T::SIZE, !GRAD && no_score(m, l) ? (f32x4){0.f, 0.f, 0.f, 0.f} : v * f);
             if (!GRAD && ch == 0) {
                 if (part) *reinterpret_cast<f32x2*>(part + (int64_t)p.qs.block * d + 2 * c) = (f32x2){m, l};
                 else if (p.lse) p.lse[h * p.ld_lse + r] = lse_of(m, l, p.scale);
@@ -357,7 +368,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs p) {
         const int r = it.q0 + c / p.qs.pack, h = hb * p.qs.pack + c % p.qs.pack;
         const float f = GRAD ? p.scale : inverse_of(m, l);
         char* to = GRAD ? p.dq + r * p.dq_row + h * p.dq_head : p.o + r * p.o_row + h * p.o_head;
-        T::store4(to + ch * T::SIZE, v * f);
+        T::store4(to + ch * T::SIZE, !GRAD && no_score(m, l) ? (f32x4){0.f, 0.f, 0.f, 0.f} : v * f);
         if (!GRAD && ch == 0 && p.lse) p.lse[h * p.ld_lse + r] = lse_of(m, l, p.scale);
     }
 }

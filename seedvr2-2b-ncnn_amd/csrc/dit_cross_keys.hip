@@ -105,10 +105,20 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
         if (n + 1 < it.count) next = table_entry(p.ks.units, it.unit0 + at);
         wait_vmem_lds<0>();
         __syncthreads();
-        if (n + 1 < it.count) fetch((n + 1) & 1);
-        const char* qt = lds + (n & 1) * STAGE;
-        const char* dt = qt + TILE_B;
+        char* qt = lds + (n & 1) * STAGE;
+        char* dt = qt + TILE_B;
         const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE_B);
+        const float mine = lse[lane];
+        if (n + 1 < it.count) fetch((n + 1) & 1);
+        // rows without scores take no part, whatever they and what comes back to them hold
+        const uint64_t none = __builtin_amdgcn_ballot_w64(mine == INFINITY);
+        if (none) {
+            for (int r = wave; r < rows; r += WAVES)
+                if ((none >> r) & 1 && lane < L::CHUNKS)
+                    reinterpret_cast<u32x4*>(qt + r * L::ROW)[lane] = reinterpret_cast<u32x4*>(dt + r * L::ROW)[lane] = (u32x4){0, 0, 0, 0};
+            __syncthreads();
+        }
+        const uint64_t out = rows == 64 ? none : none | ~(uint64_t)0 << rows;
         // 32 HALVES rows from base on (64 at once where registers allow: more products that do not wait for each other)
         auto take = [&](auto halves, int base) __attribute__((always_inline)) {
             constexpr int HALVES = decltype(halves)::value, NB = 2 * HALVES;
@@ -139,12 +149,13 @@ __global__ __launch_bounds__(64 * WKEY * SUBS, 2) void cross_keys_kernel(CrossAr
                         s[b][j][r] = e;
                     }
             }
-            if (rows < base + 32 * HALVES) {  // rows past the end hold zeros, but infinite keys times zero are not
+            if (HALVES == 2 ? out : (uint32_t)(out >> base)) {  // rows past the end hold zeros as well, but infinite keys times zero are not
+                const uint64_t its = out >> (base + 4 * g);
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (base + 16 * b + 4 * g + r >= rows)
+                        if ((its >> (16 * b + r)) & 1)
 #pragma unroll
                             for (int j = 0; j < NK; j++) s[b][j][r] = dp[b][j][r] = 0.f;
             }

@@ -147,3 +147,52 @@ def test_scores_past_fp32(ctx, dtype, nq, nk):
             (t[nq - 1, 1] if name == "out" else t[1, nq - 1:]).fill_(math.nan)
     within(out, *ref["out"], "out")
     within(lse, *ref["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nk", FORMS + [(64, 300), (97, 64)])
+@pytest.mark.parametrize("where", ["query", "key", "finite"])
+def test_rows_whose_scores_are_all_minus_infinity(ctx, dtype, nq, nk, where):
+    """Zeros, lse -infinity and no gradient, although what made the scores infinite (a query's channel, every key's, finite values
+    whose products pass fp32), the values, and what comes back to such rows, are infinite or NaN."""
+    import torch
+    g = gen(nq + nk)
+    heads, kv_heads = (4, 2) if where == "query" else (2, 2)
+    q, k, v, do = (randn(g, n, h, 64).to(dt(dtype)) for n, h in ((nq, heads), (nk, kv_heads), (nk, kv_heads), (nq, heads)))
+    none = torch.zeros(nq, heads, dtype=torch.bool, device="cuda")
+    if where == "query":
+        none[nq // 2, 1] = none[nq - 1, 3] = True
+        k[:, :, 5] = k[:, :, 5].abs() + 0.5
+    elif where == "key":  # every row of the second head
+        none[:, 1] = True
+    else:
+        none[nq // 2] = True
+    clean = [t.clone() for t in (q, k, v, do)]
+    if where == "query":
+        q[..., 5] = torch.where(none, -math.inf, q[..., 5])
+    elif where == "key":
+        q[:, 1, 5] = 1.0
+        k[:, 1, 5] = -math.inf
+        v[::7, 1, 9] = math.inf
+    else:
+        k[..., 5], clean[1][..., 5] = 3e38, 3e38
+        q[..., 5] = torch.where(none, -3e38, 0.0)
+        clean[0][..., 5] = 0.0
+    do[none] = math.nan
+    clean[0][none], clean[3][none] = 0.0, 0.0
+    ref = attention(*clean[:3], 0.125, clean[3], half_step(q.dtype) if dtype == BF16 else 0.0)
+    for name in ("out", "dq"):
+        for t in ref[name]:
+            t[none] = 0.0
+    for t, value in zip(ref["lse"], (-math.inf, 0.0)):
+        t[none.T] = value
+    plan = ctx.cross_plan(heads, 64, [nq], [nk], kv_heads=kv_heads)
+    out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+    within(out, *ref["out"], "out")
+    within(lse, *ref["lse"], "lse")
+    for name, t in zip(("dq", "dk", "dv"), ctx.cross_attn_grad(plan, do, q, k, v, out, lse)):
+        if name == "dq" and where == "finite":
+            # the fifth channel is a sum of terms dS 3e38 with |dS| up to about 1 (P at most 1, dout v of eight on the mean): its
+            # partial sums may pass fp32's 3.4e38 whatever the total is, so that it says nothing
+            t[..., 5] = torch.where(none, t[..., 5].double(), ref[name][0][..., 5])
+        within(t, *ref[name], name)
