@@ -196,3 +196,83 @@ def test_rows_whose_scores_are_all_minus_infinity(ctx, dtype, nq, nk, where):
             # partial sums may pass fp32's 3.4e38 whatever the total is, so that it says nothing
             t[..., 5] = torch.where(none, t[..., 5].double(), ref[name][0][..., 5])
         within(t, *ref[name], name)
+
+
+# ------------------------------------------------------------------ batches of more blocks than are listed by workgroup
+
+LISTED = 65536  # blocks (by heads) of a side up to which a plan lists them for each workgroup
+
+
+def uniform(g, n, nq, nk, heads, kv_heads, d, dtype):
+    """n sequences of nq queries and nk keys: (q, k, v, do) as rows, and the same for `attention` with the sequences as heads."""
+    rows = [randn(g, n * m, h, d).to(dt(dtype)) for m, h in ((nq, heads), (nk, kv_heads), (nk, kv_heads), (nq, heads))]
+    return rows, [t.unflatten(0, (n, -1)).transpose(0, 1).flatten(1, 2) for t in rows]
+
+
+def as_rows(t, n, heads):
+    """`attention`'s [m, n * heads, d] in the rows' order."""
+    return t.unflatten(1, (n, heads)).transpose(0, 1).flatten(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,nq,nk,heads,kv_heads", [(9001, 1, 5, 8, 8), (4111, 3, 66, 16, 8), (2061, 40, 70, 32, 16)])
+def test_many_blocks(ctx, dtype, n, nq, nk, heads, kv_heads):
+    """Few columns and blocks of 128, several blocks of queries' and keys' sides past the list's length."""
+    import torch
+    g = gen(n)
+    d, per = 8, heads // kv_heads
+    (q, k, v, do), wide = uniform(g, n, nq, nk, heads, kv_heads, d, dtype)
+    groups = heads if nq * per > 32 else kv_heads
+    if nq * per > 32 or per == 1:
+        assert n * groups > LISTED
+    assert n * kv_heads * ((nk + 63) // 64) > LISTED
+    mask = torch.rand(n * nk, generator=g, device="cuda") < 0.8
+    plan = ctx.cross_plan(heads, d, [nq] * n, [nk] * n, kv_heads=kv_heads)
+    some = mask.unflatten(0, (n, nk)).any(1)
+    ref = attention(*wide[:3], 0.5, wide[3], half_step(q.dtype) if dtype == BF16 else 0.0,
+                    mask.unflatten(0, (n, 1, nk)).repeat_interleave(heads, 0))
+    for name in ("out", "dq", "dk", "dv"):  # sequences without keys
+        ref[name] = [torch.where(some.repeat_interleave(t.shape[0] // n)[:, None, None], t, 0.0)
+                     for t in (as_rows(t, n, heads if name in ("out", "dq") else kv_heads) for t in ref[name])]
+    out, lse = ctx.cross_attn(plan, q, k, v, mask=mask, scale=0.5, lse=True)
+    within(out, *ref["out"], "out")
+    l, bl = (t.unflatten(0, (n, heads)).transpose(0, 1).flatten(1) for t in ref["lse"])
+    keep = some.repeat_interleave(nq)
+    within(lse[:, keep], l[:, keep], bl[:, keep], "lse")
+    assert bool((lse[:, ~keep] == -math.inf).all())
+    got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, mask=mask, scale=0.5)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        if name != "dq":
+            ref[name] = [torch.where(mask[:, None, None], r, 0.0) for r in ref[name]]
+        within(t, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("long_q,long_k", [(1, 5000), (3000, 130), (700, 2000)])
+def test_many_blocks_and_divided_ones(ctx, dtype, long_q, long_k):
+    """Past the list's length with a sequence whose keys, queries, or both, go to several workgroups and are joined."""
+    import torch
+    g = gen(long_q)
+    n, nk, heads, d = 8500, 4, 8, 16
+    assert n * heads > LISTED
+    (q, k, v, do), wide = uniform(g, n, 1, nk, heads, heads, d, dtype)
+    one = [randn(g, m, heads, d).to(dt(dtype)) for m in (long_q, long_k, long_k, long_q)]
+    # the long sequence between the short ones
+    at = n // 3
+    q, k, v, do = (torch.cat((t[: at * m], o, t[at * m:])) for t, o, m in zip((q, k, v, do), one, (1, nk, nk, 1)))
+    plan = ctx.cross_plan(heads, d, [1] * at + [long_q] + [1] * (n - at), [nk] * at + [long_k] + [nk] * (n - at))
+    code = 1 if dtype == BF16 else 0
+    kept = 2 * ((4 * heads * (n + long_q) + 255) // 256 * 256)  # what the gradients' workspace holds beside parts
+    assert plan.work(code, 0) > 0 or long_k < 1000
+    assert plan.work(code, 1) - kept > plan.work(code, 0) or long_q == 1
+    hp = half_step(q.dtype) if dtype == BF16 else 0.0
+    ref, long = attention(*wide[:3], 0.25, wide[3], hp), attention(*one[:3], 0.25, one[3], hp)
+    out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+    got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse)
+    for name, t in zip(("out", "dq", "dk", "dv"), (out, *got)):
+        m, b = (1, long_q) if name in ("out", "dq") else (nk, long_k)
+        within(t[at * m:at * m + b], *long[name], name + " of the long one")
+        short = torch.cat((t[: at * m], t[at * m + b:]))
+        within(short, *(as_rows(r, n, heads) for r in ref[name]), name)
+    within(lse[:, at:at + long_q], *long["lse"], "lse of the long one")
+    within(torch.cat((lse[:, :at], lse[:, at + long_q:]), 1), *(r.unflatten(0, (n, heads)).transpose(0, 1).flatten(1) for r in ref["lse"]), "lse")
