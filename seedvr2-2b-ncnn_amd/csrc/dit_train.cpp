@@ -384,15 +384,21 @@ int heads_ok(awa_ctx* ctx, const char* who, const char* name, const dit_heads* t
 Extent extent(const dit_heads* t, int dtype, int64_t rows, int heads, int d) {
     return {t->p, rows > 0 ? (size_t)((rows - 1) * t->row + (heads - 1) * t->head + d) * elem(dtype) : 0};
 }
-// Tensors side by side in the same rows (queries, keys and values of one projection) are apart although their extents are not.
+// Tensors side by side in the same rows (queries, keys and values of one projection), or with heads outermost in the same heads,
+// are apart although their extents are not.
 bool heads_collide(const dit_heads* a, int64_t a_rows, int a_heads, const dit_heads* b, int64_t b_rows, int b_heads, int dtype, int d) {
     if (!touches(extent(a, dtype, a_rows, a_heads, d), extent(b, dtype, b_rows, b_heads, d))) return false;
-    const int64_t size = (int64_t)elem(dtype), wa = ((a_heads - 1) * a->head + d) * size, wb = ((b_heads - 1) * b->head + d) * size;
-    const int64_t row = a->row * size;
-    if (a->row != b->row || wa > row || wb > row) return true;
+    const int64_t size = (int64_t)elem(dtype);
     const intptr_t pa = reinterpret_cast<intptr_t>(a->p), pb = reinterpret_cast<intptr_t>(b->p);
-    const int64_t off = (int64_t)((pb - pa) % row + row) % row;
-    return !(off >= wa && off + wb <= row);
+    // na and nb pieces of wa and wb elements, sa and sb apart (one piece: any)
+    auto beside = [&](int64_t na, int64_t sa, int64_t wa, int64_t nb, int64_t sb, int64_t wb) {
+        const int64_t step = (na > 1 ? sa : sb) * size;
+        if ((na > 1 && nb > 1 && sa != sb) || wa * size > step || wb * size > step) return false;
+        const int64_t off = (int64_t)((pb - pa) % step + step) % step;
+        return off >= wa * size && off + wb * size <= step;
+    };
+    return !beside(a_rows, a->row, (a_heads - 1) * a->head + d, b_rows, b->row, (b_heads - 1) * b->head + d) &&
+           !beside(a_heads, a->head, (a_rows - 1) * a->row + d, b_heads, b->head, (b_rows - 1) * b->row + d);
 }
 
 void place(const dit_heads* t, int dtype, const char*& p, int64_t& row, int64_t& head) {

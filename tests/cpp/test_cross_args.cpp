@@ -3,6 +3,8 @@
 // per failed check.
 #include <cstdarg>
 #include <cstdio>
+#include <random>
+#include <set>
 
 #include "../../seedvr2-2b-ncnn_amd/csrc/dit_train.cpp"
 
@@ -104,6 +106,46 @@ int main() {
     for (int t = 0; t < 2; t++)
         for (int grad = 0; grad < 2; grad++)
             hold("work whole", dit_cross_work(&c, t | DIT_CROSS_WHOLE, grad) == dit_cross_work(&c, t, grad) && dit_cross_work(&c, t, grad) >= 0);
+
+    // ---- outputs beside inputs and each other, in one buffer
+    const int64_t F = 1 << 20;  // bytes past which another tensor lies in the same buffer
+    // keys' gradients with heads outermost, [2 heads][dk, dv][50 rows][64]
+    check("dk, dv by heads", bwd([&](A& a) { a.dk = {Z + (1 << 30), 64, 6400}; a.dv = {Z + (1 << 30) + 6400, 64, 6400}; }), ok, 2);
+    check("dk, dv by heads, dv a row early", bwd([&](A& a) { a.dk = {Z + (1 << 30), 64, 6400}; a.dv = {Z + (1 << 30) + 6400 - 128, 64, 6400}; }), bad);
+    check("dk, dv by heads, another stride", bwd([&](A& a) { a.dk = {Z + (1 << 30), 64, 6400}; a.dv = {Z + (1 << 30) + 6400, 64, 6408}; }), bad);
+    check("out beside v by heads", fwd([&](A& a) { a.q.row = 64; a.o = {Z, 64, 12800}; a.v = {Z + 12800, 64, 12800}; }), ok);
+    c.q_rows = 1;  // one query: its stride does not matter
+    a0.q.row = a0.o.row = a0.dout.row = a0.dq.row = 0;
+    check("one query's gradient beside keys' rows", bwd([&](A& a) {
+        a.dk = {Z + F, 512, 64}; a.dv = {Z + F + 256, 512, 64}; a.dq = {Z + F + 512, 0, 64}; }), ok, 2);
+    check("one query's gradient over a key's row", bwd([&](A& a) {
+        a.dk = {Z + F, 512, 64}; a.dv = {Z + F + 256, 512, 64}; a.dq = {Z + F + 768, 0, 64}; }), bad);
+    c.q_rows = 100;
+    a0.q.row = a0.o.row = a0.dout.row = a0.dq.row = 256;
+    // against the elements themselves: nothing that overlaps is taken, and what lies side by side is
+    std::mt19937 rng(3);
+    auto upto = [&](int n) { return (int64_t)(rng() % (unsigned)(n + 1)); };
+    int taken = 0, apart = 0;
+    bool right = true;
+    for (int t = 0; t < 200000; t++) {
+        const int d = 8, ha = 1 + (int)upto(2), hb = 1 + (int)upto(2);
+        const int64_t ra = 1 + upto(3), rb = 1 + upto(3), strides[] = {8, 16, 24, 32, 48, 64, 96};
+        const bool same = upto(3) > 0;
+        dit_heads a{X + 16 * upto(40), strides[upto(6)], strides[upto(6)]}, b{X + 16 * upto(40), strides[upto(6)], strides[upto(6)]};
+        if (same) b.row = a.row, b.head = a.head;
+        std::set<char*> in;
+        for (int64_t r = 0; r < ra; r++)
+            for (int h = 0; h < ha; h++) in.insert((char*)a.p + 2 * (r * a.row + h * a.head));
+        bool over = false;
+        for (int64_t r = 0; r < rb; r++)
+            for (int h = 0; h < hb; h++) over = over || in.count((char*)b.p + 2 * (r * b.row + h * b.head));
+        const bool refused = heads_collide(&a, ra, ha, &b, rb, hb, AWA_BF16, d);
+        right = right && !(over && !refused) && refused == heads_collide(&b, rb, hb, &a, ra, ha, AWA_BF16, d);
+        apart += !over && touches(extent(&a, AWA_BF16, ra, ha, d), extent(&b, AWA_BF16, rb, hb, d));
+        taken += !over && !refused && touches(extent(&a, AWA_BF16, ra, ha, d), extent(&b, AWA_BF16, rb, hb, d));
+    }
+    hold("no overlap is taken", right);
+    hold("what lies side by side is", taken > 1000 && taken > apart / 20);
 
     printf("checks=%d failures=%d\n", checks, failures);
     return failures != 0;

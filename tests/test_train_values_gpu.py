@@ -276,3 +276,28 @@ def test_many_blocks_and_divided_ones(ctx, dtype, long_q, long_k):
         within(short, *(as_rows(r, n, heads) for r in ref[name]), name)
     within(lse[:, at:at + long_q], *long["lse"], "lse of the long one")
     within(torch.cat((lse[:, :at], lse[:, at + long_q:]), 1), *(r.unflatten(0, (n, heads)).transpose(0, 1).flatten(1) for r in ref["lse"]), "lse")
+
+
+# ------------------------------------------------------------------ tensors side by side
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq", [1, 90])
+def test_gradients_side_by_side_with_heads_outermost(ctx, dtype, nq):
+    """dk and dv in turn for each head of one buffer, dq behind both (and for one query, whose stride does not matter, beside
+    keys' rows)."""
+    import torch
+    g = gen(nq)
+    nk = 70
+    q, k, v, do = (randn(g, n, 2, 64).to(dt(dtype)) for n in (nq, nk, nk, nq))
+    plan = ctx.cross_plan(2, 64, [nq], [nk])
+    out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+    want = ctx.cross_attn_grad(plan, do, q, k, v, out, lse)
+    buf = torch.full((2, 2 * nk + nq, 64), 7.0, dtype=dt(dtype), device="cuda")
+    parts = [t.transpose(0, 1) for t in (buf[:, 2 * nk:], buf[:, :nk], buf[:, nk:2 * nk])]
+    got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, dq=parts[0], dk=parts[1], dv=parts[2])
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not bool((buf == 7).all(2).any())
+    if nq == 1:
+        buf = torch.full((nk, 3, 2, 64), 7.0, dtype=dt(dtype), device="cuda")
+        got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, dq=buf[5:6, 2], dk=buf[:, 0], dv=buf[:, 1])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert bool((buf[:5, 2] == 7).all()) and bool((buf[6:, 2] == 7).all())
