@@ -115,6 +115,10 @@ int dit_cross_create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64
                      const int64_t* h_k_len, int heads, int kv_heads, int head_d, dit_cross** out);
 /* Frees the tables; calls that use them must have finished (graphs too), and no stream may be capturing. */
 void dit_cross_destroy(dit_cross* plan);
+/* For a caller that does not know whether they have (a garbage collector), at any time: the plan is not used again; its
+ * tables are freed when the next plan is made on its device, or, if a call that used them was captured, not before the
+ * process ends. */
+void dit_cross_drop(dit_cross* plan);
 enum { DIT_CROSS_WHOLE = 256 };
 /* Bytes of d_work of dit_cross_forward (grad 0) or dit_cross_grad (1), the same with DIT_CROSS_WHOLE; negative: bad arguments. */
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad);

@@ -186,6 +186,8 @@ def lib():
         L.dit_cross_create.argtypes = [vp, C.c_int, i64p, i64p, i64p, i64p, C.c_int, C.c_int, C.c_int, C.POINTER(vp)]
         L.dit_cross_destroy.argtypes = [vp]
         L.dit_cross_destroy.restype = None
+        L.dit_cross_drop.argtypes = [vp]
+        L.dit_cross_drop.restype = None
         L.dit_cross_work.argtypes = [vp, C.c_int, C.c_int]
         L.dit_cross_forward.argtypes = [vp, vp, C.c_int] + 3 * [C.c_char_p] + [vp, C.c_float, C.c_char_p, vp, i64, vp, i64, vp]
         L.dit_cross_grad.argtypes = [vp, vp, C.c_int] + 5 * [C.c_char_p] + [vp, i64, vp, C.c_float] + 3 * [C.c_char_p] + [
@@ -1115,8 +1117,9 @@ class Context:
 
 
 class CrossPlan:
-    """dit_cross: the lengths of a batch (see Context.cross_plan); keep it until the calls that use it have finished, and as
-    long as a graph that captured them is replayed."""
+    """dit_cross: the lengths of a batch (see Context.cross_plan).  It may be dropped at any time, after its calls were made: its
+    tables go with the making of the next plan, and those that a graph captured stay.  close() frees them at once: when the calls
+    that use them have finished, graphs are no longer replayed, and no stream is captured."""
 
     def __init__(self, ctx, heads, head_d, q_len, k_len, kv_heads=None, q_at=None, k_at=None):
         def integers(v, name):
@@ -1161,14 +1164,15 @@ class CrossPlan:
             n = self._work[dtype, grad] = lib().dit_cross_work(self.ptr, dtype, grad)
         return n
 
-    def close(self):
+    def close(self, later=False):
+        """Frees the tables; later: when that is safe."""
         if self.ptr:
-            lib().dit_cross_destroy(self.ptr)
+            (lib().dit_cross_drop if later else lib().dit_cross_destroy)(self.ptr)
             self.ptr = C.c_void_p()
 
     def __del__(self):
         try:
-            self.close()
+            self.close(later=True)
         except Exception:
             pass
 

@@ -3,6 +3,7 @@
 #include <cmath>
 #include <exception>
 #include <map>
+#include <mutex>
 #include <vector>
 
 #include "dit_train_internal.hpp"
@@ -15,6 +16,7 @@ struct dit_cross {
     int heads = 0, kv_heads = 0, head_d = 0;
     int64_t q_rows = 0, k_rows = 0;  // past the last row of any sequence
     void* tables = nullptr;
+    mutable int captured = 0;  // a graph holds a call that reads the tables
     // for AWA_F32 and AWA_BF16, whose work is worth dividing differently
     CrossQueries qs[2];
     CrossKeySide ks[2];
@@ -247,6 +249,30 @@ bool ranges_ok(const std::vector<int64_t>& at, const std::vector<int64_t>& len, 
     return true;
 }
 
+// Plans of dit_cross_drop, for the next plan's making to free.  Never destroyed: a plan may be dropped while the process ends.
+struct Dropped {
+    std::mutex lock;
+    std::vector<dit_cross*> plans;
+};
+Dropped& dropped() {
+    static Dropped* const d = new Dropped;
+    return *d;
+}
+std::vector<dit_cross*> take_dropped(int device) {
+    std::vector<dit_cross*> out, keep;
+    std::lock_guard<std::mutex> hold(dropped().lock);
+    for (dit_cross* p : dropped().plans) (p->device == device ? out : keep).push_back(p);
+    dropped().plans.swap(keep);
+    return out;
+}
+
+// notes that a graph takes a call in (the default stream cannot be captured, and is not to be asked while another one is)
+void note_capture(const dit_cross* plan, hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (s && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone)
+        __atomic_store_n(&plan->captured, 1, __ATOMIC_RELAXED);
+}
+
 int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_len, const int64_t* h_k_at,
            const int64_t* h_k_len, int heads, int kv_heads, int head_d, dit_cross** out) {
     if (!out || n_seq < 0 || n_seq > DIT_CROSS_SEQ_MAX || (n_seq && (!h_q_at || !h_q_len || !h_k_at || !h_k_len)) ||
@@ -275,6 +301,7 @@ int create(awa_ctx* ctx, int n_seq, const int64_t* h_q_at, const int64_t* h_q_le
         set_err(ctx, "dit_cross_create: query rows of two sequences overlap, or key rows do and are not the same");
         return AWA_EARG;
     }
+    for (dit_cross* plan : take_dropped(ctx->device)) dit_cross_destroy(plan);
     dit_cross c;
     c.device = ctx->device;
     c.heads = heads;
@@ -606,6 +633,15 @@ void dit_cross_destroy(dit_cross* plan) {
     delete plan;
 }
 
+void dit_cross_drop(dit_cross* plan) {
+    if (!plan || __atomic_load_n(&plan->captured, __ATOMIC_RELAXED)) return;
+    try {
+        std::lock_guard<std::mutex> hold(dropped().lock);
+        dropped().plans.push_back(plan);
+    } catch (const std::exception&) {  // memory: kept
+    }
+}
+
 int64_t dit_cross_work(const dit_cross* plan, int dtype, int grad) {
     take_whole(dtype);
     if (!plan || !dtype_ok(dtype)) return AWA_EARG;
@@ -657,7 +693,9 @@ int dit_cross_forward(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_
     a.qs = plan->qs[dtype]; a.ks = plan->ks[dtype];
     a.qpart = reinterpret_cast<float*>(static_cast<char*>(d_work) + w.qpart);
     DeviceGuard dg(ctx->device);
-    HIPCK(ctx, launch_cross_forward(dtype, a, reinterpret_cast<hipStream_t>(stream)));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    note_capture(plan, s);
+    HIPCK(ctx, launch_cross_forward(dtype, a, s));
     return AWA_OK;
 }
 
@@ -727,6 +765,7 @@ int dit_cross_grad(awa_ctx* ctx, const dit_cross* plan, int dtype, const dit_hea
     a.ld_dsum = qr;
     DeviceGuard dg(ctx->device);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    note_capture(plan, s);
     HIPCK(ctx, launch_cross_grad_queries(dtype, a, s));
     HIPCK(ctx, launch_cross_grad_keys(dtype, a, s));
     return AWA_OK;

@@ -107,6 +107,31 @@ int main() {
         for (int grad = 0; grad < 2; grad++)
             hold("work whole", dit_cross_work(&c, t | DIT_CROSS_WHOLE, grad) == dit_cross_work(&c, t, grad) && dit_cross_work(&c, t, grad) >= 0);
 
+    // ---- dropped plans go with the next one's making on their device; captured ones stay
+    auto one = [&](int device, int captured) {
+        dit_cross* p = new dit_cross;
+        p->device = device;
+        p->captured = captured;
+        dit_cross_drop(p);
+        return p;
+    };
+    one(0, 0);
+    dit_cross* const other = one(1, 0);
+    dit_cross* const captured = one(0, 1);
+    one(0, 0);
+    dit_cross_drop(nullptr);
+    hold("dropped", dropped().plans.size() == 3 && dropped().plans[1] == other);
+    const int64_t none = 0;
+    dit_cross* made = nullptr;
+    check("a bad plan frees none", dit_cross_create(&ctx, 1, &none, &none, &none, &none, 0, 1, 8, &made), bad);
+    hold("a bad plan", dropped().plans.size() == 3);
+    check("a plan", dit_cross_create(&ctx, 0, &none, &none, &none, &none, 1, 1, 8, &made), ok, 0);
+    hold("freed", made && dropped().plans.size() == 1 && dropped().plans[0] == other);
+    dit_cross_destroy(made);
+    for (dit_cross* p : take_dropped(1)) dit_cross_destroy(p);
+    dit_cross_destroy(captured);
+    hold("none left", dropped().plans.empty());
+
     // ---- outputs beside inputs and each other, in one buffer
     const int64_t F = 1 << 20;  // bytes past which another tensor lies in the same buffer
     // keys' gradients with heads outermost, [2 heads][dk, dv][50 rows][64]

@@ -33,3 +33,15 @@ def test_whole_reaches_the_library(awa, monkeypatch):
             ctx.cross_attn_grad(plan, q, q, k, k, q, lse, whole=whole)
             assert [args[2] for _, args in calls] == 2 * [code | awa.DIT_CROSS_WHOLE if whole else code]
             calls.clear()
+
+
+def test_a_collected_plan_is_dropped_and_a_closed_one_destroyed(awa, monkeypatch):
+    """Collection may come while a stream is captured or a graph lives: it must not free."""
+    ctx, calls = meta_context(awa, monkeypatch)
+    for end, name in ((lambda p: p.close(), "dit_cross_destroy"), (lambda p: None, "dit_cross_drop")):
+        plan = meta_plan(awa, ctx, 10, 20)
+        del plan.close  # the class's own
+        end(plan)
+        del plan
+        assert [n for n, _ in calls] == [name]
+        calls.clear()

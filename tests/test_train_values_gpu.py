@@ -301,3 +301,39 @@ def test_gradients_side_by_side_with_heads_outermost(ctx, dtype, nq):
         got = ctx.cross_attn_grad(plan, do, q, k, v, out, lse, dq=buf[5:6, 2], dk=buf[:, 0], dv=buf[:, 1])
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert bool((buf[:5, 2] == 7).all()) and bool((buf[6:, 2] == 7).all())
+
+
+# ------------------------------------------------------------------ plans that end before what used them
+
+def test_plans_dropped_before_their_graph(ctx):
+    """A captured plan's tables outlive it; a plan that is collected during a capture does not end it."""
+    import gc
+    import torch
+    g = gen(5)
+    ql, kl = [3, 70, 1], [500, 90, 2000]
+    q, k, v, do = (randn(g, n, h, 64) for n, h in ((74, 4), (2590, 2), (2590, 2), (74, 4)))
+
+    def program(plan):
+        out, lse = ctx.cross_attn(plan, q, k, v, lse=True)
+        return [out, lse, *ctx.cross_attn_grad(plan, do, q, k, v, out, lse)]
+
+    plan, spare = ctx.cross_plan(4, 64, ql, kl, kv_heads=2), [ctx.cross_plan(4, 64, ql, kl, kv_heads=2)]
+    want = program(spare[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        spare.clear()
+        gc.collect()
+        res = program(plan)
+    del plan
+    gc.collect()
+    # plans of other lengths, in whatever memory has become free
+    others = [ctx.cross_plan(4, 64, [1 + i, 70, 1], [500, 90 + i, 2000], kv_heads=2) for i in range(30)]
+    for _ in range(4):
+        for t in res:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+        others.append(ctx.cross_plan(4, 64, ql, kl, kv_heads=2))
+        assert all(torch.equal(a, b) for a, b in zip(program(others[-1]), want))
