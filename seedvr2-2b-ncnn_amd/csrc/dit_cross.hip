@@ -381,8 +381,9 @@ void run(const CrossArgs& a, hipStream_t s) {
 template <typename T, int DP, bool GRAD>
 void run_block(const CrossArgs& a, hipStream_t s) {
     constexpr int WK = T::SIZE == 2 ? 4 : 2;
-    if (a.qs.block == 128 && T::SIZE == 2 && a.qs.most_keys <= 64) run<T, DP, 2, 4, 1, 64, GRAD, true>(a, s);
-    else if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 ? 64 : 32, GRAD>(a, s);
+    if constexpr (T::SIZE == 2)
+        if (a.qs.block == 128 && a.qs.most_keys <= 64) return run<T, DP, 2, 4, 1, 64, GRAD, true>(a, s);
+    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 ? 64 : 32, GRAD>(a, s);
     else if (a.qs.block == 32) run<T, DP, 2, 1, WK, 32, GRAD>(a, s);
     else run<T, DP, 1, 1, WK, 32, GRAD>(a, s);
 }
