@@ -337,3 +337,86 @@ def test_plans_dropped_before_their_graph(ctx):
         assert all(torch.equal(a, b) for a, b in zip(res, want))
         others.append(ctx.cross_plan(4, 64, ql, kl, kv_heads=2))
         assert all(torch.equal(a, b) for a, b in zip(program(others[-1]), want))
+
+
+# ------------------------------------------------------------------ sums that are exact
+
+def whole_numbers(g, top, *shape):
+    import torch
+    return torch.randint(-top, top + 1, shape, generator=g, device="cuda").float()
+
+
+# one wave a row to eight, rows of fewer than four columns, one row at a time; few rows and many
+@pytest.mark.parametrize("rows,cols", [(1, 3), (5001, 3), (2049, 130), (30001, 520), (4097, 1025), (9999, 1537), (2600, 2050), (12371, 2693),
+                                       (1025, 4096), (777, 4097), (3001, 8191), (515, 12289), (511, 16384)])
+@pytest.mark.parametrize("tdy,tx", [(BF16, BF16), (F32, F32), (BF16, "fp8"), (F32, "fp8")])
+def test_norm_columns_exact(ctx, rows, cols, tdy, tx):
+    """dw and db of whole numbers: |dy| up to 4, h up to 8 in halves, so that every sum is a number of halves under 2^24 and
+    exact in any order; a row or column that is lost, or taken twice, shows."""
+    import torch
+    g = gen(rows + cols)
+    dy = whole_numbers(g, 4, rows, cols + 1).to(dt(tdy))[:, 1:]
+    x = whole_numbers(g, 12, rows, cols)
+    st = torch.stack((whole_numbers(g, 4, rows), torch.full((rows,), 0.5, device="cuda")), 1).contiguous()
+    assert rows * 4 * 8 * 2 < 2 ** 24
+    h = (x.double() - st[:, :1].double()) * 0.5
+    if tx == "fp8":  # whole numbers up to 16 have at most the four bits of e4m3
+        xin, xs = ctx.quant_fp8(x)
+    else:
+        xin, xs = x.to(dt(tx)), None
+    w = whole_numbers(g, 3, cols)
+    _, dw, db = ctx.layer_norm_grad(dy, xin, st, w, x_scale=xs)
+    assert torch.equal(dw.double(), (dy.double() * h).sum(0))
+    assert torch.equal(db.double(), dy.double().sum(0))
+
+
+@pytest.mark.parametrize("rows,cols", [(5001, 130), (30001, 64), (12371, 2693), (2600, 8000), (3000, 16384)])
+def test_norm_columns_by_their_chain(ctx, rows, cols):
+    """dw and db of random data within the sums' length: the rows that a lane adds, 3 halves of a workgroup's waves, at most 66
+    parts; a term's own error is 4 U (h 2, its product, a spare one)."""
+    g = gen(rows)
+    x, dy = randn(g, rows, cols) + randn(g, rows, 1), randn(g, rows, cols)
+    _, st = ctx.layer_norm(x, stats=True)
+    _, dw, db = ctx.layer_norm_grad(dy, x, st)
+    pieces = (cols + 255) // 256
+    at_once = 8 if pieces <= 4 else 4 if pieces <= 8 else 2 if pieces <= 16 else 1
+    n = -(-rows // (min(-(-rows // at_once), 256) * at_once)) + 3 + 66 + 4
+    h = (x.double() - st[:, :1].double()) * st[:, 1:].double()
+    within(dw, (dy.double() * h).sum(0), n * U * (dy.double() * h).abs().sum(0), "dw")
+    within(db, dy.double().sum(0), n * U * dy.double().abs().sum(0), "db")
+
+
+# tiles of 128 and 256, whole, divided, and some of each; sizes beside theirs; rows of less than a stage
+WEIGHTS = [(1, 5, 7), (31, 130, 260), (33, 7, 500), (700, 300, 600), (1237, 199, 1300), (1237, 1999, 2693), (2047, 640, 2050),
+           (1300, 4353, 4353), (5498, 2560, 2560), (4100, 96, 4200)]
+
+
+@pytest.mark.parametrize("tdy", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", WEIGHTS)
+def test_weight_sums_exact(ctx, tdy, M, N, K):
+    """Whole numbers: |dy| up to 4, x up to 8 times a row's 1, 2 or 4, every sum under 2^24: dW and db are exact."""
+    import torch
+    g = gen(M + N + K)
+    dy = whole_numbers(g, 4, M, N + 3).to(dt(tdy))[:, 2:N + 2]
+    x = whole_numbers(g, 8, M, K) * torch.exp2(torch.randint(0, 3, (M, 1), generator=g, device="cuda").float())
+    assert M * 4 * 32 < 2 ** 24
+    q, s = ctx.quant_fp8(x)
+    dw, db = ctx.grad_weight_fp8(dy, q, s, cols=K, bias=True)
+    assert torch.equal(dw.double(), dy.double().t().contiguous() @ x.double())
+    assert torch.equal(db.double(), dy.double().sum(0))
+
+
+@pytest.mark.parametrize("M,N,K", [w for w in WEIGHTS if w[0] <= w[2]])
+def test_weight_fp32_values_exact(ctx, M, N, K):
+    """fp32 dy of 24 bits, each value alone in its sums (column k of x is a power of two in row k mod M and zeros): every bit of
+    every row of dy arrives."""
+    import torch
+    g = gen(M + N)
+    dy = torch.randint(-2 ** 24 + 1, 2 ** 24, (M, N), generator=g, device="cuda").float()
+    dy = dy * torch.exp2(torch.randint(-40, 20, (M, N), generator=g, device="cuda").float())
+    k = torch.arange(K, device="cuda")
+    x = torch.zeros(M, K, device="cuda")
+    x[k % M, k] = torch.where(k % 3 == 0, -2.0, torch.where(k % 3 == 1, 1.0, 0.25))
+    q, s = ctx.quant_fp8(x)
+    dw = ctx.grad_weight_fp8(dy, q, s, cols=K)
+    assert torch.equal(dw, (dy[k % M] * x[k % M, k][:, None]).t())
