@@ -51,7 +51,7 @@ enum { DIT_FP8 = 2 };
  * NULL (1 and 0).  d_stats (may be NULL): fp32 [M][2], each row's mean and rstd, for
  * the gradient.  M may be 0, K is 1 .. DIT_NORM_COLS_MAX.  Tensors need their
  * elements' alignment only (d_stats 8 bytes); y may be x itself (same type and stride).
- * A NaN or infinity makes its row NaN.  Rejected (AWA_EARG): sizes out of range, a
+ * A NaN or infinity makes its row NaN; a row whose squares sum past 2^128 has rstd 0 (y = b).  Rejected (AWA_EARG): sizes out of range, a
  * stride under K (for M > 1), eps negative or not finite, y over an input otherwise. */
 enum { DIT_NORM_COLS_MAX = 16384 };
 int dit_layer_norm(awa_ctx* ctx, int dtype_x, const void* d_x, int64_t ldx, const float* d_w, const float* d_b,

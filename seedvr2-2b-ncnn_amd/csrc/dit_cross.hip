@@ -12,11 +12,12 @@
 // generated) blocks of 16 or 32, waves that take tiles of their own in turn and add their results in LDS.
 // Runs of keys of one block that go to different workgroups leave fp32 partial results, which a second kernel joins.
 //
-// In blocks of 128 a wave's 32 columns make as many cycles of LDS reads as of products, which bounds them, two waves a SIMD
-// filling each other's waits: 27200 queries x 1024 keys x 20 heads of 128 311 us (0.92 PFLOP/s; 48 columns a wave, which spills, 320;
-// 16 425), 16384 x 384 79 (0.82).  With up to 64 keys one tile is all: half the LDS, no second maximum, four workgroups a CU
-// (5440 x 58 16.6 -> 14.9 us, 16384 x 64 32).  Few columns are bound by the keys' bytes: 32 tokens x 1500 keys, 20 heads on 4,
-// 22 us (4.4 TB/s; in blocks of 128 91), 64 x 2048, 32 on 8, 100 (5.3).  fp32 by its matrix rate.
+// In blocks of 128 a wave's 32 columns make as many cycles of LDS reads as of products, and half as many of the softmax's VALU
+// instructions (51 % issue), which bounds them, two waves a SIMD filling each other's waits: 27200 queries x 1024 keys x 20 heads of 128
+// 311 us (0.92 PFLOP/s; 48 columns a wave, which spills, 320; 16 425), 16384 x 384 83 (0.78).  With up to 64 keys one tile is all:
+// half the LDS, no second maximum, four workgroups a CU (5440 x 58 16.6 -> 14.9 us, 16384 x 64 32.5).  Few columns are bound by
+// the keys' bytes: 32 tokens x 1500 keys, 20 heads on 4, 23 us (4.3 TB/s; in blocks of 128 91), 64 x 2048, 32 on 8, 97 (5.5).  fp32
+// by its matrix rate: 5440 x 512 x 20 heads 311 us (92 TFLOP/s).
 #include "dit_cross_device.hpp"
 
 namespace awa {

@@ -62,8 +62,8 @@ struct Bf16 {
 // bf16 tensors whose probabilities (and dS) keep 16 bits, as the sum of two bf16 values and in two products (an infinity,
 // whose rest is none, becomes NaN).  Rounded to one value they cost a result as much again as its own rounding, at three
 // quarters of the time, so that a caller chooses.  2-norm of the error over the result's, heads of 128: results 2.32e-3 in one
-// product and 1.66e-3 (their rounding) in two, dq 2.37e-3 and 1.68e-3.  27200 queries x 1024 keys x 20 heads: forward 306 us and
-// 382, gradients 1137 and 1500; 16384 x 384 81 and 98, 297 and 378; 5440 x 58 15.4 and 15.8, 56 and 60.
+// product and 1.66e-3 (their rounding) in two, dq 2.37e-3 and 1.68e-3.  27200 queries x 1024 keys x 20 heads: forward 306 to
+// 311 us and 382 to 404, gradients 1137 and 1500; 16384 x 384 83 and 105, 316 and 381; 5440 x 58 15.3 and 15.5, 56 and 60.
 struct Bf16Whole : Bf16 {
     struct Packed {
         Frag top, rest;

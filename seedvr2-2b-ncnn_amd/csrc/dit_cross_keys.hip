@@ -10,8 +10,10 @@
 // kernel adds in their order.
 //
 // Bound by LDS: a wave reads 64 KB of a unit, twice the cycles of its 64 matrix instructions.  Both gradients (this kernel a little
-// over half): 16384 queries x 384 keys x 20 heads 290 us (0.78 PFLOP/s of seven products), x 128 144, x 64 110; four clips of up to
-// 5440 x 512, masked, 280.  fp32, 10 heads of 80 on 2, 2 x up to 1237 x 300: 97.
+// over half from some hundred keys on, a third at 64), on two inputs in turn: 16384 queries x 384 keys x 20 heads 316 us (0.71
+// PFLOP/s of seven products; 297 on one input, part of which stays in the memory-side cache), x 128 176, x 64 142 (130); 5440 x 58 56; four
+// clips of up to 5440 x 512, masked, 283; 32 tokens x 750 to 1500 keys, 20 heads on 4, 117.  fp32, 10 heads of 80 on 2, 2 x up to 1237 x
+// 300: 98.
 #include <type_traits>
 
 #include "dit_cross_device.hpp"

@@ -12,9 +12,9 @@
 //
 // Bound by LDS: of the 1,930 cycles of a stage of a 256 x 256 tile its 192 transposed reads (6 cycles for 512 bytes, in any
 // layout) and the 32 KB that are written take 1,400, its matrix instructions 1,024; in tiles of 128 x 128 the share is larger.
-// bf16 dy and dW: 5498 x 13824 x 2560 327 to 346 us (1.16 PFLOP/s), 5498 x 7680 x 2560 210 (1.03), 5498 x 2560 x 2560 94, 679 x 7680 x
-// 2560 46, 58 x 7680 x 2560 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a product: 1.1 PFLOP/s of
-// them), 1237 x 1999 x 2693 57.
+// bf16 dy and dW: 5498 x 13824 x 2560 327 to 346 us (1.16 PFLOP/s), 5498 x 7680 x 2560 196 to 210 (1.1), 5498 x 2560 x 2560 87 to 94,
+// 679 x 7680 x 2560 41 to 46, 58 x 7680 x 2560 15 to 16.  fp32 dy: 5498 x 13824 x 2560 1010 to 1040 (three instructions a product:
+// 1.1 PFLOP/s of them), 1237 x 1999 x 2693 57.
 #include <algorithm>
 
 #include "dit_device.hpp"

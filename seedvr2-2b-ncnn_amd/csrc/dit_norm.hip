@@ -9,10 +9,11 @@
 // all rows of their wave, waves add theirs in LDS in a fixed order, workgroups leave a row of
 // partial sums each, which a second kernel adds in their order.
 //
-// Both are bound by HBM: each value is read once and written once.  Forward, 27258 x 2560: fp32 to bf16 81 us (5.2 TB/s),
-// bf16 46 (6.1); 12370 x 2693 bf16 28; 5498 x 2560 bf16 9.8.  Gradient, bf16 dy and dx: 27258 x 2560 with bf16 x 76 us (5.5
-// TB/s), 8-bit x 79, fp32 x 103; 5498 x 2560 22 to 24; 12370 x 2693 with 8-bit x 47 to 50, where widening and two passes
-// over the row cost as much as its bytes; of these 4 us are the partial sums' kernel.
+// Both are bound by HBM: each value is read once and written once.  Calls back to back on two inputs in turn; one input alone
+// stays partly in the memory-side cache (times in brackets).  Forward, 27258 x 2560: fp32 to bf16 81 us (70; 5.2 TB/s), bf16 56 to 60
+// (48; 4.7 TB/s); 12370 x 2693 bf16 32.5; 5498 x 2560 bf16 14.7 (12.7).  Gradient, bf16 dy and dx: 27258 x 2560 with bf16 x
+// 82 us (76; 5.1 TB/s), 8-bit x 89 (79), fp32 x 104; 5498 x 2560 bf16 23, fp32 x and dx 29; 12370 x 2693 with 8-bit x 47, where rows
+// that begin anywhere cost 8 % (2688 columns 44; 82 MB are written for 67); of these 4 us are the partial sums' kernel.
 #include <algorithm>
 
 #include "dit_train_internal.hpp"

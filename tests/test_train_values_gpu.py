@@ -420,3 +420,15 @@ def test_weight_fp32_values_exact(ctx, M, N, K):
     q, s = ctx.quant_fp8(x)
     dw = ctx.grad_weight_fp8(dy, q, s, cols=K)
     assert torch.equal(dw, (dy[k % M] * x[k % M, k][:, None]).t())
+
+
+def test_norm_squares_past_fp32(ctx):
+    """Squares that sum past 2^128: rstd 0, the bias alone; the rows beside are as they would be."""
+    import torch
+    g = gen(1)
+    x, b = randn(g, 5, 300), randn(g, 300)
+    x[2] = torch.where(torch.arange(300, device="cuda") % 2 == 0, 1e25, -1e25)
+    y, st = ctx.layer_norm(x, None, b, stats=True)
+    assert torch.equal(y[2], b) and float(st[2, 1]) == 0.0
+    keep = [0, 1, 3, 4]
+    assert torch.equal(y[keep], ctx.layer_norm(x[keep], None, b))
