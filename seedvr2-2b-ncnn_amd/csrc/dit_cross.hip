@@ -27,7 +27,7 @@ using namespace cross;
 namespace {
 
 template <typename T, int DP, int NQ, int WQ, int WK, int KT, bool GRAD, bool ONE>
-__global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE ? 3 : 2) : 1)) void cross_queries_kernel(CrossArgs p) {
+__global__ __launch_bounds__(64 * WQ * WK, (T::SIZE == 2 && WK == 1 ? (ONE && !(GRAD && T::WHOLE) ? 3 : 2) : 1)) void cross_queries_kernel(CrossArgs p) {
     using Frag = typename T::Frag;
     using L = Tile<T, DP>;
     constexpr int KS = DP / 32, DB = DP / 16, KB = KT / 16, WAVES = WQ * WK;
@@ -384,7 +384,9 @@ void run_block(const CrossArgs& a, hipStream_t s) {
     constexpr int WK = T::SIZE == 2 ? 4 : 2;
     if constexpr (T::SIZE == 2)
         if (a.qs.block == 128 && a.qs.most_keys <= 64) return run<T, DP, 2, 4, 1, 64, GRAD, true>(a, s);
-    if (a.qs.block == 128) run<T, DP, 2, 4, 1, T::SIZE == 2 ? 64 : 32, GRAD>(a, s);
+    // tiles of 32 keys where 64 would spill (gradients with 16 bits a probability, 16384 x 384: 381 us with spills, 370 so)
+    constexpr int KT = T::SIZE == 4 || (GRAD && T::WHOLE && DP == 128) ? 32 : 64;
+    if (a.qs.block == 128) run<T, DP, 2, 4, 1, KT, GRAD>(a, s);
     else if (a.qs.block == 32) run<T, DP, 2, 1, WK, 32, GRAD>(a, s);
     else run<T, DP, 1, 1, WK, 32, GRAD>(a, s);
 }

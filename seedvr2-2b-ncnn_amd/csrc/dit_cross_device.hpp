@@ -26,6 +26,7 @@ typedef __attribute__((address_space(3))) bf16x4 lbf16x4_t;
 
 struct Bf16 {
     static constexpr int SIZE = 2;
+    static constexpr bool WHOLE = false;
     using Frag = bf16x8;
     static __device__ inline Frag zero() { return (bf16x8)(__bf16)0.f; }
     static __device__ inline f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
@@ -63,8 +64,9 @@ struct Bf16 {
 // whose rest is none, becomes NaN).  Rounded to one value they cost a result as much again as its own rounding, at three
 // quarters of the time, so that a caller chooses.  2-norm of the error over the result's, heads of 128: results 2.32e-3 in one
 // product and 1.66e-3 (their rounding) in two, dq 2.37e-3 and 1.68e-3.  27200 queries x 1024 keys x 20 heads: forward 306 to
-// 311 us and 382 to 404, gradients 1137 and 1500; 16384 x 384 83 and 105, 316 and 381; 5440 x 58 15.3 and 15.5, 56 and 60.
+// 311 us and 382 to 404; 16384 x 384 83 and 105 to 108, gradients 316 and 370; 5440 x 58 15.3 and 15.6, 56 and 61.
 struct Bf16Whole : Bf16 {
+    static constexpr bool WHOLE = true;
     struct Packed {
         Frag top, rest;
     };
@@ -79,6 +81,7 @@ struct Bf16Whole : Bf16 {
 };
 struct F32 {
     static constexpr int SIZE = 4;
+    static constexpr bool WHOLE = false;
     using Frag = f32x8;
     static __device__ inline Frag zero() { return (f32x8)0.f; }
     static __device__ inline f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
