@@ -51,8 +51,9 @@ enum { DIT_FP8 = 2 };
  * NULL (1 and 0).  d_stats (may be NULL): fp32 [M][2], each row's mean and rstd, for
  * the gradient.  M may be 0, K is 1 .. DIT_NORM_COLS_MAX.  Tensors need their
  * elements' alignment only (d_stats 8 bytes); y may be x itself (same type and stride).
- * A NaN or infinity makes its row NaN; a row whose squares sum past 2^128 has rstd 0 (y = b).  Rejected (AWA_EARG): sizes out of range, a
- * stride under K (for M > 1), eps negative or not finite, y over an input otherwise. */
+ * A NaN or infinity makes its row NaN; a row whose squares sum past 2^128 has rstd 0
+ * (y = b).  Rejected (AWA_EARG): sizes out of range, a stride under K (for M > 1), eps
+ * negative or not finite, y over an input otherwise. */
 enum { DIT_NORM_COLS_MAX = 16384 };
 int dit_layer_norm(awa_ctx* ctx, int dtype_x, const void* d_x, int64_t ldx, const float* d_w, const float* d_b,
                    float eps, int dtype_y, void* d_y, int64_t ldy, float* d_stats, int M, int K,
@@ -102,9 +103,9 @@ int dit_grad_weight_fp8(awa_ctx* ctx, int dtype_dy, const void* d_dy, int64_t ld
  *
  * A row for which no key is left, or whose scores are all -infinity, gets zeros, lse
  * -infinity, and no gradient, whatever it, its dout, and the keys and values that made it so, hold
- * (a row whose given lse is -infinity, too); masked keys (whatever they hold, NaN and infinities too)
- * take no part and get gradients of zero.  A row with a NaN or +infinity among its scores, or with its largest past
- * fp32 once more times log2(e), is NaN, its lse too.  Rows of tensors that belong to no sequence are
+ * (so does a row whose given lse is -infinity); masked keys (whatever they hold, NaN and infinities too)
+ * take no part and get gradients of zero.  A row with a NaN or +infinity among its scores, or whose largest
+ * score times log2(e) is past fp32, is NaN, its lse too.  Rows of tensors that belong to no sequence are
  * neither read nor written. */
 typedef struct dit_cross dit_cross;
 enum { DIT_CROSS_SEQ_MAX = 65536, DIT_CROSS_HEADS_MAX = 1024, DIT_CROSS_HEAD_D_MAX = 128 };
